@@ -53,6 +53,22 @@ class DvaeStep(ctypes.Structure):
                 ("Ge", c_void_p), ("Gd", c_void_p), ("out4", c_void_p)]
 
 
+class DvaeTensor(ctypes.Structure):
+    """Mirror of ``struct dvae_tensor``."""
+    _fields_ = [("in_", c_void_p), ("out", c_void_p), ("n", c_ll), ("in_type", c_int), ("out_type", c_int)]
+
+
+class DvaeRules(ctypes.Structure):
+    """Mirror of ``struct dvae_rules``."""
+    _fields_ = [("logits", c_void_p), ("rows", c_ll), ("ld", c_ll), ("vocab", c_int), ("dtype", c_int),
+                ("history", c_void_p), ("history_ld", c_ll), ("history_len", c_int), ("history_i64", c_int),
+                ("rows_per_history", c_ll), ("lengths", c_void_p)] + \
+               [(n, ctypes.c_double) for n in ("repetition", "frequency", "presence", "temperature")] + \
+               [(n, c_void_p) for n in ("repetition_rows", "frequency_rows", "presence_rows", "temperature_rows")] + \
+               [("bias", c_void_p), ("bias_ld", c_ll), ("mask", c_void_p), ("mask_words", c_int), ("states", c_int),
+                ("state", c_void_p)]
+
+
 class DvaeError(RuntimeError):
     pass
 
@@ -89,6 +105,15 @@ SIGNATURES = {
     "dvae_phase_read": (c_int, [c_void_p, c_void_p, c_int]),
     "dvae_adam_step": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, ctypes.c_double, ctypes.c_double,
                        ctypes.c_double, ctypes.c_double, ctypes.c_double, c_ll, c_void_p]),
+    "dvae_adam_step_scaled": (c_int, [c_void_p] * 5 + [c_size_t] + [ctypes.c_double] * 5 + [c_ll, c_void_p]),
+    "dvae_clip_ws_bytes": (c_size_t, [c_int]),
+    "dvae_grad_norm": (c_int, [c_void_p, c_int, ctypes.c_double, c_void_p, c_void_p, c_void_p]),
+    "dvae_clip_grads": (c_int, [c_void_p, c_int, ctypes.c_double, c_void_p, c_void_p, c_void_p]),
+    "dvae_rules_ws_bytes": (c_size_t, [_P(DvaeRules)]),
+    "dvae_rules_apply": (c_int, [_P(DvaeRules), c_void_p, c_ll, c_void_p]),
+    "dvae_rules_choose": (c_int, [_P(DvaeRules)] + [c_void_p] * 7),
+    "dvae_rules_logprob": (c_int, [_P(DvaeRules)] + [c_void_p] * 5),
+    "dvae_rules_logprob_bwd": (c_int, [_P(DvaeRules)] + [c_void_p] * 4 + [c_ll] + [c_void_p] * 3),
     "dvae_pair_path": (c_int, [c_int, c_int]),
     "dvae_typed_colsum": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_size_t,
                           c_void_p]),
@@ -126,6 +151,8 @@ SIGNATURES = {
     "dvae_step_part2": (c_int, [_P(DvaeStep), c_void_p, c_void_p]),
     "dvae_predict_ws_bytes": (c_size_t, [_P(DvaeDims)]),
     "dvae_decoder_predict": (c_int, [_P(DvaeDims)] + [c_void_p] * 9),
+    "dvae_predict_rules_ws_bytes": (c_size_t, [_P(DvaeDims)]),
+    "dvae_decoder_predict_rules": (c_int, [_P(DvaeDims)] + [c_void_p] * 5 + [_P(DvaeRules), c_void_p, c_int] + [c_void_p] * 3),
     "dvae_svae_dims_init": (c_int, [_P(SvaeDims)]),
     "dvae_svae_enc_param_floats": (c_size_t, [_P(SvaeDims)]),
     "dvae_svae_dec_param_floats": (c_size_t, [_P(SvaeDims)]),

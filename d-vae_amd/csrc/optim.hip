@@ -20,12 +20,17 @@ __device__ __forceinline__ void adam_one(float& p, float g, float& m, float& v, 
   p -= k.lr_over_bc1 * (m / denom);
 }
 
+// SCALED: the update of scale[0] * g (clipped gradients: 28 B per parameter still, where a pass that scales them first
+// costs 8 B more)
+template <bool SCALED>
 __global__ __launch_bounds__(256) void adam_kernel(float* __restrict__ P, const float* __restrict__ Gr, float* __restrict__ M,
-                                                   float* __restrict__ V, size_t n, AdamK k) {
+                                                   float* __restrict__ V, size_t n, AdamK k, const float* __restrict__ scale) {
   const size_t n4 = n >> 2;
+  const float c = SCALED ? scale[0] : 1.f;
   for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n4; i += (size_t)gridDim.x * blockDim.x) {
     float4 p = reinterpret_cast<float4*>(P)[i], m = reinterpret_cast<float4*>(M)[i], v = reinterpret_cast<float4*>(V)[i];
-    const float4 g = reinterpret_cast<const float4*>(Gr)[i];
+    float4 g = reinterpret_cast<const float4*>(Gr)[i];
+    if (SCALED) { g.x *= c; g.y *= c; g.z *= c; g.w *= c; }
     adam_one(p.x, g.x, m.x, v.x, k);
     adam_one(p.y, g.y, m.y, v.y, k);
     adam_one(p.z, g.z, m.z, v.z, k);
@@ -36,13 +41,11 @@ __global__ __launch_bounds__(256) void adam_kernel(float* __restrict__ P, const 
   }
   // the last n % 4 parameters
   const size_t t = (n4 << 2) + blockIdx.x * (size_t)blockDim.x + threadIdx.x;
-  if (blockIdx.x == 0 && t < n) adam_one(P[t], Gr[t], M[t], V[t], k);
+  if (blockIdx.x == 0 && t < n) adam_one(P[t], SCALED ? Gr[t] * c : Gr[t], M[t], V[t], k);
 }
 
-}  // namespace
-
-extern "C" int dvae_adam_step(float* param, const float* grad, float* exp_avg, float* exp_avg_sq, size_t n, double lr,
-                              double beta1, double beta2, double eps, double weight_decay, long long step, void* stream) {
+int adam_step(float* param, const float* grad, const float* scale, float* exp_avg, float* exp_avg_sq, size_t n, double lr,
+              double beta1, double beta2, double eps, double weight_decay, long long step, void* stream) {
   DVAE_REQUIRE(param && grad && exp_avg && exp_avg_sq, "adam_step: null pointer");
   DVAE_REQUIRE(step >= 1 && beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "adam_step: step >= 1, betas in [0, 1)");
   DVAE_REQUIRE(((uintptr_t)param & 15) == 0 && ((uintptr_t)grad & 15) == 0 && ((uintptr_t)exp_avg & 15) == 0 &&
@@ -52,7 +55,22 @@ extern "C" int dvae_adam_step(float* param, const float* grad, float* exp_avg, f
   const AdamK k{(float)(lr / bc1), (float)(1.0 / std::sqrt(bc2)), (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2),
                 (float)eps, (float)weight_decay};
   const int grid = (int)std::min<size_t>(((n >> 2) + 256) / 256, 4096);
-  hipLaunchKernelGGL(adam_kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, param, grad, exp_avg, exp_avg_sq, n, k);
+  if (scale) hipLaunchKernelGGL(adam_kernel<true>, dim3(grid), dim3(256), 0, (hipStream_t)stream, param, grad, exp_avg, exp_avg_sq, n, k, scale);
+  else hipLaunchKernelGGL(adam_kernel<false>, dim3(grid), dim3(256), 0, (hipStream_t)stream, param, grad, exp_avg, exp_avg_sq, n, k, scale);
   DVAE_LAUNCH_CHECK();
   return DVAE_OK;
+}
+
+}  // namespace
+
+extern "C" int dvae_adam_step(float* param, const float* grad, float* exp_avg, float* exp_avg_sq, size_t n, double lr,
+                              double beta1, double beta2, double eps, double weight_decay, long long step, void* stream) {
+  return adam_step(param, grad, nullptr, exp_avg, exp_avg_sq, n, lr, beta1, beta2, eps, weight_decay, step, stream);
+}
+
+extern "C" int dvae_adam_step_scaled(float* param, const float* grad, const float* scale, float* exp_avg, float* exp_avg_sq,
+                                     size_t n, double lr, double beta1, double beta2, double eps, double weight_decay,
+                                     long long step, void* stream) {
+  DVAE_REQUIRE(scale, "adam_step_scaled: null pointer");
+  return adam_step(param, grad, scale, exp_avg, exp_avg_sq, n, lr, beta1, beta2, eps, weight_decay, step, stream);
 }

@@ -6,6 +6,7 @@
 #include <algorithm>
 
 #include "layout.h"
+#include "rules.h"
 
 namespace {
 
@@ -59,6 +60,30 @@ __global__ void pick_type_kernel(int M, int N, int C, int i, const float* __rest
     type[m] = pick;
     float* oh = onehot + ((size_t)m * N + i) * C;
     for (int c = 0; c < C; ++c) oh[c] = c == pick ? 1.f : 0.f;
+  }
+}
+
+// under rules: before node 0, every latent's grammar state and its first uniform number
+__global__ void rules_start_kernel(int M, int N, int start, const float* __restrict__ u_type, int* __restrict__ state,
+                                   float* __restrict__ u) {
+  ITEM_LOOP(M) {
+    state[it] = start;
+    if (u_type) u[it] = u_type[it * N];
+  }
+}
+
+// the chosen token of node i -> type, one-hot row (all zero where the rules left nothing), the latent's history; and the
+// uniform number of node i + 1
+__global__ void rules_type_kernel(int M, int N, int C, int i, const long long* __restrict__ tokens,
+                                  const float* __restrict__ u_type, int* __restrict__ type, int* __restrict__ history,
+                                  float* __restrict__ u, float* __restrict__ onehot) {
+  ITEM_LOOP(M) {
+    const int t = (int)tokens[it];
+    type[it] = max(t, 0);
+    history[it * N + i] = t;
+    float* oh = onehot + ((size_t)it * N + i) * C;
+    for (int c = 0; c < C; ++c) oh[c] = c == t ? 1.f : 0.f;
+    if (u_type && i + 1 < N) u[it] = u_type[it * N + i + 1];
   }
 }
 
@@ -239,9 +264,39 @@ int nt(const float* X, int ldx, const float* W, int ldw, float* Y, int ldy, int 
 
 extern "C" size_t dvae_predict_ws_bytes(const dvae_dims* d) { return pred_ws(*d, nullptr).bytes; }
 
-extern "C" int dvae_decoder_predict(const dvae_dims* dp, const float* z, const float* P, void* ws,
-                                    const float* u_type, const float* u_edge, float* edges, float* onehot,
-                                    float* min_margin, void* stream) {
+namespace {
+
+// buffers of a decode under rules, behind the plain decode's
+struct RulesWs {
+  long long* tokens;
+  float *logprob, *u;
+  int *state, *history;
+  void* choose;
+  size_t bytes;
+};
+
+RulesWs rules_ws(const dvae_dims& d, void* base) {
+  RulesWs w;
+  Carver c{(char*)base, pred_ws(d, nullptr).bytes};
+  const size_t M = d.B;
+  w.tokens = reinterpret_cast<long long*>(c.f(M * 2));
+  w.logprob = c.f(M);
+  w.u = c.f(M);
+  w.state = reinterpret_cast<int*>(c.f(M));
+  w.history = reinterpret_cast<int*>(c.f(M * d.N));
+  dvae_rules q{};
+  q.rows = d.B;
+  q.vocab = d.C;
+  w.choose = c.f(dvae_rules_ws_bytes(&q) / 4 + 1);
+  w.bytes = c.off;
+  return w;
+}
+
+// rules: NULL, or the settings of the type decisions
+struct TypeRules { const dvae_rules* rules; const int* next; int start; };
+
+int decoder_predict(const dvae_dims* dp, const float* z, const float* P, void* ws, const float* u_type, const float* u_edge,
+                    float* edges, float* onehot, float* min_margin, const TypeRules* tr, void* stream) {
   DVAE_REQUIRE(dp && z && P && ws && edges && onehot, "predict: null pointer");
   DVAE_REQUIRE((u_type == nullptr) == (u_edge == nullptr), "predict: u_type and u_edge go together");
   const dvae_dims& d = *dp;
@@ -252,6 +307,12 @@ extern "C" int dvae_decoder_predict(const dvae_dims* dp, const float* z, const f
   const GruW gw = gru_at(P + L.gru, HP, d.C);
   const float* gm = P + L.gm;
   const size_t MH = (size_t)M * HP;
+  RulesWs rw{};
+  if (tr) {
+    rw = rules_ws(d, ws);
+    hipLaunchKernelGGL(rules_start_kernel, grid_for(M), dim3(256), 0, st, M, N, tr->start, u_type, rw.state, rw.u);
+    DVAE_LAUNCH_CHECK();
+  }
 
   hipLaunchKernelGGL(fill_kernel, grid_for(M), dim3(256), 0, st, w.MARG, INFINITY, (size_t)M);
   DVAE_CHECK_HIP(hipMemsetAsync(edges, 0, (size_t)M * N * N * 4, st));
@@ -263,8 +324,21 @@ extern "C" int dvae_decoder_predict(const dvae_dims* dp, const float* z, const f
     // node type (:282-291)
     DVAE_TRY(nt(gstate, HP, P + L.Wv1, HP, w.VH, d.VHP, M, d.VHP, HP, P + L.bv1, 1, w.gemm_ws, st));
     DVAE_TRY(nt(w.VH, d.VHP, P + L.Wv2, d.VHP, w.TL, d.CP, M, d.CP, d.VHP, P + L.bv2, 0, w.gemm_ws, st));
-    hipLaunchKernelGGL(pick_type_kernel, grid_for(M), dim3(256), 0, st, M, N, d.C, i, w.TL, d.CP, u_type, w.type,
-                       onehot, w.MARG);
+    if (tr) {
+      dvae_rules q = *tr->rules;
+      q.logits = w.TL; q.rows = M; q.ld = d.CP; q.vocab = d.C; q.dtype = DVAE_F32;
+      q.history = i ? rw.history : nullptr; q.history_ld = N; q.history_len = i; q.history_i64 = 0; q.rows_per_history = 1;
+      q.lengths = nullptr;
+      q.state = rw.state;
+      const int* next = q.mask ? tr->next : nullptr;
+      DVAE_TRY(dvae_rules_choose(&q, u_type ? rw.u : nullptr, next, rw.tokens, rw.logprob, next ? rw.state : nullptr,
+                                 rw.choose, st));
+      hipLaunchKernelGGL(rules_type_kernel, grid_for(M), dim3(256), 0, st, M, N, d.C, i, rw.tokens, u_type, w.type,
+                         rw.history, rw.u, onehot);
+    } else {
+      hipLaunchKernelGGL(pick_type_kernel, grid_for(M), dim3(256), 0, st, M, N, d.C, i, w.TL, d.CP, u_type, w.type,
+                         onehot, w.MARG);
+    }
     DVAE_LAUNCH_CHECK();
     // initial state (:294-298)
     float* HV = w.HD + (size_t)i * MH;
@@ -335,4 +409,28 @@ extern "C" int dvae_decoder_predict(const dvae_dims* dp, const float* z, const f
     DVAE_LAUNCH_CHECK();
   }
   return DVAE_OK;
+}
+
+}  // namespace
+
+extern "C" int dvae_decoder_predict(const dvae_dims* dp, const float* z, const float* P, void* ws,
+                                    const float* u_type, const float* u_edge, float* edges, float* onehot,
+                                    float* min_margin, void* stream) {
+  return decoder_predict(dp, z, P, ws, u_type, u_edge, edges, onehot, min_margin, nullptr, stream);
+}
+
+extern "C" size_t dvae_predict_rules_ws_bytes(const dvae_dims* d) { return rules_ws(*d, nullptr).bytes; }
+
+extern "C" int dvae_decoder_predict_rules(const dvae_dims* dp, const float* z, const float* P, void* ws,
+                                          const float* u_type, const float* u_edge, const dvae_rules* rules,
+                                          const int* next, int start, float* edges, float* onehot, void* stream) {
+  DVAE_REQUIRE(dp && rules && ws, "predict_rules: null pointer");
+  dvae_rules q = *rules;      // as every node's call will have it; the workspace stands in for what the call fills in
+  q.logits = ws; q.rows = dp->B; q.ld = dp->CP; q.vocab = dp->C; q.dtype = DVAE_F32;
+  q.history = nullptr; q.state = (const int*)ws;
+  DVAE_TRY(rules_check(q, "predict_rules"));
+  DVAE_REQUIRE(!q.mask || next, "predict_rules: a grammar mask needs the next states");
+  DVAE_REQUIRE(!q.mask || (start >= 0 && start < q.states), "predict_rules: start state %d of %d", start, q.states);
+  const TypeRules tr{rules, next, start};
+  return decoder_predict(dp, z, P, ws, u_type, u_edge, edges, onehot, nullptr, &tr, stream);
 }

@@ -1,0 +1,848 @@
+// Token rules on logits: penalties for tokens a row's history holds, a bias, a grammar mask -- and what is read from the
+// ruled values: the values themselves (apply), a token (choose), a given token's log-probability and its gradients.
+//
+//   c = how often the row's history holds v
+//   x1 = c > 0 ? (x > 0 ? x / rho : x * rho) : x;  x2 = x1 - frequency c - presence [c > 0];  x3 = x2 + bias[v]
+//   x4 = allowed(state, v) ? x3 : -inf;            p = softmax(x4 / T)
+//
+// The operations are one pass over the logits.  A row is cut into segments, one wave each (64 lanes x 16 bytes a step); a
+// lane keeps a running sum of exp against a reference of its own that moves only when a value exceeds it by 2^8 -- no
+// rescaling in the common step, no block barrier.  Segments of one row leave (maximum, sum) pairs that a second, small
+// launch joins: sum_r = sum_seg s_seg 2^((m_seg - m) k), k = log2(e) / T; the token is then looked for in ONE segment.
+//
+// Counts: a workgroup counts the history's tokens that fall into its 4 segments in LDS (integer atomics: the order does
+// not matter).
+//
+// Numbers.  A token the history does not hold has the value x + b, one fp32 rounding; a counted one is computed in
+// double and rounded once.  Decisions do not rest on that rounding: rounding is monotone, so the largest exact value is
+// among the elements whose rounded value is the largest; those few are compared by the part the rounding dropped
+// (two-sum; for counted ones double minus the rounded value).  A drawn token is decided where a running sum over the
+// whole vocabulary crosses u Z, and with thousands of probable tokens a border of fp32 sums lies within their rounding of
+// u Z for a few percent of the rows: its weights and sums are doubles, with an exp2 of 1e-12.
+#include <algorithm>
+#include <cmath>
+
+#include "rules.h"
+
+namespace {
+
+constexpr double LOG2E = 1.4426950408889634074;
+constexpr double LN2 = 0.69314718055994530942;
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+// rows start at any element (an odd vocabulary, a padded matrix): 16-byte accesses at the element's alignment
+typedef uint32_t u32x4_u2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+
+template <int T> struct Elem;
+template <> struct Elem<DVAE_F32> {
+  typedef float type;
+  static constexpr int EV = 4;
+  static __device__ __forceinline__ float at(u32x4 r, int e) { return __uint_as_float(r[e]); }
+  static __device__ __forceinline__ float one(const void* p, long long i) { return static_cast<const float*>(p)[i]; }
+  static __device__ __forceinline__ float cast(float v) { return v; }
+};
+template <> struct Elem<DVAE_BF16> {
+  typedef __bf16 type;
+  static constexpr int EV = 8;
+  static __device__ __forceinline__ float at(u32x4 r, int e) {
+    const uint32_t w = r[e >> 1];
+    return __uint_as_float((e & 1) ? (w & 0xffff0000u) : (w << 16));
+  }
+  static __device__ __forceinline__ float one(const void* p, long long i) {
+    return __uint_as_float((uint32_t)static_cast<const uint16_t*>(p)[i] << 16);
+  }
+  static __device__ __forceinline__ __bf16 cast(float v) { return (__bf16)v; }
+};
+template <> struct Elem<DVAE_F16> {
+  typedef _Float16 type;
+  static constexpr int EV = 8;
+  static __device__ __forceinline__ float at(u32x4 r, int e) {
+    const uint16_t h = (uint16_t)((e & 1) ? (r[e >> 1] >> 16) : (r[e >> 1] & 0xffffu));
+    return (float)__builtin_bit_cast(_Float16, h);
+  }
+  static __device__ __forceinline__ float one(const void* p, long long i) {
+    return (float)static_cast<const _Float16*>(p)[i];
+  }
+  static __device__ __forceinline__ _Float16 cast(float v) { return (_Float16)v; }
+};
+
+// what a wave knows about its row
+struct RowP {
+  double rho, inv_rho, freq, pres, k;      // k = log2(e) / T
+  const uint8_t* mask;            // packed bits of the row's grammar state, or NULL: everything allowed
+  const float* bias;              // or NULL
+  const char* hist;               // the row's history
+  int n_hist;
+};
+
+__device__ __forceinline__ RowP row_params(const dvae_rules& q, long long r) {
+  RowP p;
+  p.rho = q.repetition_rows ? (double)q.repetition_rows[r] : q.repetition;
+  p.inv_rho = 1.0 / p.rho;
+  p.freq = q.frequency_rows ? (double)q.frequency_rows[r] : q.frequency;
+  p.pres = q.presence_rows ? (double)q.presence_rows[r] : q.presence;
+  p.k = LOG2E / (q.temperature_rows ? (double)q.temperature_rows[r] : q.temperature);
+  p.bias = q.bias ? q.bias + r * q.bias_ld : nullptr;
+  p.mask = nullptr;
+  if (q.mask) {
+    const int s = q.state[r];
+    // a state outside the table: no mask
+    if (s >= 0 && s < q.states) p.mask = reinterpret_cast<const uint8_t*>(q.mask + (size_t)s * q.mask_words);
+  }
+  p.n_hist = 0;
+  p.hist = nullptr;
+  if (q.history) {
+    int n = q.history_len;
+    if (q.lengths) n = max(0, min(n, q.lengths[r]));
+    p.n_hist = n;
+    p.hist = static_cast<const char*>(q.history) + (r / q.rows_per_history) * q.history_ld * (q.history_i64 ? 8 : 4);
+  }
+  return p;
+}
+
+__device__ __forceinline__ long long hist_at(const RowP& p, int i64, int i) {
+  return i64 ? reinterpret_cast<const long long*>(p.hist)[i] : (long long)reinterpret_cast<const int*>(p.hist)[i];
+}
+
+// the value of a token that the history holds c > 0 times.  x / rho as x (1 / rho) with one correction step: as good as
+// the division (equal quotients stay equal, so ties stay ties) at four operations
+__device__ __forceinline__ double counted64(const RowP& p, float x, uint32_t c, float b) {
+  const double xd = x;
+  double v = xd * p.inv_rho;
+  v = fma(fma(-v, p.rho, xd), p.inv_rho, v);
+  v = x > 0.f ? v : xd * p.rho;
+  v -= p.freq * (double)c;
+  v -= p.pres;
+  return v + (double)b;
+}
+
+// NaN if either is: a NaN among the allowed values has to reach the result
+__device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+__device__ __forceinline__ float wave_max_nan(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = max_nan(v, __shfl_xor(v, o));
+  return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+// 2^(d k) in double, d k up to 1000: a = n + f, |f| <= 1/2, 2^f by its series in f ln 2 up to the 10th power (the first
+// term left out is (ln 2 / 2)^11 / 11! = 2.2e-13 of the result).  Below 2^-1000 the weight is 0.
+__device__ __forceinline__ double exp2_64(double d, double k) {
+  const double a = d * k;
+  if (!(a >= -1000.0)) return a != a ? a : 0.0;
+  const double n = rint(a);
+  const double f = (a - n) * LN2;
+  double y = 1.0 / 3628800.0;
+  y = fma(y, f, 1.0 / 362880.0);
+  y = fma(y, f, 1.0 / 40320.0);
+  y = fma(y, f, 1.0 / 5040.0);
+  y = fma(y, f, 1.0 / 720.0);
+  y = fma(y, f, 1.0 / 120.0);
+  y = fma(y, f, 1.0 / 24.0);
+  y = fma(y, f, 1.0 / 6.0);
+  y = fma(y, f, 0.5);
+  y = fma(y, f, 1.0);
+  y = fma(y, f, 1.0);
+  return ldexp(y, (int)n);
+}
+
+// what a segment leaves for the join
+struct Seg {
+  double s;       // sum of 2^((x4 - m) k)
+  float m;        // maximum (NaN when an allowed value is)
+  int pad;
+};
+
+enum { M_APPLY = 0, M_SUM = 1, M_GREEDY = 2, M_DRAW = 3, M_BWD = 4 };
+
+constexpr int SEG_MAX = 4096;   // tokens of a segment at most: the counts of a workgroup's 4 segments are 32 KB of 16 bits
+
+struct SegArgs {
+  dvae_rules q;
+  int nseg, seg_len;            // segments of a row, their tokens (a multiple of 64 x 16 bytes)
+  int wgs_per_row;              // workgroups of a row (ROWWAVE: unused)
+  void* out; long long out_ld;  // APPLY / BWD
+  Seg* seg;                     // SUM / DRAW
+  const long long* tokens;      // BWD
+  const float* stat;            // BWD: [rows][2] = maximum, 1 / Z
+  const float* d_logprob;       // BWD
+  float* d_bias_rows;           // BWD: gradient of a bias of its own per row, [rows][vocab], or NULL
+};
+
+// counts of 4 segments: u16 pairs in 32-bit words while a history has fewer than 65536 tokens, else 32 bits each
+template <int HIST> struct Counts;
+template <> struct Counts<1> { static constexpr int PER_WORD = 2; };
+template <> struct Counts<2> { static constexpr int PER_WORD = 1; };
+
+template <int HIST>
+__device__ __forceinline__ void count_one(uint32_t* lds, int d) {
+  if (HIST == 1) atomicAdd(&lds[d >> 1], (d & 1) ? 0x10000u : 1u);
+  else atomicAdd(&lds[d], 1u);
+}
+template <int HIST>
+__device__ __forceinline__ uint32_t count_at(const uint32_t* lds, int d) {
+  if (HIST == 1) return (lds[d >> 1] >> ((d & 1) * 16)) & 0xffffu;
+  return lds[d];
+}
+
+// adds the history's tokens in [v0, v0 + span) to lds; `lane` of `width` threads
+template <int HIST>
+__device__ __forceinline__ void count_history(const RowP& p, int i64, long long v0, int span, uint32_t* lds, int lane,
+                                              int width) {
+  int i = lane;
+  for (; i + 3 * width < p.n_hist; i += 4 * width) {
+    long long t[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) t[u] = hist_at(p, i64, i + u * width) - v0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if ((unsigned long long)t[u] < (unsigned long long)span) count_one<HIST>(lds, (int)t[u]);
+  }
+  for (; i < p.n_hist; i += width) {
+    const long long t = hist_at(p, i64, i) - v0;
+    if ((unsigned long long)t < (unsigned long long)span) count_one<HIST>(lds, (int)t);
+  }
+}
+
+// 16 bytes of logits from token v on; past the vocabulary zeros
+template <int T>
+__device__ __forceinline__ u32x4 load_logits(const char* lrow, int v, int V) {
+  constexpr int EV = Elem<T>::EV, BYTES = 16 / EV;
+  if (v + EV <= V) return *reinterpret_cast<const u32x4_u2*>(lrow + (size_t)v * BYTES);
+  u32x4 r = {0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < EV; ++e)
+    if (v + e < V) {
+      if (T == DVAE_F32) r[e] = reinterpret_cast<const uint32_t*>(lrow)[v + e];
+      else r[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(lrow)[v + e] << ((e & 1) * 16);
+    }
+  return r;
+}
+
+// EV tokens from v on, d their place among the counts
+template <int T, int HIST>
+struct Ruled {
+  typedef Elem<T> E;
+  static constexpr int EV = E::EV;
+  float x[EV], b[EV];
+  uint32_t c[EV];
+  uint32_t keep;                // bit e: allowed (and inside the vocabulary)
+  __device__ __forceinline__ Ruled(const RowP& p, u32x4 raw, const uint32_t* cnt, int v, int d, int V) {
+    keep = v + EV <= V ? (1u << EV) - 1 : v < V ? (1u << (V - v)) - 1 : 0u;
+    if (p.mask && v < V) {
+      const uint32_t byte = p.mask[v >> 3];
+      keep &= EV == 8 ? byte : byte >> (v & 4);
+    }
+#pragma unroll
+    for (int e = 0; e < EV; ++e) { x[e] = E::at(raw, e); b[e] = 0.f; c[e] = 0; }
+    if (p.bias) {
+      if (v + EV <= V) {
+#pragma unroll
+        for (int e = 0; e < EV; e += 4) {
+          const f32x4_u t = *reinterpret_cast<const f32x4_u*>(p.bias + v + e);
+          b[e] = t[0]; b[e + 1] = t[1]; b[e + 2] = t[2]; b[e + 3] = t[3];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < EV; ++e) if (v + e < V) b[e] = p.bias[v + e];
+      }
+    }
+    if (HIST) {
+#pragma unroll
+      for (int e = 0; e < EV; ++e) c[e] = count_at<HIST ? HIST : 1>(cnt, d + e);
+    }
+  }
+  __device__ __forceinline__ bool kept(int e) const { return (keep >> e) & 1; }
+  // rounded once to fp32
+  __device__ __forceinline__ float value(const RowP& p, int e) const {
+    float y = x[e] + b[e];
+    if (HIST) { if (c[e]) y = (float)counted64(p, x[e], c[e], b[e]); }
+    return kept(e) ? y : -INFINITY;
+  }
+  __device__ __forceinline__ double value64(const RowP& p, int e) const {
+    double y = (double)x[e] + (double)b[e];
+    if (HIST) { if (c[e]) y = counted64(p, x[e], c[e], b[e]); }
+    return kept(e) ? y : -INFINITY;
+  }
+};
+
+template <int T, int HIST, int MODE, bool ROWWAVE>
+__global__ __launch_bounds__(256) void rules_seg_kernel(SegArgs a) {
+  typedef Elem<T> E;
+  constexpr int EV = E::EV, STEP = 64 * EV;
+  constexpr int WORDS = HIST ? 4 * SEG_MAX / Counts<HIST ? HIST : 1>::PER_WORD : 4;
+  __shared__ uint32_t lds[WORDS];
+  const dvae_rules& q = a.q;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  long long row;
+  int seg;
+  if (ROWWAVE) {
+    row = (long long)blockIdx.x * 4 + wave;
+    seg = 0;
+  } else {
+    row = blockIdx.x / a.wgs_per_row;
+    seg = (blockIdx.x % a.wgs_per_row) * 4 + wave;
+  }
+  const bool live = row < q.rows && seg < a.nseg;
+  const int V = q.vocab;
+  const int v0 = live ? seg * a.seg_len : 0;
+  RowP p = row_params(q, row < q.rows ? row : q.rows - 1);
+  const uint32_t* cnt = lds;
+  if (HIST) {
+    const int words = 4 * a.seg_len / Counts<HIST ? HIST : 1>::PER_WORD;
+    for (int i = threadIdx.x * 4; i < words; i += 1024) *reinterpret_cast<u32x4*>(&lds[i]) = u32x4{0, 0, 0, 0};
+    __syncthreads();
+    if (ROWWAVE) {
+      if (live) count_history<HIST>(p, q.history_i64, 0, a.seg_len, lds + wave * (words / 4), lane, 64);
+    } else {
+      count_history<HIST>(p, q.history_i64, (long long)(seg - wave) * a.seg_len, 4 * a.seg_len, lds, threadIdx.x, 256);
+    }
+    __syncthreads();
+    cnt = lds + wave * (words / 4);
+  }
+  if (!live) return;
+  const int end = min(v0 + a.seg_len, V);
+  const char* lrow = static_cast<const char*>(q.logits) + row * q.ld * (long long)sizeof(typename E::type);
+  const float kf = (float)p.k;
+
+  if (MODE == M_APPLY || MODE == M_BWD) {
+    typename E::type* orow = static_cast<typename E::type*>(a.out) + row * a.out_ld;
+    float m = 0.f, iz = 0.f, coef = 0.f;
+    long long tok = -1;
+    bool zero = false;
+    if (MODE == M_BWD) {
+      m = a.stat[2 * row];
+      iz = a.stat[2 * row + 1];
+      coef = (float)((double)a.d_logprob[row] * (p.k * LN2));
+      tok = a.tokens[row];
+      zero = tok < 0 || tok >= V || m == -INFINITY;      // an ignored row, or one whose rules leave nothing
+    }
+    const float up = (float)p.rho, down = (float)p.inv_rho;
+    for (int v = v0 + lane * EV; v < end; v += STEP) {
+      const Ruled<T, HIST> r(p, load_logits<T>(lrow, v, V), cnt, v, v - v0, V);
+      typename E::type o[EV];
+#pragma unroll
+      for (int e = 0; e < EV; ++e) {
+        float y = r.value(p, e);
+        if (MODE == M_BWD) {
+          float g = coef * ((v + e == tok ? 1.f : 0.f) - __builtin_amdgcn_exp2f((y - m) * kf) * iz);
+          if (zero || !r.kept(e)) g = 0.f;
+          if (a.d_bias_rows && v + e < V) a.d_bias_rows[row * V + v + e] = g;
+          if (HIST) { if (r.c[e]) g *= r.x[e] > 0.f ? down : up; }
+          y = g;
+        }
+        o[e] = E::cast(y);
+      }
+      if (v + EV <= V) {
+        u32x4 w;
+        __builtin_memcpy(&w, o, 16);
+        *reinterpret_cast<u32x4_u2*>(orow + v) = w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < EV; ++e)
+          if (v + e < V) orow[v + e] = o[e];
+      }
+    }
+    return;
+  }
+
+  // reference of the lane's sum: weights are 2^((x4 - ref) k), up to 2^8 before it moves (fp32: an exponent of 8 is still
+  // exact to 2^-20) or 2^900 (double)
+  constexpr float ROOM = MODE == M_DRAW ? 900.f : 8.f;
+  const float room = ROOM / kf;
+  float ref = -3.402823466e38f, lim = ref, m = -INFINITY, z = 0.f;
+  double zd = 0.0;
+  for (int v = v0 + lane * EV; v < end; v += STEP) {
+    const Ruled<T, HIST> r(p, load_logits<T>(lrow, v, V), cnt, v, v - v0, V);
+    float s[EV];
+#pragma unroll
+    for (int e = 0; e < EV; ++e) s[e] = r.value(p, e);
+    float mx = s[0];
+#pragma unroll
+    for (int e = 1; e < EV; ++e) mx = max_nan(mx, s[e]);
+    m = max_nan(m, mx);
+    if (mx > lim) {
+      if (MODE == M_DRAW) zd *= exp2_64((double)ref - (double)mx, p.k);
+      else z *= __builtin_amdgcn_exp2f((ref - mx) * kf);
+      ref = mx;
+      lim = ref + room;
+    }
+#pragma unroll
+    for (int e = 0; e < EV; ++e) {
+      if (MODE == M_DRAW) zd += exp2_64(r.value64(p, e) - (double)ref, p.k);
+      else z += __builtin_amdgcn_exp2f((s[e] - ref) * kf);
+    }
+  }
+  m = wave_max_nan(m);
+  Seg r;
+  r.s = 0.0; r.m = m; r.pad = 0;
+  if (m > -INFINITY && m < INFINITY) {
+    if (MODE == M_DRAW) r.s = wave_sum(zd * exp2_64((double)ref - (double)m, p.k));
+    else r.s = (double)wave_sum(z * __builtin_amdgcn_exp2f((ref - m) * kf));
+  }
+  if (lane == 0) a.seg[row * a.nseg + seg] = r;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// join: one workgroup a row
+// ---------------------------------------------------------------------------------------------------------------
+struct JoinArgs {
+  dvae_rules q;
+  int nseg, seg_len;
+  const Seg* seg;
+  const float* uniforms;         // DRAW
+  const int* next;               // next state of (state, token), or NULL
+  const long long* given;        // GIVEN
+  long long* tokens;             // GREEDY / DRAW
+  float* logprob;
+  float* stat;                   // GIVEN: maximum and 1 / Z, kept for the backward pass
+  int* state_out;
+};
+
+template <typename X, typename F>
+__device__ __forceinline__ X block_reduce(X v, X* sh, F f) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = f(v, __shfl_xor(v, o));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return f(f(sh[0], sh[1]), f(sh[2], sh[3]));
+}
+
+// inclusive scan over the 256 threads; returns the thread's exclusive prefix, `total` the sum of all
+__device__ __forceinline__ double block_prefix(double v, double* sh, double& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  double x = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 63) sh[wave] = x;
+  __syncthreads();
+  double before = 0.0;
+  for (int w = 0; w < wave; ++w) before += sh[w];
+  total = sh[0] + sh[1] + sh[2] + sh[3];
+  return before + (x - v);
+}
+
+template <int T, int MODE>
+__global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
+  typedef Elem<T> E;
+  __shared__ double shd[4];
+  __shared__ float shf[4];
+  __shared__ int shi[4];
+  __shared__ int pick_seg;
+  __shared__ double pick_before;
+  __shared__ uint32_t cnt[SEG_MAX];         // counts of the segment that is searched
+  const dvae_rules& q = a.q;
+  const long long row = blockIdx.x;
+  const int V = q.vocab, tid = threadIdx.x;
+  const RowP p = row_params(q, row);
+  const Seg* seg = a.seg + row * a.nseg;
+  const typename E::type* lrow = static_cast<const typename E::type*>(q.logits) + row * q.ld;
+
+  float m = -INFINITY;
+  for (int i = tid; i < a.nseg; i += 256) m = max_nan(m, seg[i].m);
+  m = block_reduce(m, shf, [](float x, float y) { return max_nan(x, y); });
+  // a temperature that is not positive and finite makes the row NaN, as a NaN logit does
+  const bool ok = m > -INFINITY && m < INFINITY && p.k > 0.0 && p.k < INFINITY;
+  double z = 0.0;
+  // contiguous shares, so that running sums follow the vocabulary's order
+  const int per = (a.nseg + 255) / 256;
+  const int i0 = min(tid * per, a.nseg), i1 = min(i0 + per, a.nseg);
+  if (ok)
+    for (int i = i0; i < i1; ++i)
+      if (seg[i].m > -INFINITY) z += seg[i].s * exp2_64((double)seg[i].m - (double)m, p.k);
+  double Z;
+  const double before = block_prefix(z, shd, Z);
+
+  long long tok = -1;
+  if (MODE == M_SUM) {
+    tok = a.given[row];
+  } else if (ok && MODE == M_GREEDY) {
+    // the largest value's segments (hardly ever more than one), and in them the elements that round to it: among those
+    // the largest dropped part, then the lowest index
+    float lo = -INFINITY;
+    int idx = INT32_MAX;
+    const int n = a.seg_len;
+    for (int i = 0; i < a.nseg; ++i) {
+      if (seg[i].m != m) continue;
+      const int v0 = i * n;
+      for (int e = tid; e < n; e += 256) cnt[e] = 0;
+      __syncthreads();
+      count_history<2>(p, q.history_i64, v0, n, cnt, tid, 256);
+      __syncthreads();
+      for (int e = tid; e < n; e += 256) {
+        const int v = v0 + e;
+        if (v >= V || (p.mask && !((p.mask[v >> 3] >> (v & 7)) & 1))) continue;
+        const float x = E::one(lrow, v), b = p.bias ? p.bias[v] : 0.f;
+        const double y = cnt[e] ? counted64(p, x, cnt[e], b) : (double)x + (double)b;
+        if ((float)y != m) continue;
+        const float l = (float)(y - (double)m);
+        if (l > lo || (l == lo && v < idx)) { lo = l; idx = v; }
+      }
+      __syncthreads();
+    }
+    const float best = block_reduce(lo, shf, [](float x, float y) { return fmaxf(x, y); });
+    tok = block_reduce(lo == best ? idx : INT32_MAX, shi, [](int x, int y) { return min(x, y); });
+  } else if (ok && MODE == M_DRAW) {
+    const float uf = a.uniforms[row];
+    const double t = fmax((double)uf, 0.0) * Z;
+    if (uf == uf) {
+      // the segment where the running sum passes t; beyond the end (u >= 1, or rounding): the last one with a weight
+      int first = INT32_MAX, last = -1;
+      double run = before, first_before = 0.0, last_before = 0.0;
+      for (int i = i0; i < i1; ++i) {
+        if (!(seg[i].m > -INFINITY)) continue;
+        const double w = seg[i].s * exp2_64((double)seg[i].m - (double)m, p.k);
+        if (w > 0.0) { last = i; last_before = run; }
+        if (run + w > t && first == INT32_MAX) { first = i; first_before = run; }
+        run += w;
+      }
+      const int f = block_reduce(first, shi, [](int x, int y) { return min(x, y); });
+      const int l = block_reduce(last, shi, [](int x, int y) { return max(x, y); });
+      const int g = f != INT32_MAX ? f : l;
+      if (threadIdx.x == 0) pick_seg = 0;
+      __syncthreads();
+      if (g >= i0 && g < i1) {
+        pick_seg = g;
+        pick_before = f != INT32_MAX ? first_before : last_before;
+      }
+      const int n = a.seg_len;
+      for (int i = tid; i < n; i += 256) cnt[i] = 0;
+      __syncthreads();
+      const int v0 = pick_seg * n;
+      const double base = pick_before;
+      count_history<2>(p, q.history_i64, v0, n, cnt, tid, 256);
+      __syncthreads();
+      // weights of the segment's tokens, thread by thread in order
+      const int own = n / 256;
+      double mine = 0.0;
+      const auto weight = [&](int d) -> double {
+        const int v = v0 + d;
+        if (v >= V || (p.mask && !((p.mask[v >> 3] >> (v & 7)) & 1))) return 0.0;
+        const float x = E::one(lrow, v), b = p.bias ? p.bias[v] : 0.f;
+        const double y = cnt[d] ? counted64(p, x, cnt[d], b) : (double)x + (double)b;
+        return exp2_64(y - (double)m, p.k);
+      };
+      for (int e = 0; e < own; ++e) mine += weight(tid * own + e);
+      double dummy;
+      double run2 = base + block_prefix(mine, shd, dummy);
+      int hit = INT32_MAX, tail = -1;
+      for (int e = 0; e < own; ++e) {
+        const double w = weight(tid * own + e);
+        run2 += w;
+        if (w > 0.0) tail = v0 + tid * own + e;
+        if (w > 0.0 && run2 > t && hit == INT32_MAX) hit = v0 + tid * own + e;
+      }
+      hit = block_reduce(hit, shi, [](int x, int y) { return min(x, y); });
+      tail = block_reduce(tail, shi, [](int x, int y) { return max(x, y); });
+      tok = g < 0 ? -1 : hit != INT32_MAX ? hit : tail;
+    }
+  }
+
+  // the token's value: its count, then the formula
+  const bool have = tok >= 0 && tok < V;
+  int c = 0;
+  if (have)
+    for (int i = tid; i < p.n_hist; i += 256) c += hist_at(p, q.history_i64, i) == tok;
+  c = block_reduce(c, shi, [](int x, int y) { return x + y; });
+  if (tid) return;
+  float lp = -INFINITY;
+  if (MODE == M_SUM && !have) lp = 0.f;                         // an ignored row
+  else if (m == -INFINITY) lp = -INFINITY;                      // the rules leave nothing (never drawn from)
+  else if (!ok || !have) lp = NAN;                              // NaN or +inf among the allowed values (or a NaN u)
+  else if (!(p.mask && !((p.mask[tok >> 3] >> (tok & 7)) & 1))) {
+    const float x = E::one(lrow, tok), b = p.bias ? p.bias[tok] : 0.f;
+    const double y = c ? counted64(p, x, c, b) : (double)x + (double)b;
+    lp = (float)((y - (double)m) * (p.k * LN2) - log(Z));
+  }
+  a.logprob[row] = lp;
+  if (MODE == M_SUM) {
+    a.stat[2 * row] = m == -INFINITY || ok ? m : NAN;
+    a.stat[2 * row + 1] = ok ? (float)(1.0 / Z) : NAN;
+  } else {
+    a.tokens[row] = tok;
+    if (a.state_out) {
+      const int s = q.state[row];
+      a.state_out[row] = tok >= 0 && s >= 0 && s < q.states ? a.next[(size_t)s * V + tok] : s;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// gradients with a bias shared by the rows: a workgroup owns 256 EV columns and walks a share of the rows, so the
+// bias gradient's sum over rows stays in registers; shares are added in a fixed order by a second launch
+// ---------------------------------------------------------------------------------------------------------------
+struct ColArgs {
+  SegArgs s;
+  float* part;           // [shares][vocab]
+  int rows_per_share;
+};
+
+template <int T, int HIST>
+__global__ __launch_bounds__(256) void rules_bwd_col_kernel(ColArgs ca) {
+  typedef Elem<T> E;
+  constexpr int EV = E::EV, SPAN = 256 * EV;
+  __shared__ uint32_t lds[HIST ? SPAN : 1];
+  const SegArgs& a = ca.s;
+  const dvae_rules& q = a.q;
+  const int V = q.vocab, v0 = blockIdx.x * SPAN, v = v0 + threadIdx.x * EV;
+  const long long r0 = (long long)blockIdx.y * ca.rows_per_share;
+  const long long r1 = min(r0 + ca.rows_per_share, q.rows);
+  float acc[EV];
+#pragma unroll
+  for (int e = 0; e < EV; ++e) acc[e] = 0.f;
+  for (long long row = r0; row < r1; ++row) {
+    const RowP p = row_params(q, row);
+    if (HIST) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < SPAN; i += 256) lds[i] = 0;
+      __syncthreads();
+      count_history<2>(p, q.history_i64, v0, SPAN, lds, threadIdx.x, 256);
+      __syncthreads();
+    }
+    const typename E::type* lrow = static_cast<const typename E::type*>(q.logits) + row * q.ld;
+    typename E::type* orow = static_cast<typename E::type*>(a.out) + row * a.out_ld;
+    const float m = a.stat[2 * row], iz = a.stat[2 * row + 1], kf = (float)p.k;
+    const float coef = (float)((double)a.d_logprob[row] * (p.k * LN2));
+    const long long tok = a.tokens[row];
+    const bool zero = tok < 0 || tok >= V || m == -INFINITY;
+#pragma unroll
+    for (int e = 0; e < EV; ++e) {
+      const int w = v + e;
+      float g = 0.f;
+      if (w < V) {
+        const bool off = zero || (p.mask && !((p.mask[w >> 3] >> (w & 7)) & 1));
+        if (!off) {
+          const float x = E::one(lrow, w), b = p.bias ? p.bias[w] : 0.f;
+          const uint32_t c = HIST ? lds[w - v0] : 0u;
+          const float y = c ? (float)counted64(p, x, c, b) : x + b;
+          g = coef * ((w == tok ? 1.f : 0.f) - __builtin_amdgcn_exp2f((y - m) * kf) * iz);
+          acc[e] += g;
+          if (c) g *= x > 0.f ? (float)p.inv_rho : (float)p.rho;
+        }
+        orow[w] = E::cast(g);
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < EV; ++e)
+    if (v + e < V) ca.part[(size_t)blockIdx.y * V + v + e] = acc[e];
+}
+
+__global__ __launch_bounds__(256) void rules_bias_sum_kernel(const float* __restrict__ part, int shares, int V,
+                                                             float* __restrict__ d_bias) {
+  const int v = blockIdx.x * 256 + threadIdx.x;
+  if (v >= V) return;
+  float s = 0.f;
+  for (int i = 0; i < shares; ++i) s += part[(size_t)i * V + v];
+  d_bias[v] = s;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------------------------
+constexpr long long MAX_BLOCKS = (1ll << 24) - 1;     // blocks x 256 threads stay below 2^32
+
+struct Plan { int seg_len, nseg, wgs_per_row; bool row_wave; long long blocks; };
+
+int elem_bytes(int dtype) { return dtype == DVAE_F32 ? 4 : 2; }
+
+Plan plan_of(const dvae_rules& q) {
+  Plan p;
+  const int step = 64 * (16 / elem_bytes(q.dtype));      // tokens of a wave's step
+  p.seg_len = (int)std::min<long long>(SEG_MAX, ((long long)q.vocab + step - 1) / step * step);
+  p.nseg = (int)(((long long)q.vocab + p.seg_len - 1) / p.seg_len);
+  p.row_wave = p.nseg == 1;
+  p.wgs_per_row = (p.nseg + 3) / 4;
+  p.blocks = p.row_wave ? (q.rows + 3) / 4 : q.rows * p.wgs_per_row;
+  return p;
+}
+
+template <int T, int HIST, int MODE>
+void launch_seg(const SegArgs& a, const Plan& p, hipStream_t st) {
+  if (p.row_wave) hipLaunchKernelGGL((rules_seg_kernel<T, HIST, MODE, true>), dim3((unsigned)p.blocks), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((rules_seg_kernel<T, HIST, MODE, false>), dim3((unsigned)p.blocks), dim3(256), 0, st, a);
+}
+
+template <int T, int MODE>
+void pick_hist(const SegArgs& a, const Plan& p, hipStream_t st) {
+  if (!a.q.history || a.q.history_len == 0) launch_seg<T, 0, MODE>(a, p, st);
+  else if (a.q.history_len < 65536) launch_seg<T, 1, MODE>(a, p, st);
+  else launch_seg<T, 2, MODE>(a, p, st);
+}
+
+template <int MODE>
+int run_seg(SegArgs& a, const Plan& p, hipStream_t st) {
+  a.nseg = p.nseg; a.seg_len = p.seg_len; a.wgs_per_row = p.wgs_per_row;
+  switch (a.q.dtype) {
+    case DVAE_F32: pick_hist<DVAE_F32, MODE>(a, p, st); break;
+    case DVAE_BF16: pick_hist<DVAE_BF16, MODE>(a, p, st); break;
+    default: pick_hist<DVAE_F16, MODE>(a, p, st);
+  }
+  DVAE_LAUNCH_CHECK();
+  return DVAE_OK;
+}
+
+template <int MODE>
+int run_join(const JoinArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)a.q.rows), block(256);
+  switch (a.q.dtype) {
+    case DVAE_F32: hipLaunchKernelGGL((rules_join_kernel<DVAE_F32, MODE>), grid, block, 0, st, a); break;
+    case DVAE_BF16: hipLaunchKernelGGL((rules_join_kernel<DVAE_BF16, MODE>), grid, block, 0, st, a); break;
+    default: hipLaunchKernelGGL((rules_join_kernel<DVAE_F16, MODE>), grid, block, 0, st, a);
+  }
+  DVAE_LAUNCH_CHECK();
+  return DVAE_OK;
+}
+
+int bias_shares(const dvae_rules& q) {
+  const int span = 256 * (16 / elem_bytes(q.dtype));
+  const long long cols = ((long long)q.vocab + span - 1) / span;
+  return (int)std::min<long long>(q.rows, std::max<long long>(1, 2048 / cols));
+}
+
+}  // namespace
+
+int rules_check(const dvae_rules& q, const char* who) {
+  DVAE_REQUIRE(q.rows >= 0 && q.vocab >= 1, "%s: rows >= 0 and vocab >= 1", who);
+  DVAE_REQUIRE(q.dtype == DVAE_F32 || q.dtype == DVAE_BF16 || q.dtype == DVAE_F16, "%s: dtype %d", who, q.dtype);
+  DVAE_REQUIRE(q.logits || q.rows == 0, "%s: null logits", who);
+  DVAE_REQUIRE(q.rows <= 1 || q.ld >= q.vocab, "%s: rows of logits overlap (ld %lld < vocab %d)", who, q.ld, q.vocab);
+  DVAE_REQUIRE(q.vocab <= (1 << 30), "%s: vocab %d above 2^30", who, q.vocab);
+  DVAE_REQUIRE(q.repetition_rows || (q.repetition > 0.0 && std::isfinite(q.repetition)), "%s: repetition must be positive", who);
+  DVAE_REQUIRE(q.frequency_rows || std::isfinite(q.frequency), "%s: frequency must be finite", who);
+  DVAE_REQUIRE(q.presence_rows || q.presence > -INFINITY, "%s: presence must be above -inf", who);
+  DVAE_REQUIRE(q.temperature_rows || (q.temperature > 0.0 && std::isfinite(q.temperature)), "%s: temperature must be positive", who);
+  if (q.history) {
+    DVAE_REQUIRE(q.history_len >= 0 && q.history_ld >= 0, "%s: negative history length", who);
+    DVAE_REQUIRE(q.rows_per_history >= 1, "%s: rows_per_history must be at least 1", who);
+  }
+  if (q.mask) {
+    DVAE_REQUIRE(q.state && q.states >= 1, "%s: a mask needs the rows' states", who);
+    DVAE_REQUIRE(q.mask_words >= (q.vocab + 31) / 32, "%s: mask rows hold %d words, vocab %d needs %d", who, q.mask_words,
+                 q.vocab, (q.vocab + 31) / 32);
+  }
+  const Plan p = plan_of(q);
+  DVAE_REQUIRE(p.blocks <= MAX_BLOCKS && q.rows <= MAX_BLOCKS, "%s: %lld rows of %d tokens are too many for one call", who,
+               q.rows, q.vocab);
+  return DVAE_OK;
+}
+
+extern "C" size_t dvae_rules_ws_bytes(const dvae_rules* q) {
+  if (!q || q->rows <= 0 || q->vocab < 1) return 0;
+  const size_t segs = (size_t)q->rows * plan_of(*q).nseg * sizeof(Seg);
+  const size_t bias = q->bias && q->bias_ld == 0 ? (size_t)bias_shares(*q) * q->vocab * sizeof(float) : 0;
+  return std::max(segs, bias);
+}
+
+extern "C" int dvae_rules_apply(const dvae_rules* q, void* out, long long out_ld, void* stream) {
+  DVAE_REQUIRE(q, "rules_apply: null pointer");
+  DVAE_TRY(rules_check(*q, "rules_apply"));
+  if (q->rows == 0) return DVAE_OK;
+  DVAE_REQUIRE(out, "rules_apply: null pointer");
+  DVAE_REQUIRE(q->rows <= 1 || out_ld >= q->vocab, "rules_apply: rows of out overlap (ld %lld < vocab %d)", out_ld, q->vocab);
+  SegArgs a{};
+  a.q = *q;
+  const Plan p = plan_of(*q);
+  a.out = out; a.out_ld = out_ld;
+  return run_seg<M_APPLY>(a, p, (hipStream_t)stream);
+}
+
+extern "C" int dvae_rules_choose(const dvae_rules* q, const float* uniforms, const int* next, long long* tokens,
+                                 float* logprob, int* state_out, void* ws, void* stream) {
+  DVAE_REQUIRE(q, "rules_choose: null pointer");
+  DVAE_TRY(rules_check(*q, "rules_choose"));
+  if (q->rows == 0) return DVAE_OK;
+  DVAE_REQUIRE(tokens && logprob && ws, "rules_choose: null pointer");
+  DVAE_REQUIRE((next == nullptr) == (state_out == nullptr), "rules_choose: next and state_out go together");
+  DVAE_REQUIRE(!next || q->mask, "rules_choose: next states need a grammar mask");
+  const Plan p = plan_of(*q);
+  SegArgs a{};
+  a.q = *q; a.seg = (Seg*)ws;
+  JoinArgs j{};
+  j.q = *q; j.nseg = p.nseg; j.seg_len = p.seg_len; j.seg = (const Seg*)ws; j.uniforms = uniforms; j.next = next;
+  j.tokens = tokens; j.logprob = logprob; j.state_out = state_out;
+  if (uniforms) {
+    DVAE_TRY(run_seg<M_DRAW>(a, p, (hipStream_t)stream));
+    return run_join<M_DRAW>(j, (hipStream_t)stream);
+  }
+  DVAE_TRY(run_seg<M_SUM>(a, p, (hipStream_t)stream));
+  return run_join<M_GREEDY>(j, (hipStream_t)stream);
+}
+
+extern "C" int dvae_rules_logprob(const dvae_rules* q, const long long* tokens, float* logprob, float* stat, void* ws,
+                                  void* stream) {
+  DVAE_REQUIRE(q, "rules_logprob: null pointer");
+  DVAE_TRY(rules_check(*q, "rules_logprob"));
+  if (q->rows == 0) return DVAE_OK;
+  DVAE_REQUIRE(tokens && logprob && stat && ws, "rules_logprob: null pointer");
+  const Plan p = plan_of(*q);
+  SegArgs a{};
+  a.q = *q; a.seg = (Seg*)ws;
+  DVAE_TRY(run_seg<M_SUM>(a, p, (hipStream_t)stream));
+  JoinArgs j{};
+  j.q = *q; j.nseg = p.nseg; j.seg_len = p.seg_len; j.seg = (const Seg*)ws; j.given = tokens; j.logprob = logprob; j.stat = stat;
+  return run_join<M_SUM>(j, (hipStream_t)stream);
+}
+
+extern "C" int dvae_rules_logprob_bwd(const dvae_rules* q, const long long* tokens, const float* stat,
+                                      const float* d_logprob, void* d_logits, long long d_ld, float* d_bias, void* ws,
+                                      void* stream) {
+  DVAE_REQUIRE(q, "rules_logprob_bwd: null pointer");
+  DVAE_TRY(rules_check(*q, "rules_logprob_bwd"));
+  hipStream_t st = (hipStream_t)stream;
+  DVAE_REQUIRE(!d_bias || q->bias, "rules_logprob_bwd: d_bias without a bias");
+  const bool shared = d_bias && q->bias_ld == 0;
+  if (q->rows == 0) {
+    if (shared) hipLaunchKernelGGL(rules_bias_sum_kernel, dim3(cdiv(q->vocab, 256)), dim3(256), 0, st, nullptr, 0, q->vocab, d_bias);
+    DVAE_LAUNCH_CHECK();
+    return DVAE_OK;
+  }
+  DVAE_REQUIRE(tokens && stat && d_logprob && d_logits && (ws || !shared), "rules_logprob_bwd: null pointer");
+  DVAE_REQUIRE(q->rows <= 1 || d_ld >= q->vocab, "rules_logprob_bwd: rows of d_logits overlap (ld %lld < vocab %d)", d_ld,
+               q->vocab);
+  const Plan p = plan_of(*q);
+  SegArgs a{};
+  a.q = *q; a.out = d_logits; a.out_ld = d_ld; a.tokens = tokens;
+  a.stat = stat; a.d_logprob = d_logprob;
+  a.d_bias_rows = shared ? nullptr : d_bias;
+  if (!shared) return run_seg<M_BWD>(a, p, st);
+  ColArgs c{};
+  c.s = a;
+  c.part = (float*)ws;
+  const int shares = bias_shares(*q);
+  c.rows_per_share = (int)((q->rows + shares - 1) / shares);
+  const dim3 grid((unsigned)cdiv(q->vocab, 256 * (16 / elem_bytes(q->dtype))), (unsigned)shares);
+  const bool hist = q->history && q->history_len > 0;
+#define COL(T)                                                                                              \
+  do {                                                                                                      \
+    if (hist) hipLaunchKernelGGL((rules_bwd_col_kernel<T, 1>), grid, dim3(256), 0, st, c);                  \
+    else hipLaunchKernelGGL((rules_bwd_col_kernel<T, 0>), grid, dim3(256), 0, st, c);                       \
+  } while (0)
+  switch (q->dtype) {
+    case DVAE_F32: COL(DVAE_F32); break;
+    case DVAE_BF16: COL(DVAE_BF16); break;
+    default: COL(DVAE_F16);
+  }
+#undef COL
+  DVAE_LAUNCH_CHECK();
+  hipLaunchKernelGGL(rules_bias_sum_kernel, dim3(cdiv(q->vocab, 256)), dim3(256), 0, st, c.part, shares, q->vocab, d_bias);
+  DVAE_LAUNCH_CHECK();
+  return DVAE_OK;
+}

@@ -98,11 +98,18 @@ def allreduce_losses(dist, out4, group=None):
     return out4
 
 
-def predict_sharded(decoder, z, dist, is_stochastic=False, uniforms=None, group=None):
+def predict_sharded(decoder, z, dist, is_stochastic=False, uniforms=None, group=None, rules=None, temperature=1.0):
     """`Decoder.predict` over the GPUs of one node: every rank decodes its contiguous shard of the
     latent rows `z` (and of the injected uniforms, if any) and receives all (edges, onehots) in row
-    order.  Stochastic decode without injected uniforms draws them per rank on the device."""
+    order.  Stochastic decode without injected uniforms draws them per rank on the device.  `rules`
+    (of one setting for all latents) and `temperature` are `Decoder.predict`'s."""
+    kw = {}
+    if rules is not None:
+        if (rules.per_row() or torch.is_tensor(temperature)) and dist is not None and dist.is_initialized() \
+                and dist.get_world_size(group) > 1:
+            raise ValueError("predict_sharded: settings per latent do not go with sharded latents")
+        kw = dict(rules=rules, temperature=temperature)
     if uniforms is None:
-        return sharded_map(lambda zz: decoder.predict(zz, is_stochastic=is_stochastic), dist, z, group=group)
-    return sharded_map(lambda zz, ut, ue: decoder.predict(zz, is_stochastic=is_stochastic, uniforms=(ut, ue)),
+        return sharded_map(lambda zz: decoder.predict(zz, is_stochastic=is_stochastic, **kw), dist, z, group=group)
+    return sharded_map(lambda zz, ut, ue: decoder.predict(zz, is_stochastic=is_stochastic, uniforms=(ut, ue), **kw),
                        dist, z, uniforms[0], uniforms[1], group=group)

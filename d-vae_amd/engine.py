@@ -21,6 +21,21 @@ def _stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def _on_device(device, fn, *args):
+    """check(fn(*args, stream)) on `device`, whichever device is current, on the current stream there."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        check(fn(*args, _stream()))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, _stream()))
+
+
+def _written(t):
+    """Tells autograd that a kernel wrote `t` in place."""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
 def _side(side):
     """torch.cuda.Stream (or None) -> hipStream_t for the library's side stream."""
     return None if side is None else ctypes.c_void_p(side.cuda_stream)
@@ -403,6 +418,20 @@ def predict_call(dims, z, P, u_type=None, u_edge=None, want_margin=False):
     check(lib.dvae_decoder_predict(ctypes.byref(dims), _ptr(z), _ptr(P), _ptr(ws), _ptr(u_type), _ptr(u_edge),
                                    _ptr(edges), _ptr(onehot), _ptr(margin), _stream()))
     return edges, onehot, margin
+
+
+def predict_rules_call(dims, z, P, rules, next_state, start, u_type=None, u_edge=None):
+    """predict_call with the type decisions under rules: a filled _lib.DvaeRules, the grammar's next states (or None)."""
+    lib = load()
+    dev = z.device
+    M, N, C = dims.B, dims.N, dims.C
+    ws = _workspace(lib.dvae_predict_rules_ws_bytes(ctypes.byref(dims)), dev)
+    edges = _out(M, N, N, device=dev)
+    onehot = _out(M, N, C, device=dev)
+    check(lib.dvae_decoder_predict_rules(ctypes.byref(dims), _ptr(z), _ptr(P), _ptr(ws), _ptr(u_type), _ptr(u_edge),
+                                         ctypes.byref(rules), _ptr(next_state), start, _ptr(edges), _ptr(onehot),
+                                         _stream()))
+    return edges, onehot
 
 
 # ---------------------------------------------------------------------------

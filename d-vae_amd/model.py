@@ -14,6 +14,7 @@ import torch.nn as nn
 
 from . import _lib
 from . import engine as E
+from . import rules as rules_mod
 from .metrics import reconstruction_accuracy
 
 
@@ -160,12 +161,27 @@ class Decoder(nn.Module):
             call = E.DecoderCall(dims, sched, E._f32c(z), E._f32c(x), P, want_states=True)
         return call.states
 
-    def predict(self, z, is_stochastic=False, uniforms=None, return_margin=False):
+    def predict(self, z, is_stochastic=False, uniforms=None, return_margin=False, rules=None, temperature=1.0):
         """Autoregressive decode (:263-362).  Greedy by default; stochastic mode
         draws its uniforms on the device unless `uniforms` = (u_type [M,N],
-        u_edge [M,N,N]) is injected (parity tests)."""
-        E._require_cuda(z, "z")
+        u_edge [M,N,N]) is injected (parity tests).  `rules` (an addition): a
+        rules.TokenRules the node types are decided under, a latent's history
+        being the types of its earlier nodes -- e.g. rules.dag_rules(...); a
+        grammar then has next states.  A node the rules leave nothing for has
+        an all-zero one-hot row.  `temperature` goes with rules."""
         M = z.shape[0]
+        if rules is not None:
+            if return_margin:
+                raise ValueError("predict: no margin under rules")
+            if rules.grammar is not None and rules.grammar.next_state is None:
+                raise ValueError("predict: the grammar needs next states")
+            start = 0 if rules.grammar is None else rules.grammar.start
+            state = None if rules.grammar is None else torch.full((M,), start, dtype=torch.int32, device=z.device)
+            # the checks of the decisions that the decode will take
+            call = rules_mod._Call(torch.empty(M, self.num_classes, device=z.device), rules, None, None, state, temperature)
+        elif temperature != 1.0:
+            raise ValueError("predict: a temperature goes with rules")
+        E._require_cuda(z, "z")
         dims = E._dims_for(self._dims, M, self.seq_len)
         u_type = u_edge = None
         if is_stochastic or uniforms is not None:
@@ -176,6 +192,9 @@ class Decoder(nn.Module):
                 u_type, u_edge = (E._f32c(u) for u in uniforms)
         with torch.no_grad():
             P = self._pack.pack(dims, self.hip_params())
+            if rules is not None:
+                nxt = None if rules.grammar is None else rules.grammar.next_state
+                return E.predict_rules_call(dims, E._f32c(z), P, call.fill(), nxt, start, u_type, u_edge)
             edges, onehot, margin = E.predict_call(dims, E._f32c(z), P, u_type, u_edge, return_margin)
         if return_margin:
             return edges, onehot, margin
@@ -288,10 +307,12 @@ class Dvae(nn.Module):
             z = self.reparamterize(mu, logvar, eps)
         return self.decoder.predict(z, return_margin=return_margin)
 
-    def model_eval(self, X, sample_num, decode_num, is_stochastic=True, eps=None, uniforms=None, return_decoded=False):
+    def model_eval(self, X, sample_num, decode_num, is_stochastic=True, eps=None, uniforms=None, return_decoded=False,
+                   rules=None, temperature=1.0):
         """:498-524.  ``eps`` [B,sample_num,Z] replaces the reparameterisation draw, ``uniforms`` =
         (u_type [B*S*D,N], u_edge [B*S*D,N,N]) the decoder's draws (stochastic mode); both optional.
-        ``return_decoded`` adds the decoded tensors [B, D*S, N, .] to the result."""
+        ``return_decoded`` adds the decoded tensors [B, D*S, N, .] to the result; ``rules`` / ``temperature`` as in
+        ``Decoder.predict``."""
         with torch.no_grad():
             _, mu, logvar = self.encoder.predict(X)
             stack_mu = torch.stack([mu] * sample_num, dim=1)
@@ -301,7 +322,8 @@ class Dvae(nn.Module):
             assert samples == sample_num
             stack_z = stack_z.repeat(1, decode_num, 1)
             sampled_z = stack_z.view(batch_size * sample_num * decode_num, hidden_size)
-            gen_edges, gen_nodes = self.decoder.predict(sampled_z, is_stochastic, uniforms=uniforms)
+            gen_edges, gen_nodes = self.decoder.predict(sampled_z, is_stochastic, uniforms=uniforms, rules=rules,
+                                                       temperature=temperature)
             gen_edges = gen_edges.view(batch_size, decode_num * sample_num, *gen_edges.shape[1:])
             gen_nodes = gen_nodes.view(batch_size, decode_num * sample_num, *gen_nodes.shape[1:])
             recon_acc = reconstruction_accuracy(X['node_encoding'], X['graph'], gen_nodes, gen_edges)
@@ -311,17 +333,19 @@ class Dvae(nn.Module):
             return out
 
     def generation_eval(self, num_samples=None, z=None, train_batch=None, is_stochastic=False, task_type='enas',
-                        dist=None):
+                        dist=None, rules=None, temperature=1.0):
         """Addition (not in the reference; BASELINE config 5's validity/novelty path): decode
         ``num_samples`` draws from the prior N(0,I) -- or the given latents ``z`` -- and report
         validity, uniqueness and (given the training graphs) novelty of the decoded DAGs
-        (definitions in metrics.py).  ``dist``: shard the decode over the ranks (dp.predict_sharded)."""
+        (definitions in metrics.py).  ``dist``: shard the decode over the ranks (dp.predict_sharded).
+        ``rules`` / ``temperature``: as in ``Decoder.predict``."""
         from . import dp, metrics
         dev = next(self.parameters()).device
         if z is None:
             z = torch.randn(int(num_samples), self.decoder.lin1.in_features, device=dev)
         with torch.no_grad():
-            edges, onehots = dp.predict_sharded(self.decoder, z, dist, is_stochastic=is_stochastic)
+            edges, onehots = dp.predict_sharded(self.decoder, z, dist, is_stochastic=is_stochastic, rules=rules,
+                                                temperature=temperature)
         te = tx = None
         if train_batch is not None:
             te, tx = train_batch['graph'], train_batch['node_encoding']

@@ -8,14 +8,119 @@ checkpoints move between the two.  The model's parameters become views of one fl
 `nn.Parameter` objects, same values), laid out like the flat gradient buffers `Dvae.loss_and_grad` fills.
 """
 import ctypes
+import math
 
 import torch
 
+from . import _lib
 from . import engine as E
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # DVAE_F32 / DVAE_BF16 / DVAE_F16
+
+
+def _flat_order(t):
+    """Whether t's elements fill one stretch of memory, each once, in whatever order of its axes."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for n, s in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n > 1), key=lambda a: a[1]):
+        if s != want:
+            return False
+        want *= n
+    return True
+
+
+def _gradients(grads, what):
+    """The tensors of a list of gradients (None left out), checked."""
+    ts = [grads] if torch.is_tensor(grads) else [t for t in grads if t is not None]
+    for i, t in enumerate(ts):
+        if not torch.is_tensor(t) or t.layout != torch.strided or t.dtype not in _TYPES:
+            raise ValueError("%s: gradient %d must be a dense fp32, bf16 or fp16 tensor" % (what, i))
+        if t.device != ts[0].device:
+            raise ValueError("%s: gradients on %s and %s" % (what, ts[0].device, t.device))
+        if not _flat_order(t):
+            raise ValueError("%s: the elements of gradient %d %s, strides %s, are not one stretch of memory" %
+                             (what, i, tuple(t.shape), tuple(t.stride())))
+    return ts
+
+
+def _describe(ts, outs=None):
+    table = (_lib.DvaeTensor * max(len(ts), 1))()
+    for d, t, o in zip(table, ts, ts if outs is None else outs):
+        d.in_, d.out, d.n = t.data_ptr(), o.data_ptr(), t.numel()
+        d.in_type, d.out_type = _TYPES[t.dtype], _TYPES[o.dtype]
+    return table
+
+
+def _limit(max_norm, what):
+    m = float(max_norm)
+    if not m >= 0.0:
+        raise ValueError("%s: max_norm must not be negative, got %r" % (what, m))
+    return m
+
+
+def grad_norm(grads, max_norm=math.inf):
+    """-> (norm, coef): the norm of all gradients taken as one vector, and min(1, max_norm / (norm + 1e-6)), both scalars
+    on the device (nothing waits for them).  ``grads``: tensors (fp32 / bf16 / fp16, each one stretch of memory; None is
+    left out).  Sums are 64-bit in a fixed order: the same bits every time."""
+    m = _limit(max_norm, "grad_norm")
+    ts = _gradients(grads, "grad_norm")
+    if not ts:
+        return torch.zeros(()), torch.ones(())
+    E._require_cuda(ts[0], "gradient")
+    dev = ts[0].device
+    out = torch.empty(2, device=dev)
+    lib = E.load()
+    ws = E._workspace(lib.dvae_clip_ws_bytes(len(ts)), dev)
+    E._on_device(dev, lib.dvae_grad_norm, _describe(ts), len(ts), m, E._ptr(out), E._ptr(ws))
+    return out[0], out[1]
+
+
+def clip_grads(grads, max_norm, out=None):
+    """Scales the gradients so that their norm (see ``grad_norm``) is at most ``max_norm``, in place or, with ``out`` (a
+    tensor of the same shape and memory order for each; any of the three types), into other tensors -- flat buffers, or
+    single-precision copies of half-precision gradients.  Returns the norm before clipping, a scalar on the device.
+    The reference's Lightning Trainer has this as ``gradient_clip_val`` (train.py:41-47).  A NaN norm makes the gradients
+    NaN; an infinite one makes them 0 (NaN where they were infinite)."""
+    m = _limit(max_norm, "clip_grads")
+    ts = _gradients(grads, "clip_grads")
+    outs = ts
+    if out is not None:
+        outs = [out] if torch.is_tensor(out) else [t for t in out if t is not None]
+        if len(outs) != len(ts):
+            raise ValueError("clip_grads: %d outputs for %d gradients" % (len(outs), len(ts)))
+        for i, (t, o) in enumerate(zip(ts, outs)):
+            if not torch.is_tensor(o) or o.layout != torch.strided or o.dtype not in _TYPES or o.shape != t.shape or \
+                    o.device != t.device:
+                raise ValueError("clip_grads: output %d must be a dense fp32, bf16 or fp16 tensor %s on %s" %
+                                 (i, tuple(t.shape), t.device))
+            if any(n > 1 and a != b for n, a, b in zip(t.shape, t.stride(), o.stride())):
+                raise ValueError("clip_grads: output %d is laid out unlike its gradient" % i)
+    if torch.is_grad_enabled():
+        for o in outs:
+            if o.requires_grad:
+                raise ValueError("clip_grads: an output that requires a gradient is not written in place")
+    if not ts:
+        return torch.zeros(())
+    E._require_cuda(ts[0], "gradient")
+    dev = ts[0].device
+    norm = torch.empty(2, device=dev)
+    lib = E.load()
+    ws = E._workspace(lib.dvae_clip_ws_bytes(len(ts)), dev)
+    E._on_device(dev, lib.dvae_clip_grads, _describe(ts, outs), len(ts), m, E._ptr(norm), E._ptr(ws))
+    for o in outs:
+        E._written(o)
+    return norm[0]
 
 
 class FlatAdam(torch.optim.Optimizer):
-    def __init__(self, model, lr=1e-4, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0):
+    """``max_norm`` (also an attribute, changeable between steps; None = no clipping): a step's update is that of gradients
+    clipped to this norm.  ``p.grad`` keeps the gradients as they came -- the update kernel scales them as it reads them --
+    and ``grad_norm`` the last clipped step's norm (a scalar on the device)."""
+
+    def __init__(self, model, lr=1e-4, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, max_norm=None):
+        self.max_norm = None if max_norm is None else _limit(max_norm, "FlatAdam")
+        self.grad_norm = None
         enc_p, dec_p = model.encoder.hip_params(), model.decoder.hip_params()
         every = enc_p + dec_p
         if len({id(p) for p in every}) != len(every):
@@ -57,9 +162,16 @@ class FlatAdam(torch.optim.Optimizer):
                     gv.zero_()
                 elif p.grad.data_ptr() != gv.data_ptr():
                     gv.copy_(p.grad)
-            E.check(lib.dvae_adam_step(E._ptr(flat), E._ptr(fg), E._ptr(m), E._ptr(v), flat.numel(), float(g['lr']),
-                                       float(g['betas'][0]), float(g['betas'][1]), float(g['eps']),
-                                       float(g['weight_decay']), self._t, stream))
+        coef = None
+        if self.max_norm is not None:
+            self.grad_norm, coef = grad_norm((fe, fd), self.max_norm)
+        for (plist, flat, m, v), fg in zip(self._mods, (fe, fd)):
+            rest = (E._ptr(m), E._ptr(v), flat.numel(), float(g['lr']), float(g['betas'][0]), float(g['betas'][1]),
+                    float(g['eps']), float(g['weight_decay']), self._t, stream)
+            if coef is None:
+                E.check(lib.dvae_adam_step(E._ptr(flat), E._ptr(fg), *rest))
+            else:
+                E.check(lib.dvae_adam_step_scaled(E._ptr(flat), E._ptr(fg), E._ptr(coef), *rest))
         return loss
 
     def state_dict(self):

@@ -1,0 +1,377 @@
+"""Token decisions under rules: penalties for tokens a row's history holds, a bias, a grammar's mask (csrc/rules.hip).
+
+The reference decides node types by a plain argmax or draw (Decoder.predict, dvae_model.py:282-291;
+Svae._predict_from_logits, svae_model.py:112-131).  Here the same decision can be constrained, its log-probability read
+and differentiated, for any vocabulary and for fp32, bf16 and fp16 logits.  With c(v) how often the row's history holds v:
+
+    x1 = x / repetition if x > 0 else x * repetition, where c > 0
+    x2 = x1 - frequency * c - presence * [c > 0]
+    x3 = x2 + bias[v]
+    x4 = x3 where the row's grammar state allows v, -inf elsewhere;   p = softmax(x4 / temperature)
+
+``apply_rules`` returns x4, ``choose`` a token per row (greedy or drawn), ``token_logprob`` log p of given tokens with the
+gradients of the logits and the bias.  ``Decoder.predict(rules=)``, ``Svae._predict_from_logits(rules=)`` and what calls
+them (``model_eval``, ``generation_eval``) decide node types this way; ``dag_rules`` makes the rules of valid DAGs.
+
+Shapes.  Logits are ``[..., V]``; the leading axes are the rows.  ``history`` is ``[..., L]`` (int32 / int64) over the first
+of those axes (``[B, L]`` beside logits ``[B, T, V]``: the T rows of a sequence share its history; ``[L]``: all rows do);
+``lengths`` (one per row) says how many of its tokens count, entries outside ``[0, V)`` never do.  Settings are a float for
+all rows or an fp32 tensor with one per row.  Rows may lie anywhere in memory as long as a row's logits are adjacent (other
+layouts are copied).  Everything is queued on the current stream of the logits' device.
+
+A row whose rules leave nothing: token -1, log-probability -inf, no gradient.  A row that allows a NaN or a +inf, or whose
+own temperature is not positive and finite: token -1, log-probability NaN.
+"""
+import collections
+import ctypes
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from . import engine as E
+from ._lib import check, load
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # DVAE_F32 / DVAE_BF16 / DVAE_F16
+_INDEX = (torch.int32, torch.int64)
+
+Choice = collections.namedtuple("Choice", "tokens logprob state")
+
+
+class Grammar:
+    """A grammar as a table: ``allowed`` bool [S, V] -- state s allows token v -- and ``next_state`` int [S, V], the state
+    after token v (optional; a value outside [0, S) is a state that allows everything).  ``start``: the state before the
+    first token.  ``masks`` holds ``allowed`` as packed bits: bit v % 32 of word v // 32."""
+
+    def __init__(self, allowed, next_state=None, start=0):
+        if not torch.is_tensor(allowed) or allowed.dtype != torch.bool or allowed.dim() != 2 or 0 in allowed.shape:
+            raise ValueError("Grammar: allowed must be a bool tensor [states, vocab]")
+        self.states, self.vocab = (int(n) for n in allowed.shape)
+        if not 0 <= int(start) < self.states:
+            raise ValueError("Grammar: start state %d of %d" % (int(start), self.states))
+        self.start = int(start)
+        words = (self.vocab + 31) // 32
+        bits = torch.zeros(self.states, words * 32, dtype=torch.int64, device=allowed.device)
+        bits[:, :self.vocab] = allowed
+        weight = torch.ones((), dtype=torch.int64, device=allowed.device) << torch.arange(32, device=allowed.device)
+        packed = (bits.view(self.states, words, 32) * weight).sum(2)
+        # two's complement: the 32 bits of an unsigned word in an int32
+        self.masks = torch.where(packed >= 1 << 31, packed - (1 << 32), packed).to(torch.int32).contiguous()
+        self.next_state = None
+        if next_state is not None:
+            if not torch.is_tensor(next_state) or next_state.dtype not in _INDEX or next_state.shape != allowed.shape:
+                raise ValueError("Grammar: next_state must be an int32 / int64 tensor [states, vocab]")
+            if next_state.device != allowed.device:
+                raise ValueError("Grammar: next_state is on %s, allowed on %s" % (next_state.device, allowed.device))
+            self.next_state = next_state.clamp(-1, self.states).to(torch.int32).contiguous()
+
+    def to(self, device):
+        g = object.__new__(Grammar)
+        g.__dict__.update(self.__dict__)
+        g.masks = self.masks.to(device)
+        g.next_state = None if self.next_state is None else self.next_state.to(device)
+        return g
+
+
+class TokenRules:
+    """What a decision follows: ``repetition`` (> 0, 1 = none), ``frequency``, ``presence`` (inf: no token twice) -- floats,
+    or fp32 tensors with one value per row --, ``bias`` fp32 [V] or one row per row [..., V], and a ``Grammar``."""
+
+    def __init__(self, repetition=1.0, frequency=0.0, presence=0.0, bias=None, grammar=None):
+        for name, v in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
+            if torch.is_tensor(v):
+                _per_row_check(v, name)
+                continue
+            v = float(v)
+            if name == "repetition" and not (v > 0.0 and math.isfinite(v)):
+                raise ValueError("TokenRules: repetition must be positive and finite, got %r" % v)
+            if name == "frequency" and not math.isfinite(v):
+                raise ValueError("TokenRules: frequency must be finite, got %r" % v)
+            if name == "presence" and not v > -math.inf:
+                raise ValueError("TokenRules: presence must be above -inf, got %r" % v)
+        if bias is not None and (not torch.is_tensor(bias) or bias.dtype != torch.float32 or bias.dim() < 1):
+            raise ValueError("TokenRules: bias must be an fp32 tensor [V] or [..., V]")
+        if grammar is not None and not isinstance(grammar, Grammar):
+            raise ValueError("TokenRules: grammar must be a Grammar")
+        self.repetition, self.frequency, self.presence = repetition, frequency, presence
+        self.bias, self.grammar = bias, grammar
+
+    def per_row(self):
+        """Whether any setting is one per row (such rules fit one set of rows only)."""
+        return any(torch.is_tensor(v) for v in (self.repetition, self.frequency, self.presence)) or (
+            self.bias is not None and self.bias.dim() > 1)
+
+    def to(self, device):
+        def move(v):
+            return v.to(device) if torch.is_tensor(v) else v
+        r = TokenRules(move(self.repetition), move(self.frequency), move(self.presence), move(self.bias))
+        r.grammar = None if self.grammar is None else self.grammar.to(device)
+        return r
+
+
+def dag_rules(num_classes, max_seq, task_type='enas', start=0, device=None):
+    """Rules under which a type string can be one of ``metrics.dag_validity``'s valid graphs (dataloader.py:57-88: node 0
+    has the start type num_classes - 2, node max_seq - 1 the end type num_classes - 1, no other node either).  'bn': the
+    variable nodes carry distinct types as well.  ``start``: the node of the first decision (1 for S-VAE strings, which
+    leave the start node out)."""
+    if task_type not in ('enas', 'bn'):
+        raise NotImplementedError
+    C, N = int(num_classes), int(max_seq)
+    if C < 3 or N < 2:
+        raise ValueError("dag_rules: at least 3 types and 2 nodes")
+    if task_type == 'bn' and N > C:
+        raise ValueError("dag_rules: %d variable nodes have no %d distinct types" % (N - 2, C - 2))
+    allowed = torch.zeros(N, C, dtype=torch.bool)
+    allowed[:, :C - 2] = True
+    allowed[0] = allowed[N - 1] = False
+    allowed[0, C - 2] = allowed[N - 1, C - 1] = True
+    following = torch.arange(1, N + 1, dtype=torch.int32).clamp(max=N - 1).view(N, 1).repeat(1, C)
+    rules = TokenRules(presence=math.inf if task_type == 'bn' else 0.0, grammar=Grammar(allowed, following, start))
+    return rules if device is None else rules.to(device)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# arguments
+# ---------------------------------------------------------------------------------------------------------------
+def _per_row_check(t, name):
+    if t.dtype != torch.float32:
+        raise ValueError("%s: one value per row is an fp32 tensor, got %s" % (name, t.dtype))
+    if t.requires_grad:
+        raise ValueError("%s has no gradient: detach it" % name)
+
+
+def _rows2d(t):
+    """[..., n] -> [rows, n] with adjacent rows' elements; a view where the layout allows."""
+    t = t.reshape(-1, t.shape[-1]) if t.dim() != 2 else t
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t
+
+
+class _Call:
+    """The C descriptor of one call and the tensors behind its pointers."""
+
+    def __init__(self, logits, rules, history, lengths, state, temperature):
+        if not torch.is_tensor(logits) or logits.dtype not in _DTYPES:
+            raise ValueError("logits must be an fp32, bf16 or fp16 tensor [..., V]")
+        if logits.dim() < 1 or logits.shape[-1] < 1:
+            raise ValueError("logits must have a vocabulary axis, got %s" % (tuple(logits.shape),))
+        rules = TokenRules() if rules is None else rules
+        if not isinstance(rules, TokenRules):
+            raise ValueError("rules must be a TokenRules")
+        self.lead, self.V = tuple(logits.shape[:-1]), int(logits.shape[-1])
+        self.rows = math.prod(self.lead)
+        self.device = logits.device
+        self.rules = rules
+        self.logits = _rows2d(logits)
+        self.history = None
+        if history is not None:
+            if not torch.is_tensor(history) or history.dtype not in _INDEX or history.dim() < 1:
+                raise ValueError("history must be an int32 / int64 tensor [..., L]")
+            if tuple(history.shape[:-1]) != self.lead[:history.dim() - 1]:
+                raise ValueError("history %s does not go with the rows %s" % (tuple(history.shape), self.lead))
+            if history.shape[-1] > 0 and self.rows > 0:
+                h = history.reshape(-1, history.shape[-1])
+                if h.shape[1] > 1 and h.stride(1) != 1:
+                    h = h.contiguous()
+                self.history = self._here(h, "history")
+        elif lengths is not None:
+            raise ValueError("lengths without a history")
+        self.lengths = None
+        if lengths is not None:
+            self._per_row(lengths, "lengths", _INDEX)
+            if lengths.dtype != torch.int32:
+                lengths = lengths.clamp(0, history.shape[-1])
+            self.lengths = lengths.to(torch.int32).contiguous()
+        self.grammar, self.state = rules.grammar, None
+        if self.grammar is not None:
+            if self.grammar.vocab != self.V:
+                raise ValueError("the grammar has %d tokens, the logits %d" % (self.grammar.vocab, self.V))
+            self._here(self.grammar.masks, "grammar")
+            if state is None:
+                raise ValueError("a grammar needs the rows' state")
+            self._per_row(state, "state", _INDEX)
+            if state.dtype != torch.int32:
+                state = state.clamp(-1, self.grammar.states)
+            self.state = state.to(torch.int32).contiguous()
+        elif state is not None:
+            raise ValueError("state without a grammar")
+        self.bias = None
+        if rules.bias is not None:
+            b = self._here(rules.bias, "bias")
+            if b.shape[-1] != self.V or (b.dim() > 1 and tuple(b.shape[:-1]) != self.lead):
+                raise ValueError("bias %s does not go with logits %s" % (tuple(b.shape), tuple(logits.shape)))
+            self.bias = (b if b.stride(0) == 1 or self.V == 1 else b.contiguous()) if b.dim() == 1 else _rows2d(b)
+        self.settings = []
+        for name, v in (("repetition", rules.repetition), ("frequency", rules.frequency), ("presence", rules.presence),
+                        ("temperature", temperature)):
+            if torch.is_tensor(v):
+                _per_row_check(v, name)
+                self._per_row(v, name, (torch.float32,))
+                v = v.contiguous()
+            else:
+                v = float(v)
+                if name == "temperature" and not (v > 0.0 and math.isfinite(v)):
+                    raise ValueError("temperature must be positive and finite, got %r" % v)
+            self.settings.append((name, v))
+        E._require_cuda(logits, "logits")
+
+    def _here(self, t, name):
+        if t.device != self.device:
+            raise _lib.DvaeError("%s is on %s, the logits on %s" % (name, t.device, self.device))
+        return t
+
+    def _per_row(self, t, name, dtypes):
+        if not torch.is_tensor(t) or t.dtype not in dtypes or tuple(t.shape) != self.lead:
+            raise ValueError("%s must hold one value per row: a tensor %s of %s" %
+                             (name, self.lead, " / ".join(str(d) for d in dtypes)))
+        return self._here(t, name)
+
+    def fill(self):
+        q = _lib.DvaeRules()
+        x = self.logits
+        q.logits, q.rows, q.vocab, q.dtype = x.data_ptr(), self.rows, self.V, _DTYPES[x.dtype]
+        q.ld = x.stride(0) if self.rows > 1 else self.V
+        q.rows_per_history = 1
+        if self.history is not None:
+            h = self.history
+            q.history, q.history_len = h.data_ptr(), h.shape[1]
+            q.history_ld = h.stride(0) if h.shape[0] > 1 else 0
+            q.history_i64 = int(h.dtype == torch.int64)
+            q.rows_per_history = self.rows // h.shape[0]
+        if self.lengths is not None:
+            q.lengths = self.lengths.data_ptr()
+        for name, v in self.settings:
+            if torch.is_tensor(v):
+                setattr(q, name + "_rows", v.data_ptr())
+            else:
+                setattr(q, name, v)
+        if self.bias is not None:
+            q.bias = self.bias.data_ptr()
+            q.bias_ld = 0 if self.bias.dim() == 1 else (self.bias.stride(0) if self.rows > 1 else self.V)
+        if self.grammar is not None:
+            g = self.grammar.masks
+            q.mask, q.mask_words, q.states, q.state = g.data_ptr(), g.shape[1], g.shape[0], self.state.data_ptr()
+        return q
+
+    def workspace(self, q):
+        return E._workspace(load().dvae_rules_ws_bytes(ctypes.byref(q)), self.device)
+
+    def launch(self, fn, *args):
+        E._on_device(self.device, fn, *args)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# operators
+# ---------------------------------------------------------------------------------------------------------------
+def apply_rules(logits, rules, history=None, lengths=None, state=None, out=None):
+    """-> x4 in the logits' type (one rounding).  ``out``: a tensor like the logits to write, which may be the logits
+    themselves; its rows must have adjacent elements.  No gradient: see ``token_logprob``."""
+    if torch.is_grad_enabled() and torch.is_tensor(logits) and logits.requires_grad:
+        raise ValueError("apply_rules has no gradient: detach the logits, or use token_logprob")
+    c = _Call(logits, rules, history, lengths, state, 1.0)
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    else:
+        if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
+            raise ValueError("out must be like the logits: %s %s on %s" % (tuple(logits.shape), logits.dtype, logits.device))
+        if torch.is_grad_enabled() and out.requires_grad:
+            raise ValueError("out requires a gradient")
+    o2 = out if out.dim() == 2 else out.view(-1, c.V)
+    if c.rows and ((c.V > 1 and o2.stride(1) != 1) or (c.rows > 1 and o2.stride(0) < c.V)):
+        raise ValueError("out: a row's elements must be adjacent")
+    ld = o2.stride(0) if c.rows > 1 else c.V
+    if c.rows and out.data_ptr() != c.logits.data_ptr():
+        _apart(o2, c.logits, "out overlaps the logits")
+    elif c.rows > 1 and ld != c.logits.stride(0):
+        raise ValueError("out overlaps the logits")
+    q = c.fill()
+    c.launch(load().dvae_rules_apply, ctypes.byref(q), E._ptr(out), ld)
+    E._written(out)
+    return out
+
+
+def _span(t):
+    n = 1 + sum((s - 1) * st for s, st in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + n * t.element_size()
+
+
+def _apart(a, b, text):
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    if a0 < b1 and b0 < a1:
+        raise ValueError(text)
+
+
+def choose(logits, rules=None, history=None, lengths=None, state=None, temperature=1.0, uniforms=None):
+    """One token per row -> ``Choice(tokens int64, logprob fp32, state int32 or None)``.
+
+    Without ``uniforms`` the largest x4, the lowest index of equal ones.  With ``uniforms`` (fp32, one per row, in [0, 1)) the
+    first token at which the running sum of p exceeds u; either decision is the one of 64-bit arithmetic.  ``logprob`` is
+    log p of the token (detached), ``state`` the grammar's next state where the grammar has ``next_state`` (a row without
+    a token keeps its state)."""
+    if torch.is_tensor(logits):
+        logits = logits.detach()
+    c = _Call(logits, rules, history, lengths, state, temperature)
+    u = None
+    if uniforms is not None:
+        u = c._per_row(uniforms, "uniforms", (torch.float32,)).contiguous()
+    dev = c.device
+    tokens = torch.empty(c.lead, dtype=torch.int64, device=dev)
+    logprob = torch.empty(c.lead, dtype=torch.float32, device=dev)
+    following = nxt = None
+    if c.grammar is not None and c.grammar.next_state is not None:
+        nxt = c._here(c.grammar.next_state, "grammar")
+        following = torch.empty(c.lead, dtype=torch.int32, device=dev)
+    q = c.fill()
+    ws = c.workspace(q)
+    c.launch(load().dvae_rules_choose, ctypes.byref(q), E._ptr(u), E._ptr(nxt), E._ptr(tokens), E._ptr(logprob),
+             E._ptr(following), E._ptr(ws))
+    return Choice(tokens, logprob, following)
+
+
+class _LogprobFn(torch.autograd.Function):
+    # every tensor behind a pointer goes through save_for_backward: a change between forward and backward is an error
+    @staticmethod
+    def forward(ctx, call, logits, bias, tokens, *others):
+        q = call.fill()
+        ws = call.workspace(q)
+        logprob = torch.empty(call.rows, dtype=torch.float32, device=call.device)
+        stat = torch.empty(call.rows, 2, dtype=torch.float32, device=call.device)
+        call.launch(load().dvae_rules_logprob, ctypes.byref(q), E._ptr(tokens), E._ptr(logprob), E._ptr(stat), E._ptr(ws))
+        ctx.call = call
+        ctx.save_for_backward(logits, bias, tokens, stat, *others)
+        return logprob
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_logprob):
+        call = ctx.call
+        tokens, stat = ctx.saved_tensors[2:4]          # checks every saved tensor's version
+        q = call.fill()
+        d_logprob = d_logprob.to(torch.float32).contiguous()
+        d_logits = torch.empty(call.logits.shape, dtype=call.logits.dtype, device=call.device)
+        d_bias = None
+        if ctx.needs_input_grad[2]:
+            d_bias = torch.empty(call.bias.shape, dtype=torch.float32, device=call.device)
+        ws = call.workspace(q)
+        call.launch(load().dvae_rules_logprob_bwd, ctypes.byref(q), E._ptr(tokens), E._ptr(stat), E._ptr(d_logprob),
+                    E._ptr(d_logits), call.V, E._ptr(d_bias), E._ptr(ws))
+        grads = (None, d_logits if ctx.needs_input_grad[1] else None, d_bias, None)
+        return grads + (None,) * (len(ctx.needs_input_grad) - 4)
+
+
+def token_logprob(logits, tokens, rules=None, history=None, lengths=None, state=None, temperature=1.0):
+    """log p of ``tokens`` (int32 / int64, one per row) under the rules, fp32, one per row; differentiable once with respect
+    to the logits and the rules' bias.  A token outside [0, V) marks a row to ignore: 0 and no gradient.  A token the
+    grammar forbids has -inf (and still the gradient -p / temperature of the allowed ones)."""
+    c = _Call(logits, rules, history, lengths, state, temperature)
+    c._per_row(tokens, "tokens", _INDEX)
+    tokens = tokens.to(torch.int64).contiguous().view(-1)
+    others = [t for t in (c.history, c.lengths, c.state) if t is not None]
+    if c.grammar is not None:
+        others.append(c.grammar.masks)
+    others += [v for _, v in c.settings if torch.is_tensor(v)]
+    x, b = c.logits, c.bias
+    c.logits, c.bias = x.detach(), None if b is None else b.detach()
+    return _LogprobFn.apply(c, x, b, tokens, *others).view(c.lead)

@@ -20,6 +20,7 @@ from . import _lib
 from . import engine as E
 from ._lib import check, load
 from .engine import _f32c, _ptr, _stream
+from .rules import choose
 
 
 class GruWeights(nn.Module):
@@ -163,6 +164,24 @@ class _ElboFn(torch.autograd.Function):
         return None, gt * (d[1] + d[3]), ge * (d[0] + d[3]), None, gm * sk, gl * sk, None
 
 
+def decide_string(scores, rules, uniforms=None, temperature=1.0):
+    """Types [B, T] of strings whose scores [B, T, C] are all known: one ``rules.choose`` a step, the earlier steps' types
+    as history."""
+    B, T, C = scores.shape
+    tokens = torch.full((B, T), -1, dtype=torch.int64, device=scores.device)
+    state = None
+    if rules.grammar is not None:
+        if rules.grammar.next_state is None:
+            raise ValueError("decide_string: the grammar needs next states")
+        state = torch.full((B,), rules.grammar.start, dtype=torch.int32, device=scores.device)
+    for t in range(T):
+        picked = choose(scores[:, t], rules, history=tokens[:, :t] if t else None, state=state, temperature=temperature,
+                        uniforms=None if uniforms is None else uniforms[:, t])
+        tokens[:, t] = picked.tokens
+        state = picked.state
+    return tokens
+
+
 class Encoder(nn.Module):
     """svae_model.py:13-44."""
 
@@ -255,10 +274,17 @@ class Svae(nn.Module):
             eps = torch.randn_like(mu)
         return E.ReparamFn.apply(mu, logvar, eps)
 
-    def _predict_from_logits(self, type_scores, edge_scores, is_stochastic=False, uniforms=None):
+    def _predict_from_logits(self, type_scores, edge_scores, is_stochastic=False, uniforms=None, rules=None,
+                             temperature=1.0):
         """-> (one-hot types, parent flags), exact 0/1 (:112-131).  Stochastic draws use the
         uniforms given as (u_type [..], u_edge [.., N]) or fresh ``torch.rand`` ones, through the
-        inverse CDF (the reference draws with torch.multinomial / torch.bernoulli)."""
+        inverse CDF (the reference draws with torch.multinomial / torch.bernoulli).  ``rules`` (an addition): a
+        rules.TokenRules the types [B, T, C] are decided under, step by step with the string's earlier types as history
+        (rules.dag_rules(..., start=1)); a step the rules leave nothing for has an all-zero one-hot row."""
+        if rules is None and temperature != 1.0:
+            raise ValueError("a temperature goes with rules")
+        if rules is not None and type_scores.dim() != 3:
+            raise ValueError("rules need the strings' type scores [B, T, C]")
         ts, es = _f32c(type_scores), _f32c(edge_scores)
         E._require_cuda(ts, "type_scores")
         rows = ts.numel() // ts.shape[-1]
@@ -272,6 +298,9 @@ class Svae(nn.Module):
         onehot, flags = torch.empty_like(ts), torch.empty_like(es)
         check(load().dvae_svae_predict(ctypes.byref(d), rows, _ptr(ts), _ptr(es), _ptr(ut), _ptr(ue), _ptr(onehot),
                                        _ptr(flags), _stream()))
+        if rules is not None:
+            tokens = decide_string(ts, rules, ut.view(ts.shape[:-1]) if is_stochastic else None, temperature)
+            onehot = (tokens.unsqueeze(-1) == torch.arange(ts.shape[-1], device=ts.device)).to(ts.dtype)
         return onehot, flags
 
     def predict(self, X):
@@ -399,7 +428,8 @@ class Svae(nn.Module):
     def test_dataloader(self):
         return self.test_loader
 
-    def model_eval(self, X, sample_num, decode_num, is_stochastic=True, eps=None, uniforms=None):
+    def model_eval(self, X, sample_num, decode_num, is_stochastic=True, eps=None, uniforms=None, rules=None,
+                   temperature=1.0):
         with torch.no_grad():
             true_graph = X["graph"]
             mu, logvar = self.encoder(true_graph)
@@ -412,7 +442,7 @@ class Svae(nn.Module):
             sampled_z = stack_z.view(batch_size * sample_num * decode_num, hidden_size)
             type_scores, edge_scores = self.decoder(sampled_z)
             onehot, flags = self._predict_from_logits(type_scores, edge_scores, is_stochastic=is_stochastic,
-                                                      uniforms=uniforms)
+                                                      uniforms=uniforms, rules=rules, temperature=temperature)
             pred_graph = torch.cat((onehot, flags), dim=-1)
             pred_graph = pred_graph.view(batch_size, decode_num * samples, *pred_graph.shape[1:])
             correct = (true_graph.unsqueeze(1) == pred_graph).all(dim=-1).all(dim=-1)

@@ -10,6 +10,8 @@ import os
 
 import torch
 
+from .optim import clip_grads
+
 
 def save_checkpoint(path, model, optimizer=None, scheduler=None, epoch=0, extra=None):
     """`{'epoch', 'state_dict', 'optimizer_states', 'lr_schedulers'}` -- the keys a Lightning
@@ -62,6 +64,8 @@ class Trainer:
                       `training_step(...)['loss'].backward()` through autograd
     flat_adam         with `fused`: the model's Adam as one launch per module over flat buffers (optim.FlatAdam; same
                       update, same checkpoint layout as torch.optim.Adam) when `configure_optimizers` offers it
+    gradient_clip_val largest norm of all gradients taken together, as Lightning's Trainer has it (0 = no clipping): applied
+                      before every optimizer step, after the gradients' all-reduce
     dist              torch.distributed module (initialised) for data-parallel runs: every rank
                       trains on its shard of each batch, gradients are SUM all-reduced (dp.py)
     A batch dict may carry 'eps' [B,Z]: the reparameterisation draw per GLOBAL graph index (sharded with the
@@ -69,7 +73,10 @@ class Trainer:
     """
 
     def __init__(self, max_epochs=300, save_dir=None, fused=True, dist=None, keep_all=False, log=print,
-                 max_steps_per_epoch=None, flat_adam=True):
+                 max_steps_per_epoch=None, flat_adam=True, gradient_clip_val=0.0):
+        if not float(gradient_clip_val) >= 0.0:
+            raise ValueError("Trainer: gradient_clip_val must not be negative, got %r" % (gradient_clip_val,))
+        self.gradient_clip_val = float(gradient_clip_val)
         self.max_epochs, self.save_dir, self.fused, self.dist = int(max_epochs), save_dir, fused, dist
         self.flat_adam = flat_adam
         self.keep_all, self.log, self.max_steps = keep_all, log, max_steps_per_epoch
@@ -82,6 +89,15 @@ class Trainer:
     def _world(self):
         d = self.dist
         return (d.get_rank(), d.get_world_size()) if d is not None and d.is_initialized() else (0, 1)
+
+    def _step(self, opt):
+        """The optimizer's step on gradients of at most gradient_clip_val."""
+        if self.gradient_clip_val > 0.0:
+            if hasattr(opt, 'max_norm'):        # FlatAdam scales the gradients inside its update
+                opt.max_norm = self.gradient_clip_val
+            else:
+                clip_grads([p.grad for g in opt.param_groups for p in g['params']], self.gradient_clip_val)
+        opt.step()
 
     def fit(self, model, resume_from=None):
         from . import dp
@@ -128,7 +144,7 @@ class Trainer:
                 if prepared:
                     batch, level_sched = item
                     out4 = model.loss_and_grad(batch, eps=batch.get('eps'), grad_sync=sync, sched=level_sched)
-                    opt.step()
+                    self._step(opt)
                     sums += dp.allreduce_losses(self.dist, out4.detach().clone()).double().cpu()
                     steps += 1
                     continue
@@ -149,7 +165,7 @@ class Trainer:
                                 sync(p.grad).wait()
                     out4 = torch.tensor([out['log'][k] for k in ('train/edge_loss', 'train/vertex_loss',
                                                                  'train/kl_loss', 'train/loss')])
-                opt.step()
+                self._step(opt)
                 sums += dp.allreduce_losses(self.dist, out4.detach().clone()).double().cpu()
                 steps += 1
             rec = {'epoch': self.epoch, 'steps': steps}

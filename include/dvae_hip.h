@@ -327,6 +327,11 @@ int dvae_adam_step(float* param, const float* grad, float* exp_avg, float* exp_a
  * joined).  dvae_phase_read waits for the device, returns the marks' times in ms since the first one and their tags
  * (at most max), and forgets them.  tools/lab/phases.py prints the per-phase means. */
 int dvae_phase_read(double* out_ms, int* tags, int max);
+/* dvae_adam_step on the gradients scale[0] * grad: scale is one float in device memory, e.g. the coefficient that
+ * dvae_grad_norm leaves, so that a clipped step costs no pass over the gradients of its own. */
+int dvae_adam_step_scaled(float* param, const float* grad, const float* scale, float* exp_avg, float* exp_avg_sq, size_t n,
+                          double lr, double beta1, double beta2, double eps, double weight_decay, long long step,
+                          void* stream);
 /* test surface (no counterpart in the reference): which kernels score add_edge's pairs (dvae_model.py:210-220) for
  * graphs of up to N nodes at add_edge width EHP (dvae_dims.EHP).  Bits: 1 forward on the LDS-sliced scorer, 2 with more
  * than one window of candidate rows, 4 backward fused per graph (accumulators on chip), 8 backward windowed one-pass;
@@ -465,6 +470,91 @@ int dvae_svae_elbo(const dvae_svae_dims* d, const float* type_scores, const floa
 int dvae_svae_predict(const dvae_svae_dims* d, long long rows, const float* type_scores,
                       const float* edge_scores, const float* u_type, const float* u_edge,
                       float* onehot, float* flags, void* stream);
+
+/* element types of the calls below */
+enum { DVAE_F32 = 0, DVAE_BF16 = 1, DVAE_F16 = 2 };
+
+/* ------------------------------------------------------------------------
+ * Global gradient norm and clipping (the reference trains through a Lightning Trainer, train.py:41-47, whose
+ * gradient_clip_val this is; no kernel of the reference's own).  norm = sqrt of the sum of squares over ALL tensors;
+ * coef = min(1, max_norm / (norm + 1e-6)); norm_coef[2] (device) = {norm, coef}.  Squares and sums are doubles added in a
+ * fixed order: the same bits every call.  A NaN gradient makes norm and coef NaN, an infinite one coef 0.
+ *   dvae_grad_norm   reads the tensors' `in` only
+ *   dvae_clip_grads  also writes out = coef * in, rounded once to out_type; `out` may be `in` (then nothing is written
+ *                    while coef is 1); any other overlap of an output with a tensor is refused
+ * Tensors are flat: n elements from `in` (aligned to their type only).  `tensors` is host memory, read before the call
+ * returns.  ws: dvae_clip_ws_bytes(n) bytes of device memory, free again once the call's work is done.
+ * ---------------------------------------------------------------------- */
+typedef struct dvae_tensor {
+  const void* in;
+  void* out;
+  long long n;
+  int in_type, out_type;
+} dvae_tensor;
+size_t dvae_clip_ws_bytes(int n);
+int dvae_grad_norm(const dvae_tensor* tensors, int n, double max_norm, float* norm_coef, void* ws, void* stream);
+int dvae_clip_grads(const dvae_tensor* tensors, int n, double max_norm, float* norm_coef, void* ws, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Token rules on rows of logits (for the type decisions of Decoder.predict, dvae_model.py:282-291, and
+ * Svae._predict_from_logits, svae_model.py:112-131, which take the plain argmax or draw; the reference has no rules).
+ * c(v) = how often the row's history holds v:
+ *   x1 = c > 0 ? (x > 0 ? x / repetition : x * repetition) : x
+ *   x2 = x1 - frequency * c - presence * [c > 0]
+ *   x3 = x2 + bias[v]
+ *   x4 = the row's grammar state allows v ? x3 : -inf;  p = softmax(x4 / temperature)
+ * Each setting is one double for all rows, or an array of one float per row (the *_rows pointers) where that is not NULL.
+ * repetition and temperature are positive, temperature finite; a row whose own temperature is not, or that allows a NaN or
+ * +inf logit, has token -1 and a NaN log-probability.
+ * ---------------------------------------------------------------------- */
+typedef struct dvae_rules {
+  const void* logits;         /* [rows][ld], ld >= vocab, any alignment of the type                                   */
+  long long rows, ld;
+  int vocab, dtype;           /* DVAE_F32 / DVAE_BF16 / DVAE_F16                                                      */
+  const void* history;        /* int32 or int64 tokens, NULL = none; entries outside [0, vocab) count nothing         */
+  long long history_ld;       /* elements between two histories                                                       */
+  int history_len;            /* tokens of a history                                                                  */
+  int history_i64;            /* 1: int64 entries                                                                     */
+  long long rows_per_history; /* row r has history r / rows_per_history                                               */
+  const int* lengths;         /* [rows]: only the first lengths[r] tokens count (clamped to 0..history_len), or NULL  */
+  double repetition, frequency, presence, temperature;
+  const float *repetition_rows, *frequency_rows, *presence_rows, *temperature_rows;
+  const float* bias;          /* [vocab] (bias_ld 0) or [rows][bias_ld], or NULL                                      */
+  long long bias_ld;
+  const uint32_t* mask;       /* [states][mask_words]: bit v % 32 of word v / 32 = state allows v; NULL = no grammar  */
+  int mask_words, states;
+  const int* state;           /* [rows]: the row's state; one outside [0, states) allows everything                   */
+} dvae_rules;
+/* ws of choose / logprob / logprob_bwd; 0 for arguments they refuse */
+size_t dvae_rules_ws_bytes(const dvae_rules* rules);
+/* out [rows][out_ld] (of the logits' type; may be the logits) = x4 */
+int dvae_rules_apply(const dvae_rules* rules, void* out, long long out_ld, void* stream);
+/* One token per row and its log-probability log p.  uniforms NULL: the largest x4, the lowest index of equal ones.
+ * uniforms [rows] in [0, 1): the first v at which the running sum of p exceeds u (u below 0 counts as 0, from 1 on the
+ * last token with a probability, NaN as token -1).  The decision is that of 64-bit arithmetic.  A row whose rules leave
+ * nothing has token -1 and log-probability -inf.  next [states][vocab] / state_out [rows] (together, or NULL):
+ * state_out[r] = next[state[r]][token]; a row without a token or a state keeps its state.  state_out may be `state`. */
+int dvae_rules_choose(const dvae_rules* rules, const float* uniforms, const int* next, long long* tokens, float* logprob,
+                      int* state_out, void* ws, void* stream);
+/* log p of the given tokens [rows]; a token outside [0, vocab) makes an ignored row (0).  stat [rows][2]: kept by the
+ * caller for the backward call. */
+int dvae_rules_logprob(const dvae_rules* rules, const long long* tokens, float* logprob, float* stat, void* ws,
+                       void* stream);
+/* d_logits [rows][d_ld] (the logits' type) = slope * d_logprob[r] / temperature * ([v = token] - p), slope the derivative
+ * of x2 (1, 1 / repetition or repetition), 0 where the grammar forbids v, in ignored rows and in rows with nothing
+ * allowed.  d_bias (or NULL): the same without the slope, summed over the rows in a fixed order for a shared bias
+ * ([vocab]), else [rows][vocab].  d_logits may be the logits. */
+int dvae_rules_logprob_bwd(const dvae_rules* rules, const long long* tokens, const float* stat, const float* d_logprob,
+                           void* d_logits, long long d_ld, float* d_bias, void* ws, void* stream);
+
+/* dvae_decoder_predict with its type decisions (dvae_model.py:282-291) under rules: repetition .. temperature (and their
+ * per-latent arrays), bias and mask of `rules` count; logits, rows, history, lengths and state are the decode's own (a
+ * latent's history: the types of its earlier nodes; its state: `start`, then next[state][type]).  A node whose rules leave
+ * nothing has an all-zero one-hot row, and the decode goes on as after type 0.  ws: dvae_predict_rules_ws_bytes(d). */
+size_t dvae_predict_rules_ws_bytes(const dvae_dims* d);
+int dvae_decoder_predict_rules(const dvae_dims* d, const float* z, const float* P, void* ws, const float* u_type,
+                               const float* u_edge, const dvae_rules* rules, const int* next, int start, float* edges,
+                               float* onehot, void* stream);
 
 #ifdef __cplusplus
 }
