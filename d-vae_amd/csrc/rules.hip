@@ -76,13 +76,22 @@ struct RowP {
   int n_hist;
 };
 
-__device__ __forceinline__ RowP row_params(const dvae_rules& q, long long r) {
+// one setting for all rows: its quotients are formed on the host
+struct Rules : dvae_rules {
+  double inv_rho, k;
+};
+
+__device__ __forceinline__ RowP row_params(const Rules& q, long long r) {
   RowP p;
-  p.rho = q.repetition_rows ? (double)q.repetition_rows[r] : q.repetition;
-  p.inv_rho = 1.0 / p.rho;
+  p.rho = q.repetition;
+  p.inv_rho = q.inv_rho;
+  if (q.repetition_rows) {
+    p.rho = q.repetition_rows[r];
+    p.inv_rho = 1.0 / p.rho;
+  }
   p.freq = q.frequency_rows ? (double)q.frequency_rows[r] : q.frequency;
   p.pres = q.presence_rows ? (double)q.presence_rows[r] : q.presence;
-  p.k = LOG2E / (q.temperature_rows ? (double)q.temperature_rows[r] : q.temperature);
+  p.k = q.temperature_rows ? LOG2E / (double)q.temperature_rows[r] : q.k;
   p.bias = q.bias ? q.bias + r * q.bias_ld : nullptr;
   p.mask = nullptr;
   if (q.mask) {
@@ -169,7 +178,7 @@ enum { M_APPLY = 0, M_SUM = 1, M_GREEDY = 2, M_DRAW = 3, M_BWD = 4 };
 constexpr int SEG_MAX = 4096;   // tokens of a segment at most: the counts of a workgroup's 4 segments are 32 KB of 16 bits
 
 struct SegArgs {
-  dvae_rules q;
+  Rules q;
   int nseg, seg_len;            // segments of a row, their tokens (a multiple of 64 x 16 bytes)
   int wgs_per_row;              // workgroups of a row (ROWWAVE: unused)
   void* out; long long out_ld;  // APPLY / BWD
@@ -283,7 +292,7 @@ __global__ __launch_bounds__(256) void rules_seg_kernel(SegArgs a) {
   constexpr int EV = E::EV, STEP = 64 * EV;
   constexpr int WORDS = HIST ? 4 * SEG_MAX / Counts<HIST ? HIST : 1>::PER_WORD : 4;
   __shared__ uint32_t lds[WORDS];
-  const dvae_rules& q = a.q;
+  const Rules& q = a.q;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   long long row;
@@ -399,7 +408,7 @@ __global__ __launch_bounds__(256) void rules_seg_kernel(SegArgs a) {
 // join: one workgroup a row
 // ---------------------------------------------------------------------------------------------------------------
 struct JoinArgs {
-  dvae_rules q;
+  Rules q;
   int nseg, seg_len;
   const Seg* seg;
   const float* uniforms;         // DRAW
@@ -448,7 +457,7 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
   __shared__ int pick_seg;
   __shared__ double pick_before;
   __shared__ uint32_t cnt[SEG_MAX];         // counts of the segment that is searched
-  const dvae_rules& q = a.q;
+  const Rules& q = a.q;
   const long long row = blockIdx.x;
   const int V = q.vocab, tid = threadIdx.x;
   const RowP p = row_params(q, row);
@@ -585,6 +594,135 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------
+// small vocabularies: W lanes a row (W the power of two from the vocabulary on, up to a wave), one token a lane, one
+// launch that ends each row -- everything in double, sums and searches by shuffles inside the group
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int SMALL_VOCAB = 64, SMALL_HISTORY = 256;
+
+struct SmallArgs {
+  Rules q;
+  int w;                          // lanes of a row
+  const float* uniforms; const int* next; long long* tokens; float* logprob; int* state_out;   // GREEDY / DRAW
+  const long long* given; float* stat;                                                         // SUM, BWD
+  const float* d_logprob; void* out; long long out_ld; float* d_bias; float* part;             // APPLY, BWD
+};
+
+template <typename X>
+__device__ __forceinline__ X group_sum(X v, int w) {
+  for (int o = w >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+template <int T, int MODE>
+__global__ __launch_bounds__(256) void rules_small_kernel(SmallArgs a) {
+  typedef Elem<T> E;
+  __shared__ float acc_sh[256];
+  const Rules& q = a.q;
+  const int W = a.w, V = q.vocab;
+  const int v = threadIdx.x & (W - 1);
+  const int groups = 256 / W;
+  float acc = 0.f;
+  for (long long row = (long long)blockIdx.x * groups + threadIdx.x / W; row < q.rows; row += (long long)gridDim.x * groups) {
+    const RowP p = row_params(q, row);
+    const bool in = v < V;
+    const float x = in ? E::one(q.logits, row * q.ld + v) : 0.f;
+    uint32_t c = 0;
+    int i = 0;
+    for (; i + 3 < p.n_hist; i += 4) {
+      long long t[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) t[u] = hist_at(p, q.history_i64, i + u);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) c += t[u] == v;
+    }
+    for (; i < p.n_hist; ++i) c += hist_at(p, q.history_i64, i) == v;
+    const bool kept = in && !(p.mask && !((p.mask[v >> 3] >> (v & 7)) & 1));
+    const float b = p.bias && in ? p.bias[v] : 0.f;
+    const double y = !kept ? -INFINITY : c ? counted64(p, x, c, b) : (double)x + (double)b;
+    if (MODE == M_APPLY) {
+      if (in) static_cast<typename E::type*>(a.out)[row * a.out_ld + v] = E::cast((float)y);
+      continue;
+    }
+    if (MODE == M_BWD) {
+      const float m = a.stat[2 * row];
+      const long long tok = a.given[row];
+      double g = 0.0;
+      if (kept && tok >= 0 && tok < V && m != -INFINITY)
+        g = (double)a.d_logprob[row] * (p.k * LN2) * ((v == tok ? 1.0 : 0.0) - exp2_64(y - (double)m, p.k) * (double)a.stat[2 * row + 1]);
+      const float gf = (float)g;
+      if (a.part) acc += gf;
+      else if (a.d_bias && in) a.d_bias[row * V + v] = gf;
+      if (c) g *= x > 0.f ? p.inv_rho : p.rho;
+      if (in) static_cast<typename E::type*>(a.out)[row * a.out_ld + v] = E::cast((float)g);
+      continue;
+    }
+    float m = (float)y;
+    for (int o = W >> 1; o > 0; o >>= 1) m = max_nan(m, __shfl_xor(m, o));
+    const bool ok = m > -INFINITY && m < INFINITY && p.k > 0.0 && p.k < INFINITY;
+    const double w = kept && ok ? exp2_64(y - (double)m, p.k) : 0.0;
+    double run = w;                                   // running sum in the vocabulary's order
+    for (int o = 1; o < W; o <<= 1) {
+      const double t = __shfl_up(run, o, W);
+      if (v >= o) run += t;
+    }
+    const double Z = __shfl(run, W - 1, W);
+    long long tok = -1;
+    if (MODE == M_SUM) {
+      tok = a.given[row];
+    } else if (ok && MODE == M_GREEDY) {
+      double best = y;
+      int idx = v;
+      for (int o = W >> 1; o > 0; o >>= 1) {
+        const double b2 = __shfl_xor(best, o);
+        const int i2 = __shfl_xor(idx, o);
+        if (b2 > best || (b2 == best && i2 < idx)) { best = b2; idx = i2; }
+      }
+      tok = idx;
+    } else if (ok && MODE == M_DRAW) {
+      const float u = a.uniforms[row];
+      if (u == u) {
+        int hit = w > 0.0 && run > fmax((double)u, 0.0) * Z ? v : INT32_MAX;
+        int last = w > 0.0 ? v : -1;
+        for (int o = W >> 1; o > 0; o >>= 1) {
+          hit = min(hit, __shfl_xor(hit, o));
+          last = max(last, __shfl_xor(last, o));
+        }
+        tok = hit != INT32_MAX ? hit : last;
+      }
+    }
+    const bool have = tok >= 0 && tok < V;
+    const double at = __shfl(y, have ? (int)tok : 0, W);
+    if (v) continue;
+    float lp;
+    if (MODE == M_SUM && !have) lp = 0.f;
+    else if (m == -INFINITY) lp = -INFINITY;
+    else if (!ok || !have) lp = NAN;
+    else lp = (float)((at - (double)m) * (p.k * LN2) - log(Z));
+    a.logprob[row] = lp;
+    if (MODE == M_SUM) {
+      a.stat[2 * row] = m == -INFINITY || ok ? m : NAN;
+      a.stat[2 * row + 1] = ok ? (float)(1.0 / Z) : NAN;
+    } else {
+      a.tokens[row] = tok;
+      if (a.state_out) {
+        const int s = q.state[row];
+        a.state_out[row] = tok >= 0 && s >= 0 && s < q.states ? a.next[(size_t)s * V + tok] : s;
+      }
+    }
+  }
+  if (MODE == M_BWD) {
+    if (!a.part) return;
+    // the workgroup's share of the bias gradient: its groups in order
+    acc_sh[threadIdx.x] = acc;
+    __syncthreads();
+    if (threadIdx.x >= V) return;
+    float s = 0.f;
+    for (int g = 0; g < groups; ++g) s += acc_sh[g * W + threadIdx.x];
+    a.part[(size_t)blockIdx.x * V + threadIdx.x] = s;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
 // gradients with a bias shared by the rows: a workgroup owns 256 EV columns and walks a share of the rows, so the
 // bias gradient's sum over rows stays in registers; shares are added in a fixed order by a second launch
 // ---------------------------------------------------------------------------------------------------------------
@@ -600,7 +738,7 @@ __global__ __launch_bounds__(256) void rules_bwd_col_kernel(ColArgs ca) {
   constexpr int EV = E::EV, SPAN = 256 * EV;
   __shared__ uint32_t lds[HIST ? SPAN : 1];
   const SegArgs& a = ca.s;
-  const dvae_rules& q = a.q;
+  const Rules& q = a.q;
   const int V = q.vocab, v0 = blockIdx.x * SPAN, v = v0 + threadIdx.x * EV;
   const long long r0 = (long long)blockIdx.y * ca.rows_per_share;
   const long long r1 = min(r0 + ca.rows_per_share, q.rows);
@@ -645,12 +783,20 @@ __global__ __launch_bounds__(256) void rules_bwd_col_kernel(ColArgs ca) {
     if (v + e < V) ca.part[(size_t)blockIdx.y * V + v + e] = acc[e];
 }
 
+// 16 columns a workgroup, 16 threads a column: shares in a fixed order
 __global__ __launch_bounds__(256) void rules_bias_sum_kernel(const float* __restrict__ part, int shares, int V,
                                                              float* __restrict__ d_bias) {
-  const int v = blockIdx.x * 256 + threadIdx.x;
-  if (v >= V) return;
+  __shared__ float sh[16][17];
+  const int c = threadIdx.x & 15, r = threadIdx.x >> 4, v = blockIdx.x * 16 + c;
   float s = 0.f;
-  for (int i = 0; i < shares; ++i) s += part[(size_t)i * V + v];
+  if (v < V) {
+#pragma unroll 4
+    for (int i = r; i < shares; i += 16) s += part[(size_t)i * V + v];
+  }
+  sh[r][c] = s;
+  __syncthreads();
+  if (r || v >= V) return;
+  for (int i = 1; i < 16; ++i) s += sh[i][c];
   d_bias[v] = s;
 }
 
@@ -662,6 +808,14 @@ constexpr long long MAX_BLOCKS = (1ll << 24) - 1;     // blocks x 256 threads st
 struct Plan { int seg_len, nseg, wgs_per_row; bool row_wave; long long blocks; };
 
 int elem_bytes(int dtype) { return dtype == DVAE_F32 ? 4 : 2; }
+
+Rules with_constants(const dvae_rules& q) {
+  Rules r;
+  static_cast<dvae_rules&>(r) = q;
+  r.inv_rho = 1.0 / q.repetition;
+  r.k = LOG2E / q.temperature;
+  return r;
+}
 
 Plan plan_of(const dvae_rules& q) {
   Plan p;
@@ -711,7 +865,37 @@ int run_join(const JoinArgs& a, hipStream_t st) {
   return DVAE_OK;
 }
 
+// a lane a token and its history read by every lane of the group: pays while both are short
+bool is_small(const dvae_rules& q) {
+  return q.vocab <= SMALL_VOCAB && (!q.history || q.history_len <= SMALL_HISTORY);
+}
+
+int small_lanes(const dvae_rules& q) {
+  int w = 1;
+  while (w < q.vocab) w <<= 1;
+  return w;
+}
+
+long long small_blocks(const dvae_rules& q) {
+  const int groups = 256 / small_lanes(q);
+  return std::min<long long>((q.rows + groups - 1) / groups, MAX_BLOCKS);
+}
+
+template <int MODE>
+int run_small(SmallArgs& a, long long blocks, hipStream_t st) {
+  a.w = small_lanes(a.q);
+  const dim3 grid((unsigned)blocks), block(256);
+  switch (a.q.dtype) {
+    case DVAE_F32: hipLaunchKernelGGL((rules_small_kernel<DVAE_F32, MODE>), grid, block, 0, st, a); break;
+    case DVAE_BF16: hipLaunchKernelGGL((rules_small_kernel<DVAE_BF16, MODE>), grid, block, 0, st, a); break;
+    default: hipLaunchKernelGGL((rules_small_kernel<DVAE_F16, MODE>), grid, block, 0, st, a);
+  }
+  DVAE_LAUNCH_CHECK();
+  return DVAE_OK;
+}
+
 int bias_shares(const dvae_rules& q) {
+  if (is_small(q)) return (int)std::min<long long>(small_blocks(q), 1024);
   const int span = 256 * (16 / elem_bytes(q.dtype));
   const long long cols = ((long long)q.vocab + span - 1) / span;
   return (int)std::min<long long>(q.rows, std::max<long long>(1, 2048 / cols));
@@ -757,8 +941,13 @@ extern "C" int dvae_rules_apply(const dvae_rules* q, void* out, long long out_ld
   if (q->rows == 0) return DVAE_OK;
   DVAE_REQUIRE(out, "rules_apply: null pointer");
   DVAE_REQUIRE(q->rows <= 1 || out_ld >= q->vocab, "rules_apply: rows of out overlap (ld %lld < vocab %d)", out_ld, q->vocab);
+  if (is_small(*q)) {
+    SmallArgs m{};
+    m.q = with_constants(*q); m.out = out; m.out_ld = out_ld;
+    return run_small<M_APPLY>(m, small_blocks(*q), (hipStream_t)stream);
+  }
   SegArgs a{};
-  a.q = *q;
+  a.q = with_constants(*q);
   const Plan p = plan_of(*q);
   a.out = out; a.out_ld = out_ld;
   return run_seg<M_APPLY>(a, p, (hipStream_t)stream);
@@ -772,11 +961,17 @@ extern "C" int dvae_rules_choose(const dvae_rules* q, const float* uniforms, con
   DVAE_REQUIRE(tokens && logprob && ws, "rules_choose: null pointer");
   DVAE_REQUIRE((next == nullptr) == (state_out == nullptr), "rules_choose: next and state_out go together");
   DVAE_REQUIRE(!next || q->mask, "rules_choose: next states need a grammar mask");
+  if (is_small(*q)) {
+    SmallArgs m{};
+    m.q = with_constants(*q); m.uniforms = uniforms; m.next = next; m.tokens = tokens; m.logprob = logprob; m.state_out = state_out;
+    return uniforms ? run_small<M_DRAW>(m, small_blocks(*q), (hipStream_t)stream)
+                    : run_small<M_GREEDY>(m, small_blocks(*q), (hipStream_t)stream);
+  }
   const Plan p = plan_of(*q);
   SegArgs a{};
-  a.q = *q; a.seg = (Seg*)ws;
+  a.q = with_constants(*q); a.seg = (Seg*)ws;
   JoinArgs j{};
-  j.q = *q; j.nseg = p.nseg; j.seg_len = p.seg_len; j.seg = (const Seg*)ws; j.uniforms = uniforms; j.next = next;
+  j.q = a.q; j.nseg = p.nseg; j.seg_len = p.seg_len; j.seg = (const Seg*)ws; j.uniforms = uniforms; j.next = next;
   j.tokens = tokens; j.logprob = logprob; j.state_out = state_out;
   if (uniforms) {
     DVAE_TRY(run_seg<M_DRAW>(a, p, (hipStream_t)stream));
@@ -792,12 +987,17 @@ extern "C" int dvae_rules_logprob(const dvae_rules* q, const long long* tokens, 
   DVAE_TRY(rules_check(*q, "rules_logprob"));
   if (q->rows == 0) return DVAE_OK;
   DVAE_REQUIRE(tokens && logprob && stat && ws, "rules_logprob: null pointer");
+  if (is_small(*q)) {
+    SmallArgs m{};
+    m.q = with_constants(*q); m.given = tokens; m.logprob = logprob; m.stat = stat;
+    return run_small<M_SUM>(m, small_blocks(*q), (hipStream_t)stream);
+  }
   const Plan p = plan_of(*q);
   SegArgs a{};
-  a.q = *q; a.seg = (Seg*)ws;
+  a.q = with_constants(*q); a.seg = (Seg*)ws;
   DVAE_TRY(run_seg<M_SUM>(a, p, (hipStream_t)stream));
   JoinArgs j{};
-  j.q = *q; j.nseg = p.nseg; j.seg_len = p.seg_len; j.seg = (const Seg*)ws; j.given = tokens; j.logprob = logprob; j.stat = stat;
+  j.q = a.q; j.nseg = p.nseg; j.seg_len = p.seg_len; j.seg = (const Seg*)ws; j.given = tokens; j.logprob = logprob; j.stat = stat;
   return run_join<M_SUM>(j, (hipStream_t)stream);
 }
 
@@ -810,23 +1010,36 @@ extern "C" int dvae_rules_logprob_bwd(const dvae_rules* q, const long long* toke
   DVAE_REQUIRE(!d_bias || q->bias, "rules_logprob_bwd: d_bias without a bias");
   const bool shared = d_bias && q->bias_ld == 0;
   if (q->rows == 0) {
-    if (shared) hipLaunchKernelGGL(rules_bias_sum_kernel, dim3(cdiv(q->vocab, 256)), dim3(256), 0, st, nullptr, 0, q->vocab, d_bias);
+    if (shared) hipLaunchKernelGGL(rules_bias_sum_kernel, dim3(cdiv(q->vocab, 16)), dim3(256), 0, st, nullptr, 0, q->vocab, d_bias);
     DVAE_LAUNCH_CHECK();
     return DVAE_OK;
   }
   DVAE_REQUIRE(tokens && stat && d_logprob && d_logits && (ws || !shared), "rules_logprob_bwd: null pointer");
   DVAE_REQUIRE(q->rows <= 1 || d_ld >= q->vocab, "rules_logprob_bwd: rows of d_logits overlap (ld %lld < vocab %d)", d_ld,
                q->vocab);
+  const int shares = bias_shares(*q);
+  const auto sum_shares = [&]() -> int {
+    hipLaunchKernelGGL(rules_bias_sum_kernel, dim3(cdiv(q->vocab, 16)), dim3(256), 0, st, (const float*)ws, shares, q->vocab,
+                       d_bias);
+    DVAE_LAUNCH_CHECK();
+    return DVAE_OK;
+  };
+  if (is_small(*q)) {
+    SmallArgs m{};
+    m.q = with_constants(*q); m.given = tokens; m.stat = const_cast<float*>(stat); m.d_logprob = d_logprob;
+    m.out = d_logits; m.out_ld = d_ld; m.d_bias = shared ? nullptr : d_bias; m.part = shared ? (float*)ws : nullptr;
+    DVAE_TRY(run_small<M_BWD>(m, shared ? shares : small_blocks(*q), st));
+    return shared ? sum_shares() : DVAE_OK;
+  }
   const Plan p = plan_of(*q);
   SegArgs a{};
-  a.q = *q; a.out = d_logits; a.out_ld = d_ld; a.tokens = tokens;
+  a.q = with_constants(*q); a.out = d_logits; a.out_ld = d_ld; a.tokens = tokens;
   a.stat = stat; a.d_logprob = d_logprob;
   a.d_bias_rows = shared ? nullptr : d_bias;
   if (!shared) return run_seg<M_BWD>(a, p, st);
   ColArgs c{};
   c.s = a;
   c.part = (float*)ws;
-  const int shares = bias_shares(*q);
   c.rows_per_share = (int)((q->rows + shares - 1) / shares);
   const dim3 grid((unsigned)cdiv(q->vocab, 256 * (16 / elem_bytes(q->dtype))), (unsigned)shares);
   const bool hist = q->history && q->history_len > 0;
@@ -842,7 +1055,5 @@ extern "C" int dvae_rules_logprob_bwd(const dvae_rules* q, const long long* toke
   }
 #undef COL
   DVAE_LAUNCH_CHECK();
-  hipLaunchKernelGGL(rules_bias_sum_kernel, dim3(cdiv(q->vocab, 256)), dim3(256), 0, st, c.part, shares, q->vocab, d_bias);
-  DVAE_LAUNCH_CHECK();
-  return DVAE_OK;
+  return sum_shares();
 }

@@ -21,19 +21,22 @@ def _stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def _on_device(device, fn, *args):
-    """check(fn(*args, stream)) on `device`, whichever device is current, on the current stream there."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        check(fn(*args, _stream()))
+def _on_device(index, fn, *args):
+    """check(fn(*args, stream)) on device `index`, whichever device is current, on the current stream there."""
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            check(fn(*args, _stream()))
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc)
 
 
-def _written(t):
-    """Tells autograd that a kernel wrote `t` in place."""
-    if not t.is_inference():
-        torch.autograd.graph.increment_version(t)
+def _written(tensors):
+    """Tells autograd that a kernel wrote these tensors in place."""
+    tensors = [t for t in tensors if not t.is_inference()]
+    if tensors:
+        torch.autograd.graph.increment_version(tensors)
 
 
 def _side(side):
@@ -429,7 +432,7 @@ def predict_rules_call(dims, z, P, rules, next_state, start, u_type=None, u_edge
     edges = _out(M, N, N, device=dev)
     onehot = _out(M, N, C, device=dev)
     check(lib.dvae_decoder_predict_rules(ctypes.byref(dims), _ptr(z), _ptr(P), _ptr(ws), _ptr(u_type), _ptr(u_edge),
-                                         ctypes.byref(rules), _ptr(next_state), start, _ptr(edges), _ptr(onehot),
+                                         rules, _ptr(next_state), start, _ptr(edges), _ptr(onehot),
                                          _stream()))
     return edges, onehot
 

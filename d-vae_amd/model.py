@@ -194,7 +194,7 @@ class Decoder(nn.Module):
             P = self._pack.pack(dims, self.hip_params())
             if rules is not None:
                 nxt = None if rules.grammar is None else rules.grammar.next_state
-                return E.predict_rules_call(dims, E._f32c(z), P, call.fill(), nxt, start, u_type, u_edge)
+                return E.predict_rules_call(dims, E._f32c(z), P, call.q, nxt, start, u_type, u_edge)
             edges, onehot, margin = E.predict_call(dims, E._f32c(z), P, u_type, u_edge, return_margin)
         if return_margin:
             return edges, onehot, margin

@@ -12,7 +12,6 @@ import math
 
 import torch
 
-from . import _lib
 from . import engine as E
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # DVAE_F32 / DVAE_BF16 / DVAE_F16
@@ -30,26 +29,33 @@ def _flat_order(t):
     return True
 
 
-def _gradients(grads, what):
-    """The tensors of a list of gradients (None left out), checked."""
-    ts = [grads] if torch.is_tensor(grads) else [t for t in grads if t is not None]
+def _flat_list(ts, what, name):
+    """Dense fp32 / bf16 / fp16 tensors on one device -> (addresses, sizes, types); each is one stretch of memory."""
+    where = None
     for i, t in enumerate(ts):
-        if not torch.is_tensor(t) or t.layout != torch.strided or t.dtype not in _TYPES:
-            raise ValueError("%s: gradient %d must be a dense fp32, bf16 or fp16 tensor" % (what, i))
-        if t.device != ts[0].device:
-            raise ValueError("%s: gradients on %s and %s" % (what, ts[0].device, t.device))
-        if not _flat_order(t):
-            raise ValueError("%s: the elements of gradient %d %s, strides %s, are not one stretch of memory" %
-                             (what, i, tuple(t.shape), tuple(t.stride())))
-    return ts
+        if not isinstance(t, torch.Tensor) or t.layout != torch.strided or t.dtype not in _TYPES:
+            raise ValueError("%s: %s %d must be a dense fp32, bf16 or fp16 tensor" % (what, name, i))
+        if where is None:
+            where = t.get_device()
+        elif t.get_device() != where:
+            raise ValueError("%s: %ss on %s and %s" % (what, name, ts[0].device, t.device))
+        if not (t.is_contiguous() or _flat_order(t)):
+            raise ValueError("%s: the elements of %s %d %s, strides %s, are not one stretch of memory" %
+                             (what, name, i, tuple(t.shape), tuple(t.stride())))
+    return [t.data_ptr() for t in ts], [t.numel() for t in ts], [_TYPES[t.dtype] for t in ts]
 
 
-def _describe(ts, outs=None):
-    table = (_lib.DvaeTensor * max(len(ts), 1))()
-    for d, t, o in zip(table, ts, ts if outs is None else outs):
-        d.in_, d.out, d.n = t.data_ptr(), o.data_ptr(), t.numel()
-        d.in_type, d.out_type = _TYPES[t.dtype], _TYPES[o.dtype]
-    return table
+def _table(ins, outs):
+    """An array of struct dvae_tensor: per tensor its two addresses, its size and (in one word) its two types."""
+    (pi, n, ti), (po, _, to) = ins, outs
+    flat = [0] * (4 * len(pi))
+    flat[0::4], flat[1::4], flat[2::4] = pi, po, n
+    flat[3::4] = [a | b << 32 for a, b in zip(ti, to)]
+    return (ctypes.c_longlong * max(len(flat), 4))(*flat)
+
+
+def _as_list(ts):
+    return [ts] if isinstance(ts, torch.Tensor) else [t for t in ts if t is not None]
 
 
 def _limit(max_norm, what):
@@ -64,15 +70,15 @@ def grad_norm(grads, max_norm=math.inf):
     on the device (nothing waits for them).  ``grads``: tensors (fp32 / bf16 / fp16, each one stretch of memory; None is
     left out).  Sums are 64-bit in a fixed order: the same bits every time."""
     m = _limit(max_norm, "grad_norm")
-    ts = _gradients(grads, "grad_norm")
+    ts = _as_list(grads)
+    ins = _flat_list(ts, "grad_norm", "gradient")
     if not ts:
         return torch.zeros(()), torch.ones(())
     E._require_cuda(ts[0], "gradient")
-    dev = ts[0].device
-    out = torch.empty(2, device=dev)
+    out = torch.empty(2, device=ts[0].device)
     lib = E.load()
-    ws = E._workspace(lib.dvae_clip_ws_bytes(len(ts)), dev)
-    E._on_device(dev, lib.dvae_grad_norm, _describe(ts), len(ts), m, E._ptr(out), E._ptr(ws))
+    ws = E._workspace(lib.dvae_clip_ws_bytes(len(ts)), ts[0].device)
+    E._on_device(ts[0].get_device(), lib.dvae_grad_norm, _table(ins, ins), len(ts), m, out.data_ptr(), ws.data_ptr())
     return out[0], out[1]
 
 
@@ -83,33 +89,30 @@ def clip_grads(grads, max_norm, out=None):
     The reference's Lightning Trainer has this as ``gradient_clip_val`` (train.py:41-47).  A NaN norm makes the gradients
     NaN; an infinite one makes them 0 (NaN where they were infinite)."""
     m = _limit(max_norm, "clip_grads")
-    ts = _gradients(grads, "clip_grads")
-    outs = ts
+    ts = _as_list(grads)
+    ins = _flat_list(ts, "clip_grads", "gradient")
+    os_, outs = ts, ins
     if out is not None:
-        outs = [out] if torch.is_tensor(out) else [t for t in out if t is not None]
-        if len(outs) != len(ts):
-            raise ValueError("clip_grads: %d outputs for %d gradients" % (len(outs), len(ts)))
-        for i, (t, o) in enumerate(zip(ts, outs)):
-            if not torch.is_tensor(o) or o.layout != torch.strided or o.dtype not in _TYPES or o.shape != t.shape or \
-                    o.device != t.device:
-                raise ValueError("clip_grads: output %d must be a dense fp32, bf16 or fp16 tensor %s on %s" %
-                                 (i, tuple(t.shape), t.device))
-            if any(n > 1 and a != b for n, a, b in zip(t.shape, t.stride(), o.stride())):
+        os_ = _as_list(out)
+        if len(os_) != len(ts):
+            raise ValueError("clip_grads: %d outputs for %d gradients" % (len(os_), len(ts)))
+        outs = _flat_list(os_, "clip_grads", "output")
+        for i, (t, o) in enumerate(zip(ts, os_)):
+            if o.shape != t.shape or o.get_device() != t.get_device():
+                raise ValueError("clip_grads: output %d must be %s on %s" % (i, tuple(t.shape), t.device))
+            if not (t.is_contiguous() and o.is_contiguous()) and \
+                    any(n > 1 and a != b for n, a, b in zip(t.shape, t.stride(), o.stride())):
                 raise ValueError("clip_grads: output %d is laid out unlike its gradient" % i)
-    if torch.is_grad_enabled():
-        for o in outs:
-            if o.requires_grad:
-                raise ValueError("clip_grads: an output that requires a gradient is not written in place")
+    if torch.is_grad_enabled() and any(o.requires_grad for o in os_):
+        raise ValueError("clip_grads: an output that requires a gradient is not written in place")
     if not ts:
         return torch.zeros(())
     E._require_cuda(ts[0], "gradient")
-    dev = ts[0].device
-    norm = torch.empty(2, device=dev)
+    norm = torch.empty(2, device=ts[0].device)
     lib = E.load()
-    ws = E._workspace(lib.dvae_clip_ws_bytes(len(ts)), dev)
-    E._on_device(dev, lib.dvae_clip_grads, _describe(ts, outs), len(ts), m, E._ptr(norm), E._ptr(ws))
-    for o in outs:
-        E._written(o)
+    ws = E._workspace(lib.dvae_clip_ws_bytes(len(ts)), ts[0].device)
+    E._on_device(ts[0].get_device(), lib.dvae_clip_grads, _table(ins, outs), len(ts), m, norm.data_ptr(), ws.data_ptr())
+    E._written(os_)
     return norm[0]
 
 

@@ -23,7 +23,6 @@ A row whose rules leave nothing: token -1, log-probability -inf, no gradient.  A
 own temperature is not positive and finite: token -1, log-probability NaN.
 """
 import collections
-import ctypes
 import math
 
 import torch
@@ -31,7 +30,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from . import engine as E
-from ._lib import check, load
+from ._lib import load
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # DVAE_F32 / DVAE_BF16 / DVAE_F16
 _INDEX = (torch.int32, torch.int64)
@@ -143,123 +142,126 @@ def _per_row_check(t, name):
 
 def _rows2d(t):
     """[..., n] -> [rows, n] with adjacent rows' elements; a view where the layout allows."""
-    t = t.reshape(-1, t.shape[-1]) if t.dim() != 2 else t
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    rows, n = t.shape
+    s0, s1 = t.stride()
+    if (n > 1 and s1 != 1) or (rows > 1 and s0 < n):
         t = t.contiguous()
     return t
 
 
 class _Call:
-    """The C descriptor of one call and the tensors behind its pointers."""
+    """The checked arguments of one call: the C descriptor `q` and the tensors behind its pointers."""
 
     def __init__(self, logits, rules, history, lengths, state, temperature):
-        if not torch.is_tensor(logits) or logits.dtype not in _DTYPES:
+        if not isinstance(logits, torch.Tensor) or logits.dtype not in _DTYPES:
             raise ValueError("logits must be an fp32, bf16 or fp16 tensor [..., V]")
-        if logits.dim() < 1 or logits.shape[-1] < 1:
-            raise ValueError("logits must have a vocabulary axis, got %s" % (tuple(logits.shape),))
-        rules = TokenRules() if rules is None else rules
-        if not isinstance(rules, TokenRules):
+        shape = logits.shape
+        if len(shape) < 1 or shape[-1] < 1:
+            raise ValueError("logits must have a vocabulary axis, got %s" % (tuple(shape),))
+        if rules is None:
+            rules = TokenRules()
+        elif not isinstance(rules, TokenRules):
             raise ValueError("rules must be a TokenRules")
-        self.lead, self.V = tuple(logits.shape[:-1]), int(logits.shape[-1])
-        self.rows = math.prod(self.lead)
-        self.device = logits.device
-        self.rules = rules
-        self.logits = _rows2d(logits)
-        self.history = None
+        self.lead, self.V = lead, V = shape[:-1], shape[-1]
+        self.rows = rows = math.prod(lead)
+        self.index = index = logits.get_device()           # -1: the CPU
+        self.logits = x = _rows2d(logits)
+        q = _lib.DvaeRules(logits=x.data_ptr(), rows=rows, ld=x.stride(0) if rows > 1 else V, vocab=V,
+                           dtype=_DTYPES[x.dtype], rows_per_history=1)
+        self.tensors = keep = []                           # behind q's pointers, besides logits and bias
         if history is not None:
-            if not torch.is_tensor(history) or history.dtype not in _INDEX or history.dim() < 1:
+            if not isinstance(history, torch.Tensor) or history.dtype not in _INDEX or history.dim() < 1:
                 raise ValueError("history must be an int32 / int64 tensor [..., L]")
-            if tuple(history.shape[:-1]) != self.lead[:history.dim() - 1]:
-                raise ValueError("history %s does not go with the rows %s" % (tuple(history.shape), self.lead))
-            if history.shape[-1] > 0 and self.rows > 0:
-                h = history.reshape(-1, history.shape[-1])
-                if h.shape[1] > 1 and h.stride(1) != 1:
+            if history.shape[:-1] != lead[:history.dim() - 1]:
+                raise ValueError("history %s does not go with the rows %s" % (tuple(history.shape), tuple(lead)))
+            self._here(history, "history")
+            L = history.shape[-1]
+            if L > 0 and rows > 0:
+                h = history if history.dim() == 2 else history.reshape(-1, L)
+                if L > 1 and h.stride(1) != 1:
                     h = h.contiguous()
-                self.history = self._here(h, "history")
+                n = h.shape[0]
+                q.history, q.history_len, q.history_ld = h.data_ptr(), L, h.stride(0) if n > 1 else 0
+                q.history_i64 = h.dtype == torch.int64
+                q.rows_per_history = rows // n
+                keep.append(h)
+            if lengths is not None:
+                self._per_row(lengths, "lengths", _INDEX)
+                if lengths.dtype != torch.int32:
+                    lengths = lengths.clamp(0, L).to(torch.int32)
+                lengths = lengths.contiguous()
+                q.lengths = lengths.data_ptr()
+                keep.append(lengths)
         elif lengths is not None:
             raise ValueError("lengths without a history")
-        self.lengths = None
-        if lengths is not None:
-            self._per_row(lengths, "lengths", _INDEX)
-            if lengths.dtype != torch.int32:
-                lengths = lengths.clamp(0, history.shape[-1])
-            self.lengths = lengths.to(torch.int32).contiguous()
-        self.grammar, self.state = rules.grammar, None
-        if self.grammar is not None:
-            if self.grammar.vocab != self.V:
-                raise ValueError("the grammar has %d tokens, the logits %d" % (self.grammar.vocab, self.V))
-            self._here(self.grammar.masks, "grammar")
+        grammar = rules.grammar
+        if grammar is not None:
+            if grammar.vocab != V:
+                raise ValueError("the grammar has %d tokens, the logits %d" % (grammar.vocab, V))
             if state is None:
                 raise ValueError("a grammar needs the rows' state")
+            masks = self._here(grammar.masks, "grammar")
             self._per_row(state, "state", _INDEX)
             if state.dtype != torch.int32:
-                state = state.clamp(-1, self.grammar.states)
-            self.state = state.to(torch.int32).contiguous()
+                state = state.clamp(-1, grammar.states).to(torch.int32)
+            state = state.contiguous()
+            q.mask, q.mask_words, q.states, q.state = masks.data_ptr(), masks.shape[1], masks.shape[0], state.data_ptr()
+            keep.append(masks)
+            keep.append(state)
         elif state is not None:
             raise ValueError("state without a grammar")
         self.bias = None
         if rules.bias is not None:
             b = self._here(rules.bias, "bias")
-            if b.shape[-1] != self.V or (b.dim() > 1 and tuple(b.shape[:-1]) != self.lead):
-                raise ValueError("bias %s does not go with logits %s" % (tuple(b.shape), tuple(logits.shape)))
-            self.bias = (b if b.stride(0) == 1 or self.V == 1 else b.contiguous()) if b.dim() == 1 else _rows2d(b)
-        self.settings = []
-        for name, v in (("repetition", rules.repetition), ("frequency", rules.frequency), ("presence", rules.presence),
-                        ("temperature", temperature)):
-            if torch.is_tensor(v):
-                _per_row_check(v, name)
-                self._per_row(v, name, (torch.float32,))
-                v = v.contiguous()
+            if b.shape[-1] != V or (b.dim() > 1 and b.shape[:-1] != lead):
+                raise ValueError("bias %s does not go with logits %s" % (tuple(b.shape), tuple(shape)))
+            if b.dim() == 1:
+                self.bias = b if V == 1 or b.stride(0) == 1 else b.contiguous()
             else:
-                v = float(v)
-                if name == "temperature" and not (v > 0.0 and math.isfinite(v)):
-                    raise ValueError("temperature must be positive and finite, got %r" % v)
-            self.settings.append((name, v))
-        E._require_cuda(logits, "logits")
+                self.bias = _rows2d(b)
+                q.bias_ld = self.bias.stride(0) if rows > 1 else V
+            q.bias = self.bias.data_ptr()
+        q.repetition = self._setting(q, "repetition", rules.repetition)
+        q.frequency = self._setting(q, "frequency", rules.frequency)
+        q.presence = self._setting(q, "presence", rules.presence)
+        q.temperature = t = self._setting(q, "temperature", temperature)
+        if not (t > 0.0 and t < math.inf):
+            raise ValueError("temperature must be positive and finite, got %r" % t)
+        if index < 0:
+            E._require_cuda(logits, "logits")
+        self.q = q
+
+    def _setting(self, q, name, v):
+        if not isinstance(v, torch.Tensor):
+            return float(v)
+        _per_row_check(v, name)
+        v = self._per_row(v, name, (torch.float32,)).contiguous()
+        setattr(q, name + "_rows", v.data_ptr())
+        self.tensors.append(v)
+        return 1.0
 
     def _here(self, t, name):
-        if t.device != self.device:
-            raise _lib.DvaeError("%s is on %s, the logits on %s" % (name, t.device, self.device))
+        if t.get_device() != self.index:
+            raise _lib.DvaeError("%s is on %s, the logits on %s" % (name, t.device, self.logits.device))
         return t
 
     def _per_row(self, t, name, dtypes):
-        if not torch.is_tensor(t) or t.dtype not in dtypes or tuple(t.shape) != self.lead:
+        if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.shape != self.lead:
             raise ValueError("%s must hold one value per row: a tensor %s of %s" %
-                             (name, self.lead, " / ".join(str(d) for d in dtypes)))
+                             (name, tuple(self.lead), " / ".join(str(d) for d in dtypes)))
         return self._here(t, name)
 
-    def fill(self):
-        q = _lib.DvaeRules()
-        x = self.logits
-        q.logits, q.rows, q.vocab, q.dtype = x.data_ptr(), self.rows, self.V, _DTYPES[x.dtype]
-        q.ld = x.stride(0) if self.rows > 1 else self.V
-        q.rows_per_history = 1
-        if self.history is not None:
-            h = self.history
-            q.history, q.history_len = h.data_ptr(), h.shape[1]
-            q.history_ld = h.stride(0) if h.shape[0] > 1 else 0
-            q.history_i64 = int(h.dtype == torch.int64)
-            q.rows_per_history = self.rows // h.shape[0]
-        if self.lengths is not None:
-            q.lengths = self.lengths.data_ptr()
-        for name, v in self.settings:
-            if torch.is_tensor(v):
-                setattr(q, name + "_rows", v.data_ptr())
-            else:
-                setattr(q, name, v)
-        if self.bias is not None:
-            q.bias = self.bias.data_ptr()
-            q.bias_ld = 0 if self.bias.dim() == 1 else (self.bias.stride(0) if self.rows > 1 else self.V)
-        if self.grammar is not None:
-            g = self.grammar.masks
-            q.mask, q.mask_words, q.states, q.state = g.data_ptr(), g.shape[1], g.shape[0], self.state.data_ptr()
-        return q
-
-    def workspace(self, q):
-        return E._workspace(load().dvae_rules_ws_bytes(ctypes.byref(q)), self.device)
+    def workspace(self):
+        return E._workspace(load().dvae_rules_ws_bytes(self.q), self.logits.device)
 
     def launch(self, fn, *args):
-        E._on_device(self.device, fn, *args)
+        E._on_device(self.index, fn, self.q, *args)
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
 
 
 # ---------------------------------------------------------------------------------------------------------------
@@ -273,11 +275,12 @@ def apply_rules(logits, rules, history=None, lengths=None, state=None, out=None)
     c = _Call(logits, rules, history, lengths, state, 1.0)
     if out is None:
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    else:
-        if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
-            raise ValueError("out must be like the logits: %s %s on %s" % (tuple(logits.shape), logits.dtype, logits.device))
-        if torch.is_grad_enabled() and out.requires_grad:
-            raise ValueError("out requires a gradient")
+        c.launch(load().dvae_rules_apply, out.data_ptr(), c.V)
+        return out
+    if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
+        raise ValueError("out must be like the logits: %s %s on %s" % (tuple(logits.shape), logits.dtype, logits.device))
+    if torch.is_grad_enabled() and out.requires_grad:
+        raise ValueError("out requires a gradient")
     o2 = out if out.dim() == 2 else out.view(-1, c.V)
     if c.rows and ((c.V > 1 and o2.stride(1) != 1) or (c.rows > 1 and o2.stride(0) < c.V)):
         raise ValueError("out: a row's elements must be adjacent")
@@ -286,9 +289,8 @@ def apply_rules(logits, rules, history=None, lengths=None, state=None, out=None)
         _apart(o2, c.logits, "out overlaps the logits")
     elif c.rows > 1 and ld != c.logits.stride(0):
         raise ValueError("out overlaps the logits")
-    q = c.fill()
-    c.launch(load().dvae_rules_apply, ctypes.byref(q), E._ptr(out), ld)
-    E._written(out)
+    c.launch(load().dvae_rules_apply, out.data_ptr(), ld)
+    E._written([out])
     return out
 
 
@@ -310,23 +312,20 @@ def choose(logits, rules=None, history=None, lengths=None, state=None, temperatu
     first token at which the running sum of p exceeds u; either decision is the one of 64-bit arithmetic.  ``logprob`` is
     log p of the token (detached), ``state`` the grammar's next state where the grammar has ``next_state`` (a row without
     a token keeps its state)."""
-    if torch.is_tensor(logits):
-        logits = logits.detach()
     c = _Call(logits, rules, history, lengths, state, temperature)
     u = None
     if uniforms is not None:
         u = c._per_row(uniforms, "uniforms", (torch.float32,)).contiguous()
-    dev = c.device
+    dev = logits.device
     tokens = torch.empty(c.lead, dtype=torch.int64, device=dev)
     logprob = torch.empty(c.lead, dtype=torch.float32, device=dev)
     following = nxt = None
-    if c.grammar is not None and c.grammar.next_state is not None:
-        nxt = c._here(c.grammar.next_state, "grammar")
+    if rules is not None and rules.grammar is not None and rules.grammar.next_state is not None:
+        nxt = c._here(rules.grammar.next_state, "grammar")
         following = torch.empty(c.lead, dtype=torch.int32, device=dev)
-    q = c.fill()
-    ws = c.workspace(q)
-    c.launch(load().dvae_rules_choose, ctypes.byref(q), E._ptr(u), E._ptr(nxt), E._ptr(tokens), E._ptr(logprob),
-             E._ptr(following), E._ptr(ws))
+    ws = c.workspace()
+    c.launch(load().dvae_rules_choose, _address(u), _address(nxt), tokens.data_ptr(), logprob.data_ptr(),
+             _address(following), ws.data_ptr())
     return Choice(tokens, logprob, following)
 
 
@@ -334,31 +333,30 @@ class _LogprobFn(torch.autograd.Function):
     # every tensor behind a pointer goes through save_for_backward: a change between forward and backward is an error
     @staticmethod
     def forward(ctx, call, logits, bias, tokens, *others):
-        q = call.fill()
-        ws = call.workspace(q)
-        logprob = torch.empty(call.rows, dtype=torch.float32, device=call.device)
-        stat = torch.empty(call.rows, 2, dtype=torch.float32, device=call.device)
-        call.launch(load().dvae_rules_logprob, ctypes.byref(q), E._ptr(tokens), E._ptr(logprob), E._ptr(stat), E._ptr(ws))
-        ctx.call = call
-        ctx.save_for_backward(logits, bias, tokens, stat, *others)
+        dev = logits.device
+        ws = call.workspace()
+        logprob = torch.empty(call.rows, dtype=torch.float32, device=dev)
+        stat = torch.empty(call.rows, 2, dtype=torch.float32, device=dev)
+        call.launch(load().dvae_rules_logprob, tokens.data_ptr(), logprob.data_ptr(), stat.data_ptr(), ws.data_ptr())
+        ctx.call, ctx.stat = call, stat
+        ctx.save_for_backward(logits, bias, tokens, *others)
         return logprob
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_logprob):
-        call = ctx.call
-        tokens, stat = ctx.saved_tensors[2:4]          # checks every saved tensor's version
-        q = call.fill()
-        d_logprob = d_logprob.to(torch.float32).contiguous()
-        d_logits = torch.empty(call.logits.shape, dtype=call.logits.dtype, device=call.device)
+        call, stat = ctx.call, ctx.stat
+        logits, bias, tokens = ctx.saved_tensors[:3]          # checks every saved tensor's version
+        if d_logprob.dtype != torch.float32 or not d_logprob.is_contiguous():
+            d_logprob = d_logprob.to(torch.float32).contiguous()
+        d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         d_bias = None
         if ctx.needs_input_grad[2]:
-            d_bias = torch.empty(call.bias.shape, dtype=torch.float32, device=call.device)
-        ws = call.workspace(q)
-        call.launch(load().dvae_rules_logprob_bwd, ctypes.byref(q), E._ptr(tokens), E._ptr(stat), E._ptr(d_logprob),
-                    E._ptr(d_logits), call.V, E._ptr(d_bias), E._ptr(ws))
-        grads = (None, d_logits if ctx.needs_input_grad[1] else None, d_bias, None)
-        return grads + (None,) * (len(ctx.needs_input_grad) - 4)
+            d_bias = torch.empty(bias.shape, dtype=torch.float32, device=logits.device)
+        ws = call.workspace()
+        call.launch(load().dvae_rules_logprob_bwd, tokens.data_ptr(), stat.data_ptr(), d_logprob.data_ptr(),
+                    d_logits.data_ptr(), call.V, _address(d_bias), ws.data_ptr())
+        return (None, d_logits if ctx.needs_input_grad[1] else None, d_bias) + (None,) * (len(ctx.needs_input_grad) - 3)
 
 
 def token_logprob(logits, tokens, rules=None, history=None, lengths=None, state=None, temperature=1.0):
@@ -367,11 +365,8 @@ def token_logprob(logits, tokens, rules=None, history=None, lengths=None, state=
     grammar forbids has -inf (and still the gradient -p / temperature of the allowed ones)."""
     c = _Call(logits, rules, history, lengths, state, temperature)
     c._per_row(tokens, "tokens", _INDEX)
-    tokens = tokens.to(torch.int64).contiguous().view(-1)
-    others = [t for t in (c.history, c.lengths, c.state) if t is not None]
-    if c.grammar is not None:
-        others.append(c.grammar.masks)
-    others += [v for _, v in c.settings if torch.is_tensor(v)]
+    tokens = (tokens if tokens.dtype == torch.int64 else tokens.to(torch.int64)).contiguous()
     x, b = c.logits, c.bias
-    c.logits, c.bias = x.detach(), None if b is None else b.detach()
-    return _LogprobFn.apply(c, x, b, tokens, *others).view(c.lead)
+    c.logits, c.bias = x.detach(), None                   # the graph holds what needs a gradient, not the call
+    lp = _LogprobFn.apply(c, x, b, tokens, *c.tensors)
+    return lp if len(c.lead) == 1 else lp.view(c.lead)
