@@ -30,41 +30,90 @@ static_assert(sizeof(Batch) <= 3584, "kernel arguments");
 
 typedef uint32_t u32x4_u2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_u2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-__device__ __forceinline__ float load1(const void* p, int type, long long i) {
-  if (type == DVAE_F32) return static_cast<const float*>(p)[i];
-  if (type == DVAE_BF16) return __uint_as_float((uint32_t)static_cast<const uint16_t*>(p)[i] << 16);
-  return (float)static_cast<const _Float16*>(p)[i];
-}
-__device__ __forceinline__ void store1(void* p, int type, long long i, float v) {
-  if (type == DVAE_F32) static_cast<float*>(p)[i] = v;
-  else if (type == DVAE_BF16) static_cast<__bf16*>(p)[i] = (__bf16)v;
-  else static_cast<_Float16*>(p)[i] = (_Float16)v;
-}
-
-// tensor of a chunk (uniform over the workgroup)
-__device__ __forceinline__ int tensor_of(const Batch& b, int chunk) {
-  int lo = 0, hi = b.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (b.start[mid] <= chunk) lo = mid; else hi = mid - 1;
+template <int T> struct Elem;
+template <> struct Elem<DVAE_F32> {
+  typedef float type;
+  static constexpr int EV = 4;
+  static __device__ __forceinline__ float at(u32x4 r, int e) { return __uint_as_float(r[e]); }
+  static __device__ __forceinline__ float wide(float v) { return v; }
+  static __device__ __forceinline__ float cast(float v) { return v; }
+};
+template <> struct Elem<DVAE_BF16> {
+  typedef __bf16 type;
+  static constexpr int EV = 8;
+  static __device__ __forceinline__ float at(u32x4 r, int e) {
+    return __uint_as_float((e & 1) ? (r[e >> 1] & 0xffff0000u) : (r[e >> 1] << 16));
   }
-  return lo;
+  static __device__ __forceinline__ float wide(__bf16 v) { return (float)v; }
+  static __device__ __forceinline__ __bf16 cast(float v) { return (__bf16)v; }
+};
+template <> struct Elem<DVAE_F16> {
+  typedef _Float16 type;
+  static constexpr int EV = 8;
+  static __device__ __forceinline__ float at(u32x4 r, int e) {
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)((e & 1) ? (r[e >> 1] >> 16) : (r[e >> 1] & 0xffffu)));
+  }
+  static __device__ __forceinline__ float wide(_Float16 v) { return (float)v; }
+  static __device__ __forceinline__ _Float16 cast(float v) { return (_Float16)v; }
+};
+
+// The tensor of a chunk: every lane of a wave holds two chunk starts, the wave counts those at or before the chunk -- no
+// search through memory between two chunks.
+struct Lookup {
+  int s0, s1;
+  __device__ __forceinline__ explicit Lookup(const Batch& b) {
+    const int lane = threadIdx.x & 63;
+    s0 = lane < b.count ? b.start[lane] : INT32_MAX;
+    s1 = lane + 64 < b.count ? b.start[lane + 64] : INT32_MAX;
+  }
+  __device__ __forceinline__ int operator()(int chunk) const {
+    return __popcll(__ballot(s0 <= chunk)) + __popcll(__ballot(s1 <= chunk)) - 1;
+  }
+};
+static_assert(CLIP_BATCH <= 128, "two chunk starts a lane");
+
+// squares of one chunk, in four sums
+template <int T>
+__device__ __forceinline__ void norm_chunk(const void* in, long long base, int n, double (&s)[4]) {
+  typedef Elem<T> E;
+  constexpr int EV = E::EV, NV = CHUNK / (256 * EV);
+  const typename E::type* p = static_cast<const typename E::type*>(in) + base;
+  if (n == CHUNK) {
+    u32x4 r[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) r[j] = *reinterpret_cast<const u32x4_u2*>(p + (j * 256 + threadIdx.x) * EV);
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < EV; ++e) {
+        const double v = E::at(r[j], e);
+        s[e & 3] = fma(v, v, s[e & 3]);
+      }
+  } else {
+    for (int i = threadIdx.x; i < n; i += 256) {
+      const double v = E::wide(p[i]);
+      s[0] = fma(v, v, s[0]);
+    }
+  }
 }
 
 __global__ __launch_bounds__(256) void norm_kernel(Batch b, double* __restrict__ part) {
   __shared__ double sh[4];
-  double s = 0.0;
+  double s4[4] = {0.0, 0.0, 0.0, 0.0};
   const int chunks = b.start[b.count];
+  const Lookup tensor_of(b);
   for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
-    const int t = tensor_of(b, c);
+    const int t = tensor_of(c);
     const long long base = (long long)(c - b.start[t]) * CHUNK;
-    const long long end = min(base + CHUNK, b.n[t]);
-    for (long long i = base + threadIdx.x; i < end; i += 256) {
-      const double v = load1(b.in[t], b.in_type[t], i);
-      s = fma(v, v, s);
-    }
+    const int n = (int)min((long long)CHUNK, b.n[t] - base);
+    if (b.in_type[t] == DVAE_F32) norm_chunk<DVAE_F32>(b.in[t], base, n, s4);
+    else if (b.in_type[t] == DVAE_BF16) norm_chunk<DVAE_BF16>(b.in[t], base, n, s4);
+    else norm_chunk<DVAE_F16>(b.in[t], base, n, s4);
   }
+  double s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
@@ -88,16 +137,62 @@ __global__ __launch_bounds__(256) void norm_join_kernel(const double* __restrict
   out2[1] = coef > 1.0 ? 1.f : (float)coef;       // a NaN norm stays NaN
 }
 
+template <int TI, int TO>
+__device__ __forceinline__ void scale_chunk(const void* in, void* out, long long base, int n, float k) {
+  typedef Elem<TI> I;
+  typedef Elem<TO> O;
+  constexpr int EV = I::EV, NV = CHUNK / (256 * EV);
+  const typename I::type* p = static_cast<const typename I::type*>(in) + base;
+  typename O::type* q = static_cast<typename O::type*>(out) + base;
+  if (n == CHUNK) {
+    u32x4 r[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) r[j] = *reinterpret_cast<const u32x4_u2*>(p + (j * 256 + threadIdx.x) * EV);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      typename O::type o[EV];
+#pragma unroll
+      for (int e = 0; e < EV; ++e) o[e] = O::cast(I::at(r[j], e) * k);
+      typename O::type* w = q + (j * 256 + threadIdx.x) * EV;
+      constexpr int BYTES = EV * (int)sizeof(o[0]);          // 8 (fp32 to half), 16 or 32 (half to fp32)
+      if (BYTES == 8) {
+        u32x2 v;
+        __builtin_memcpy(&v, o, 8);
+        *reinterpret_cast<u32x2_u2*>(w) = v;
+      } else {
+#pragma unroll
+        for (int h = 0; h < BYTES / 16; ++h) {
+          u32x4 v;
+          __builtin_memcpy(&v, reinterpret_cast<const char*>(o) + 16 * h, 16);
+          *reinterpret_cast<u32x4_u2*>(reinterpret_cast<char*>(w) + 16 * h) = v;
+        }
+      }
+    }
+  } else {
+    for (int i = threadIdx.x; i < n; i += 256) q[i] = O::cast(I::wide(p[i]) * k);
+  }
+}
+
+template <int TI>
+__device__ __forceinline__ void scale_to(int out_type, const void* in, void* out, long long base, int n, float k) {
+  if (out_type == DVAE_F32) scale_chunk<TI, DVAE_F32>(in, out, base, n, k);
+  else if (out_type == DVAE_BF16) scale_chunk<TI, DVAE_BF16>(in, out, base, n, k);
+  else scale_chunk<TI, DVAE_F16>(in, out, base, n, k);
+}
+
+// Chunks from the last to the first: the norm pass read the last ones last, so they are still in the 256 MB cache.
 __global__ __launch_bounds__(256) void scale_kernel(Batch b, const float* __restrict__ out2) {
   const float k = out2[1];
   const int chunks = b.start[b.count];
-  for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
-    const int t = tensor_of(b, c);
+  const Lookup tensor_of(b);
+  for (int c = chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
+    const int t = tensor_of(c);
     if (k == 1.f && b.in[t] == b.out[t]) continue;              // in place, nothing to clip
     const long long base = (long long)(c - b.start[t]) * CHUNK;
-    const long long end = min(base + CHUNK, b.n[t]);
-    for (long long i = base + threadIdx.x; i < end; i += 256)
-      store1(b.out[t], b.out_type[t], i, load1(b.in[t], b.in_type[t], i) * k);
+    const int n = (int)min((long long)CHUNK, b.n[t] - base);
+    if (b.in_type[t] == DVAE_F32) scale_to<DVAE_F32>(b.out_type[t], b.in[t], b.out[t], base, n, k);
+    else if (b.in_type[t] == DVAE_BF16) scale_to<DVAE_BF16>(b.out_type[t], b.in[t], b.out[t], base, n, k);
+    else scale_to<DVAE_F16>(b.out_type[t], b.in[t], b.out[t], base, n, k);
   }
 }
 
