@@ -10,7 +10,7 @@
 #include <new>
 #include <vector>
 
-#include "common.h"
+#include "elem.h"
 
 namespace {
 
@@ -27,38 +27,6 @@ struct Batch {
   int count;
 };
 static_assert(sizeof(Batch) <= 3584, "kernel arguments");
-
-typedef uint32_t u32x4_u2 __attribute__((ext_vector_type(4), aligned(2)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2_u2 __attribute__((ext_vector_type(2), aligned(2)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-
-template <int T> struct Elem;
-template <> struct Elem<DVAE_F32> {
-  typedef float type;
-  static constexpr int EV = 4;
-  static __device__ __forceinline__ float at(u32x4 r, int e) { return __uint_as_float(r[e]); }
-  static __device__ __forceinline__ float wide(float v) { return v; }
-  static __device__ __forceinline__ float cast(float v) { return v; }
-};
-template <> struct Elem<DVAE_BF16> {
-  typedef __bf16 type;
-  static constexpr int EV = 8;
-  static __device__ __forceinline__ float at(u32x4 r, int e) {
-    return __uint_as_float((e & 1) ? (r[e >> 1] & 0xffff0000u) : (r[e >> 1] << 16));
-  }
-  static __device__ __forceinline__ float wide(__bf16 v) { return (float)v; }
-  static __device__ __forceinline__ __bf16 cast(float v) { return (__bf16)v; }
-};
-template <> struct Elem<DVAE_F16> {
-  typedef _Float16 type;
-  static constexpr int EV = 8;
-  static __device__ __forceinline__ float at(u32x4 r, int e) {
-    return (float)__builtin_bit_cast(_Float16, (uint16_t)((e & 1) ? (r[e >> 1] >> 16) : (r[e >> 1] & 0xffffu)));
-  }
-  static __device__ __forceinline__ float wide(_Float16 v) { return (float)v; }
-  static __device__ __forceinline__ _Float16 cast(float v) { return (_Float16)v; }
-};
 
 // The tensor of a chunk: every lane of a wave holds two chunk starts, the wave counts those at or before the chunk -- no
 // search through memory between two chunks.
@@ -84,7 +52,7 @@ __device__ __forceinline__ void norm_chunk(const void* in, long long base, int n
   if (n == CHUNK) {
     u32x4 r[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) r[j] = *reinterpret_cast<const u32x4_u2*>(p + (j * 256 + threadIdx.x) * EV);
+    for (int j = 0; j < NV; ++j) r[j] = *reinterpret_cast<const u32x4_u*>(p + (j * 256 + threadIdx.x) * EV);
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -94,7 +62,7 @@ __device__ __forceinline__ void norm_chunk(const void* in, long long base, int n
       }
   } else {
     for (int i = threadIdx.x; i < n; i += 256) {
-      const double v = E::wide(p[i]);
+      const double v = E::one(p, i);
       s[0] = fma(v, v, s[0]);
     }
   }
@@ -147,7 +115,7 @@ __device__ __forceinline__ void scale_chunk(const void* in, void* out, long long
   if (n == CHUNK) {
     u32x4 r[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) r[j] = *reinterpret_cast<const u32x4_u2*>(p + (j * 256 + threadIdx.x) * EV);
+    for (int j = 0; j < NV; ++j) r[j] = *reinterpret_cast<const u32x4_u*>(p + (j * 256 + threadIdx.x) * EV);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       typename O::type o[EV];
@@ -158,18 +126,18 @@ __device__ __forceinline__ void scale_chunk(const void* in, void* out, long long
       if (BYTES == 8) {
         u32x2 v;
         __builtin_memcpy(&v, o, 8);
-        *reinterpret_cast<u32x2_u2*>(w) = v;
+        *reinterpret_cast<u32x2_u*>(w) = v;
       } else {
 #pragma unroll
         for (int h = 0; h < BYTES / 16; ++h) {
           u32x4 v;
           __builtin_memcpy(&v, reinterpret_cast<const char*>(o) + 16 * h, 16);
-          *reinterpret_cast<u32x4_u2*>(reinterpret_cast<char*>(w) + 16 * h) = v;
+          *reinterpret_cast<u32x4_u*>(reinterpret_cast<char*>(w) + 16 * h) = v;
         }
       }
     }
   } else {
-    for (int i = threadIdx.x; i < n; i += 256) q[i] = O::cast(I::wide(p[i]) * k);
+    for (int i = threadIdx.x; i < n; i += 256) q[i] = O::cast(I::one(p, i) * k);
   }
 }
 
@@ -196,8 +164,6 @@ __global__ __launch_bounds__(256) void scale_kernel(Batch b, const float* __rest
   }
 }
 
-int type_bytes(int t) { return t == DVAE_F32 ? 4 : 2; }
-
 struct Span { uintptr_t lo, hi; int tensor; bool write; };
 
 // no output may overlap another tensor; an input may be its own output
@@ -207,11 +173,11 @@ int check_tensors(const dvae_tensor* t, int n, bool write, const char* who) {
     DVAE_REQUIRE(t[i].n >= 0, "%s: tensor %d has %lld elements", who, i, t[i].n);
     DVAE_REQUIRE(t[i].in_type >= DVAE_F32 && t[i].in_type <= DVAE_F16, "%s: tensor %d has type %d", who, i, t[i].in_type);
     DVAE_REQUIRE(t[i].in || t[i].n == 0, "%s: tensor %d is null", who, i);
-    DVAE_REQUIRE((uintptr_t)t[i].in % type_bytes(t[i].in_type) == 0, "%s: tensor %d is not aligned to its type", who, i);
+    DVAE_REQUIRE((uintptr_t)t[i].in % elem_bytes(t[i].in_type) == 0, "%s: tensor %d is not aligned to its type", who, i);
     if (!write) continue;
     DVAE_REQUIRE(t[i].out_type >= DVAE_F32 && t[i].out_type <= DVAE_F16, "%s: output %d has type %d", who, i, t[i].out_type);
     DVAE_REQUIRE(t[i].out || t[i].n == 0, "%s: output %d is null", who, i);
-    DVAE_REQUIRE((uintptr_t)t[i].out % type_bytes(t[i].out_type) == 0, "%s: output %d is not aligned to its type", who, i);
+    DVAE_REQUIRE((uintptr_t)t[i].out % elem_bytes(t[i].out_type) == 0, "%s: output %d is not aligned to its type", who, i);
     DVAE_REQUIRE(t[i].n == 0 || t[i].in != t[i].out || t[i].in_type == t[i].out_type, "%s: tensor %d is its own output in another type", who, i);
   }
   if (!write) return DVAE_OK;
@@ -221,8 +187,8 @@ int check_tensors(const dvae_tensor* t, int n, bool write, const char* who) {
     for (int i = 0; i < n; ++i) {
       if (t[i].n == 0) continue;
       const uintptr_t o = (uintptr_t)t[i].out, p = (uintptr_t)t[i].in;
-      v.push_back({o, o + (uintptr_t)t[i].n * type_bytes(t[i].out_type), i, true});
-      if (p != o) v.push_back({p, p + (uintptr_t)t[i].n * type_bytes(t[i].in_type), i, false});
+      v.push_back({o, o + (uintptr_t)t[i].n * elem_bytes(t[i].out_type), i, true});
+      if (p != o) v.push_back({p, p + (uintptr_t)t[i].n * elem_bytes(t[i].in_type), i, false});
     }
     std::sort(v.begin(), v.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
     // the farthest end seen so far, of any span and of the written ones

@@ -18,54 +18,17 @@
 // among the elements whose rounded value is the largest; those few are compared by the part the rounding dropped
 // (two-sum; for counted ones double minus the rounded value).  A drawn token is decided where a running sum over the
 // whole vocabulary crosses u Z, and with thousands of probable tokens a border of fp32 sums lies within their rounding of
-// u Z for a few percent of the rows: its weights and sums are doubles, with an exp2 of 1e-12.
+// u Z for a few percent of the rows: its weights and sums are doubles, with an exp2 of 4e-14.
 #include <algorithm>
 #include <cmath>
 
+#include "elem.h"
 #include "rules.h"
 
 namespace {
 
 constexpr double LOG2E = 1.4426950408889634074;
 constexpr double LN2 = 0.69314718055994530942;
-
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-// rows start at any element (an odd vocabulary, a padded matrix): 16-byte accesses at the element's alignment
-typedef uint32_t u32x4_u2 __attribute__((ext_vector_type(4), aligned(2)));
-typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
-
-template <int T> struct Elem;
-template <> struct Elem<DVAE_F32> {
-  typedef float type;
-  static constexpr int EV = 4;
-  static __device__ __forceinline__ float at(u32x4 r, int e) { return __uint_as_float(r[e]); }
-  static __device__ __forceinline__ float one(const void* p, long long i) { return static_cast<const float*>(p)[i]; }
-  static __device__ __forceinline__ float cast(float v) { return v; }
-};
-template <> struct Elem<DVAE_BF16> {
-  typedef __bf16 type;
-  static constexpr int EV = 8;
-  static __device__ __forceinline__ float at(u32x4 r, int e) {
-    const uint32_t w = r[e >> 1];
-    return __uint_as_float((e & 1) ? (w & 0xffff0000u) : (w << 16));
-  }
-  static __device__ __forceinline__ float one(const void* p, long long i) {
-    return __uint_as_float((uint32_t)static_cast<const uint16_t*>(p)[i] << 16);
-  }
-  static __device__ __forceinline__ __bf16 cast(float v) { return (__bf16)v; }
-};
-template <> struct Elem<DVAE_F16> {
-  typedef _Float16 type;
-  static constexpr int EV = 8;
-  static __device__ __forceinline__ float at(u32x4 r, int e) {
-    const uint16_t h = (uint16_t)((e & 1) ? (r[e >> 1] >> 16) : (r[e >> 1] & 0xffffu));
-    return (float)__builtin_bit_cast(_Float16, h);
-  }
-  static __device__ __forceinline__ float one(const void* p, long long i) {
-    return (float)static_cast<const _Float16*>(p)[i];
-  }
-  static __device__ __forceinline__ _Float16 cast(float v) { return (_Float16)v; }
-};
 
 // what a wave knows about its row
 struct RowP {
@@ -145,25 +108,32 @@ __device__ __forceinline__ double wave_sum(double v) {
   return v;
 }
 
-// 2^(d k) in double, d k up to 1000: a = n + f, |f| <= 1/2, 2^f by its series in f ln 2 up to the 10th power (the first
-// term left out is (ln 2 / 2)^11 / 11! = 2.2e-13 of the result).  Below 2^-1000 the weight is 0.
+// 2^(d k) in double for d k from -1000 (`low` = -1000 / k; what lies below counts as 2^-1000) to 1000: a = d k = n + f,
+// |f| <= 1/2; n by adding 1.5 2^52, which leaves it in the low bits; 2^f as 1 + f q(f), q the polynomial that
+// meets (2^f - 1) / f in the nine Chebyshev nodes of [-1/2, 1/2] (off by at most 3.7e-14 of the result, exact at 0); n goes into the exponent by an integer addition.
+// 15 operations of full rate: the accurate exp of the math library and its branches took three times as long.
+__device__ __forceinline__ double exp2_fast(double d, double k, double low) {
+  constexpr double SHIFT = 6755399441055744.0;
+  d = fmax(d, low);
+  const double t = fma(d, k, SHIFT);
+  const double f = fma(d, k, -(t - SHIFT));
+  double y = 1.0203121138901363e-07;
+  y = fma(y, f, 1.325522487892511e-06);
+  y = fma(y, f, 1.525268684597521e-05);
+  y = fma(y, f, 0.00015403455852451678);
+  y = fma(y, f, 0.0013333558179043376);
+  y = fma(y, f, 0.009618129159402562);
+  y = fma(y, f, 0.055504108664760424);
+  y = fma(y, f, 0.2402265069581299);
+  y = fma(y, f, 0.6931471805599453);
+  y = fma(y, f, 1.0);
+  return __hiloint2double(__double2hiint(y) + (__double2loint(t) << 20), __double2loint(y));
+}
+
+// the same, 0 below 2^-1000 and NaN for NaN
 __device__ __forceinline__ double exp2_64(double d, double k) {
-  const double a = d * k;
-  if (!(a >= -1000.0)) return a != a ? a : 0.0;
-  const double n = rint(a);
-  const double f = (a - n) * LN2;
-  double y = 1.0 / 3628800.0;
-  y = fma(y, f, 1.0 / 362880.0);
-  y = fma(y, f, 1.0 / 40320.0);
-  y = fma(y, f, 1.0 / 5040.0);
-  y = fma(y, f, 1.0 / 720.0);
-  y = fma(y, f, 1.0 / 120.0);
-  y = fma(y, f, 1.0 / 24.0);
-  y = fma(y, f, 1.0 / 6.0);
-  y = fma(y, f, 0.5);
-  y = fma(y, f, 1.0);
-  y = fma(y, f, 1.0);
-  return ldexp(y, (int)n);
+  const double a = d * k, w = exp2_fast(d, k, -1000.0 / k);
+  return a != a ? a : a < -1000.0 ? 0.0 : w;
 }
 
 // what a segment leaves for the join
@@ -228,7 +198,7 @@ __device__ __forceinline__ void count_history(const RowP& p, int i64, long long 
 template <int T>
 __device__ __forceinline__ u32x4 load_logits(const char* lrow, int v, int V) {
   constexpr int EV = Elem<T>::EV, BYTES = 16 / EV;
-  if (v + EV <= V) return *reinterpret_cast<const u32x4_u2*>(lrow + (size_t)v * BYTES);
+  if (v + EV <= V) return *reinterpret_cast<const u32x4_u*>(lrow + (size_t)v * BYTES);
   u32x4 r = {0, 0, 0, 0};
 #pragma unroll
   for (int e = 0; e < EV; ++e)
@@ -239,7 +209,17 @@ __device__ __forceinline__ u32x4 load_logits(const char* lrow, int v, int V) {
   return r;
 }
 
-// EV tokens from v on, d their place among the counts
+// a step's loads, begun one step ahead: its logits and its byte of the mask
+struct Loaded { u32x4 raw; uint32_t byte; };
+template <int T>
+__device__ __forceinline__ Loaded load_step(const RowP& p, const char* lrow, int v, int V) {
+  Loaded l;
+  l.raw = load_logits<T>(lrow, v, V);
+  l.byte = p.mask ? p.mask[v >> 3] : 0xffu;
+  return l;
+}
+
+// EV tokens from v < V on, d their place among the counts
 template <int T, int HIST>
 struct Ruled {
   typedef Elem<T> E;
@@ -247,12 +227,10 @@ struct Ruled {
   float x[EV], b[EV];
   uint32_t c[EV];
   uint32_t keep;                // bit e: allowed (and inside the vocabulary)
-  __device__ __forceinline__ Ruled(const RowP& p, u32x4 raw, const uint32_t* cnt, int v, int d, int V) {
-    keep = v + EV <= V ? (1u << EV) - 1 : v < V ? (1u << (V - v)) - 1 : 0u;
-    if (p.mask && v < V) {
-      const uint32_t byte = p.mask[v >> 3];
-      keep &= EV == 8 ? byte : byte >> (v & 4);
-    }
+  __device__ __forceinline__ Ruled(const RowP& p, const Loaded& in, const uint32_t* cnt, int v, int d, int V) {
+    const u32x4 raw = in.raw;
+    keep = v + EV <= V ? (1u << EV) - 1 : (1u << (V - v)) - 1;
+    keep &= EV == 8 ? in.byte : in.byte >> (v & 4);
 #pragma unroll
     for (int e = 0; e < EV; ++e) { x[e] = E::at(raw, e); b[e] = 0.f; c[e] = 0; }
     if (p.bias) {
@@ -339,8 +317,12 @@ __global__ __launch_bounds__(256) void rules_seg_kernel(SegArgs a) {
       zero = tok < 0 || tok >= V || m == -INFINITY;      // an ignored row, or one whose rules leave nothing
     }
     const float up = (float)p.rho, down = (float)p.inv_rho;
+    Loaded ahead;
+    if (v0 + lane * EV < end) ahead = load_step<T>(p, lrow, v0 + lane * EV, V);
     for (int v = v0 + lane * EV; v < end; v += STEP) {
-      const Ruled<T, HIST> r(p, load_logits<T>(lrow, v, V), cnt, v, v - v0, V);
+      const Loaded in = ahead;
+      if (v + STEP < end) ahead = load_step<T>(p, lrow, v + STEP, V);
+      const Ruled<T, HIST> r(p, in, cnt, v, v - v0, V);
       typename E::type o[EV];
 #pragma unroll
       for (int e = 0; e < EV; ++e) {
@@ -357,7 +339,7 @@ __global__ __launch_bounds__(256) void rules_seg_kernel(SegArgs a) {
       if (v + EV <= V) {
         u32x4 w;
         __builtin_memcpy(&w, o, 16);
-        *reinterpret_cast<u32x4_u2*>(orow + v) = w;
+        *reinterpret_cast<u32x4_u*>(orow + v) = w;
       } else {
 #pragma unroll
         for (int e = 0; e < EV; ++e)
@@ -373,8 +355,13 @@ __global__ __launch_bounds__(256) void rules_seg_kernel(SegArgs a) {
   const float room = ROOM / kf;
   float ref = -3.402823466e38f, lim = ref, m = -INFINITY, z = 0.f;
   double zd = 0.0;
+  const double low = -1000.0 / p.k;
+  Loaded ahead;
+  if (v0 + lane * EV < end) ahead = load_step<T>(p, lrow, v0 + lane * EV, V);
   for (int v = v0 + lane * EV; v < end; v += STEP) {
-    const Ruled<T, HIST> r(p, load_logits<T>(lrow, v, V), cnt, v, v - v0, V);
+    const Loaded in = ahead;
+    if (v + STEP < end) ahead = load_step<T>(p, lrow, v + STEP, V);
+    const Ruled<T, HIST> r(p, in, cnt, v, v - v0, V);
     float s[EV];
 #pragma unroll
     for (int e = 0; e < EV; ++e) s[e] = r.value(p, e);
@@ -388,10 +375,17 @@ __global__ __launch_bounds__(256) void rules_seg_kernel(SegArgs a) {
       ref = mx;
       lim = ref + room;
     }
+    if (MODE == M_DRAW) {
+      if (!HIST && !p.bias) {          // the fp32 values are exact
 #pragma unroll
-    for (int e = 0; e < EV; ++e) {
-      if (MODE == M_DRAW) zd += exp2_64(r.value64(p, e) - (double)ref, p.k);
-      else z += __builtin_amdgcn_exp2f((s[e] - ref) * kf);
+        for (int e = 0; e < EV; ++e) zd += exp2_fast((double)s[e] - (double)ref, p.k, low);
+      } else {
+#pragma unroll
+        for (int e = 0; e < EV; ++e) zd += exp2_fast(r.value64(p, e) - (double)ref, p.k, low);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < EV; ++e) z += __builtin_amdgcn_exp2f((s[e] - ref) * kf);
     }
   }
   m = wave_max_nan(m);
@@ -448,149 +442,195 @@ __device__ __forceinline__ double block_prefix(double v, double* sh, double& tot
   return before + (x - v);
 }
 
+constexpr int HIST_STAGE = 4096;       // tokens of a history that the join keeps in LDS
+
+// value of one token in 64 bits, -inf where the grammar forbids it
+template <int T>
+__device__ __forceinline__ double token_value(const Rules& q, const RowP& p, long long row, int v, uint32_t c) {
+  if (p.mask && !((p.mask[v >> 3] >> (v & 7)) & 1)) return -INFINITY;
+  const float x = Elem<T>::one(q.logits, row * q.ld + v), b = p.bias ? p.bias[v] : 0.f;
+  return c ? counted64(p, x, c, b) : (double)x + (double)b;
+}
+
+// One workgroup a row.  What it reads depends on what it has read (partials, then the segment they point to), so the
+// loads that do not -- the history, a given token's logit -- are begun first, and the partials stay in registers.
 template <int T, int MODE>
 __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
-  typedef Elem<T> E;
+  constexpr bool SEARCH = MODE != M_SUM;
   __shared__ double shd[4];
   __shared__ float shf[4];
   __shared__ int shi[4];
-  __shared__ int pick_seg;
   __shared__ double pick_before;
-  __shared__ uint32_t cnt[SEG_MAX];         // counts of the segment that is searched
+  __shared__ int hist[SEARCH ? HIST_STAGE : 1];
+  __shared__ uint32_t cnt[SEARCH ? SEG_MAX : 1];      // counts of the segment that is searched
   const Rules& q = a.q;
   const long long row = blockIdx.x;
-  const int V = q.vocab, tid = threadIdx.x;
+  const int V = q.vocab, tid = threadIdx.x, n = a.seg_len;
   const RowP p = row_params(q, row);
   const Seg* seg = a.seg + row * a.nseg;
-  const typename E::type* lrow = static_cast<const typename E::type*>(q.logits) + row * q.ld;
 
-  float m = -INFINITY;
-  for (int i = tid; i < a.nseg; i += 256) m = max_nan(m, seg[i].m);
-  m = block_reduce(m, shf, [](float x, float y) { return max_nan(x, y); });
-  // a temperature that is not positive and finite makes the row NaN, as a NaN logit does
-  const bool ok = m > -INFINITY && m < INFINITY && p.k > 0.0 && p.k < INFINITY;
-  double z = 0.0;
   // contiguous shares, so that running sums follow the vocabulary's order
   const int per = (a.nseg + 255) / 256;
   const int i0 = min(tid * per, a.nseg), i1 = min(i0 + per, a.nseg);
-  if (ok)
-    for (int i = i0; i < i1; ++i)
-      if (seg[i].m > -INFINITY) z += seg[i].s * exp2_64((double)seg[i].m - (double)m, p.k);
+  Seg mine;
+  mine.s = 0.0; mine.m = -INFINITY; mine.pad = 0;
+  if (i0 < i1) mine = seg[i0];
+
+  long long tok = -1;
+  double given_y = 0.0;
+  int c = 0;
+  if (SEARCH) {
+    for (int i = tid; i < min(p.n_hist, HIST_STAGE); i += 256) {
+      const long long t = hist_at(p, q.history_i64, i);
+      hist[i] = t >= 0 && t < V ? (int)t : -1;
+    }
+  } else {
+    tok = a.given[row];
+    if (tok >= 0 && tok < V) {
+      for (int i = tid; i < p.n_hist; i += 256) c += hist_at(p, q.history_i64, i) == tok;
+      if (p.n_hist) c = block_reduce(c, shi, [](int x, int y) { return x + y; });
+      given_y = token_value<T>(q, p, row, (int)tok, c);
+    }
+  }
+
+  float m = mine.m;
+  for (int i = i0 + 1; i < i1; ++i) m = max_nan(m, seg[i].m);
+  m = block_reduce(m, shf, [](float x, float y) { return max_nan(x, y); });
+  // a temperature that is not positive and finite makes the row NaN, as a NaN logit does
+  const bool ok = m > -INFINITY && m < INFINITY && p.k > 0.0 && p.k < INFINITY;
+  const auto scaled = [&](const Seg& s) { return s.m > -INFINITY ? s.s * exp2_64((double)s.m - (double)m, p.k) : 0.0; };
+  double z0 = 0.0, z = 0.0;
+  if (ok) {
+    z0 = scaled(mine);
+    z = z0;
+    for (int i = i0 + 1; i < i1; ++i) z += scaled(seg[i]);
+  }
   double Z;
   const double before = block_prefix(z, shd, Z);
 
-  long long tok = -1;
+  const auto finish = [&](long long t, double y) {
+    float lp = -INFINITY;
+    if (MODE == M_SUM && !(t >= 0 && t < V)) lp = 0.f;          // an ignored row
+    else if (m == -INFINITY) lp = -INFINITY;                    // the rules leave nothing
+    else if (!ok || t < 0) lp = NAN;                            // NaN or +inf among the allowed values (or a NaN u)
+    else lp = (float)((y - (double)m) * (p.k * LN2) - log(Z));
+    a.logprob[row] = lp;
+    if (MODE == M_SUM) {
+      a.stat[2 * row] = m == -INFINITY || ok ? m : NAN;
+      a.stat[2 * row + 1] = ok ? (float)(1.0 / Z) : NAN;
+    } else {
+      a.tokens[row] = t;
+      if (a.state_out) {
+        const int s = q.state[row];
+        a.state_out[row] = t >= 0 && s >= 0 && s < q.states ? a.next[(size_t)s * V + t] : s;
+      }
+    }
+  };
   if (MODE == M_SUM) {
-    tok = a.given[row];
-  } else if (ok && MODE == M_GREEDY) {
+    if (tid == 0) finish(tok, given_y);
+    return;
+  }
+  const float uf = MODE == M_DRAW ? a.uniforms[row] : 0.f;
+  if (!ok || uf != uf) {
+    if (tid == 0) finish(-1, 0.0);
+    return;
+  }
+  // counts of the tokens [v0, v0 + n)
+  const auto count = [&](int v0) {
+    for (int i = tid; i < n; i += 256) cnt[i] = 0;
+    __syncthreads();
+    const int staged = min(p.n_hist, HIST_STAGE);
+    for (int i = tid; i < staged; i += 256) {
+      const int d = hist[i] - v0;
+      if (hist[i] >= 0 && d >= 0 && d < n) atomicAdd(&cnt[d], 1u);
+    }
+    for (int i = staged + tid; i < p.n_hist; i += 256) {
+      const long long d = hist_at(p, q.history_i64, i) - v0;
+      if ((unsigned long long)d < (unsigned long long)n) atomicAdd(&cnt[(int)d], 1u);
+    }
+    __syncthreads();
+  };
+
+  if (MODE == M_GREEDY) {
     // the largest value's segments (hardly ever more than one), and in them the elements that round to it: among those
     // the largest dropped part, then the lowest index
     float lo = -INFINITY;
     int idx = INT32_MAX;
-    const int n = a.seg_len;
-    for (int i = 0; i < a.nseg; ++i) {
-      if (seg[i].m != m) continue;
-      const int v0 = i * n;
-      for (int e = tid; e < n; e += 256) cnt[e] = 0;
-      __syncthreads();
-      count_history<2>(p, q.history_i64, v0, n, cnt, tid, 256);
-      __syncthreads();
-      for (int e = tid; e < n; e += 256) {
-        const int v = v0 + e;
-        if (v >= V || (p.mask && !((p.mask[v >> 3] >> (v & 7)) & 1))) continue;
-        const float x = E::one(lrow, v), b = p.bias ? p.bias[v] : 0.f;
-        const double y = cnt[e] ? counted64(p, x, cnt[e], b) : (double)x + (double)b;
+    double best_y = 0.0;
+    int from = 0;
+    while (true) {
+      int g = mine.m == m && i0 >= from ? i0 : INT32_MAX;
+      for (int i = i0 + 1; i < i1; ++i)
+        if (i >= from && i < g && seg[i].m == m) g = i;
+      g = block_reduce(g, shi, [](int x, int y) { return min(x, y); });
+      if (g == INT32_MAX) break;
+      from = g + 1;
+      const int v0 = g * n;
+      count(v0);
+      for (int e = tid; e < n && v0 + e < V; e += 256) {
+        const double y = token_value<T>(q, p, row, v0 + e, cnt[e]);
         if ((float)y != m) continue;
         const float l = (float)(y - (double)m);
-        if (l > lo || (l == lo && v < idx)) { lo = l; idx = v; }
+        if (l > lo || (l == lo && v0 + e < idx)) { lo = l; idx = v0 + e; best_y = y; }
       }
       __syncthreads();
     }
     const float best = block_reduce(lo, shf, [](float x, float y) { return fmaxf(x, y); });
-    tok = block_reduce(lo == best ? idx : INT32_MAX, shi, [](int x, int y) { return min(x, y); });
-  } else if (ok && MODE == M_DRAW) {
-    const float uf = a.uniforms[row];
-    const double t = fmax((double)uf, 0.0) * Z;
-    if (uf == uf) {
-      // the segment where the running sum passes t; beyond the end (u >= 1, or rounding): the last one with a weight
-      int first = INT32_MAX, last = -1;
-      double run = before, first_before = 0.0, last_before = 0.0;
-      for (int i = i0; i < i1; ++i) {
-        if (!(seg[i].m > -INFINITY)) continue;
-        const double w = seg[i].s * exp2_64((double)seg[i].m - (double)m, p.k);
-        if (w > 0.0) { last = i; last_before = run; }
-        if (run + w > t && first == INT32_MAX) { first = i; first_before = run; }
-        run += w;
-      }
-      const int f = block_reduce(first, shi, [](int x, int y) { return min(x, y); });
-      const int l = block_reduce(last, shi, [](int x, int y) { return max(x, y); });
-      const int g = f != INT32_MAX ? f : l;
-      if (threadIdx.x == 0) pick_seg = 0;
-      __syncthreads();
-      if (g >= i0 && g < i1) {
-        pick_seg = g;
-        pick_before = f != INT32_MAX ? first_before : last_before;
-      }
-      const int n = a.seg_len;
-      for (int i = tid; i < n; i += 256) cnt[i] = 0;
-      __syncthreads();
-      const int v0 = pick_seg * n;
-      const double base = pick_before;
-      count_history<2>(p, q.history_i64, v0, n, cnt, tid, 256);
-      __syncthreads();
-      // weights of the segment's tokens, thread by thread in order
-      const int own = n / 256;
-      double mine = 0.0;
-      const auto weight = [&](int d) -> double {
-        const int v = v0 + d;
-        if (v >= V || (p.mask && !((p.mask[v >> 3] >> (v & 7)) & 1))) return 0.0;
-        const float x = E::one(lrow, v), b = p.bias ? p.bias[v] : 0.f;
-        const double y = cnt[d] ? counted64(p, x, cnt[d], b) : (double)x + (double)b;
-        return exp2_64(y - (double)m, p.k);
-      };
-      for (int e = 0; e < own; ++e) mine += weight(tid * own + e);
-      double dummy;
-      double run2 = base + block_prefix(mine, shd, dummy);
-      int hit = INT32_MAX, tail = -1;
-      for (int e = 0; e < own; ++e) {
-        const double w = weight(tid * own + e);
-        run2 += w;
-        if (w > 0.0) tail = v0 + tid * own + e;
-        if (w > 0.0 && run2 > t && hit == INT32_MAX) hit = v0 + tid * own + e;
-      }
-      hit = block_reduce(hit, shi, [](int x, int y) { return min(x, y); });
-      tail = block_reduce(tail, shi, [](int x, int y) { return max(x, y); });
-      tok = g < 0 ? -1 : hit != INT32_MAX ? hit : tail;
-    }
+    const int t = block_reduce(lo == best ? idx : INT32_MAX, shi, [](int x, int y) { return min(x, y); });
+    if (idx == t) finish(t, best_y);
+    return;
   }
 
-  // the token's value: its count, then the formula
-  const bool have = tok >= 0 && tok < V;
-  int c = 0;
-  if (have)
-    for (int i = tid; i < p.n_hist; i += 256) c += hist_at(p, q.history_i64, i) == tok;
-  c = block_reduce(c, shi, [](int x, int y) { return x + y; });
-  if (tid) return;
-  float lp = -INFINITY;
-  if (MODE == M_SUM && !have) lp = 0.f;                         // an ignored row
-  else if (m == -INFINITY) lp = -INFINITY;                      // the rules leave nothing (never drawn from)
-  else if (!ok || !have) lp = NAN;                              // NaN or +inf among the allowed values (or a NaN u)
-  else if (!(p.mask && !((p.mask[tok >> 3] >> (tok & 7)) & 1))) {
-    const float x = E::one(lrow, tok), b = p.bias ? p.bias[tok] : 0.f;
-    const double y = c ? counted64(p, x, c, b) : (double)x + (double)b;
-    lp = (float)((y - (double)m) * (p.k * LN2) - log(Z));
+  // the segment where the running sum passes u Z; beyond the end (u >= 1, or rounding): the last one with a weight
+  const double edge = fmax((double)uf, 0.0) * Z;
+  int first = INT32_MAX, last = -1;
+  double first_before = 0.0, last_before = 0.0, run = before;
+  for (int i = i0; i < i1; ++i) {
+    const double w = i == i0 ? z0 : scaled(seg[i]);
+    if (w > 0.0) { last = i; last_before = run; }
+    if (run + w > edge && first == INT32_MAX) { first = i; first_before = run; }
+    run += w;
   }
-  a.logprob[row] = lp;
-  if (MODE == M_SUM) {
-    a.stat[2 * row] = m == -INFINITY || ok ? m : NAN;
-    a.stat[2 * row + 1] = ok ? (float)(1.0 / Z) : NAN;
-  } else {
-    a.tokens[row] = tok;
-    if (a.state_out) {
-      const int s = q.state[row];
-      a.state_out[row] = tok >= 0 && s >= 0 && s < q.states ? a.next[(size_t)s * V + tok] : s;
+  const int f = block_reduce(first, shi, [](int x, int y) { return min(x, y); });
+  int g = f;
+  if (f == INT32_MAX) g = block_reduce(last, shi, [](int x, int y) { return max(x, y); });
+  if (g < 0) {      // no weight at all: not with a finite maximum
+    if (tid == 0) finish(-1, 0.0);
+    return;
+  }
+  if (g >= i0 && g < i1) {
+    pick_before = f != INT32_MAX ? first_before : last_before;
+  }
+  const int v0 = g * n;
+  count(v0);
+  // weights of the segment's tokens, thread by thread in order
+  constexpr int OWN = SEG_MAX / 256;
+  const int own = n / 256, d0 = tid * own;
+  double w[OWN], sum = 0.0;
+#pragma unroll
+  for (int e = 0; e < OWN; ++e) {
+    w[e] = 0.0;
+    if (e < own && v0 + d0 + e < V) w[e] = exp2_64(token_value<T>(q, p, row, v0 + d0 + e, cnt[d0 + e]) - (double)m, p.k);
+    sum += w[e];
+  }
+  double all;
+  double at = pick_before + block_prefix(sum, shd, all);
+  int hit = INT32_MAX, tail = -1;
+#pragma unroll
+  for (int e = 0; e < OWN; ++e) {
+    at += w[e];
+    if (w[e] > 0.0) {
+      tail = v0 + d0 + e;
+      if (at > edge && hit == INT32_MAX) hit = v0 + d0 + e;
     }
   }
+  int t = block_reduce(hit, shi, [](int x, int y) { return min(x, y); });
+  if (t == INT32_MAX) t = block_reduce(tail, shi, [](int x, int y) { return max(x, y); });
+  if (t < 0) {
+    if (tid == 0) finish(-1, 0.0);
+    return;
+  }
+  if (t - v0 >= d0 && t - v0 < d0 + own) finish(t, token_value<T>(q, p, row, t, cnt[t - v0]));
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -807,8 +847,6 @@ constexpr long long MAX_BLOCKS = (1ll << 24) - 1;     // blocks x 256 threads st
 
 struct Plan { int seg_len, nseg, wgs_per_row; bool row_wave; long long blocks; };
 
-int elem_bytes(int dtype) { return dtype == DVAE_F32 ? 4 : 2; }
-
 Rules with_constants(const dvae_rules& q) {
   Rules r;
   static_cast<dvae_rules&>(r) = q;
@@ -820,7 +858,9 @@ Rules with_constants(const dvae_rules& q) {
 Plan plan_of(const dvae_rules& q) {
   Plan p;
   const int step = 64 * (16 / elem_bytes(q.dtype));      // tokens of a wave's step
-  p.seg_len = (int)std::min<long long>(SEG_MAX, ((long long)q.vocab + step - 1) / step * step);
+  // segments as long as 4096 waves (four for each SIMD) leave them: few rows are spread over the whole card
+  p.seg_len = step;
+  while (p.seg_len < SEG_MAX && p.seg_len < q.vocab && q.rows * ((q.vocab + p.seg_len - 1) / p.seg_len) > 4096) p.seg_len *= 2;
   p.nseg = (int)(((long long)q.vocab + p.seg_len - 1) / p.seg_len);
   p.row_wave = p.nseg == 1;
   p.wgs_per_row = (p.nseg + 3) / 4;
