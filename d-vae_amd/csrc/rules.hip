@@ -21,6 +21,7 @@
 // u Z for a few percent of the rows: its weights and sums are doubles, with an exp2 of 4e-14.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "elem.h"
 #include "rules.h"
@@ -32,12 +33,20 @@ constexpr double LN2 = 0.69314718055994530942;
 
 // what a wave knows about its row
 struct RowP {
-  double rho, inv_rho, freq, pres, k;      // k = log2(e) / T
+  double rho, inv_rho, freq, pres, temp, k;      // k = log2(e) / T
   const uint8_t* mask;            // packed bits of the row's grammar state, or NULL: everything allowed
   const float* bias;              // or NULL
   const char* hist;               // the row's history
   int n_hist;
 };
+
+// 1 / v to the last bits: the hardware's approximation and two Newton steps (no infinities or zeros inside: those rows
+// are refused by their k)
+__device__ __forceinline__ double reciprocal(double v) {
+  double r = __builtin_amdgcn_rcp(v);
+  r = fma(fma(-v, r, 1.0), r, r);
+  return fma(fma(-v, r, 1.0), r, r);
+}
 
 // one setting for all rows: its quotients are formed on the host
 struct Rules : dvae_rules {
@@ -50,11 +59,16 @@ __device__ __forceinline__ RowP row_params(const Rules& q, long long r) {
   p.inv_rho = q.inv_rho;
   if (q.repetition_rows) {
     p.rho = q.repetition_rows[r];
-    p.inv_rho = 1.0 / p.rho;
+    p.inv_rho = reciprocal(p.rho);
   }
   p.freq = q.frequency_rows ? (double)q.frequency_rows[r] : q.frequency;
   p.pres = q.presence_rows ? (double)q.presence_rows[r] : q.presence;
-  p.k = q.temperature_rows ? LOG2E / (double)q.temperature_rows[r] : q.k;
+  p.temp = q.temperature;
+  p.k = q.k;
+  if (q.temperature_rows) {
+    p.temp = q.temperature_rows[r];
+    p.k = LOG2E * reciprocal(p.temp);
+  }
   p.bias = q.bias ? q.bias + r * q.bias_ld : nullptr;
   p.mask = nullptr;
   if (q.mask) {
@@ -84,7 +98,7 @@ __device__ __forceinline__ double counted64(const RowP& p, float x, uint32_t c, 
   double v = xd * p.inv_rho;
   v = fma(fma(-v, p.rho, xd), p.inv_rho, v);
   v = x > 0.f ? v : xd * p.rho;
-  v -= p.freq * (double)c;
+  v = fma(-p.freq, (double)c, v);        // one operation everywhere: two kernels compute a value and have to agree
   v -= p.pres;
   return v + (double)b;
 }
@@ -132,15 +146,16 @@ __device__ __forceinline__ double exp2_fast(double d, double k, double low) {
 
 // the same, 0 below 2^-1000 and NaN for NaN
 __device__ __forceinline__ double exp2_64(double d, double k) {
-  const double a = d * k, w = exp2_fast(d, k, -1000.0 / k);
+  const double a = d * k;
+  const double w = exp2_fast(a < -1000.0 ? 0.0 : d, k, -INFINITY);
   return a != a ? a : a < -1000.0 ? 0.0 : w;
 }
 
 // what a segment leaves for the join
 struct Seg {
-  double s;       // sum of 2^((x4 - m) k)
+  double s;       // sum of 2^((x4 - ref) k)
   float m;        // maximum (NaN when an allowed value is)
-  int pad;
+  float ref;
 };
 
 enum { M_APPLY = 0, M_SUM = 1, M_GREEDY = 2, M_DRAW = 3, M_BWD = 4 };
@@ -165,76 +180,95 @@ template <> struct Counts<1> { static constexpr int PER_WORD = 2; };
 template <> struct Counts<2> { static constexpr int PER_WORD = 1; };
 
 template <int HIST>
-__device__ __forceinline__ void count_one(uint32_t* lds, int d) {
-  if (HIST == 1) atomicAdd(&lds[d >> 1], (d & 1) ? 0x10000u : 1u);
-  else atomicAdd(&lds[d], 1u);
-}
-template <int HIST>
 __device__ __forceinline__ uint32_t count_at(const uint32_t* lds, int d) {
   if (HIST == 1) return (lds[d >> 1] >> ((d & 1) * 16)) & 0xffffu;
   return lds[d];
 }
 
-// adds the history's tokens in [v0, v0 + span) to lds; `lane` of `width` threads
+// adds the history's tokens in [v0, v0 + span) to lds and, if there is one, marks them in the bitmap; `lane` of `width`
+// threads
 template <int HIST>
-__device__ __forceinline__ void count_history(const RowP& p, int i64, long long v0, int span, uint32_t* lds, int lane,
-                                              int width) {
+__device__ __forceinline__ void count_history(const RowP& p, int i64, long long v0, int span, uint32_t* lds, uint32_t* bits,
+                                              int lane, int width) {
+  const auto add = [&](long long t) {
+    if ((unsigned long long)t < (unsigned long long)span) {
+      const int d = (int)t;
+      if (HIST == 1) atomicAdd(&lds[d >> 1], (d & 1) ? 0x10000u : 1u);
+      else atomicAdd(&lds[d], 1u);
+      if (bits) atomicOr(&bits[d >> 5], 1u << (d & 31));
+    }
+  };
   int i = lane;
   for (; i + 3 * width < p.n_hist; i += 4 * width) {
     long long t[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) t[u] = hist_at(p, i64, i + u * width) - v0;
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if ((unsigned long long)t[u] < (unsigned long long)span) count_one<HIST>(lds, (int)t[u]);
+    for (int u = 0; u < 4; ++u) add(t[u]);
   }
-  for (; i < p.n_hist; i += width) {
-    const long long t = hist_at(p, i64, i) - v0;
-    if ((unsigned long long)t < (unsigned long long)span) count_one<HIST>(lds, (int)t);
-  }
+  for (; i < p.n_hist; i += width) add(hist_at(p, i64, i) - v0);
 }
 
-// 16 bytes of logits from token v on; past the vocabulary zeros
+// A step of a wave: 64 x EV tokens, from v on in this lane.  Every step but a row's last is whole in every lane (`whole`, the
+// same for the wave): no bounds in it.
+struct Loaded { u32x4 raw; uint32_t keep; };       // keep, bit e: allowed (and inside the vocabulary)
+
 template <int T>
-__device__ __forceinline__ u32x4 load_logits(const char* lrow, int v, int V) {
+__device__ __forceinline__ Loaded load_step(const RowP& p, const char* lrow, int v, int V, bool whole) {
   constexpr int EV = Elem<T>::EV, BYTES = 16 / EV;
-  if (v + EV <= V) return *reinterpret_cast<const u32x4_u*>(lrow + (size_t)v * BYTES);
-  u32x4 r = {0, 0, 0, 0};
-#pragma unroll
-  for (int e = 0; e < EV; ++e)
-    if (v + e < V) {
-      if (T == DVAE_F32) r[e] = reinterpret_cast<const uint32_t*>(lrow)[v + e];
-      else r[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(lrow)[v + e] << ((e & 1) * 16);
-    }
-  return r;
-}
-
-// a step's loads, begun one step ahead: its logits and its byte of the mask
-struct Loaded { u32x4 raw; uint32_t byte; };
-template <int T>
-__device__ __forceinline__ Loaded load_step(const RowP& p, const char* lrow, int v, int V) {
   Loaded l;
-  l.raw = load_logits<T>(lrow, v, V);
-  l.byte = p.mask ? p.mask[v >> 3] : 0xffu;
+  l.keep = (1u << EV) - 1;
+  if (whole || v + EV <= V) {
+    l.raw = *reinterpret_cast<const u32x4_u*>(lrow + (size_t)v * BYTES);
+  } else {
+    l.raw = u32x4{0, 0, 0, 0};
+    l.keep = v < V ? (1u << (V - v)) - 1 : 0u;
+#pragma unroll
+    for (int e = 0; e < EV; ++e)
+      if (v + e < V) {
+        if (T == DVAE_F32) l.raw[e] = reinterpret_cast<const uint32_t*>(lrow)[v + e];
+        else l.raw[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(lrow)[v + e] << ((e & 1) * 16);
+      }
+  }
+  if (p.mask && (whole || v < V)) {
+    const uint32_t byte = p.mask[v >> 3];
+    l.keep &= EV == 8 ? byte : byte >> (v & 4);
+  }
   return l;
 }
 
-// EV tokens from v < V on, d their place among the counts
+// The values under the rules.  Forbidden places: x = -inf and b = 0 before anything is computed, so that nothing they hold
+// shows.  Counted tokens are few: one test for the whole step, then one branch each.
 template <int T, int HIST>
 struct Ruled {
   typedef Elem<T> E;
   static constexpr int EV = E::EV;
-  float x[EV], b[EV];
-  uint32_t c[EV];
-  uint32_t keep;                // bit e: allowed (and inside the vocabulary)
-  __device__ __forceinline__ Ruled(const RowP& p, const Loaded& in, const uint32_t* cnt, int v, int d, int V) {
-    const u32x4 raw = in.raw;
-    keep = v + EV <= V ? (1u << EV) - 1 : (1u << (V - v)) - 1;
-    keep &= EV == 8 ? in.byte : in.byte >> (v & 4);
+  static constexpr int CW = HIST == 1 ? EV / 2 : HIST == 2 ? EV : 1;
+  float x[EV], s[EV];
+  uint32_t cw[CW];
+  uint32_t any;                 // nonzero: the history holds one of the step's tokens in this lane
+
+  __device__ __forceinline__ uint32_t count(int e) const {
+    if (HIST == 1) return (cw[e >> 1] >> ((e & 1) * 16)) & 0xffffu;
+    return HIST == 2 ? cw[e] : 0u;
+  }
+  // cnt: the counts from this lane's first token on
+  __device__ __forceinline__ Ruled(const RowP& p, const Loaded& in, const uint32_t* cnt, int v, int V, bool whole) {
+    const auto on = [&](int e) { return (uint32_t)((int)(in.keep << (31 - e)) >> 31); };
 #pragma unroll
-    for (int e = 0; e < EV; ++e) { x[e] = E::at(raw, e); b[e] = 0.f; c[e] = 0; }
+    for (int e = 0; e < EV; ++e) x[e] = E::at(in.raw, e);
+    if (p.mask || !whole) {
+#pragma unroll
+      for (int e = 0; e < EV; ++e) x[e] = __uint_as_float((__float_as_uint(x[e]) & on(e)) | (0xff800000u & ~on(e)));
+    }
+    any = 0;
+    if (HIST) {
+#pragma unroll
+      for (int i = 0; i < CW; ++i) { cw[i] = cnt[i]; any |= cw[i]; }
+    }
+    float b[EV];
     if (p.bias) {
-      if (v + EV <= V) {
+      if (whole || v + EV <= V) {
 #pragma unroll
         for (int e = 0; e < EV; e += 4) {
           const f32x4_u t = *reinterpret_cast<const f32x4_u*>(p.bias + v + e);
@@ -242,158 +276,341 @@ struct Ruled {
         }
       } else {
 #pragma unroll
-        for (int e = 0; e < EV; ++e) if (v + e < V) b[e] = p.bias[v + e];
+        for (int e = 0; e < EV; ++e) b[e] = v + e < V ? p.bias[v + e] : 0.f;
+      }
+      if (p.mask) {
+#pragma unroll
+        for (int e = 0; e < EV; ++e) b[e] = __uint_as_float(__float_as_uint(b[e]) & on(e));
+      }
+#pragma unroll
+      for (int e = 0; e < EV; ++e) s[e] = x[e] + b[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < EV; ++e) {
+        b[e] = 0.f;
+        s[e] = x[e];
       }
     }
-    if (HIST) {
+    if (HIST && any) {
 #pragma unroll
-      for (int e = 0; e < EV; ++e) c[e] = count_at<HIST ? HIST : 1>(cnt, d + e);
+      for (int e = 0; e < EV; ++e)
+        if (count(e)) {
+          s[e] = (in.keep >> e) & 1 ? (float)counted64(p, x[e], count(e), b[e]) : -INFINITY;
+        }
     }
-  }
-  __device__ __forceinline__ bool kept(int e) const { return (keep >> e) & 1; }
-  // rounded once to fp32
-  __device__ __forceinline__ float value(const RowP& p, int e) const {
-    float y = x[e] + b[e];
-    if (HIST) { if (c[e]) y = (float)counted64(p, x[e], c[e], b[e]); }
-    return kept(e) ? y : -INFINITY;
-  }
-  __device__ __forceinline__ double value64(const RowP& p, int e) const {
-    double y = (double)x[e] + (double)b[e];
-    if (HIST) { if (c[e]) y = counted64(p, x[e], c[e], b[e]); }
-    return kept(e) ? y : -INFINITY;
   }
 };
 
+// APPLY and BWD: a value written for every logit
 template <int T, int HIST, int MODE, bool ROWWAVE>
-__global__ __launch_bounds__(256) void rules_seg_kernel(SegArgs a) {
+__global__ __launch_bounds__(256) void rules_map_kernel(SegArgs a) {
   typedef Elem<T> E;
   constexpr int EV = E::EV, STEP = 64 * EV;
-  constexpr int WORDS = HIST ? 4 * SEG_MAX / Counts<HIST ? HIST : 1>::PER_WORD : 4;
-  __shared__ uint32_t lds[WORDS];
+  extern __shared__ uint32_t lds[];          // counts of the workgroup's 4 segments
   const Rules& q = a.q;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  long long row;
-  int seg;
-  if (ROWWAVE) {
-    row = (long long)blockIdx.x * 4 + wave;
-    seg = 0;
-  } else {
-    row = blockIdx.x / a.wgs_per_row;
-    seg = (blockIdx.x % a.wgs_per_row) * 4 + wave;
-  }
+  const long long row = ROWWAVE ? (long long)blockIdx.x * 4 + wave : blockIdx.x / a.wgs_per_row;
+  const int seg = ROWWAVE ? 0 : (blockIdx.x % a.wgs_per_row) * 4 + wave;
   const bool live = row < q.rows && seg < a.nseg;
   const int V = q.vocab;
   const int v0 = live ? seg * a.seg_len : 0;
-  RowP p = row_params(q, row < q.rows ? row : q.rows - 1);
+  const RowP p = row_params(q, row < q.rows ? row : q.rows - 1);
+  const int end = min(v0 + a.seg_len, V);
+  const char* lrow = static_cast<const char*>(q.logits) + row * q.ld * (long long)sizeof(typename E::type);
+  const int full = (end - v0) / STEP, steps = (end - v0 + STEP - 1) / STEP;
+  int v = v0 + lane * EV;
+  Loaded ahead{};                                 // the first step's loads are on their way while the history is counted
+  if (live) ahead = load_step<T>(p, lrow, v, V, full > 0);
   const uint32_t* cnt = lds;
   if (HIST) {
     const int words = 4 * a.seg_len / Counts<HIST ? HIST : 1>::PER_WORD;
     for (int i = threadIdx.x * 4; i < words; i += 1024) *reinterpret_cast<u32x4*>(&lds[i]) = u32x4{0, 0, 0, 0};
     __syncthreads();
     if (ROWWAVE) {
-      if (live) count_history<HIST>(p, q.history_i64, 0, a.seg_len, lds + wave * (words / 4), lane, 64);
+      if (live) count_history<HIST>(p, q.history_i64, 0, V, lds + wave * (words / 4), nullptr, lane, 64);
     } else {
-      count_history<HIST>(p, q.history_i64, (long long)(seg - wave) * a.seg_len, 4 * a.seg_len, lds, threadIdx.x, 256);
+      const int first = (seg - wave) * a.seg_len;
+      count_history<HIST>(p, q.history_i64, first, min(4 * a.seg_len, V - first), lds, nullptr, threadIdx.x, 256);
     }
     __syncthreads();
     cnt = lds + wave * (words / 4);
   }
   if (!live) return;
-  const int end = min(v0 + a.seg_len, V);
-  const char* lrow = static_cast<const char*>(q.logits) + row * q.ld * (long long)sizeof(typename E::type);
   const float kf = (float)p.k;
+  constexpr int PER = HIST ? Counts<HIST ? HIST : 1>::PER_WORD : 1;
 
-  if (MODE == M_APPLY || MODE == M_BWD) {
-    typename E::type* orow = static_cast<typename E::type*>(a.out) + row * a.out_ld;
-    float m = 0.f, iz = 0.f, coef = 0.f;
-    long long tok = -1;
-    bool zero = false;
-    if (MODE == M_BWD) {
-      m = a.stat[2 * row];
-      iz = a.stat[2 * row + 1];
-      coef = (float)((double)a.d_logprob[row] * (p.k * LN2));
-      tok = a.tokens[row];
-      zero = tok < 0 || tok >= V || m == -INFINITY;      // an ignored row, or one whose rules leave nothing
-    }
-    const float up = (float)p.rho, down = (float)p.inv_rho;
-    Loaded ahead;
-    if (v0 + lane * EV < end) ahead = load_step<T>(p, lrow, v0 + lane * EV, V);
-    for (int v = v0 + lane * EV; v < end; v += STEP) {
-      const Loaded in = ahead;
-      if (v + STEP < end) ahead = load_step<T>(p, lrow, v + STEP, V);
-      const Ruled<T, HIST> r(p, in, cnt, v, v - v0, V);
-      typename E::type o[EV];
+  typename E::type* orow = static_cast<typename E::type*>(a.out) + row * a.out_ld;
+  float m = 0.f, iz = 0.f, coef = 0.f;
+  long long tok = -1;
+  bool zero = false;
+  if (MODE == M_BWD) {
+    m = a.stat[2 * row];
+    iz = a.stat[2 * row + 1];
+    coef = (float)((double)a.d_logprob[row] * (p.k * LN2));
+    tok = a.tokens[row];
+    // an ignored row, or one whose rules leave nothing
+    zero = tok < 0 || tok >= V || m == -INFINITY;
+  }
+  const float up = (float)p.rho, down = (float)p.inv_rho, spread = -coef * iz;
+  for (int i = 0; i < steps; ++i, v += STEP) {
+    const Loaded in = ahead;
+    const bool whole = i < full;
+    if (i + 1 < steps) ahead = load_step<T>(p, lrow, v + STEP, V, i + 1 < full);
+    if (v >= end) continue;
+    const Ruled<T, HIST> r(p, in, cnt + (v - v0) / PER, v, V, whole);
+    float y[EV];
 #pragma unroll
-      for (int e = 0; e < EV; ++e) {
-        float y = r.value(p, e);
-        if (MODE == M_BWD) {
-          float g = coef * ((v + e == tok ? 1.f : 0.f) - __builtin_amdgcn_exp2f((y - m) * kf) * iz);
-          if (zero || !r.kept(e)) g = 0.f;
-          if (a.d_bias_rows && v + e < V) a.d_bias_rows[row * V + v + e] = g;
-          if (HIST) { if (r.c[e]) g *= r.x[e] > 0.f ? down : up; }
-          y = g;
-        }
-        o[e] = E::cast(y);
+    for (int e = 0; e < EV; ++e) y[e] = r.s[e];
+    if (MODE == M_BWD) {
+      // -g / T p; forbidden places have the weight 0 by themselves
+#pragma unroll
+      for (int e = 0; e < EV; ++e) y[e] = spread * __builtin_amdgcn_exp2f((y[e] - m) * kf);
+      const unsigned at = (unsigned)((int)tok - v);
+      if (at < EV) {                           // the lane of the given token
+#pragma unroll
+        for (int e = 0; e < EV; ++e) y[e] += at == e ? coef : 0.f;
       }
-      if (v + EV <= V) {
-        u32x4 w;
-        __builtin_memcpy(&w, o, 16);
-        *reinterpret_cast<u32x4_u*>(orow + v) = w;
-      } else {
+      if (zero || !(fabsf(spread) < INFINITY) || at < EV) {    // no gradient, a NaN or infinite one, a forbidden token
 #pragma unroll
         for (int e = 0; e < EV; ++e)
-          if (v + e < V) orow[v + e] = o[e];
+          if (zero || !((in.keep >> e) & 1)) y[e] = 0.f;
+      }
+      if (a.d_bias_rows) {
+#pragma unroll
+        for (int e = 0; e < EV; ++e)
+          if (v + e < V) a.d_bias_rows[row * V + v + e] = y[e];
+      }
+      if (HIST && r.any) {
+#pragma unroll
+        for (int e = 0; e < EV; ++e)
+          if (r.count(e)) y[e] *= r.x[e] > 0.f ? down : up;
       }
     }
-    return;
+    typename E::type o[EV];
+#pragma unroll
+    for (int e = 0; e < EV; ++e) o[e] = E::cast(y[e]);
+    if (whole || v + EV <= V) {
+      u32x4 w;
+      __builtin_memcpy(&w, o, 16);
+      *reinterpret_cast<u32x4_u*>(orow + v) = w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < EV; ++e)
+        if (v + e < V) orow[v + e] = o[e];
+    }
   }
+}
 
-  // reference of the lane's sum: weights are 2^((x4 - ref) k), up to 2^8 before it moves (fp32: an exponent of 8 is still
-  // exact to 2^-20) or 2^900 (double)
-  constexpr float ROOM = MODE == M_DRAW ? 900.f : 8.f;
-  const float room = ROOM / kf;
-  float ref = -3.402823466e38f, lim = ref, m = -INFINITY, z = 0.f;
+// value of one token in 64 bits, -inf where the grammar forbids it
+template <int T>
+__device__ __forceinline__ double token_value(const Rules& q, const RowP& p, long long row, int v, uint32_t c) {
+  if (p.mask && !((p.mask[v >> 3] >> (v & 7)) & 1)) return -INFINITY;
+  const float x = Elem<T>::one(q.logits, row * q.ld + v), b = p.bias ? p.bias[v] : 0.f;
+  return c ? counted64(p, x, c, b) : (double)x + (double)b;
+}
+
+// a counted token's loads (none waits for another), and its value
+struct Counted { float x, b; uint32_t c; bool kept; };
+template <int T, int HIST>
+__device__ __forceinline__ Counted load_counted(const Rules& q, const RowP& p, const char* lrow, const uint32_t* cnt, int v0, int d) {
+  const int v = v0 + d;
+  Counted t;
+  t.x = Elem<T>::one(lrow, v);
+  t.b = p.bias ? p.bias[v] : 0.f;
+  t.kept = !p.mask || ((p.mask[v >> 3] >> (v & 7)) & 1);
+  t.c = count_at<HIST ? HIST : 1>(cnt, d);
+  return t;
+}
+template <int T>
+__device__ __forceinline__ double counted_value(const RowP& p, const Counted& t) {
+  return t.kept ? counted64(p, t.x, t.c, t.b) : -INFINITY;
+}
+
+constexpr int LIST = 512;       // counted tokens of a segment that are listed; more are looked up bit by bit
+
+// A segment's maximum and sum of weights.  Tokens that the history holds are left out of the steps (one more bit mask) and
+// taken afterwards, a lane each: they are few, and the steps stay free of branches.
+// DRAW: sums of doubles, against 0 as reference -- an exponent of a double has room for every ordinary row; where the
+// maximum is no ordinary one (beyond 2^-400 .. 2^900) the segment is summed again against it.  Else fp32 sums, against a
+// reference of the lane's own that moves when a value exceeds it by 2^8 (an exponent of 8 is still exact to 2^-20).
+template <int T, int HIST, bool DRAW, bool ROWWAVE>
+__global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
+  typedef Elem<T> E;
+  constexpr int EV = E::EV, STEP = 64 * EV;
+  extern __shared__ uint32_t lds[];          // counts of the workgroup's 4 segments, a bit for each token, and the lists of counted ones
+  const Rules& q = a.q;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long long row = ROWWAVE ? (long long)blockIdx.x * 4 + wave : blockIdx.x / a.wgs_per_row;
+  const int seg = ROWWAVE ? 0 : (blockIdx.x % a.wgs_per_row) * 4 + wave;
+  const bool live = row < q.rows && seg < a.nseg;
+  const int V = q.vocab;
+  const int v0 = live ? seg * a.seg_len : 0;
+  const RowP p = row_params(q, row < q.rows ? row : q.rows - 1);
+  const int end = min(v0 + a.seg_len, V);
+  const char* lrow = static_cast<const char*>(q.logits) + row * q.ld * (long long)sizeof(typename E::type);
+  const int full = (end - v0) / STEP, steps = (end - v0 + STEP - 1) / STEP;
+  Loaded begun{};                                 // the first step's loads are on their way while the history is counted
+  if (live) begun = load_step<T>(p, lrow, v0 + lane * EV, V, full > 0);
+  const uint32_t *cnt = lds, *seen = lds;
+  if (HIST) {
+    const int words = 4 * a.seg_len / Counts<HIST ? HIST : 1>::PER_WORD, marks = 4 * a.seg_len / 32;
+    uint32_t* bits = lds + words;
+    for (int i = threadIdx.x * 4; i < words + marks; i += 1024) *reinterpret_cast<u32x4*>(&lds[i]) = u32x4{0, 0, 0, 0};
+    __syncthreads();
+    if (ROWWAVE) {
+      if (live) count_history<HIST>(p, q.history_i64, 0, V, lds + wave * (words / 4), bits + wave * (marks / 4), lane, 64);
+    } else {
+      const int first = (seg - wave) * a.seg_len;
+      count_history<HIST>(p, q.history_i64, first, min(4 * a.seg_len, V - first), lds, bits, threadIdx.x, 256);
+    }
+    __syncthreads();
+    cnt = lds + wave * (words / 4);
+    seen = bits + wave * (marks / 4);
+  }
+  if (!live) return;
+  const float kf = (float)p.k;
+
+  float m = -INFINITY, z = 0.f;
+  float ref = -3.402823466e38f, lim = ref;           // fp32 sums: the lane's reference, and where it moves
+  const float room = 8.f * (float)(p.temp * LN2);
   double zd = 0.0;
-  const double low = -1000.0 / p.k;
-  Loaded ahead;
-  if (v0 + lane * EV < end) ahead = load_step<T>(p, lrow, v0 + lane * EV, V);
-  for (int v = v0 + lane * EV; v < end; v += STEP) {
-    const Loaded in = ahead;
-    if (v + STEP < end) ahead = load_step<T>(p, lrow, v + STEP, V);
-    const Ruled<T, HIST> r(p, in, cnt, v, v - v0, V);
-    float s[EV];
+  const double low = -1000.0 * LN2 * p.temp;        // -1000 / k
+
+  // the segment's counted tokens as a list (in a fixed order); the first 64 are loaded ahead of the steps, which hide the way
+  uint16_t* list = reinterpret_cast<uint16_t*>(lds + (HIST ? 4 * a.seg_len / Counts<HIST ? HIST : 1>::PER_WORD + a.seg_len / 8 : 0)) + wave * LIST;
+  int held = 0;
+  Counted first_held{};
+  if (HIST) {
+    const int words = a.seg_len / 32;
+    uint32_t w0 = lane < words ? seen[lane] : 0u, w1 = lane + 64 < words ? seen[lane + 64] : 0u;
+    int at = __popc(w0) + __popc(w1);
+    const int own = at;
 #pragma unroll
-    for (int e = 0; e < EV; ++e) s[e] = r.value(p, e);
-    float mx = s[0];
-#pragma unroll
-    for (int e = 1; e < EV; ++e) mx = max_nan(mx, s[e]);
+    for (int o = 1; o < 64; o <<= 1) {
+      const int t = __shfl_up(at, o);
+      if (lane >= o) at += t;
+    }
+    held = __shfl(at, 63);
+    if (held <= LIST) {
+      at -= own;
+      for (; w0; w0 &= w0 - 1) list[at++] = (uint16_t)(lane * 32 + __ffs(w0) - 1);
+      for (; w1; w1 &= w1 - 1) list[at++] = (uint16_t)((lane + 64) * 32 + __ffs(w1) - 1);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (lane < held) first_held = load_counted<T, HIST>(q, p, lrow, cnt, v0, list[lane]);
+    }
+  }
+  const auto take = [&](float mx) {
     m = max_nan(m, mx);
-    if (mx > lim) {
-      if (MODE == M_DRAW) zd *= exp2_64((double)ref - (double)mx, p.k);
-      else z *= __builtin_amdgcn_exp2f((ref - mx) * kf);
+    if (!DRAW && mx > lim) {
+      z *= __builtin_amdgcn_exp2f((ref - mx) * kf);
       ref = mx;
       lim = ref + room;
     }
-    if (MODE == M_DRAW) {
-      if (!HIST && !p.bias) {          // the fp32 values are exact
+  };
+  const auto scan = [&](auto shifted, double base) {
+    const auto weigh = [&](double y) { zd += exp2_fast(decltype(shifted)::value ? y - base : y, p.k, low); };
+    int v = v0 + lane * EV;
+    Loaded ahead = decltype(shifted)::value ? load_step<T>(p, lrow, v, V, full > 0) : begun;
+    for (int i = 0; i < steps; ++i, v += STEP) {
+      Loaded in = ahead;
+      const bool whole = i < full;
+      if (i + 1 < steps) ahead = load_step<T>(p, lrow, v + STEP, V, i + 1 < full);
+      if (v >= end) continue;
+      if (HIST) {
+        const uint32_t byte = reinterpret_cast<const uint8_t*>(seen)[(v - v0) >> 3];
+        in.keep &= ~(EV == 8 ? byte : byte >> (v & 4));
+      }
+      float x[EV], s[EV];
 #pragma unroll
-        for (int e = 0; e < EV; ++e) zd += exp2_fast((double)s[e] - (double)ref, p.k, low);
+      for (int e = 0; e < EV; ++e) x[e] = E::at(in.raw, e);
+      const auto on = [&](int e) { return (uint32_t)((int)(in.keep << (31 - e)) >> 31); };
+      if (HIST || p.mask || !whole) {
+#pragma unroll
+        for (int e = 0; e < EV; ++e) x[e] = __uint_as_float((__float_as_uint(x[e]) & on(e)) | (0xff800000u & ~on(e)));
+      }
+      if (p.bias) {
+        float b[EV];
+        if (whole || v + EV <= V) {
+#pragma unroll
+          for (int e = 0; e < EV; e += 4) {
+            const f32x4_u t = *reinterpret_cast<const f32x4_u*>(p.bias + v + e);
+            b[e] = t[0]; b[e + 1] = t[1]; b[e + 2] = t[2]; b[e + 3] = t[3];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < EV; ++e) b[e] = v + e < V ? p.bias[v + e] : 0.f;
+        }
+        if (HIST || p.mask) {
+#pragma unroll
+          for (int e = 0; e < EV; ++e) b[e] = __uint_as_float(__float_as_uint(b[e]) & on(e));
+        }
+#pragma unroll
+        for (int e = 0; e < EV; ++e) s[e] = x[e] + b[e];
+        if (DRAW) {
+#pragma unroll
+          for (int e = 0; e < EV; ++e) weigh((double)x[e] + (double)b[e]);
+        }
       } else {
 #pragma unroll
-        for (int e = 0; e < EV; ++e) zd += exp2_fast(r.value64(p, e) - (double)ref, p.k, low);
-      }
-    } else {
+        for (int e = 0; e < EV; ++e) s[e] = x[e];
+        if (DRAW) {
 #pragma unroll
-      for (int e = 0; e < EV; ++e) z += __builtin_amdgcn_exp2f((s[e] - ref) * kf);
+          for (int e = 0; e < EV; ++e) weigh((double)x[e]);
+        }
+      }
+      float mx = s[0];
+#pragma unroll
+      for (int e = 1; e < EV; ++e) mx = max_nan(mx, s[e]);
+      take(mx);
+      if (!DRAW) {
+#pragma unroll
+        for (int e = 0; e < EV; ++e) z += __builtin_amdgcn_exp2f((s[e] - ref) * kf);
+      }
     }
-  }
+    if (HIST) {
+      const auto one = [&](double y) {
+        take((float)y);
+        if (DRAW) weigh(y);
+        else z += __builtin_amdgcn_exp2f(((float)y - ref) * kf);
+      };
+      if (held <= LIST) {
+        if (lane < held) one(counted_value<T>(p, first_held));
+        for (int i = lane + 64; i < held; i += 256) {          // four in flight
+          Counted t[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (i + 64 * u < held) t[u] = load_counted<T, HIST>(q, p, lrow, cnt, v0, list[i + 64 * u]);
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (i + 64 * u < held) one(counted_value<T>(p, t[u]));
+        }
+      } else {
+        for (int w = lane; w < a.seg_len / 32; w += 64)
+          for (uint32_t left = seen[w]; left; left &= left - 1)
+            one(counted_value<T>(p, load_counted<T, HIST>(q, p, lrow, cnt, v0, w * 32 + __ffs(left) - 1)));
+      }
+    }
+  };
+  scan(std::false_type{}, 0.0);
   m = wave_max_nan(m);
   Seg r;
-  r.s = 0.0; r.m = m; r.pad = 0;
+  r.s = 0.0; r.m = m; r.ref = m;
   if (m > -INFINITY && m < INFINITY) {
-    if (MODE == M_DRAW) r.s = wave_sum(zd * exp2_64((double)ref - (double)m, p.k));
-    else r.s = (double)wave_sum(z * __builtin_amdgcn_exp2f((ref - m) * kf));
+    if (DRAW) {
+      const double top = (double)m * p.k;
+      r.ref = 0.f;
+      if (!(top > -400.0 && top < 900.0)) {
+        r.ref = m;
+        zd = 0.0;
+        scan(std::true_type{}, (double)m);
+      }
+      r.s = wave_sum(zd);
+    } else {
+      r.s = (double)wave_sum(z * __builtin_amdgcn_exp2f((ref - m) * kf));
+    }
   }
   if (lane == 0) a.seg[row * a.nseg + seg] = r;
 }
@@ -444,14 +661,6 @@ __device__ __forceinline__ double block_prefix(double v, double* sh, double& tot
 
 constexpr int HIST_STAGE = 4096;       // tokens of a history that the join keeps in LDS
 
-// value of one token in 64 bits, -inf where the grammar forbids it
-template <int T>
-__device__ __forceinline__ double token_value(const Rules& q, const RowP& p, long long row, int v, uint32_t c) {
-  if (p.mask && !((p.mask[v >> 3] >> (v & 7)) & 1)) return -INFINITY;
-  const float x = Elem<T>::one(q.logits, row * q.ld + v), b = p.bias ? p.bias[v] : 0.f;
-  return c ? counted64(p, x, c, b) : (double)x + (double)b;
-}
-
 // One workgroup a row.  What it reads depends on what it has read (partials, then the segment they point to), so the
 // loads that do not -- the history, a given token's logit -- are begun first, and the partials stay in registers.
 template <int T, int MODE>
@@ -473,9 +682,10 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
   const int per = (a.nseg + 255) / 256;
   const int i0 = min(tid * per, a.nseg), i1 = min(i0 + per, a.nseg);
   Seg mine;
-  mine.s = 0.0; mine.m = -INFINITY; mine.pad = 0;
+  mine.s = 0.0; mine.m = -INFINITY; mine.ref = 0.f;
   if (i0 < i1) mine = seg[i0];
 
+  const float uf = MODE == M_DRAW ? a.uniforms[row] : 0.f;
   long long tok = -1;
   double given_y = 0.0;
   int c = 0;
@@ -498,7 +708,7 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
   m = block_reduce(m, shf, [](float x, float y) { return max_nan(x, y); });
   // a temperature that is not positive and finite makes the row NaN, as a NaN logit does
   const bool ok = m > -INFINITY && m < INFINITY && p.k > 0.0 && p.k < INFINITY;
-  const auto scaled = [&](const Seg& s) { return s.m > -INFINITY ? s.s * exp2_64((double)s.m - (double)m, p.k) : 0.0; };
+  const auto scaled = [&](const Seg& s) { return s.m > -INFINITY ? s.s * exp2_64((double)s.ref - (double)m, p.k) : 0.0; };
   double z0 = 0.0, z = 0.0;
   if (ok) {
     z0 = scaled(mine);
@@ -530,7 +740,6 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
     if (tid == 0) finish(tok, given_y);
     return;
   }
-  const float uf = MODE == M_DRAW ? a.uniforms[row] : 0.f;
   if (!ok || uf != uf) {
     if (tid == 0) finish(-1, 0.0);
     return;
@@ -577,7 +786,11 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
     }
     const float best = block_reduce(lo, shf, [](float x, float y) { return fmaxf(x, y); });
     const int t = block_reduce(lo == best ? idx : INT32_MAX, shi, [](int x, int y) { return min(x, y); });
-    if (idx == t) finish(t, best_y);
+    if (t == INT32_MAX) {                // (the sum pass computed the same values: one of them is the maximum)
+      if (tid == 0) finish(-1, 0.0);
+    } else if (idx == t) {
+      finish(t, best_y);
+    }
     return;
   }
 
@@ -588,7 +801,7 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
   for (int i = i0; i < i1; ++i) {
     const double w = i == i0 ? z0 : scaled(seg[i]);
     if (w > 0.0) { last = i; last_before = run; }
-    if (run + w > edge && first == INT32_MAX) { first = i; first_before = run; }
+    if (w > 0.0 && run + w > edge && first == INT32_MAX) { first = i; first_before = run; }
     run += w;
   }
   const int f = block_reduce(first, shi, [](int x, int y) { return min(x, y); });
@@ -603,34 +816,62 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
   }
   const int v0 = g * n;
   count(v0);
-  // weights of the segment's tokens, thread by thread in order
-  constexpr int OWN = SEG_MAX / 256;
-  const int own = n / 256, d0 = tid * own;
-  double w[OWN], sum = 0.0;
+  // weights of the segment's tokens: a quarter for each wave, in strips of 64 tokens
+  constexpr int STRIPS = SEG_MAX / 256;
+  const int strips = n / 256, lane = tid & 63, wave = tid >> 6;
+  const int d0 = wave * (n / 4) + lane;
+  double w[STRIPS], sum = 0.0;
 #pragma unroll
-  for (int e = 0; e < OWN; ++e) {
+  for (int e = 0; e < STRIPS; ++e) {
     w[e] = 0.0;
-    if (e < own && v0 + d0 + e < V) w[e] = exp2_64(token_value<T>(q, p, row, v0 + d0 + e, cnt[d0 + e]) - (double)m, p.k);
+    const int d = d0 + e * 64;
+    if (e < strips && v0 + d < V) w[e] = exp2_64(token_value<T>(q, p, row, v0 + d, cnt[d]) - (double)m, p.k);
     sum += w[e];
   }
-  double all;
-  double at = pick_before + block_prefix(sum, shd, all);
-  int hit = INT32_MAX, tail = -1;
 #pragma unroll
-  for (int e = 0; e < OWN; ++e) {
-    at += w[e];
-    if (w[e] > 0.0) {
-      tail = v0 + d0 + e;
-      if (at > edge && hit == INT32_MAX) hit = v0 + d0 + e;
-    }
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+  __syncthreads();
+  if (lane == 0) shd[wave] = sum;
+  __syncthreads();
+  double at = pick_before;
+  int in = -1;
+  for (int i = 0; i < 4; ++i) {
+    if (shd[i] > 0.0 && at + shd[i] > edge) { in = i; break; }
+    at += shd[i];
   }
-  int t = block_reduce(hit, shi, [](int x, int y) { return min(x, y); });
-  if (t == INT32_MAX) t = block_reduce(tail, shi, [](int x, int y) { return max(x, y); });
-  if (t < 0) {
-    if (tid == 0) finish(-1, 0.0);
+  if (in < 0) {      // by rounding, or u >= 1: the last token with a weight
+    int tail = -1;
+#pragma unroll
+    for (int e = 0; e < STRIPS; ++e)
+      if (w[e] > 0.0) tail = d0 + e * 64;
+    tail = block_reduce(tail, shi, [](int x, int y) { return max(x, y); });
+    if (tail < 0) {
+      if (tid == 0) finish(-1, 0.0);
+    } else if (tail >= d0 && ((tail - d0) & 63) == 0 && tail < wave * (n / 4) + n / 4) {
+      finish(v0 + tail, token_value<T>(q, p, row, v0 + tail, cnt[tail]));
+    }
     return;
   }
-  if (t - v0 >= d0 && t - v0 < d0 + own) finish(t, token_value<T>(q, p, row, t, cnt[t - v0]));
+  if (wave != in) return;
+  int hit = INT32_MAX, tail = -1;
+#pragma unroll
+  for (int e = 0; e < STRIPS; ++e) {
+    if (e < strips && hit == INT32_MAX) {
+      double run = w[e];
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const double t = __shfl_up(run, o);
+        if (lane >= o) run += t;
+      }
+      const unsigned long long over = __ballot(w[e] > 0.0 && at + run > edge), any = __ballot(w[e] > 0.0);
+      if (any) tail = e * 64 + 63 - __clzll(any);
+      if (over) hit = e * 64 + __ffsll(over) - 1;
+      at += __shfl(run, 63);
+    }
+  }
+  // (sums of another order may end a rounding short of the edge: then the wave's last token with a weight)
+  const int d = wave * (n / 4) + (hit != INT32_MAX ? hit : tail);
+  if (((d - d0) & 63) == 0) finish(v0 + d, token_value<T>(q, p, row, v0 + d, cnt[d]));
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -791,7 +1032,7 @@ __global__ __launch_bounds__(256) void rules_bwd_col_kernel(ColArgs ca) {
       __syncthreads();
       for (int i = threadIdx.x; i < SPAN; i += 256) lds[i] = 0;
       __syncthreads();
-      count_history<2>(p, q.history_i64, v0, SPAN, lds, threadIdx.x, 256);
+      count_history<2>(p, q.history_i64, v0, min(SPAN, V - v0), lds, nullptr, threadIdx.x, 256);
       __syncthreads();
     }
     const typename E::type* lrow = static_cast<const typename E::type*>(q.logits) + row * q.ld;
@@ -859,8 +1100,10 @@ Plan plan_of(const dvae_rules& q) {
   Plan p;
   const int step = 64 * (16 / elem_bytes(q.dtype));      // tokens of a wave's step
   // segments as long as 4096 waves (four for each SIMD) leave them: few rows are spread over the whole card
+  // (a workgroup counts the whole history, so a long one asks for long segments; 32-bit counts take twice the room)
+  const int cap = q.history && q.history_len > 4096 && q.history_len < 65536 ? SEG_MAX : 2048;
   p.seg_len = step;
-  while (p.seg_len < SEG_MAX && p.seg_len < q.vocab && q.rows * ((q.vocab + p.seg_len - 1) / p.seg_len) > 4096) p.seg_len *= 2;
+  while (p.seg_len < cap && p.seg_len < q.vocab && q.rows * ((q.vocab + p.seg_len - 1) / p.seg_len) > 4096) p.seg_len *= 2;
   p.nseg = (int)(((long long)q.vocab + p.seg_len - 1) / p.seg_len);
   p.row_wave = p.nseg == 1;
   p.wgs_per_row = (p.nseg + 3) / 4;
@@ -870,8 +1113,17 @@ Plan plan_of(const dvae_rules& q) {
 
 template <int T, int HIST, int MODE>
 void launch_seg(const SegArgs& a, const Plan& p, hipStream_t st) {
-  if (p.row_wave) hipLaunchKernelGGL((rules_seg_kernel<T, HIST, MODE, true>), dim3((unsigned)p.blocks), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((rules_seg_kernel<T, HIST, MODE, false>), dim3((unsigned)p.blocks), dim3(256), 0, st, a);
+  const dim3 grid((unsigned)p.blocks), block(256);
+  // counts of 4 segments and, for sums, a bit for each token and the lists: 38 KB at most
+  unsigned lds = HIST ? 16u * p.seg_len / Counts<HIST ? HIST : 1>::PER_WORD : 0u;
+  if constexpr (MODE == M_APPLY || MODE == M_BWD) {
+    if (p.row_wave) hipLaunchKernelGGL((rules_map_kernel<T, HIST, MODE, true>), grid, block, lds, st, a);
+    else hipLaunchKernelGGL((rules_map_kernel<T, HIST, MODE, false>), grid, block, lds, st, a);
+  } else {
+    if (HIST) lds += p.seg_len / 2 + 4 * LIST * 2;
+    if (p.row_wave) hipLaunchKernelGGL((rules_sum_kernel<T, HIST, MODE == M_DRAW, true>), grid, block, lds, st, a);
+    else hipLaunchKernelGGL((rules_sum_kernel<T, HIST, MODE == M_DRAW, false>), grid, block, lds, st, a);
+  }
 }
 
 template <int T, int MODE>
