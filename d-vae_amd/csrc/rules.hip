@@ -301,6 +301,51 @@ struct Ruled {
   }
 };
 
+// a row's part of the gradient: y = -g / T p, + g / T at the given token
+struct Bwd {
+  float m, coef, spread, kf, up, down;
+  int tok;
+  bool zero;                      // an ignored row, or one whose rules leave nothing
+  __device__ __forceinline__ Bwd() {}
+  __device__ __forceinline__ Bwd(const SegArgs& a, const RowP& p, long long row) {
+    const long long t = a.tokens[row];
+    m = a.stat[2 * row];
+    kf = (float)p.k;
+    coef = (float)((double)a.d_logprob[row] * (p.k * LN2));
+    spread = -coef * a.stat[2 * row + 1];
+    up = (float)p.rho;
+    down = (float)p.inv_rho;
+    zero = t < 0 || t >= a.q.vocab || m == -INFINITY;
+    tok = zero ? 0 : (int)t;
+  }
+  // d values of the step's tokens, from v on
+  template <typename R, int EV>
+  __device__ __forceinline__ void values(const R& r, uint32_t keep, int v, float (&y)[EV]) const {
+    // forbidden places have the weight 0 by themselves
+#pragma unroll
+    for (int e = 0; e < EV; ++e) y[e] = spread * __builtin_amdgcn_exp2f((r.s[e] - m) * kf);
+    const unsigned at = (unsigned)(tok - v);
+    if (at < EV) {
+#pragma unroll
+      for (int e = 0; e < EV; ++e) y[e] += at == e ? coef : 0.f;
+    }
+    if (zero || !(fabsf(spread) < INFINITY) || at < EV) {      // no gradient, a NaN or infinite one, a forbidden token
+#pragma unroll
+      for (int e = 0; e < EV; ++e)
+        if (zero || !((keep >> e) & 1)) y[e] = 0.f;
+    }
+  }
+  // d values -> d logits
+  template <typename R, int EV>
+  __device__ __forceinline__ void slope(const R& r, float (&y)[EV]) const {
+    if (r.any) {
+#pragma unroll
+      for (int e = 0; e < EV; ++e)
+        if (r.count(e)) y[e] *= r.x[e] > 0.f ? down : up;
+    }
+  }
+};
+
 // APPLY and BWD: a value written for every logit
 template <int T, int HIST, int MODE, bool ROWWAVE>
 __global__ __launch_bounds__(256) void rules_map_kernel(SegArgs a) {
@@ -341,18 +386,8 @@ __global__ __launch_bounds__(256) void rules_map_kernel(SegArgs a) {
   constexpr int PER = HIST ? Counts<HIST ? HIST : 1>::PER_WORD : 1;
 
   typename E::type* orow = static_cast<typename E::type*>(a.out) + row * a.out_ld;
-  float m = 0.f, iz = 0.f, coef = 0.f;
-  long long tok = -1;
-  bool zero = false;
-  if (MODE == M_BWD) {
-    m = a.stat[2 * row];
-    iz = a.stat[2 * row + 1];
-    coef = (float)((double)a.d_logprob[row] * (p.k * LN2));
-    tok = a.tokens[row];
-    // an ignored row, or one whose rules leave nothing
-    zero = tok < 0 || tok >= V || m == -INFINITY;
-  }
-  const float up = (float)p.rho, down = (float)p.inv_rho, spread = -coef * iz;
+  Bwd b;
+  if (MODE == M_BWD) b = Bwd(a, p, row);
   for (int i = 0; i < steps; ++i, v += STEP) {
     const Loaded in = ahead;
     const bool whole = i < full;
@@ -363,29 +398,13 @@ __global__ __launch_bounds__(256) void rules_map_kernel(SegArgs a) {
 #pragma unroll
     for (int e = 0; e < EV; ++e) y[e] = r.s[e];
     if (MODE == M_BWD) {
-      // -g / T p; forbidden places have the weight 0 by themselves
-#pragma unroll
-      for (int e = 0; e < EV; ++e) y[e] = spread * __builtin_amdgcn_exp2f((y[e] - m) * kf);
-      const unsigned at = (unsigned)((int)tok - v);
-      if (at < EV) {                           // the lane of the given token
-#pragma unroll
-        for (int e = 0; e < EV; ++e) y[e] += at == e ? coef : 0.f;
-      }
-      if (zero || !(fabsf(spread) < INFINITY) || at < EV) {    // no gradient, a NaN or infinite one, a forbidden token
-#pragma unroll
-        for (int e = 0; e < EV; ++e)
-          if (zero || !((in.keep >> e) & 1)) y[e] = 0.f;
-      }
+      b.values(r, in.keep, v, y);
       if (a.d_bias_rows) {
 #pragma unroll
         for (int e = 0; e < EV; ++e)
           if (v + e < V) a.d_bias_rows[row * V + v + e] = y[e];
       }
-      if (HIST && r.any) {
-#pragma unroll
-        for (int e = 0; e < EV; ++e)
-          if (r.count(e)) y[e] *= r.x[e] > 0.f ? down : up;
-      }
+      b.slope(r, y);
     }
     typename E::type o[EV];
 #pragma unroll
@@ -1004,8 +1023,9 @@ __global__ __launch_bounds__(256) void rules_small_kernel(SmallArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// gradients with a bias shared by the rows: a workgroup owns 256 EV columns and walks a share of the rows, so the
-// bias gradient's sum over rows stays in registers; shares are added in a fixed order by a second launch
+// gradients with a bias shared by the rows: a workgroup owns 256 EV columns and a share of the rows, each of its waves
+// every fourth of them, so that the bias gradient's sum over rows stays in registers and no row costs a barrier (a wave
+// counts its row's history by itself); shares are added in a fixed order by a second launch
 // ---------------------------------------------------------------------------------------------------------------
 struct ColArgs {
   SegArgs s;
@@ -1013,55 +1033,75 @@ struct ColArgs {
   int rows_per_share;
 };
 
+constexpr int COL_STEPS = 4;
+
 template <int T, int HIST>
 __global__ __launch_bounds__(256) void rules_bwd_col_kernel(ColArgs ca) {
   typedef Elem<T> E;
-  constexpr int EV = E::EV, SPAN = 256 * EV;
-  __shared__ uint32_t lds[HIST ? SPAN : 1];
+  constexpr int EV = E::EV, STEP = 64 * EV, SPAN = COL_STEPS * STEP, PER = HIST ? Counts<HIST ? HIST : 1>::PER_WORD : 1;
+  __shared__ uint32_t lds[4 * SPAN];              // counts of each wave's row, then each wave's sums
   const SegArgs& a = ca.s;
   const Rules& q = a.q;
-  const int V = q.vocab, v0 = blockIdx.x * SPAN, v = v0 + threadIdx.x * EV;
+  const int V = q.vocab, v0 = blockIdx.x * SPAN, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const long long r0 = (long long)blockIdx.y * ca.rows_per_share;
   const long long r1 = min(r0 + ca.rows_per_share, q.rows);
-  float acc[EV];
+  uint32_t* cnt = lds + wave * (SPAN / PER);
+  float acc[COL_STEPS][EV];
 #pragma unroll
-  for (int e = 0; e < EV; ++e) acc[e] = 0.f;
-  for (long long row = r0; row < r1; ++row) {
+  for (int j = 0; j < COL_STEPS; ++j)
+#pragma unroll
+    for (int e = 0; e < EV; ++e) acc[j][e] = 0.f;
+  for (long long row = r0 + wave; row < r1; row += 4) {
     const RowP p = row_params(q, row);
-    if (HIST) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < SPAN; i += 256) lds[i] = 0;
-      __syncthreads();
-      count_history<2>(p, q.history_i64, v0, min(SPAN, V - v0), lds, nullptr, threadIdx.x, 256);
-      __syncthreads();
-    }
-    const typename E::type* lrow = static_cast<const typename E::type*>(q.logits) + row * q.ld;
+    const Bwd b(a, p, row);
+    const char* lrow = static_cast<const char*>(q.logits) + row * q.ld * (long long)sizeof(typename E::type);
     typename E::type* orow = static_cast<typename E::type*>(a.out) + row * a.out_ld;
-    const float m = a.stat[2 * row], iz = a.stat[2 * row + 1], kf = (float)p.k;
-    const float coef = (float)((double)a.d_logprob[row] * (p.k * LN2));
-    const long long tok = a.tokens[row];
-    const bool zero = tok < 0 || tok >= V || m == -INFINITY;
+    Loaded in[COL_STEPS];
 #pragma unroll
-    for (int e = 0; e < EV; ++e) {
-      const int w = v + e;
-      float g = 0.f;
-      if (w < V) {
-        const bool off = zero || (p.mask && !((p.mask[w >> 3] >> (w & 7)) & 1));
-        if (!off) {
-          const float x = E::one(lrow, w), b = p.bias ? p.bias[w] : 0.f;
-          const uint32_t c = HIST ? lds[w - v0] : 0u;
-          const float y = c ? (float)counted64(p, x, c, b) : x + b;
-          g = coef * ((w == tok ? 1.f : 0.f) - __builtin_amdgcn_exp2f((y - m) * kf) * iz);
-          acc[e] += g;
-          if (c) g *= x > 0.f ? (float)p.inv_rho : (float)p.rho;
-        }
-        orow[w] = E::cast(g);
+    for (int j = 0; j < COL_STEPS; ++j) in[j] = load_step<T>(p, lrow, v0 + j * STEP + lane * EV, V, v0 + (j + 1) * STEP <= V);
+    if (HIST) {
+      for (int i = lane * 4; i < SPAN / PER; i += 256) *reinterpret_cast<u32x4*>(&cnt[i]) = u32x4{0, 0, 0, 0};
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      count_history<HIST>(p, q.history_i64, v0, min(SPAN, V - v0), cnt, nullptr, lane, 64);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+#pragma unroll
+    for (int j = 0; j < COL_STEPS; ++j) {
+      const int d = j * STEP + lane * EV, v = v0 + d;
+      const bool whole = v0 + (j + 1) * STEP <= V;
+      if (v >= V) continue;
+      const Ruled<T, HIST> r(p, in[j], cnt + d / PER, v, V, whole);
+      float y[EV];
+      b.values(r, in[j].keep, v, y);
+#pragma unroll
+      for (int e = 0; e < EV; ++e) acc[j][e] += y[e];
+      b.slope(r, y);
+      typename E::type o[EV];
+#pragma unroll
+      for (int e = 0; e < EV; ++e) o[e] = E::cast(y[e]);
+      if (whole || v + EV <= V) {
+        u32x4 w;
+        __builtin_memcpy(&w, o, 16);
+        *reinterpret_cast<u32x4_u*>(orow + v) = w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < EV; ++e)
+          if (v + e < V) orow[v + e] = o[e];
       }
     }
   }
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(lds);
 #pragma unroll
-  for (int e = 0; e < EV; ++e)
-    if (v + e < V) ca.part[(size_t)blockIdx.y * V + v + e] = acc[e];
+  for (int j = 0; j < COL_STEPS; ++j)
+#pragma unroll
+    for (int e = 0; e < EV; ++e) sums[wave * SPAN + j * STEP + lane * EV + e] = acc[j][e];
+  __syncthreads();
+  for (int d = threadIdx.x; d < SPAN && v0 + d < V; d += 256)
+    ca.part[(size_t)blockIdx.y * V + v0 + d] = (sums[d] + sums[SPAN + d]) + (sums[2 * SPAN + d] + sums[3 * SPAN + d]);
 }
 
 // 16 columns a workgroup, 16 threads a column: shares in a fixed order
@@ -1188,9 +1228,9 @@ int run_small(SmallArgs& a, long long blocks, hipStream_t st) {
 
 int bias_shares(const dvae_rules& q) {
   if (is_small(q)) return (int)std::min<long long>(small_blocks(q), 1024);
-  const int span = 256 * (16 / elem_bytes(q.dtype));
+  const int span = 64 * COL_STEPS * (16 / elem_bytes(q.dtype));
   const long long cols = ((long long)q.vocab + span - 1) / span;
-  return (int)std::min<long long>(q.rows, std::max<long long>(1, 2048 / cols));
+  return (int)std::min<long long>((q.rows + 3) / 4, std::max<long long>(1, 1024 / cols));
 }
 
 }  // namespace
@@ -1333,11 +1373,12 @@ extern "C" int dvae_rules_logprob_bwd(const dvae_rules* q, const long long* toke
   c.s = a;
   c.part = (float*)ws;
   c.rows_per_share = (int)((q->rows + shares - 1) / shares);
-  const dim3 grid((unsigned)cdiv(q->vocab, 256 * (16 / elem_bytes(q->dtype))), (unsigned)shares);
-  const bool hist = q->history && q->history_len > 0;
+  const dim3 grid((unsigned)cdiv(q->vocab, 64 * COL_STEPS * (16 / elem_bytes(q->dtype))), (unsigned)shares);
+  const int hist = !q->history || q->history_len == 0 ? 0 : q->history_len < 65536 ? 1 : 2;
 #define COL(T)                                                                                              \
   do {                                                                                                      \
-    if (hist) hipLaunchKernelGGL((rules_bwd_col_kernel<T, 1>), grid, dim3(256), 0, st, c);                  \
+    if (hist == 1) hipLaunchKernelGGL((rules_bwd_col_kernel<T, 1>), grid, dim3(256), 0, st, c);             \
+    else if (hist) hipLaunchKernelGGL((rules_bwd_col_kernel<T, 2>), grid, dim3(256), 0, st, c);             \
     else hipLaunchKernelGGL((rules_bwd_col_kernel<T, 0>), grid, dim3(256), 0, st, c);                       \
   } while (0)
   switch (q->dtype) {
