@@ -89,20 +89,30 @@ __global__ __launch_bounds__(256) void norm_kernel(Batch b, double* __restrict__
   if (threadIdx.x == 0) part[blockIdx.x] = (sh[0] + sh[1]) + (sh[2] + sh[3]);
 }
 
-__global__ __launch_bounds__(256) void norm_join_kernel(const double* __restrict__ part, int n, double max_norm,
-                                                        float* __restrict__ out2) {
+// {norm, coef} from the partial sums, the same in every workgroup that forms them
+struct Sum { double norm, coef; };
+__device__ __forceinline__ Sum join(const double* __restrict__ part, int n, double max_norm) {
   __shared__ double sh[4];
   double s = 0.0;
+#pragma unroll 4
   for (int i = threadIdx.x; i < n; i += 256) s += part[i];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
   __syncthreads();
+  Sum r;
+  r.norm = sqrt((sh[0] + sh[1]) + (sh[2] + sh[3]));
+  const double coef = max_norm / (r.norm + 1e-6);
+  r.coef = coef > 1.0 ? 1.0 : coef;               // a NaN norm stays NaN
+  return r;
+}
+
+__global__ __launch_bounds__(256) void norm_join_kernel(const double* __restrict__ part, int n, double max_norm,
+                                                        float* __restrict__ out2) {
+  const Sum s = join(part, n, max_norm);
   if (threadIdx.x) return;
-  const double norm = sqrt((sh[0] + sh[1]) + (sh[2] + sh[3]));
-  const double coef = max_norm / (norm + 1e-6);
-  out2[0] = (float)norm;
-  out2[1] = coef > 1.0 ? 1.f : (float)coef;       // a NaN norm stays NaN
+  out2[0] = (float)s.norm;
+  out2[1] = (float)s.coef;
 }
 
 template <int TI, int TO>
@@ -148,9 +158,16 @@ __device__ __forceinline__ void scale_to(int out_type, const void* in, void* out
   else scale_chunk<TI, DVAE_F16>(in, out, base, n, k);
 }
 
-// Chunks from the last to the first: the norm pass read the last ones last, so they are still in the 256 MB cache.
-__global__ __launch_bounds__(256) void scale_kernel(Batch b, const float* __restrict__ out2) {
-  const float k = out2[1];
+// Chunks from the last to the first: the norm pass read the last ones last, so they are still in the 256 MB cache.  Every
+// workgroup adds the partial sums (a few thousand at most, 4 us less than a launch of their own).
+__global__ __launch_bounds__(256) void scale_kernel(Batch b, const double* __restrict__ part, int n_part, double max_norm,
+                                                    float* __restrict__ out2) {
+  const Sum sum = join(part, n_part, max_norm);
+  const float k = (float)sum.coef;
+  if (out2 && blockIdx.x == 0 && threadIdx.x == 0) {
+    out2[0] = (float)sum.norm;
+    out2[1] = k;
+  }
   const int chunks = b.start[b.count];
   const Lookup tensor_of(b);
   for (int c = chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
@@ -245,32 +262,51 @@ extern "C" size_t dvae_clip_ws_bytes(int n) {
   return n < 0 ? 0 : ((size_t)n / CLIP_BATCH + 1) * 2 * MAX_GRID * sizeof(double);
 }
 
-extern "C" int dvae_grad_norm(const dvae_tensor* tensors, int n, double max_norm, float* norm_coef, void* ws, void* stream) {
-  DVAE_TRY(check_tensors(tensors, n, false, "grad_norm"));
-  DVAE_REQUIRE(norm_coef && ws, "grad_norm: null pointer");
-  DVAE_REQUIRE(max_norm >= 0.0, "grad_norm: max_norm must not be negative");
-  hipStream_t st = (hipStream_t)stream;
+namespace {
+
+// partial sums of all tensors -> ws; `used` their number
+int partials(const dvae_tensor* tensors, int n, double max_norm, const float* norm_coef, void* ws, int* used, const char* who,
+             hipStream_t st) {
+  DVAE_REQUIRE(norm_coef && ws, "%s: null pointer", who);
+  DVAE_REQUIRE(max_norm >= 0.0, "%s: max_norm must not be negative", who);
   double* part = (double*)ws;
   const size_t room = dvae_clip_ws_bytes(n) / sizeof(double);
-  size_t used = 0;
-  DVAE_TRY(for_batches(tensors, n, [&](const Batch& b, int grid) -> int {
-    DVAE_REQUIRE(used + grid <= room, "grad_norm: too many batches");
-    hipLaunchKernelGGL(norm_kernel, dim3(grid), dim3(256), 0, st, b, part + used);
+  *used = 0;
+  return for_batches(tensors, n, [&](const Batch& b, int grid) -> int {
+    DVAE_REQUIRE((size_t)*used + grid <= room, "%s: too many batches", who);
+    hipLaunchKernelGGL(norm_kernel, dim3(grid), dim3(256), 0, st, b, part + *used);
     DVAE_LAUNCH_CHECK();
-    used += grid;
+    *used += grid;
     return DVAE_OK;
-  }));
-  hipLaunchKernelGGL(norm_join_kernel, dim3(1), dim3(256), 0, st, part, (int)used, max_norm, norm_coef);
+  });
+}
+
+}  // namespace
+
+extern "C" int dvae_grad_norm(const dvae_tensor* tensors, int n, double max_norm, float* norm_coef, void* ws, void* stream) {
+  DVAE_TRY(check_tensors(tensors, n, false, "grad_norm"));
+  int used;
+  DVAE_TRY(partials(tensors, n, max_norm, norm_coef, ws, &used, "grad_norm", (hipStream_t)stream));
+  hipLaunchKernelGGL(norm_join_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, (const double*)ws, used, max_norm, norm_coef);
   DVAE_LAUNCH_CHECK();
   return DVAE_OK;
 }
 
 extern "C" int dvae_clip_grads(const dvae_tensor* tensors, int n, double max_norm, float* norm_coef, void* ws, void* stream) {
   DVAE_TRY(check_tensors(tensors, n, true, "clip_grads"));
-  DVAE_TRY(dvae_grad_norm(tensors, n, max_norm, norm_coef, ws, stream));
-  return for_batches(tensors, n, [&](const Batch& b, int grid) -> int {
-    hipLaunchKernelGGL(scale_kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, b, norm_coef);
+  hipStream_t st = (hipStream_t)stream;
+  int used;
+  DVAE_TRY(partials(tensors, n, max_norm, norm_coef, ws, &used, "clip_grads", st));
+  float* out2 = norm_coef;              // written by the first batch's launch
+  DVAE_TRY(for_batches(tensors, n, [&](const Batch& b, int grid) -> int {
+    hipLaunchKernelGGL(scale_kernel, dim3(grid), dim3(256), 0, st, b, (const double*)ws, used, max_norm, out2);
     DVAE_LAUNCH_CHECK();
+    out2 = nullptr;
     return DVAE_OK;
-  });
+  }));
+  if (out2) {                           // no elements at all
+    hipLaunchKernelGGL(norm_join_kernel, dim3(1), dim3(256), 0, st, (const double*)ws, 0, max_norm, norm_coef);
+    DVAE_LAUNCH_CHECK();
+  }
+  return DVAE_OK;
 }

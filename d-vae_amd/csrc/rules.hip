@@ -151,6 +151,25 @@ __device__ __forceinline__ double exp2_64(double d, double k) {
   return a != a ? a : a < -1000.0 ? 0.0 : w;
 }
 
+// log Z for Z > 0 in double: Z = 2^n c, c in [sqrt 1/2, sqrt 2), log c = 2 atanh t, t = (c - 1) / (c + 1), |t| < 0.172; the
+// first term left out of the series is t^18 / 19 of the result (9e-16).  A third of the math library's operations.
+__device__ __forceinline__ double log_64(double z) {
+  int n;
+  double c = frexp(z, &n);
+  if (c < 0.70710678118654752) { c += c; --n; }
+  const double t = (c - 1.0) * reciprocal(c + 1.0), u = t * t;
+  double s = 1.0 / 17.0;
+  s = fma(s, u, 1.0 / 15.0);
+  s = fma(s, u, 1.0 / 13.0);
+  s = fma(s, u, 1.0 / 11.0);
+  s = fma(s, u, 1.0 / 9.0);
+  s = fma(s, u, 1.0 / 7.0);
+  s = fma(s, u, 1.0 / 5.0);
+  s = fma(s, u, 1.0 / 3.0);
+  s = fma(s, u, 1.0);
+  return fma((double)n, LN2, 2.0 * t * s);
+}
+
 // what a segment leaves for the join
 struct Seg {
   double s;       // sum of 2^((x4 - ref) k)
@@ -742,7 +761,7 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
     if (MODE == M_SUM && !(t >= 0 && t < V)) lp = 0.f;          // an ignored row
     else if (m == -INFINITY) lp = -INFINITY;                    // the rules leave nothing
     else if (!ok || t < 0) lp = NAN;                            // NaN or +inf among the allowed values (or a NaN u)
-    else lp = (float)((y - (double)m) * (p.k * LN2) - log(Z));
+    else lp = (float)((y - (double)m) * (p.k * LN2) - log_64(Z));
     a.logprob[row] = lp;
     if (MODE == M_SUM) {
       a.stat[2 * row] = m == -INFINITY || ok ? m : NAN;
@@ -913,6 +932,178 @@ __device__ __forceinline__ X group_sum(X v, int w) {
   return v;
 }
 
+// a row's results: its token, `at` the token's value, m and Z the row's maximum and sum
+template <int MODE>
+__device__ __forceinline__ void end_row(const SmallArgs& a, const RowP& p, long long row, long long tok, double at, float m,
+                                        bool ok, double Z) {
+  const Rules& q = a.q;
+  const bool have = tok >= 0 && tok < q.vocab;
+  float lp;
+  if (MODE == M_SUM && !have) lp = 0.f;                   // an ignored row
+  else if (m == -INFINITY) lp = -INFINITY;                // the rules leave nothing
+  else if (!ok || !have) lp = NAN;                        // NaN or +inf among the allowed values (or a NaN u)
+  else lp = (float)((at - (double)m) * (p.k * LN2) - log_64(Z));
+  a.logprob[row] = lp;
+  if (MODE == M_SUM) {
+    a.stat[2 * row] = m == -INFINITY || ok ? m : NAN;
+    a.stat[2 * row + 1] = ok ? (float)reciprocal(Z) : NAN;
+  } else {
+    a.tokens[row] = tok;
+    if (a.state_out) {
+      const int s = q.state[row];
+      a.state_out[row] = tok >= 0 && s >= 0 && s < q.states ? a.next[(size_t)s * q.vocab + tok] : s;
+    }
+  }
+}
+
+// Vocabularies of up to VM = 8 or 16 tokens with many rows: a lane a row.  No sums or searches across lanes, and an eighth of
+// the operations of a group of lanes, whose single exp, log and decision each take a whole wave's time: 100000 x 8 drawn with
+// seven tokens of history 8.6 us (15.6 in groups).  But 64 rows a wave make few waves: at 32768 x 8 the two are even
+// (log p 5.2 / 6.1, gradients 5.4 / 4.4 us), so fewer rows take the groups.
+constexpr int TINY_VOCAB = 16, TINY_ROWS = 32768, TINY_HISTORY = 255;      // counts are bytes of a register
+
+template <int T, int VM, int MODE>
+__global__ __launch_bounds__(256) void rules_tiny_kernel(SmallArgs a) {
+  typedef Elem<T> E;
+  constexpr int EV = E::EV;
+  __shared__ float acc_sh[4][VM];
+  const Rules& q = a.q;
+  const int V = q.vocab;
+  float acc[VM];
+#pragma unroll
+  for (int v = 0; v < VM; ++v) acc[v] = 0.f;
+  for (long long row = (long long)blockIdx.x * 256 + threadIdx.x; row < q.rows; row += (long long)gridDim.x * 256) {
+    const RowP p = row_params(q, row);
+    const char* lrow = static_cast<const char*>(q.logits) + row * q.ld * (long long)sizeof(typename E::type);
+    float x[VM];
+    if (V == VM) {
+#pragma unroll
+      for (int i = 0; i < VM / EV; ++i) {
+        const u32x4 raw = *reinterpret_cast<const u32x4_u*>(lrow + 16 * i);
+#pragma unroll
+        for (int e = 0; e < EV; ++e) x[i * EV + e] = E::at(raw, e);
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < VM; ++v) x[v] = v < V ? E::one(lrow, v) : 0.f;
+    }
+    uint32_t keep = p.mask ? *reinterpret_cast<const uint32_t*>(p.mask) : 0xffffffffu;
+    keep &= (1u << V) - 1;
+    uint64_t c0 = 0, c1 = 0;
+    const auto add = [&](long long t) {
+      const uint64_t one = (unsigned long long)t < (unsigned long long)V ? 1ull << (8 * (t & 7)) : 0ull;
+      if (VM == 8 || t < 8) c0 += one;
+      else c1 += one;
+    };
+    int i = 0;
+    for (; i + 3 < p.n_hist; i += 4) {
+      long long t[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) t[u] = hist_at(p, q.history_i64, i + u);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) add(t[u]);
+    }
+    for (; i < p.n_hist; ++i) add(hist_at(p, q.history_i64, i));
+    const auto count = [&](int v) { return (uint32_t)((v < 8 ? c0 : c1) >> (8 * (v & 7))) & 0xffu; };
+    double y[VM];
+#pragma unroll
+    for (int v = 0; v < VM; ++v) {
+      const float b = p.bias && v < V ? p.bias[v] : 0.f;
+      y[v] = -INFINITY;
+      if ((keep >> v) & 1) y[v] = count(v) ? counted64(p, x[v], count(v), b) : (double)x[v] + (double)b;
+    }
+    if (MODE == M_APPLY || MODE == M_BWD) {
+      typename E::type o[VM];
+      if (MODE == M_BWD) {
+        const float m = a.stat[2 * row];
+        const long long tok = a.given[row];
+        const bool zero = tok < 0 || tok >= V || m == -INFINITY;
+        const double coef = (double)a.d_logprob[row] * (p.k * LN2), iz = a.stat[2 * row + 1];
+#pragma unroll
+        for (int v = 0; v < VM; ++v) {
+          double g = 0.0;
+          if (!zero && ((keep >> v) & 1)) g = coef * ((v == tok ? 1.0 : 0.0) - exp2_64(y[v] - (double)m, p.k) * iz);
+          const float gf = (float)g;
+          if (a.part) acc[v] += gf;
+          else if (a.d_bias && v < V) a.d_bias[row * V + v] = gf;
+          if (count(v)) g *= x[v] > 0.f ? p.inv_rho : p.rho;
+          o[v] = E::cast((float)g);
+        }
+      } else {
+#pragma unroll
+        for (int v = 0; v < VM; ++v) o[v] = E::cast((float)y[v]);
+      }
+      typename E::type* orow = static_cast<typename E::type*>(a.out) + row * a.out_ld;
+      if (V == VM) {
+#pragma unroll
+        for (int j = 0; j < VM / EV; ++j) {
+          u32x4 w;
+          __builtin_memcpy(&w, o + j * EV, 16);
+          *reinterpret_cast<u32x4_u*>(orow + j * EV) = w;
+        }
+      } else {
+#pragma unroll
+        for (int v = 0; v < VM; ++v)
+          if (v < V) orow[v] = o[v];
+      }
+      continue;
+    }
+    float m = (float)y[0];
+#pragma unroll
+    for (int v = 1; v < VM; ++v) m = max_nan(m, (float)y[v]);
+    const bool ok = m > -INFINITY && m < INFINITY && p.k > 0.0 && p.k < INFINITY;
+    double w[VM], Z = 0.0;
+#pragma unroll
+    for (int v = 0; v < VM; ++v) {
+      w[v] = ok && ((keep >> v) & 1) ? exp2_64(y[v] - (double)m, p.k) : 0.0;
+      Z += w[v];
+    }
+    int tok = -1;
+    if (MODE == M_SUM) {
+      const long long t = a.given[row];
+      tok = t >= 0 && t < V ? (int)t : -1;
+    } else if (ok && MODE == M_GREEDY) {
+      double best = -INFINITY;
+#pragma unroll
+      for (int v = 0; v < VM; ++v)
+        if (y[v] > best) { best = y[v]; tok = v; }
+    } else if (ok && MODE == M_DRAW) {
+      const float u = a.uniforms[row];
+      const double edge = fmax((double)u, 0.0) * Z;
+      double run = 0.0;
+      int last = -1;
+#pragma unroll
+      for (int v = 0; v < VM; ++v) {
+        run += w[v];
+        if (w[v] > 0.0) {
+          last = v;
+          if (run > edge && tok < 0) tok = v;
+        }
+      }
+      if (tok < 0) tok = last;
+      if (u != u) tok = -1;
+    }
+    double at = 0.0;
+#pragma unroll
+    for (int v = 0; v < VM; ++v)
+      if (v == tok) at = y[v];
+    end_row<MODE>(a, p, row, tok, at, m, ok, Z);
+  }
+  if (MODE == M_BWD) {
+    if (!a.part) return;
+    // the workgroup's share of the bias gradient, summed in a fixed order
+#pragma unroll
+    for (int v = 0; v < VM; ++v) {
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) acc[v] += __shfl_xor(acc[v], o);
+      if ((threadIdx.x & 63) == 0) acc_sh[threadIdx.x >> 6][v] = acc[v];
+    }
+    __syncthreads();
+    const int v = threadIdx.x;
+    if (v < V) a.part[(size_t)blockIdx.x * V + v] = (acc_sh[0][v] + acc_sh[1][v]) + (acc_sh[2][v] + acc_sh[3][v]);
+  }
+}
+
 template <int T, int MODE>
 __global__ __launch_bounds__(256) void rules_small_kernel(SmallArgs a) {
   typedef Elem<T> E;
@@ -990,25 +1181,8 @@ __global__ __launch_bounds__(256) void rules_small_kernel(SmallArgs a) {
         tok = hit != INT32_MAX ? hit : last;
       }
     }
-    const bool have = tok >= 0 && tok < V;
-    const double at = __shfl(y, have ? (int)tok : 0, W);
-    if (v) continue;
-    float lp;
-    if (MODE == M_SUM && !have) lp = 0.f;
-    else if (m == -INFINITY) lp = -INFINITY;
-    else if (!ok || !have) lp = NAN;
-    else lp = (float)((at - (double)m) * (p.k * LN2) - log(Z));
-    a.logprob[row] = lp;
-    if (MODE == M_SUM) {
-      a.stat[2 * row] = m == -INFINITY || ok ? m : NAN;
-      a.stat[2 * row + 1] = ok ? (float)(1.0 / Z) : NAN;
-    } else {
-      a.tokens[row] = tok;
-      if (a.state_out) {
-        const int s = q.state[row];
-        a.state_out[row] = tok >= 0 && s >= 0 && s < q.states ? a.next[(size_t)s * V + tok] : s;
-      }
-    }
+    const double at = __shfl(y, tok >= 0 && tok < V ? (int)tok : 0, W);
+    if (v == 0) end_row<MODE>(a, p, row, tok, at, m, ok, Z);
   }
   if (MODE == M_BWD) {
     if (!a.part) return;
@@ -1208,7 +1382,12 @@ int small_lanes(const dvae_rules& q) {
   return w;
 }
 
+bool is_tiny(const dvae_rules& q) {
+  return q.vocab <= TINY_VOCAB && q.rows >= TINY_ROWS && (!q.history || q.history_len <= TINY_HISTORY);
+}
+
 long long small_blocks(const dvae_rules& q) {
+  if (is_tiny(q)) return (q.rows + 255) / 256;
   const int groups = 256 / small_lanes(q);
   return std::min<long long>((q.rows + groups - 1) / groups, MAX_BLOCKS);
 }
@@ -1217,11 +1396,19 @@ template <int MODE>
 int run_small(SmallArgs& a, long long blocks, hipStream_t st) {
   a.w = small_lanes(a.q);
   const dim3 grid((unsigned)blocks), block(256);
+  const bool tiny = is_tiny(a.q), eight = a.q.vocab <= 8;
+#define SMALL(T)                                                                                                  \
+  do {                                                                                                            \
+    if (tiny && eight) hipLaunchKernelGGL((rules_tiny_kernel<T, 8, MODE>), grid, block, 0, st, a);                \
+    else if (tiny) hipLaunchKernelGGL((rules_tiny_kernel<T, 16, MODE>), grid, block, 0, st, a);                   \
+    else hipLaunchKernelGGL((rules_small_kernel<T, MODE>), grid, block, 0, st, a);                                \
+  } while (0)
   switch (a.q.dtype) {
-    case DVAE_F32: hipLaunchKernelGGL((rules_small_kernel<DVAE_F32, MODE>), grid, block, 0, st, a); break;
-    case DVAE_BF16: hipLaunchKernelGGL((rules_small_kernel<DVAE_BF16, MODE>), grid, block, 0, st, a); break;
-    default: hipLaunchKernelGGL((rules_small_kernel<DVAE_F16, MODE>), grid, block, 0, st, a);
+    case DVAE_F32: SMALL(DVAE_F32); break;
+    case DVAE_BF16: SMALL(DVAE_BF16); break;
+    default: SMALL(DVAE_F16);
   }
+#undef SMALL
   DVAE_LAUNCH_CHECK();
   return DVAE_OK;
 }
@@ -1262,7 +1449,7 @@ int rules_check(const dvae_rules& q, const char* who) {
 
 extern "C" size_t dvae_rules_ws_bytes(const dvae_rules* q) {
   if (!q || q->rows <= 0 || q->vocab < 1) return 0;
-  const size_t segs = (size_t)q->rows * plan_of(*q).nseg * sizeof(Seg);
+  const size_t segs = is_small(*q) ? 0 : (size_t)q->rows * plan_of(*q).nseg * sizeof(Seg);
   const size_t bias = q->bias && q->bias_ld == 0 ? (size_t)bias_shares(*q) * q->vocab * sizeof(float) : 0;
   return std::max(segs, bias);
 }
@@ -1290,7 +1477,7 @@ extern "C" int dvae_rules_choose(const dvae_rules* q, const float* uniforms, con
   DVAE_REQUIRE(q, "rules_choose: null pointer");
   DVAE_TRY(rules_check(*q, "rules_choose"));
   if (q->rows == 0) return DVAE_OK;
-  DVAE_REQUIRE(tokens && logprob && ws, "rules_choose: null pointer");
+  DVAE_REQUIRE(tokens && logprob && (ws || is_small(*q)), "rules_choose: null pointer");
   DVAE_REQUIRE((next == nullptr) == (state_out == nullptr), "rules_choose: next and state_out go together");
   DVAE_REQUIRE(!next || q->mask, "rules_choose: next states need a grammar mask");
   if (is_small(*q)) {
@@ -1318,7 +1505,7 @@ extern "C" int dvae_rules_logprob(const dvae_rules* q, const long long* tokens, 
   DVAE_REQUIRE(q, "rules_logprob: null pointer");
   DVAE_TRY(rules_check(*q, "rules_logprob"));
   if (q->rows == 0) return DVAE_OK;
-  DVAE_REQUIRE(tokens && logprob && stat && ws, "rules_logprob: null pointer");
+  DVAE_REQUIRE(tokens && logprob && stat && (ws || is_small(*q)), "rules_logprob: null pointer");
   if (is_small(*q)) {
     SmallArgs m{};
     m.q = with_constants(*q); m.given = tokens; m.logprob = logprob; m.stat = stat;

@@ -34,9 +34,7 @@ def _on_device(index, fn, *args):
 
 def _written(tensors):
     """Tells autograd that a kernel wrote these tensors in place."""
-    tensors = [t for t in tensors if not t.is_inference()]
-    if tensors:
-        torch.autograd.graph.increment_version(tensors)
+    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
 
 
 def _side(side):

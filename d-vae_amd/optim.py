@@ -31,18 +31,23 @@ def _flat_order(t):
 
 def _flat_list(ts, what, name):
     """Dense fp32 / bf16 / fp16 tensors on one device -> (addresses, sizes, types); each is one stretch of memory."""
-    where = None
-    for i, t in enumerate(ts):
+    try:
+        types = [_TYPES[t.dtype] for t in ts]
+        fine = all([t.layout is torch.strided and (t.is_contiguous() or _flat_order(t)) for t in ts]) and \
+            len({t.get_device() for t in ts}) <= 1
+        if fine:
+            return [t.data_ptr() for t in ts], [t.numel() for t in ts], types
+    except (AttributeError, KeyError):
+        pass
+    for i, t in enumerate(ts):           # which one it is
         if not isinstance(t, torch.Tensor) or t.layout != torch.strided or t.dtype not in _TYPES:
             raise ValueError("%s: %s %d must be a dense fp32, bf16 or fp16 tensor" % (what, name, i))
-        if where is None:
-            where = t.get_device()
-        elif t.get_device() != where:
+        if t.device != ts[0].device:
             raise ValueError("%s: %ss on %s and %s" % (what, name, ts[0].device, t.device))
-        if not (t.is_contiguous() or _flat_order(t)):
+        if not _flat_order(t):
             raise ValueError("%s: the elements of %s %d %s, strides %s, are not one stretch of memory" %
                              (what, name, i, tuple(t.shape), tuple(t.stride())))
-    return [t.data_ptr() for t in ts], [t.numel() for t in ts], [_TYPES[t.dtype] for t in ts]
+    raise ValueError("%s: %ss must be tensors" % (what, name))
 
 
 def _table(ins, outs):
@@ -84,7 +89,7 @@ def grad_norm(grads, max_norm=math.inf):
 
 def clip_grads(grads, max_norm, out=None):
     """Scales the gradients so that their norm (see ``grad_norm``) is at most ``max_norm``, in place or, with ``out`` (a
-    tensor of the same shape and memory order for each; any of the three types), into other tensors -- flat buffers, or
+    tensor for each, of any of the three types: contiguous as the gradient is, or of its shape and strides), into other tensors -- flat buffers, or
     single-precision copies of half-precision gradients.  Returns the norm before clipping, a scalar on the device.
     The reference's Lightning Trainer has this as ``gradient_clip_val`` (train.py:41-47).  A NaN norm makes the gradients
     NaN; an infinite one makes them 0 (NaN where they were infinite)."""
@@ -97,13 +102,13 @@ def clip_grads(grads, max_norm, out=None):
         if len(os_) != len(ts):
             raise ValueError("clip_grads: %d outputs for %d gradients" % (len(os_), len(ts)))
         outs = _flat_list(os_, "clip_grads", "output")
+        if outs[1] != ins[1] or (ts and os_[0].get_device() != ts[0].get_device()):
+            raise ValueError("clip_grads: outputs unlike the gradients: sizes %s for %s" % (outs[1], ins[1]))
         for i, (t, o) in enumerate(zip(ts, os_)):
-            if o.shape != t.shape or o.get_device() != t.get_device():
-                raise ValueError("clip_grads: output %d must be %s on %s" % (i, tuple(t.shape), t.device))
-            if not (t.is_contiguous() and o.is_contiguous()) and \
-                    any(n > 1 and a != b for n, a, b in zip(t.shape, t.stride(), o.stride())):
+            if not (t.is_contiguous() and o.is_contiguous()) and (t.shape != o.shape or any(
+                    n > 1 and a != b for n, a, b in zip(t.shape, t.stride(), o.stride()))):
                 raise ValueError("clip_grads: output %d is laid out unlike its gradient" % i)
-    if torch.is_grad_enabled() and any(o.requires_grad for o in os_):
+    if torch.is_grad_enabled() and any([o.requires_grad for o in os_]):
         raise ValueError("clip_grads: an output that requires a gradient is not written in place")
     if not ts:
         return torch.zeros(())

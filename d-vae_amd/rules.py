@@ -254,7 +254,12 @@ class _Call:
         return self._here(t, name)
 
     def workspace(self):
-        return E._workspace(load().dvae_rules_ws_bytes(self.q), self.logits.device)
+        """-> (address or None, tensor): the tensor is to live until the launch is queued."""
+        n = load().dvae_rules_ws_bytes(self.q)
+        if not n:
+            return None, None
+        ws = E._workspace(n, self.logits.device)
+        return ws.data_ptr(), ws
 
     def launch(self, fn, *args):
         E._on_device(self.index, fn, self.q, *args)
@@ -316,47 +321,55 @@ def choose(logits, rules=None, history=None, lengths=None, state=None, temperatu
     u = None
     if uniforms is not None:
         u = c._per_row(uniforms, "uniforms", (torch.float32,)).contiguous()
-    dev = logits.device
-    tokens = torch.empty(c.lead, dtype=torch.int64, device=dev)
-    logprob = torch.empty(c.lead, dtype=torch.float32, device=dev)
+    tokens = logits.new_empty(c.lead, dtype=torch.int64)
+    logprob = logits.new_empty(c.lead, dtype=torch.float32)
     following = nxt = None
     if rules is not None and rules.grammar is not None and rules.grammar.next_state is not None:
         nxt = c._here(rules.grammar.next_state, "grammar")
-        following = torch.empty(c.lead, dtype=torch.int32, device=dev)
-    ws = c.workspace()
+        following = logits.new_empty(c.lead, dtype=torch.int32)
+    at, ws = c.workspace()
     c.launch(load().dvae_rules_choose, _address(u), _address(nxt), tokens.data_ptr(), logprob.data_ptr(),
-             _address(following), ws.data_ptr())
+             _address(following), at)
     return Choice(tokens, logprob, following)
 
 
 class _LogprobFn(torch.autograd.Function):
-    # every tensor behind a pointer goes through save_for_backward: a change between forward and backward is an error
+    # Every tensor behind a pointer goes through save_for_backward: a change between forward and backward is an error.  The
+    # backward pass runs on autograd's own thread, where Python is slowest: what it needs is at hand when the forward pass ends.
     @staticmethod
     def forward(ctx, call, logits, bias, tokens, *others):
-        dev = logits.device
-        ws = call.workspace()
-        logprob = torch.empty(call.rows, dtype=torch.float32, device=dev)
-        stat = torch.empty(call.rows, 2, dtype=torch.float32, device=dev)
-        call.launch(load().dvae_rules_logprob, tokens.data_ptr(), logprob.data_ptr(), stat.data_ptr(), ws.data_ptr())
-        ctx.call, ctx.stat = call, stat
+        lib = load()
+        ws, keep = call.workspace()
+        logprob = logits.new_empty(call.rows, dtype=torch.float32)
+        stat = logits.new_empty((call.rows, 2), dtype=torch.float32)
+        at = tokens.data_ptr(), stat.data_ptr()
+        call.launch(lib.dvae_rules_logprob, at[0], logprob.data_ptr(), at[1], ws)
+        ctx.call, ctx.stat, ctx.at, ctx.fn = call, stat, at, lib.dvae_rules_logprob_bwd
         ctx.save_for_backward(logits, bias, tokens, *others)
         return logprob
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, d_logprob):
-        call, stat = ctx.call, ctx.stat
-        logits, bias, tokens = ctx.saved_tensors[:3]          # checks every saved tensor's version
+        if torch.is_grad_enabled():                           # create_graph: the result refuses to be differentiated
+            return once_differentiable(_LogprobFn._gradients)(ctx, d_logprob)
+        return _LogprobFn._gradients(ctx, d_logprob)
+
+    @staticmethod
+    def _gradients(ctx, d_logprob):
+        call = ctx.call
+        saved = ctx.saved_tensors                             # checks every saved tensor's version
+        logits = saved[0]
         if d_logprob.dtype != torch.float32 or not d_logprob.is_contiguous():
             d_logprob = d_logprob.to(torch.float32).contiguous()
-        d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        d_bias = None
-        if ctx.needs_input_grad[2]:
-            d_bias = torch.empty(bias.shape, dtype=torch.float32, device=logits.device)
-        ws = call.workspace()
-        call.launch(load().dvae_rules_logprob_bwd, tokens.data_ptr(), stat.data_ptr(), d_logprob.data_ptr(),
-                    d_logits.data_ptr(), call.V, _address(d_bias), ws.data_ptr())
-        return (None, d_logits if ctx.needs_input_grad[1] else None, d_bias) + (None,) * (len(ctx.needs_input_grad) - 3)
+        d_logits = torch.empty_like(logits, memory_format=torch.contiguous_format)
+        d_bias = ws = None
+        _, want_logits, want_bias, *rest = ctx.needs_input_grad
+        if want_bias:
+            d_bias = torch.empty_like(saved[1], memory_format=torch.contiguous_format)
+            ws, keep = call.workspace()
+        call.launch(ctx.fn, *ctx.at, d_logprob.data_ptr(), d_logits.data_ptr(), call.V,
+                    None if d_bias is None else d_bias.data_ptr(), ws)
+        return None, d_logits if want_logits else None, d_bias, *([None] * len(rest))
 
 
 def token_logprob(logits, tokens, rules=None, history=None, lengths=None, state=None, temperature=1.0):

@@ -525,7 +525,7 @@ typedef struct dvae_rules {
   int mask_words, states;
   const int* state;           /* [rows]: the row's state; one outside [0, states) allows everything                   */
 } dvae_rules;
-/* ws of choose / logprob / logprob_bwd; 0 for arguments they refuse */
+/* ws of choose / logprob / logprob_bwd; 0: they take NULL (and for arguments they refuse) */
 size_t dvae_rules_ws_bytes(const dvae_rules* rules);
 /* out [rows][out_ld] (of the logits' type; may be the logits) = x4 */
 int dvae_rules_apply(const dvae_rules* rules, void* out, long long out_ld, void* stream);

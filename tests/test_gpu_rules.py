@@ -240,6 +240,55 @@ def test_many_rows_share_one_bias(cuda):
     check_logprob(cuda, case, x, b, lp, dx, db, case.g)
 
 
+@pytest.mark.parametrize("shape", [dict(vocab=8, L=7, index=torch.int32, states=5, free=True),
+                                   dict(vocab=5, L=200, ragged=True, dtype="bf16", bias="shared", per_row=True, junk=True),
+                                   dict(vocab=16, L=9, dtype="fp16", bias="rows", states=3, per_row=True, pad=1),
+                                   dict(vocab=11, L=3, states=4), dict(vocab=1), dict(vocab=8, L=255),
+                                   dict(vocab=13, L=256, states=2)], ids=ident)
+def test_many_rows_of_a_few_tokens(cuda, shape):
+    """32800 rows: a lane a row.  The oracle sees 200 rows spread over them (the bias gradient: all)."""
+    from dvae_amd.rules import apply_rules, choose, token_logprob
+    rows = 32800
+    case = Case(rows=rows, seed=12, drawn=True, **shape)
+    x, kw, temp = case.big.to(cuda)[:, :case.vocab], case.kw(cuda), case.temperature(cuda)
+    some = list(range(0, rows, 167)) + [rows - 1]
+    got = apply_rules(x, case.rules(cuda), **kw).double().cpu().numpy()
+    draw = choose(x, case.rules(cuda), temperature=temp, uniforms=case.u.to(cuda), **kw)
+    best = choose(x, case.rules(cuda), temperature=temp, **kw)
+    picked = [(c.tokens.tolist(), c.logprob.tolist(), None if c.state is None else c.state.tolist()) for c in (draw, best)]
+    x = x.requires_grad_(True)
+    shared = case.bias is not None and case.bias.dim() == 1
+    b = case.bias.to(cuda).requires_grad_(True) if case.bias is not None else None
+    lp = token_logprob(x, case.tokens.to(cuda), case.rules(cuda, b), temperature=temp, **kw)
+    grads = torch.autograd.grad(lp, [x] + ([] if b is None else [b]), case.g.to(cuda))
+    dx, values = grads[0].double().cpu().numpy(), lp.tolist()
+    total, off = np.zeros(case.vocab), np.zeros(case.vocab)
+    for r in (range(rows) if shared else some):
+        y, slope, al, t = case.row(r)
+        want, d, dv = R.logprob_row(y, slope, int(case.tokens[r]), t, float(case.g[r]), al)
+        same_or_close(values[r], want, U * abs(want) + 1e-11 if math.isfinite(want) else 0.0, "log p of row %d" % r)
+        # doubles but for 1 / Z and the maximum, each rounded once: 2 roundings of p, one of d and the type's
+        p = np.exp(R.log_softmax(y, t)[0])
+        scale = abs(float(case.g[r])) / t
+        fin = np.where(np.isfinite(y), np.abs(y), 0.0).max()
+        err = scale * p * (2 * U + U * fin / t) + U * np.abs(dv)
+        same_or_close(dx[r], d, err * slope + (half(case.dtype) + U) * np.abs(d) + TINY[case.dtype], "d logits of row %d" % r)
+        total, off = total + dv, off + err + rows * U * np.abs(dv)
+        if r in (some if not shared else some[:50]):
+            same_or_close(got[r], y, (half(case.dtype) + U) * np.abs(np.where(np.isfinite(y), y, 0)) + TINY[case.dtype], "row %d" % r)
+            for (tok, lps, st), u in zip(picked, (float(case.u[r]), None)):
+                k, l = R.choose_row(y, t, u)
+                assert tok[r] == k, (r, tok[r], k)
+                same_or_close(lps[r], l, U * abs(l) + 1e-11 if math.isfinite(l) else 0.0, "row %d" % r)
+                if st is not None:
+                    s = int(case.state[r])
+                    assert st[r] == (int(case.next[s, k]) if k >= 0 and 0 <= s < case.next.shape[0] else s)
+    if shared:
+        same_or_close(grads[1].double().cpu().numpy(), total, off, "d bias")
+    elif b is not None:
+        assert grads[1].shape == b.shape
+
+
 def test_gradient_against_differences(cuda):
     """Central differences of the kernel's own log p along directions of +-1: the third derivative of a log-sum-exp along
     such a direction is a third central moment of a variable of +-1/T, at most 0.77 / T^3 (the Bernoulli extreme,

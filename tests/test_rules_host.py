@@ -167,7 +167,10 @@ def test_c_abi_refuses_missing_pointers():
     assert lib.dvae_rules_apply(r, None, 16, None) == -1
     assert lib.dvae_rules_apply(r, p, 15, None) == -1
     assert lib.dvae_rules_choose(r, None, None, None, p, None, p, None) == -1
-    assert lib.dvae_rules_choose(r, None, None, p, p, None, None, None) == -1
+    large = _q(vocab=4000, ld=4000)
+    assert lib.dvae_rules_ws_bytes(r) == 0 and lib.dvae_rules_ws_bytes(ctypes.byref(large)) > 0
+    assert lib.dvae_rules_choose(ctypes.byref(large), None, None, p, p, None, None, None) == -1
+    assert lib.dvae_rules_logprob(ctypes.byref(large), p, p, p, None, None) == -1
     assert lib.dvae_rules_choose(r, None, p, p, p, None, p, None) == -1          # next without state_out
     assert lib.dvae_rules_choose(r, None, p, p, p, p, p, None) == -1             # next without a mask
     assert lib.dvae_rules_logprob(r, None, p, p, p, None) == -1
