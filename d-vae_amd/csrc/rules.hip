@@ -228,17 +228,18 @@ __device__ __forceinline__ void count_history(const RowP& p, int i64, long long 
   for (; i < p.n_hist; i += width) add(hist_at(p, i64, i) - v0);
 }
 
-// A step of a wave: 64 x EV tokens, from v on in this lane.  Every step but a row's last is whole in every lane (`whole`, the
-// same for the wave): no bounds in it.
+// A step of a wave: 64 x EV tokens, from v on in this lane.  WHOLE: inside the vocabulary in every lane, as every step but a
+// row's last is.
 struct Loaded { u32x4 raw; uint32_t keep; };       // keep, bit e: allowed (and inside the vocabulary)
 
-template <int T>
-__device__ __forceinline__ Loaded load_step(const RowP& p, const char* lrow, int v, int V, bool whole) {
+template <int T, bool WHOLE>
+__device__ __forceinline__ Loaded load_step(const RowP& p, const char* lrow, int v, int V) {
   constexpr int EV = Elem<T>::EV, BYTES = 16 / EV;
   Loaded l;
   l.keep = (1u << EV) - 1;
-  if (whole || v + EV <= V) {
-    l.raw = *reinterpret_cast<const u32x4_u*>(lrow + (size_t)v * BYTES);
+  if (WHOLE || v + EV <= V) {
+    // read once: not to push out what is read again
+    l.raw = __builtin_nontemporal_load(reinterpret_cast<const u32x4_u*>(lrow + (size_t)v * BYTES));
   } else {
     l.raw = u32x4{0, 0, 0, 0};
     l.keep = v < V ? (1u << (V - v)) - 1 : 0u;
@@ -249,12 +250,77 @@ __device__ __forceinline__ Loaded load_step(const RowP& p, const char* lrow, int
         else l.raw[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(lrow)[v + e] << ((e & 1) * 16);
       }
   }
-  if (p.mask && (whole || v < V)) {
+  if (p.mask && (WHOLE || v < V)) {
     const uint32_t byte = p.mask[v >> 3];
     l.keep &= EV == 8 ? byte : byte >> (v & 4);
   }
   return l;
 }
+
+// bias of the step's tokens, 0 past the vocabulary
+template <int EV, bool WHOLE>
+__device__ __forceinline__ void load_bias(const float* bias, int v, int V, float (&b)[EV]) {
+  if (WHOLE || v + EV <= V) {
+#pragma unroll
+    for (int e = 0; e < EV; e += 4) {
+      const f32x4_u t = *reinterpret_cast<const f32x4_u*>(bias + v + e);
+      b[e] = t[0]; b[e + 1] = t[1]; b[e + 2] = t[2]; b[e + 3] = t[3];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < EV; ++e) b[e] = v + e < V ? bias[v + e] : 0.f;
+  }
+}
+
+template <int T, bool WHOLE>
+__device__ __forceinline__ void store_step(typename Elem<T>::type* orow, int v, int V, const float (&y)[Elem<T>::EV]) {
+  constexpr int EV = Elem<T>::EV;
+  typename Elem<T>::type o[EV];
+#pragma unroll
+  for (int e = 0; e < EV; ++e) o[e] = Elem<T>::cast(y[e]);
+  if (WHOLE || v + EV <= V) {
+    u32x4 w;
+    __builtin_memcpy(&w, o, 16);
+    __builtin_nontemporal_store(w, reinterpret_cast<u32x4_u*>(orow + v));
+  } else {
+#pragma unroll
+    for (int e = 0; e < EV; ++e)
+      if (v + e < V) orow[v + e] = o[e];
+  }
+}
+
+// A segment's steps: D of the whole ones in flight (each in registers of its own: moving a load from one to another would
+// wait for it), then the partial one, if there is one.  begin() before the history is counted, so that the loads travel
+// meanwhile; f(loaded, v, whole) for each step.
+template <int T, int D>
+struct Steps {
+  static constexpr int EV = Elem<T>::EV, STEP = 64 * EV;
+  Loaded l[D];
+  int full, v, end;                // v: this lane's first token
+  __device__ __forceinline__ void begin(const RowP& p, const char* lrow, int v0, int stop, int lane, int V) {
+    full = (stop - v0) / STEP;
+    v = v0 + lane * EV;
+    end = stop;
+#pragma unroll
+    for (int j = 0; j < D; ++j)
+      if (j < full) l[j] = load_step<T, true>(p, lrow, v + j * STEP, V);
+  }
+  template <typename F>
+  __device__ __forceinline__ void run(const RowP& p, const char* lrow, int V, F f) {
+    int at = v;
+    for (int g = 0; g < full; g += D) {
+#pragma unroll
+      for (int j = 0; j < D; ++j)
+        if (g + j < full) {
+          const Loaded in = l[j];
+          if (g + j + D < full) l[j] = load_step<T, true>(p, lrow, at + D * STEP, V);
+          f(in, at, std::true_type{});
+          at += STEP;
+        }
+    }
+    if (at < end) f(load_step<T, false>(p, lrow, at, V), at, std::false_type{});
+  }
+};
 
 // The values under the rules.  Forbidden places: x = -inf and b = 0 before anything is computed, so that nothing they hold
 // shows.  Counted tokens are few: one test for the whole step, then one branch each.
@@ -272,11 +338,13 @@ struct Ruled {
     return HIST == 2 ? cw[e] : 0u;
   }
   // cnt: the counts from this lane's first token on
-  __device__ __forceinline__ Ruled(const RowP& p, const Loaded& in, const uint32_t* cnt, int v, int V, bool whole) {
+  template <typename W>
+  __device__ __forceinline__ Ruled(const RowP& p, const Loaded& in, const uint32_t* cnt, int v, int V, W) {
+    constexpr bool WHOLE = W::value;
     const auto on = [&](int e) { return (uint32_t)((int)(in.keep << (31 - e)) >> 31); };
 #pragma unroll
     for (int e = 0; e < EV; ++e) x[e] = E::at(in.raw, e);
-    if (p.mask || !whole) {
+    if (p.mask || !WHOLE) {
 #pragma unroll
       for (int e = 0; e < EV; ++e) x[e] = __uint_as_float((__float_as_uint(x[e]) & on(e)) | (0xff800000u & ~on(e)));
     }
@@ -287,16 +355,7 @@ struct Ruled {
     }
     float b[EV];
     if (p.bias) {
-      if (whole || v + EV <= V) {
-#pragma unroll
-        for (int e = 0; e < EV; e += 4) {
-          const f32x4_u t = *reinterpret_cast<const f32x4_u*>(p.bias + v + e);
-          b[e] = t[0]; b[e + 1] = t[1]; b[e + 2] = t[2]; b[e + 3] = t[3];
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < EV; ++e) b[e] = v + e < V ? p.bias[v + e] : 0.f;
-      }
+      load_bias<EV, WHOLE>(p.bias, v, V, b);
       if (p.mask) {
 #pragma unroll
         for (int e = 0; e < EV; ++e) b[e] = __uint_as_float(__float_as_uint(b[e]) & on(e));
@@ -382,10 +441,8 @@ __global__ __launch_bounds__(256) void rules_map_kernel(SegArgs a) {
   const RowP p = row_params(q, row < q.rows ? row : q.rows - 1);
   const int end = min(v0 + a.seg_len, V);
   const char* lrow = static_cast<const char*>(q.logits) + row * q.ld * (long long)sizeof(typename E::type);
-  const int full = (end - v0) / STEP, steps = (end - v0 + STEP - 1) / STEP;
-  int v = v0 + lane * EV;
-  Loaded ahead{};                                 // the first step's loads are on their way while the history is counted
-  if (live) ahead = load_step<T>(p, lrow, v, V, full > 0);
+  Steps<T, 4> steps;
+  if (live) steps.begin(p, lrow, v0, end, lane, V);
   const uint32_t* cnt = lds;
   if (HIST) {
     const int words = 4 * a.seg_len / Counts<HIST ? HIST : 1>::PER_WORD;
@@ -407,11 +464,7 @@ __global__ __launch_bounds__(256) void rules_map_kernel(SegArgs a) {
   typename E::type* orow = static_cast<typename E::type*>(a.out) + row * a.out_ld;
   Bwd b;
   if (MODE == M_BWD) b = Bwd(a, p, row);
-  for (int i = 0; i < steps; ++i, v += STEP) {
-    const Loaded in = ahead;
-    const bool whole = i < full;
-    if (i + 1 < steps) ahead = load_step<T>(p, lrow, v + STEP, V, i + 1 < full);
-    if (v >= end) continue;
+  steps.run(p, lrow, V, [&](const Loaded& in, int v, auto whole) {
     const Ruled<T, HIST> r(p, in, cnt + (v - v0) / PER, v, V, whole);
     float y[EV];
 #pragma unroll
@@ -425,19 +478,8 @@ __global__ __launch_bounds__(256) void rules_map_kernel(SegArgs a) {
       }
       b.slope(r, y);
     }
-    typename E::type o[EV];
-#pragma unroll
-    for (int e = 0; e < EV; ++e) o[e] = E::cast(y[e]);
-    if (whole || v + EV <= V) {
-      u32x4 w;
-      __builtin_memcpy(&w, o, 16);
-      *reinterpret_cast<u32x4_u*>(orow + v) = w;
-    } else {
-#pragma unroll
-      for (int e = 0; e < EV; ++e)
-        if (v + e < V) orow[v + e] = o[e];
-    }
-  }
+    store_step<T, decltype(whole)::value>(orow, v, V, y);
+  });
 }
 
 // value of one token in 64 bits, -inf where the grammar forbids it
@@ -488,9 +530,8 @@ __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
   const RowP p = row_params(q, row < q.rows ? row : q.rows - 1);
   const int end = min(v0 + a.seg_len, V);
   const char* lrow = static_cast<const char*>(q.logits) + row * q.ld * (long long)sizeof(typename E::type);
-  const int full = (end - v0) / STEP, steps = (end - v0 + STEP - 1) / STEP;
-  Loaded begun{};                                 // the first step's loads are on their way while the history is counted
-  if (live) begun = load_step<T>(p, lrow, v0 + lane * EV, V, full > 0);
+  Steps<T, DRAW ? 2 : 4> steps;
+  if (live) steps.begin(p, lrow, v0, end, lane, V);
   const uint32_t *cnt = lds, *seen = lds;
   if (HIST) {
     const int words = 4 * a.seg_len / Counts<HIST ? HIST : 1>::PER_WORD, marks = 4 * a.seg_len / 32;
@@ -550,13 +591,8 @@ __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
   };
   const auto scan = [&](auto shifted, double base) {
     const auto weigh = [&](double y) { zd += exp2_fast(decltype(shifted)::value ? y - base : y, p.k, low); };
-    int v = v0 + lane * EV;
-    Loaded ahead = decltype(shifted)::value ? load_step<T>(p, lrow, v, V, full > 0) : begun;
-    for (int i = 0; i < steps; ++i, v += STEP) {
-      Loaded in = ahead;
-      const bool whole = i < full;
-      if (i + 1 < steps) ahead = load_step<T>(p, lrow, v + STEP, V, i + 1 < full);
-      if (v >= end) continue;
+    steps.run(p, lrow, V, [&](Loaded in, int v, auto whole) {
+      constexpr bool WHOLE = decltype(whole)::value;
       if (HIST) {
         const uint32_t byte = reinterpret_cast<const uint8_t*>(seen)[(v - v0) >> 3];
         in.keep &= ~(EV == 8 ? byte : byte >> (v & 4));
@@ -565,22 +601,13 @@ __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
 #pragma unroll
       for (int e = 0; e < EV; ++e) x[e] = E::at(in.raw, e);
       const auto on = [&](int e) { return (uint32_t)((int)(in.keep << (31 - e)) >> 31); };
-      if (HIST || p.mask || !whole) {
+      if (HIST || p.mask || !WHOLE) {
 #pragma unroll
         for (int e = 0; e < EV; ++e) x[e] = __uint_as_float((__float_as_uint(x[e]) & on(e)) | (0xff800000u & ~on(e)));
       }
       if (p.bias) {
         float b[EV];
-        if (whole || v + EV <= V) {
-#pragma unroll
-          for (int e = 0; e < EV; e += 4) {
-            const f32x4_u t = *reinterpret_cast<const f32x4_u*>(p.bias + v + e);
-            b[e] = t[0]; b[e + 1] = t[1]; b[e + 2] = t[2]; b[e + 3] = t[3];
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < EV; ++e) b[e] = v + e < V ? p.bias[v + e] : 0.f;
-        }
+        load_bias<EV, WHOLE>(p.bias, v, V, b);
         if (HIST || p.mask) {
 #pragma unroll
           for (int e = 0; e < EV; ++e) b[e] = __uint_as_float(__float_as_uint(b[e]) & on(e));
@@ -607,7 +634,7 @@ __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
 #pragma unroll
         for (int e = 0; e < EV; ++e) z += __builtin_amdgcn_exp2f((s[e] - ref) * kf);
       }
-    }
+    });
     if (HIST) {
       const auto one = [&](double y) {
         take((float)y);
@@ -643,6 +670,7 @@ __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
       if (!(top > -400.0 && top < 900.0)) {
         r.ref = m;
         zd = 0.0;
+        steps.begin(p, lrow, v0, end, lane, V);
         scan(std::true_type{}, (double)m);
       }
       r.s = wave_sum(zd);
@@ -1233,7 +1261,11 @@ __global__ __launch_bounds__(256) void rules_bwd_col_kernel(ColArgs ca) {
     typename E::type* orow = static_cast<typename E::type*>(a.out) + row * a.out_ld;
     Loaded in[COL_STEPS];
 #pragma unroll
-    for (int j = 0; j < COL_STEPS; ++j) in[j] = load_step<T>(p, lrow, v0 + j * STEP + lane * EV, V, v0 + (j + 1) * STEP <= V);
+    for (int j = 0; j < COL_STEPS; ++j) {
+      const int v = v0 + j * STEP + lane * EV;
+      if (v0 + (j + 1) * STEP <= V) in[j] = load_step<T, true>(p, lrow, v, V);
+      else in[j] = load_step<T, false>(p, lrow, v, V);
+    }
     if (HIST) {
       for (int i = lane * 4; i < SPAN / PER; i += 256) *reinterpret_cast<u32x4*>(&cnt[i]) = u32x4{0, 0, 0, 0};
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -1245,26 +1277,17 @@ __global__ __launch_bounds__(256) void rules_bwd_col_kernel(ColArgs ca) {
 #pragma unroll
     for (int j = 0; j < COL_STEPS; ++j) {
       const int d = j * STEP + lane * EV, v = v0 + d;
-      const bool whole = v0 + (j + 1) * STEP <= V;
-      if (v >= V) continue;
-      const Ruled<T, HIST> r(p, in[j], cnt + d / PER, v, V, whole);
-      float y[EV];
-      b.values(r, in[j].keep, v, y);
+      const auto step = [&](auto whole) {
+        const Ruled<T, HIST> r(p, in[j], cnt + d / PER, v, V, whole);
+        float y[EV];
+        b.values(r, in[j].keep, v, y);
 #pragma unroll
-      for (int e = 0; e < EV; ++e) acc[j][e] += y[e];
-      b.slope(r, y);
-      typename E::type o[EV];
-#pragma unroll
-      for (int e = 0; e < EV; ++e) o[e] = E::cast(y[e]);
-      if (whole || v + EV <= V) {
-        u32x4 w;
-        __builtin_memcpy(&w, o, 16);
-        *reinterpret_cast<u32x4_u*>(orow + v) = w;
-      } else {
-#pragma unroll
-        for (int e = 0; e < EV; ++e)
-          if (v + e < V) orow[v + e] = o[e];
-      }
+        for (int e = 0; e < EV; ++e) acc[j][e] += y[e];
+        b.slope(r, y);
+        store_step<T, decltype(whole)::value>(orow, v, V, y);
+      };
+      if (v0 + (j + 1) * STEP <= V) step(std::true_type{});
+      else if (v < V) step(std::false_type{});
     }
   }
   __syncthreads();

@@ -7,7 +7,7 @@ unchanged) and its `state_dict()` has torch Adam's layout (`step`, `exp_avg`, `e
 checkpoints move between the two.  The model's parameters become views of one flat buffer per module (same
 `nn.Parameter` objects, same values), laid out like the flat gradient buffers `Dvae.loss_and_grad` fills.
 """
-import ctypes
+import array
 import math
 
 import torch
@@ -56,7 +56,7 @@ def _table(ins, outs):
     flat = [0] * (4 * len(pi))
     flat[0::4], flat[1::4], flat[2::4] = pi, po, n
     flat[3::4] = [a | b << 32 for a, b in zip(ti, to)]
-    return (ctypes.c_longlong * max(len(flat), 4))(*flat)
+    return array.array('q', flat or [0])
 
 
 def _as_list(ts):
@@ -83,14 +83,15 @@ def grad_norm(grads, max_norm=math.inf):
     out = torch.empty(2, device=ts[0].device)
     lib = E.load()
     ws = E._workspace(lib.dvae_clip_ws_bytes(len(ts)), ts[0].device)
-    E._on_device(ts[0].get_device(), lib.dvae_grad_norm, _table(ins, ins), len(ts), m, out.data_ptr(), ws.data_ptr())
+    table = _table(ins, ins)
+    E._on_device(ts[0].get_device(), lib.dvae_grad_norm, table.buffer_info()[0], len(ts), m, out.data_ptr(), ws.data_ptr())
     return out[0], out[1]
 
 
 def clip_grads(grads, max_norm, out=None):
     """Scales the gradients so that their norm (see ``grad_norm``) is at most ``max_norm``, in place or, with ``out`` (a
-    tensor for each, of any of the three types: contiguous as the gradient is, or of its shape and strides), into other tensors -- flat buffers, or
-    single-precision copies of half-precision gradients.  Returns the norm before clipping, a scalar on the device.
+    tensor for each, of any of the three types: contiguous as the gradient is, or of its shape and strides), into other
+    tensors -- flat buffers, or single-precision copies of half-precision gradients.  Returns the norm before clipping, a scalar on the device.
     The reference's Lightning Trainer has this as ``gradient_clip_val`` (train.py:41-47).  A NaN norm makes the gradients
     NaN; an infinite one makes them 0 (NaN where they were infinite)."""
     m = _limit(max_norm, "clip_grads")
@@ -116,7 +117,8 @@ def clip_grads(grads, max_norm, out=None):
     norm = torch.empty(2, device=ts[0].device)
     lib = E.load()
     ws = E._workspace(lib.dvae_clip_ws_bytes(len(ts)), ts[0].device)
-    E._on_device(ts[0].get_device(), lib.dvae_clip_grads, _table(ins, outs), len(ts), m, norm.data_ptr(), ws.data_ptr())
+    table = _table(ins, outs)
+    E._on_device(ts[0].get_device(), lib.dvae_clip_grads, table.buffer_info()[0], len(ts), m, norm.data_ptr(), ws.data_ptr())
     E._written(os_)
     return norm[0]
 
