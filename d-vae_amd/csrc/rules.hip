@@ -91,6 +91,20 @@ __device__ __forceinline__ long long hist_at(const RowP& p, int i64, int i) {
   return i64 ? reinterpret_cast<const long long*>(p.hist)[i] : (long long)reinterpret_cast<const int*>(p.hist)[i];
 }
 
+// f(token) for the history's tokens from `from` on, `lane` of `width` threads; N loads in flight, whatever the length
+template <int N, typename F>
+__device__ __forceinline__ void for_history(const RowP& p, int i64, int from, int lane, int width, F f) {
+  for (int i = from + lane; i < p.n_hist; i += N * width) {
+    long long t[N];
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+      if (i + u * width < p.n_hist) t[u] = hist_at(p, i64, i + u * width);
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+      if (i + u * width < p.n_hist) f(t[u]);
+  }
+}
+
 // the value of a token that the history holds c > 0 times.  x / rho as x (1 / rho) with one correction step: as good as
 // the division (equal quotients stay equal, so ties stay ties) at four operations
 __device__ __forceinline__ double counted64(const RowP& p, float x, uint32_t c, float b) {
@@ -209,7 +223,8 @@ __device__ __forceinline__ uint32_t count_at(const uint32_t* lds, int d) {
 template <int HIST>
 __device__ __forceinline__ void count_history(const RowP& p, int i64, long long v0, int span, uint32_t* lds, uint32_t* bits,
                                               int lane, int width) {
-  const auto add = [&](long long t) {
+  const auto add = [&](long long token) {
+    const long long t = token - v0;
     if ((unsigned long long)t < (unsigned long long)span) {
       const int d = (int)t;
       if (HIST == 1) atomicAdd(&lds[d >> 1], (d & 1) ? 0x10000u : 1u);
@@ -217,15 +232,8 @@ __device__ __forceinline__ void count_history(const RowP& p, int i64, long long 
       if (bits) atomicOr(&bits[d >> 5], 1u << (d & 31));
     }
   };
-  int i = lane;
-  for (; i + 3 * width < p.n_hist; i += 4 * width) {
-    long long t[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) t[u] = hist_at(p, i64, i + u * width) - v0;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) add(t[u]);
-  }
-  for (; i < p.n_hist; i += width) add(hist_at(p, i64, i) - v0);
+  if (p.n_hist > 4 * width) for_history<8>(p, i64, 0, lane, width, add);
+  else for_history<4>(p, i64, 0, lane, width, add);
 }
 
 // A step of a wave: 64 x EV tokens, from v on in this lane.  WHOLE: inside the vocabulary in every lane, as every step but a
@@ -428,7 +436,7 @@ struct Bwd {
 template <int T, int HIST, int MODE, bool ROWWAVE>
 __global__ __launch_bounds__(256) void rules_map_kernel(SegArgs a) {
   typedef Elem<T> E;
-  constexpr int EV = E::EV, STEP = 64 * EV;
+  constexpr int EV = E::EV;
   extern __shared__ uint32_t lds[];          // counts of the workgroup's 4 segments
   const Rules& q = a.q;
   const int lane = threadIdx.x & 63;
@@ -458,7 +466,6 @@ __global__ __launch_bounds__(256) void rules_map_kernel(SegArgs a) {
     cnt = lds + wave * (words / 4);
   }
   if (!live) return;
-  const float kf = (float)p.k;
   constexpr int PER = HIST ? Counts<HIST ? HIST : 1>::PER_WORD : 1;
 
   typename E::type* orow = static_cast<typename E::type*>(a.out) + row * a.out_ld;
@@ -517,7 +524,7 @@ constexpr int LIST = 512;       // counted tokens of a segment that are listed; 
 template <int T, int HIST, bool DRAW, bool ROWWAVE>
 __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
   typedef Elem<T> E;
-  constexpr int EV = E::EV, STEP = 64 * EV;
+  constexpr int EV = E::EV;
   extern __shared__ uint32_t lds[];          // counts of the workgroup's 4 segments, a bit for each token, and the lists of counted ones
   const Rules& q = a.q;
   const int lane = threadIdx.x & 63;
@@ -756,14 +763,17 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
   double given_y = 0.0;
   int c = 0;
   if (SEARCH) {
-    for (int i = tid; i < min(p.n_hist, HIST_STAGE); i += 256) {
-      const long long t = hist_at(p, q.history_i64, i);
-      hist[i] = t >= 0 && t < V ? (int)t : -1;
-    }
+    RowP staged = p;
+    staged.n_hist = min(p.n_hist, HIST_STAGE);
+    int at = tid;
+    for_history<8>(staged, q.history_i64, 0, tid, 256, [&](long long t) {
+      hist[at] = t >= 0 && t < V ? (int)t : -1;
+      at += 256;
+    });
   } else {
     tok = a.given[row];
     if (tok >= 0 && tok < V) {
-      for (int i = tid; i < p.n_hist; i += 256) c += hist_at(p, q.history_i64, i) == tok;
+      for_history<8>(p, q.history_i64, 0, tid, 256, [&](long long t) { c += t == tok; });
       if (p.n_hist) c = block_reduce(c, shi, [](int x, int y) { return x + y; });
       given_y = token_value<T>(q, p, row, (int)tok, c);
     }
@@ -815,14 +825,15 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
     for (int i = tid; i < n; i += 256) cnt[i] = 0;
     __syncthreads();
     const int staged = min(p.n_hist, HIST_STAGE);
+#pragma unroll 4
     for (int i = tid; i < staged; i += 256) {
-      const int d = hist[i] - v0;
-      if (hist[i] >= 0 && d >= 0 && d < n) atomicAdd(&cnt[d], 1u);
+      const int t = hist[i], d = t - v0;
+      if (t >= 0 && d >= 0 && d < n) atomicAdd(&cnt[d], 1u);
     }
-    for (int i = staged + tid; i < p.n_hist; i += 256) {
-      const long long d = hist_at(p, q.history_i64, i) - v0;
+    for_history<8>(p, q.history_i64, HIST_STAGE, tid, 256, [&](long long t) {
+      const long long d = t - v0;
       if ((unsigned long long)d < (unsigned long long)n) atomicAdd(&cnt[(int)d], 1u);
-    }
+    });
     __syncthreads();
   };
 
