@@ -514,6 +514,13 @@ __device__ __forceinline__ double counted_value(const RowP& p, const Counted& t)
   return t.kept ? counted64(p, t.x, t.c, t.b) : -INFINITY;
 }
 
+// the value of a token, counted or not
+template <int T>
+__device__ __forceinline__ double any_value(const RowP& p, const Counted& t) {
+  if (!t.kept) return -INFINITY;
+  return t.c ? counted64(p, t.x, t.c, t.b) : (double)t.x + (double)t.b;
+}
+
 constexpr int LIST = 512;       // counted tokens of a segment that are listed; more are looked up bit by bit
 
 // A segment's maximum and sum of weights.  Tokens that the history holds are left out of the steps (one more bit mask) and
@@ -750,6 +757,7 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
   const int V = q.vocab, tid = threadIdx.x, n = a.seg_len;
   const RowP p = row_params(q, row);
   const Seg* seg = a.seg + row * a.nseg;
+  const char* lrow = static_cast<const char*>(q.logits) + row * q.ld * (long long)sizeof(typename Elem<T>::type);
 
   // contiguous shares, so that running sums follow the vocabulary's order
   const int per = (a.nseg + 255) / 256;
@@ -853,11 +861,20 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
       from = g + 1;
       const int v0 = g * n;
       count(v0);
-      for (int e = tid; e < n && v0 + e < V; e += 256) {
-        const double y = token_value<T>(q, p, row, v0 + e, cnt[e]);
-        if ((float)y != m) continue;
-        const float l = (float)(y - (double)m);
-        if (l > lo || (l == lo && v0 + e < idx)) { lo = l; idx = v0 + e; best_y = y; }
+      for (int e = tid; e < n && v0 + e < V; e += 1024) {
+        Counted t[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (e + 256 * u < n && v0 + e + 256 * u < V) t[u] = load_counted<T, 2>(q, p, lrow, cnt, v0, e + 256 * u);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int v = v0 + e + 256 * u;
+          if (e + 256 * u >= n || v >= V) continue;
+          const double y = any_value<T>(p, t[u]);
+          if ((float)y != m) continue;
+          const float l = (float)(y - (double)m);
+          if (l > lo || (l == lo && v < idx)) { lo = l; idx = v; best_y = y; }
+        }
       }
       __syncthreads();
     }
@@ -897,12 +914,15 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
   constexpr int STRIPS = SEG_MAX / 256;
   const int strips = n / 256, lane = tid & 63, wave = tid >> 6;
   const int d0 = wave * (n / 4) + lane;
+  Counted tokens[STRIPS];
+#pragma unroll
+  for (int e = 0; e < STRIPS; ++e)
+    if (e < strips && v0 + d0 + e * 64 < V) tokens[e] = load_counted<T, 2>(q, p, lrow, cnt, v0, d0 + e * 64);
   double w[STRIPS], sum = 0.0;
 #pragma unroll
   for (int e = 0; e < STRIPS; ++e) {
     w[e] = 0.0;
-    const int d = d0 + e * 64;
-    if (e < strips && v0 + d < V) w[e] = exp2_64(token_value<T>(q, p, row, v0 + d, cnt[d]) - (double)m, p.k);
+    if (e < strips && v0 + d0 + e * 64 < V) w[e] = exp2_64(any_value<T>(p, tokens[e]) - (double)m, p.k);
     sum += w[e];
   }
 #pragma unroll
@@ -932,18 +952,26 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
   if (wave != in) return;
   int hit = INT32_MAX, tail = -1;
 #pragma unroll
-  for (int e = 0; e < STRIPS; ++e) {
-    if (e < strips && hit == INT32_MAX) {
-      double run = w[e];
+  for (int g = 0; g < STRIPS; g += 4) {             // four strips' running sums at once: a step of one waits for its shuffles
+    if (g < strips && hit == INT32_MAX) {
+      double run[4] = {w[g], w[g + 1], w[g + 2], w[g + 3]};
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
-        const double t = __shfl_up(run, o);
-        if (lane >= o) run += t;
+        double t[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t[j] = __shfl_up(run[j], o);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) run[j] += lane >= o ? t[j] : 0.0;
       }
-      const unsigned long long over = __ballot(w[e] > 0.0 && at + run > edge), any = __ballot(w[e] > 0.0);
-      if (any) tail = e * 64 + 63 - __clzll(any);
-      if (over) hit = e * 64 + __ffsll(over) - 1;
-      at += __shfl(run, 63);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const unsigned long long over = __ballot(w[g + j] > 0.0 && at + run[j] > edge), any = __ballot(w[g + j] > 0.0);
+        if (hit == INT32_MAX) {
+          if (any) tail = (g + j) * 64 + 63 - __clzll(any);
+          if (over) hit = (g + j) * 64 + __ffsll(over) - 1;
+        }
+        at += __shfl(run[j], 63);
+      }
     }
   }
   // (sums of another order may end a rounding short of the edge: then the wave's last token with a weight)
