@@ -195,14 +195,24 @@ enum { M_APPLY = 0, M_SUM = 1, M_GREEDY = 2, M_DRAW = 3, M_BWD = 4 };
 
 constexpr int SEG_MAX = 4096;   // tokens of a segment at most: the counts of a workgroup's 4 segments are 32 KB of 16 bits
 
+// what a row's decision reads and leaves
+struct RowOut {
+  const float* uniforms;         // DRAW
+  const int* next;               // next state of (state, token), or NULL
+  const long long* given;        // SUM, BWD: the given tokens
+  long long* tokens;             // GREEDY / DRAW
+  float* logprob;
+  float* stat;                   // SUM, BWD: [rows][2] = maximum and 1 / Z, kept for the backward pass
+  int* state_out;
+};
+
 struct SegArgs {
   Rules q;
+  RowOut o;
   int nseg, seg_len;            // segments of a row, their tokens (a multiple of 64 x 16 bytes)
   int wgs_per_row;              // workgroups of a row (ROWWAVE: unused)
   void* out; long long out_ld;  // APPLY / BWD
-  Seg* seg;                     // SUM / DRAW
-  const long long* tokens;      // BWD
-  const float* stat;            // BWD: [rows][2] = maximum, 1 / Z
+  Seg* seg;                     // sums: a segment's (ROWWAVE: unused)
   const float* d_logprob;       // BWD
   float* d_bias_rows;           // BWD: gradient of a bias of its own per row, [rows][vocab], or NULL
 };
@@ -394,11 +404,11 @@ struct Bwd {
   bool zero;                      // an ignored row, or one whose rules leave nothing
   __device__ __forceinline__ Bwd() {}
   __device__ __forceinline__ Bwd(const SegArgs& a, const RowP& p, long long row) {
-    const long long t = a.tokens[row];
-    m = a.stat[2 * row];
+    const long long t = a.o.given[row];
+    m = a.o.stat[2 * row];
     kf = (float)p.k;
     coef = (float)((double)a.d_logprob[row] * (p.k * LN2));
-    spread = -coef * a.stat[2 * row + 1];
+    spread = -coef * a.o.stat[2 * row + 1];
     up = (float)p.rho;
     down = (float)p.inv_rho;
     zero = t < 0 || t >= a.q.vocab || m == -INFINITY;
@@ -497,6 +507,29 @@ __device__ __forceinline__ double token_value(const Rules& q, const RowP& p, lon
   return c ? counted64(p, x, c, b) : (double)x + (double)b;
 }
 
+// a row's results: its token, `at` the token's value, m and Z the row's maximum and sum
+template <int MODE>
+__device__ __forceinline__ void end_row(const Rules& q, const RowOut& o, const RowP& p, long long row, long long tok,
+                                        double at, float m, bool ok, double Z) {
+  const bool have = tok >= 0 && tok < q.vocab;
+  float lp;
+  if (MODE == M_SUM && !have) lp = 0.f;                   // an ignored row
+  else if (m == -INFINITY) lp = -INFINITY;                // the rules leave nothing
+  else if (!ok || !have) lp = NAN;                        // NaN or +inf among the allowed values (or a NaN u)
+  else lp = (float)((at - (double)m) * (p.k * LN2) - log_64(Z));
+  o.logprob[row] = lp;
+  if (MODE == M_SUM) {
+    o.stat[2 * row] = m == -INFINITY || ok ? m : NAN;
+    o.stat[2 * row + 1] = ok ? (float)reciprocal(Z) : NAN;
+  } else {
+    o.tokens[row] = tok;
+    if (o.state_out) {
+      const int s = q.state[row];
+      o.state_out[row] = tok >= 0 && s >= 0 && s < q.states ? o.next[(size_t)s * q.vocab + tok] : s;
+    }
+  }
+}
+
 // a counted token's loads (none waits for another), and its value
 struct Counted { float x, b; uint32_t c; bool kept; };
 template <int T, int HIST>
@@ -528,8 +561,9 @@ constexpr int LIST = 512;       // counted tokens of a segment that are listed; 
 // DRAW: sums of doubles, against 0 as reference -- an exponent of a double has room for every ordinary row; where the
 // maximum is no ordinary one (beyond 2^-400 .. 2^900) the segment is summed again against it.  Else fp32 sums, against a
 // reference of the lane's own that moves when a value exceeds it by 2^8 (an exponent of 8 is still exact to 2^-20).
-template <int T, int HIST, bool DRAW, bool ROWWAVE>
+template <int T, int HIST, int MODE, bool ROWWAVE>
 __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
+  constexpr bool DRAW = MODE == M_DRAW;
   typedef Elem<T> E;
   constexpr int EV = E::EV;
   extern __shared__ uint32_t lds[];          // counts of the workgroup's 4 segments, a bit for each token, and the lists of counted ones
@@ -692,7 +726,94 @@ __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
       r.s = (double)wave_sum(z * __builtin_amdgcn_exp2f((ref - m) * kf));
     }
   }
-  if (lane == 0) a.seg[row * a.nseg + seg] = r;
+  if (!ROWWAVE) {
+    if (lane == 0) a.seg[row * a.nseg + seg] = r;
+    return;
+  }
+  // a row of one segment: its wave decides it
+  const bool ok = m > -INFINITY && m < INFINITY && p.k > 0.0 && p.k < INFINITY;
+  long long tok = -1;
+  const auto count = [&](int v) { return HIST ? count_at<HIST ? HIST : 1>(cnt, v) : 0u; };
+  // values of EV tokens, -inf where there is none
+  const auto values = [&](int v, double (&y)[EV]) {
+    const Loaded in = load_step<T, false>(p, lrow, v, V);
+    float b[EV];
+    if (p.bias) load_bias<EV, false>(p.bias, v, V, b);
+#pragma unroll
+    for (int e = 0; e < EV; ++e) {
+      y[e] = -INFINITY;
+      if (!((in.keep >> e) & 1)) continue;
+      const uint32_t c = count(v + e);
+      const float be = p.bias ? b[e] : 0.f;
+      y[e] = c ? counted64(p, E::at(in.raw, e), c, be) : (double)E::at(in.raw, e) + (double)be;
+    }
+  };
+  if (MODE == M_SUM) {
+    tok = a.o.given[row];
+  } else if (ok && MODE == M_GREEDY) {
+    float lo = -INFINITY;
+    int idx = INT32_MAX;
+    for (int v = lane * EV; v < end; v += 64 * EV) {
+      double y[EV];
+      values(v, y);
+#pragma unroll
+      for (int e = 0; e < EV; ++e) {
+        const float l = (float)y[e] == m ? (float)(y[e] - (double)m) : -INFINITY;
+        if (l > lo) { lo = l; idx = v + e; }
+      }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      const float l2 = __shfl_xor(lo, o);
+      const int i2 = __shfl_xor(idx, o);
+      if (l2 > lo || (l2 == lo && i2 < idx)) { lo = l2; idx = i2; }
+    }
+    if (idx < V) tok = idx;
+  } else if (ok && MODE == M_DRAW) {
+    const float u = a.o.uniforms[row];
+    if (u == u) {
+      const double edge = fmax((double)u, 0.0) * r.s;
+      double before = 0.0;
+      int last = -1;
+      for (int first = 0; first < end && tok < 0; first += 64 * EV) {
+        const int v = first + lane * EV;
+        double w[EV], sum = 0.0;
+        if (v < end) values(v, w);
+#pragma unroll
+        for (int e = 0; e < EV; ++e) {
+          w[e] = v < end ? exp2_64(w[e] - (double)r.ref, p.k) : 0.0;
+          sum += w[e];
+          if (w[e] > 0.0) last = v + e;
+        }
+        double run = sum;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const double t = __shfl_up(run, o);
+          if (lane >= o) run += t;
+        }
+        const double all = __shfl(run, 63);
+        run = before + (run - sum);
+        int hit = INT32_MAX;
+#pragma unroll
+        for (int e = 0; e < EV; ++e) {
+          run += w[e];
+          if (w[e] > 0.0 && run > edge && hit == INT32_MAX) hit = v + e;
+        }
+        const unsigned long long over = __ballot(hit != INT32_MAX);
+        if (over) tok = __shfl(hit, __ffsll(over) - 1);
+        before += all;
+      }
+      if (tok < 0) {                       // u >= 1, or by rounding: the last token with a weight
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) last = max(last, __shfl_xor(last, o));
+        tok = last;
+      }
+    }
+  }
+  if (lane) return;
+  const bool have = tok >= 0 && tok < V;
+  const double at = have ? token_value<T>(q, p, row, (int)tok, count((int)tok)) : 0.0;
+  end_row<MODE>(q, a.o, p, row, tok, at, m, ok, ok ? r.s * exp2_64((double)r.ref - (double)m, p.k) : 0.0);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -700,15 +821,9 @@ __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
 // ---------------------------------------------------------------------------------------------------------------
 struct JoinArgs {
   Rules q;
+  RowOut o;
   int nseg, seg_len;
   const Seg* seg;
-  const float* uniforms;         // DRAW
-  const int* next;               // next state of (state, token), or NULL
-  const long long* given;        // GIVEN
-  long long* tokens;             // GREEDY / DRAW
-  float* logprob;
-  float* stat;                   // GIVEN: maximum and 1 / Z, kept for the backward pass
-  int* state_out;
 };
 
 template <typename X, typename F>
@@ -766,7 +881,7 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
   mine.s = 0.0; mine.m = -INFINITY; mine.ref = 0.f;
   if (i0 < i1) mine = seg[i0];
 
-  const float uf = MODE == M_DRAW ? a.uniforms[row] : 0.f;
+  const float uf = MODE == M_DRAW ? a.o.uniforms[row] : 0.f;
   long long tok = -1;
   double given_y = 0.0;
   int c = 0;
@@ -779,7 +894,7 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
       at += 256;
     });
   } else {
-    tok = a.given[row];
+    tok = a.o.given[row];
     if (tok >= 0 && tok < V) {
       for_history<8>(p, q.history_i64, 0, tid, 256, [&](long long t) { c += t == tok; });
       if (p.n_hist) c = block_reduce(c, shi, [](int x, int y) { return x + y; });
@@ -802,24 +917,7 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
   double Z;
   const double before = block_prefix(z, shd, Z);
 
-  const auto finish = [&](long long t, double y) {
-    float lp = -INFINITY;
-    if (MODE == M_SUM && !(t >= 0 && t < V)) lp = 0.f;          // an ignored row
-    else if (m == -INFINITY) lp = -INFINITY;                    // the rules leave nothing
-    else if (!ok || t < 0) lp = NAN;                            // NaN or +inf among the allowed values (or a NaN u)
-    else lp = (float)((y - (double)m) * (p.k * LN2) - log_64(Z));
-    a.logprob[row] = lp;
-    if (MODE == M_SUM) {
-      a.stat[2 * row] = m == -INFINITY || ok ? m : NAN;
-      a.stat[2 * row + 1] = ok ? (float)(1.0 / Z) : NAN;
-    } else {
-      a.tokens[row] = t;
-      if (a.state_out) {
-        const int s = q.state[row];
-        a.state_out[row] = t >= 0 && s >= 0 && s < q.states ? a.next[(size_t)s * V + t] : s;
-      }
-    }
-  };
+  const auto finish = [&](long long t, double y) { end_row<MODE>(q, a.o, p, row, t, y, m, ok, Z); };
   if (MODE == M_SUM) {
     if (tid == 0) finish(tok, given_y);
     return;
@@ -987,9 +1085,8 @@ constexpr int SMALL_VOCAB = 64, SMALL_HISTORY = 256;
 
 struct SmallArgs {
   Rules q;
+  RowOut o;
   int w;                          // lanes of a row
-  const float* uniforms; const int* next; long long* tokens; float* logprob; int* state_out;   // GREEDY / DRAW
-  const long long* given; float* stat;                                                         // SUM, BWD
   const float* d_logprob; void* out; long long out_ld; float* d_bias; float* part;             // APPLY, BWD
 };
 
@@ -997,30 +1094,6 @@ template <typename X>
 __device__ __forceinline__ X group_sum(X v, int w) {
   for (int o = w >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o);
   return v;
-}
-
-// a row's results: its token, `at` the token's value, m and Z the row's maximum and sum
-template <int MODE>
-__device__ __forceinline__ void end_row(const SmallArgs& a, const RowP& p, long long row, long long tok, double at, float m,
-                                        bool ok, double Z) {
-  const Rules& q = a.q;
-  const bool have = tok >= 0 && tok < q.vocab;
-  float lp;
-  if (MODE == M_SUM && !have) lp = 0.f;                   // an ignored row
-  else if (m == -INFINITY) lp = -INFINITY;                // the rules leave nothing
-  else if (!ok || !have) lp = NAN;                        // NaN or +inf among the allowed values (or a NaN u)
-  else lp = (float)((at - (double)m) * (p.k * LN2) - log_64(Z));
-  a.logprob[row] = lp;
-  if (MODE == M_SUM) {
-    a.stat[2 * row] = m == -INFINITY || ok ? m : NAN;
-    a.stat[2 * row + 1] = ok ? (float)reciprocal(Z) : NAN;
-  } else {
-    a.tokens[row] = tok;
-    if (a.state_out) {
-      const int s = q.state[row];
-      a.state_out[row] = tok >= 0 && s >= 0 && s < q.states ? a.next[(size_t)s * q.vocab + tok] : s;
-    }
-  }
 }
 
 // Vocabularies of up to VM = 8 or 16 tokens with many rows: a lane a row.  No sums or searches across lanes, and an eighth of
@@ -1082,10 +1155,10 @@ __global__ __launch_bounds__(256) void rules_tiny_kernel(SmallArgs a) {
     if (MODE == M_APPLY || MODE == M_BWD) {
       typename E::type o[VM];
       if (MODE == M_BWD) {
-        const float m = a.stat[2 * row];
-        const long long tok = a.given[row];
+        const float m = a.o.stat[2 * row];
+        const long long tok = a.o.given[row];
         const bool zero = tok < 0 || tok >= V || m == -INFINITY;
-        const double coef = (double)a.d_logprob[row] * (p.k * LN2), iz = a.stat[2 * row + 1];
+        const double coef = (double)a.d_logprob[row] * (p.k * LN2), iz = a.o.stat[2 * row + 1];
 #pragma unroll
         for (int v = 0; v < VM; ++v) {
           double g = 0.0;
@@ -1127,7 +1200,7 @@ __global__ __launch_bounds__(256) void rules_tiny_kernel(SmallArgs a) {
     }
     int tok = -1;
     if (MODE == M_SUM) {
-      const long long t = a.given[row];
+      const long long t = a.o.given[row];
       tok = t >= 0 && t < V ? (int)t : -1;
     } else if (ok && MODE == M_GREEDY) {
       double best = -INFINITY;
@@ -1135,7 +1208,7 @@ __global__ __launch_bounds__(256) void rules_tiny_kernel(SmallArgs a) {
       for (int v = 0; v < VM; ++v)
         if (y[v] > best) { best = y[v]; tok = v; }
     } else if (ok && MODE == M_DRAW) {
-      const float u = a.uniforms[row];
+      const float u = a.o.uniforms[row];
       const double edge = fmax((double)u, 0.0) * Z;
       double run = 0.0;
       int last = -1;
@@ -1154,7 +1227,7 @@ __global__ __launch_bounds__(256) void rules_tiny_kernel(SmallArgs a) {
 #pragma unroll
     for (int v = 0; v < VM; ++v)
       if (v == tok) at = y[v];
-    end_row<MODE>(a, p, row, tok, at, m, ok, Z);
+    end_row<MODE>(q, a.o, p, row, tok, at, m, ok, Z);
   }
   if (MODE == M_BWD) {
     if (!a.part) return;
@@ -1202,11 +1275,11 @@ __global__ __launch_bounds__(256) void rules_small_kernel(SmallArgs a) {
       continue;
     }
     if (MODE == M_BWD) {
-      const float m = a.stat[2 * row];
-      const long long tok = a.given[row];
+      const float m = a.o.stat[2 * row];
+      const long long tok = a.o.given[row];
       double g = 0.0;
       if (kept && tok >= 0 && tok < V && m != -INFINITY)
-        g = (double)a.d_logprob[row] * (p.k * LN2) * ((v == tok ? 1.0 : 0.0) - exp2_64(y - (double)m, p.k) * (double)a.stat[2 * row + 1]);
+        g = (double)a.d_logprob[row] * (p.k * LN2) * ((v == tok ? 1.0 : 0.0) - exp2_64(y - (double)m, p.k) * (double)a.o.stat[2 * row + 1]);
       const float gf = (float)g;
       if (a.part) acc += gf;
       else if (a.d_bias && in) a.d_bias[row * V + v] = gf;
@@ -1226,7 +1299,7 @@ __global__ __launch_bounds__(256) void rules_small_kernel(SmallArgs a) {
     const double Z = __shfl(run, W - 1, W);
     long long tok = -1;
     if (MODE == M_SUM) {
-      tok = a.given[row];
+      tok = a.o.given[row];
     } else if (ok && MODE == M_GREEDY) {
       double best = y;
       int idx = v;
@@ -1237,7 +1310,7 @@ __global__ __launch_bounds__(256) void rules_small_kernel(SmallArgs a) {
       }
       tok = idx;
     } else if (ok && MODE == M_DRAW) {
-      const float u = a.uniforms[row];
+      const float u = a.o.uniforms[row];
       if (u == u) {
         int hit = w > 0.0 && run > fmax((double)u, 0.0) * Z ? v : INT32_MAX;
         int last = w > 0.0 ? v : -1;
@@ -1249,7 +1322,7 @@ __global__ __launch_bounds__(256) void rules_small_kernel(SmallArgs a) {
       }
     }
     const double at = __shfl(y, tok >= 0 && tok < V ? (int)tok : 0, W);
-    if (v == 0) end_row<MODE>(a, p, row, tok, at, m, ok, Z);
+    if (v == 0) end_row<MODE>(q, a.o, p, row, tok, at, m, ok, Z);
   }
   if (MODE == M_BWD) {
     if (!a.part) return;
@@ -1397,8 +1470,8 @@ void launch_seg(const SegArgs& a, const Plan& p, hipStream_t st) {
     else hipLaunchKernelGGL((rules_map_kernel<T, HIST, MODE, false>), grid, block, lds, st, a);
   } else {
     if (HIST) lds += p.seg_len / 2 + 4 * LIST * 2;
-    if (p.row_wave) hipLaunchKernelGGL((rules_sum_kernel<T, HIST, MODE == M_DRAW, true>), grid, block, lds, st, a);
-    else hipLaunchKernelGGL((rules_sum_kernel<T, HIST, MODE == M_DRAW, false>), grid, block, lds, st, a);
+    if (p.row_wave) hipLaunchKernelGGL((rules_sum_kernel<T, HIST, MODE, true>), grid, block, lds, st, a);
+    else hipLaunchKernelGGL((rules_sum_kernel<T, HIST, MODE == M_DRAW ? M_DRAW : M_SUM, false>), grid, block, lds, st, a);
   }
 }
 
@@ -1421,8 +1494,14 @@ int run_seg(SegArgs& a, const Plan& p, hipStream_t st) {
   return DVAE_OK;
 }
 
+// sums of all segments, then the rows' decisions (ROWWAVE: in the same launch)
 template <int MODE>
-int run_join(const JoinArgs& a, hipStream_t st) {
+int run_join(SegArgs& s, hipStream_t st) {
+  const Plan p = plan_of(s.q);
+  DVAE_TRY(run_seg<MODE>(s, p, st));
+  if (p.row_wave) return DVAE_OK;
+  JoinArgs a{};
+  a.q = s.q; a.o = s.o; a.nseg = p.nseg; a.seg_len = p.seg_len; a.seg = s.seg;
   const dim3 grid((unsigned)a.q.rows), block(256);
   switch (a.q.dtype) {
     case DVAE_F32: hipLaunchKernelGGL((rules_join_kernel<DVAE_F32, MODE>), grid, block, 0, st, a); break;
@@ -1437,6 +1516,8 @@ int run_join(const JoinArgs& a, hipStream_t st) {
 bool is_small(const dvae_rules& q) {
   return q.vocab <= SMALL_VOCAB && (!q.history || q.history_len <= SMALL_HISTORY);
 }
+
+bool needs_segments(const dvae_rules& q) { return !is_small(q) && !plan_of(q).row_wave; }
 
 int small_lanes(const dvae_rules& q) {
   int w = 1;
@@ -1511,7 +1592,7 @@ int rules_check(const dvae_rules& q, const char* who) {
 
 extern "C" size_t dvae_rules_ws_bytes(const dvae_rules* q) {
   if (!q || q->rows <= 0 || q->vocab < 1) return 0;
-  const size_t segs = is_small(*q) ? 0 : (size_t)q->rows * plan_of(*q).nseg * sizeof(Seg);
+  const size_t segs = !needs_segments(*q) ? 0 : (size_t)q->rows * plan_of(*q).nseg * sizeof(Seg);
   const size_t bias = q->bias && q->bias_ld == 0 ? (size_t)bias_shares(*q) * q->vocab * sizeof(float) : 0;
   return std::max(segs, bias);
 }
@@ -1539,27 +1620,20 @@ extern "C" int dvae_rules_choose(const dvae_rules* q, const float* uniforms, con
   DVAE_REQUIRE(q, "rules_choose: null pointer");
   DVAE_TRY(rules_check(*q, "rules_choose"));
   if (q->rows == 0) return DVAE_OK;
-  DVAE_REQUIRE(tokens && logprob && (ws || is_small(*q)), "rules_choose: null pointer");
+  DVAE_REQUIRE(tokens && logprob && (ws || !needs_segments(*q)), "rules_choose: null pointer");
   DVAE_REQUIRE((next == nullptr) == (state_out == nullptr), "rules_choose: next and state_out go together");
   DVAE_REQUIRE(!next || q->mask, "rules_choose: next states need a grammar mask");
+  RowOut o{};
+  o.uniforms = uniforms; o.next = next; o.tokens = tokens; o.logprob = logprob; o.state_out = state_out;
+  hipStream_t st = (hipStream_t)stream;
   if (is_small(*q)) {
     SmallArgs m{};
-    m.q = with_constants(*q); m.uniforms = uniforms; m.next = next; m.tokens = tokens; m.logprob = logprob; m.state_out = state_out;
-    return uniforms ? run_small<M_DRAW>(m, small_blocks(*q), (hipStream_t)stream)
-                    : run_small<M_GREEDY>(m, small_blocks(*q), (hipStream_t)stream);
+    m.q = with_constants(*q); m.o = o;
+    return uniforms ? run_small<M_DRAW>(m, small_blocks(*q), st) : run_small<M_GREEDY>(m, small_blocks(*q), st);
   }
-  const Plan p = plan_of(*q);
   SegArgs a{};
-  a.q = with_constants(*q); a.seg = (Seg*)ws;
-  JoinArgs j{};
-  j.q = a.q; j.nseg = p.nseg; j.seg_len = p.seg_len; j.seg = (const Seg*)ws; j.uniforms = uniforms; j.next = next;
-  j.tokens = tokens; j.logprob = logprob; j.state_out = state_out;
-  if (uniforms) {
-    DVAE_TRY(run_seg<M_DRAW>(a, p, (hipStream_t)stream));
-    return run_join<M_DRAW>(j, (hipStream_t)stream);
-  }
-  DVAE_TRY(run_seg<M_SUM>(a, p, (hipStream_t)stream));
-  return run_join<M_GREEDY>(j, (hipStream_t)stream);
+  a.q = with_constants(*q); a.o = o; a.seg = (Seg*)ws;
+  return uniforms ? run_join<M_DRAW>(a, st) : run_join<M_GREEDY>(a, st);
 }
 
 extern "C" int dvae_rules_logprob(const dvae_rules* q, const long long* tokens, float* logprob, float* stat, void* ws,
@@ -1567,19 +1641,17 @@ extern "C" int dvae_rules_logprob(const dvae_rules* q, const long long* tokens, 
   DVAE_REQUIRE(q, "rules_logprob: null pointer");
   DVAE_TRY(rules_check(*q, "rules_logprob"));
   if (q->rows == 0) return DVAE_OK;
-  DVAE_REQUIRE(tokens && logprob && stat && (ws || is_small(*q)), "rules_logprob: null pointer");
+  DVAE_REQUIRE(tokens && logprob && stat && (ws || !needs_segments(*q)), "rules_logprob: null pointer");
+  RowOut o{};
+  o.given = tokens; o.logprob = logprob; o.stat = stat;
   if (is_small(*q)) {
     SmallArgs m{};
-    m.q = with_constants(*q); m.given = tokens; m.logprob = logprob; m.stat = stat;
+    m.q = with_constants(*q); m.o = o;
     return run_small<M_SUM>(m, small_blocks(*q), (hipStream_t)stream);
   }
-  const Plan p = plan_of(*q);
   SegArgs a{};
-  a.q = with_constants(*q); a.seg = (Seg*)ws;
-  DVAE_TRY(run_seg<M_SUM>(a, p, (hipStream_t)stream));
-  JoinArgs j{};
-  j.q = a.q; j.nseg = p.nseg; j.seg_len = p.seg_len; j.seg = (const Seg*)ws; j.given = tokens; j.logprob = logprob; j.stat = stat;
-  return run_join<M_SUM>(j, (hipStream_t)stream);
+  a.q = with_constants(*q); a.o = o; a.seg = (Seg*)ws;
+  return run_join<M_SUM>(a, (hipStream_t)stream);
 }
 
 extern "C" int dvae_rules_logprob_bwd(const dvae_rules* q, const long long* tokens, const float* stat,
@@ -1607,15 +1679,15 @@ extern "C" int dvae_rules_logprob_bwd(const dvae_rules* q, const long long* toke
   };
   if (is_small(*q)) {
     SmallArgs m{};
-    m.q = with_constants(*q); m.given = tokens; m.stat = const_cast<float*>(stat); m.d_logprob = d_logprob;
+    m.q = with_constants(*q); m.o.given = tokens; m.o.stat = const_cast<float*>(stat); m.d_logprob = d_logprob;
     m.out = d_logits; m.out_ld = d_ld; m.d_bias = shared ? nullptr : d_bias; m.part = shared ? (float*)ws : nullptr;
     DVAE_TRY(run_small<M_BWD>(m, shared ? shares : small_blocks(*q), st));
     return shared ? sum_shares() : DVAE_OK;
   }
   const Plan p = plan_of(*q);
   SegArgs a{};
-  a.q = with_constants(*q); a.out = d_logits; a.out_ld = d_ld; a.tokens = tokens;
-  a.stat = stat; a.d_logprob = d_logprob;
+  a.q = with_constants(*q); a.out = d_logits; a.out_ld = d_ld; a.o.given = tokens;
+  a.o.stat = const_cast<float*>(stat); a.d_logprob = d_logprob;
   a.d_bias_rows = shared ? nullptr : d_bias;
   if (!shared) return run_seg<M_BWD>(a, p, st);
   ColArgs c{};

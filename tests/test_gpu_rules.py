@@ -191,10 +191,10 @@ def test_choose(cuda, shape, drawn):
         assert got.state is None
 
 
-def check_logprob(cuda, case, x, bias, lp, dx, db, g):
+def check_logprob(cuda, case, x, bias, lp, dx, db, g, some=None):
     want_db = np.zeros((case.nrows, case.vocab))
     tol_db = np.zeros((case.nrows, case.vocab))
-    for r in range(case.nrows):
+    for r in range(case.nrows) if some is None else some:
         y, slope, al, temp = case.row(r)
         want, d, dv = R.logprob_row(y, slope, int(case.tokens[r]), temp, float(g[r]), al)
         lz = log_z_tol(case, y, temp)
@@ -287,6 +287,38 @@ def test_many_rows_of_a_few_tokens(cuda, shape):
         same_or_close(grads[1].double().cpu().numpy(), total, off, "d bias")
     elif b is not None:
         assert grads[1].shape == b.shape
+
+
+@pytest.mark.parametrize("shape", [dict(vocab=700, L=40, ragged=True, states=4, free=True, per_row=True),
+                                   dict(vocab=1900, dtype="bf16", L=9, bias="rows", index=torch.int32, pad=3),
+                                   dict(vocab=2048, dtype="fp16", states=3), dict(vocab=1025, L=600, junk=True)], ids=ident)
+def test_many_rows_of_a_middle_vocabulary(cuda, shape):
+    """4200 rows: a wave a row, all in one launch.  The oracle sees 60 of them."""
+    from dvae_amd.rules import apply_rules, choose, token_logprob
+    rows = 4200
+    case = Case(rows=rows, seed=13, drawn=True, **shape)
+    x, kw, temp = case.big.to(cuda)[:, :case.vocab], case.kw(cuda), case.temperature(cuda)
+    got = apply_rules(x, case.rules(cuda), **kw)
+    draw = choose(x, case.rules(cuda), temperature=temp, uniforms=case.u.to(cuda), **kw)
+    best = choose(x, case.rules(cuda), temperature=temp, **kw)
+    picked = [(c.tokens.tolist(), c.logprob.tolist(), None if c.state is None else c.state.tolist()) for c in (draw, best)]
+    x = x.requires_grad_(True)
+    lp = token_logprob(x, case.tokens.to(cuda), case.rules(cuda), temperature=temp, **kw)
+    (dx,) = torch.autograd.grad(lp, x, case.g.to(cuda))
+    some = list(range(0, rows, 71)) + [rows - 1]
+    for r in some:
+        y, _, _, t = case.row(r)
+        same_or_close(got[r].double().cpu().numpy(), y,
+                      (half(case.dtype) + U) * np.abs(np.where(np.isfinite(y), y, 0)) + TINY[case.dtype], "row %d" % r)
+        for (tok, lps, st), u in zip(picked, (float(case.u[r]), None)):
+            k, l = R.choose_row(y, t, u)
+            assert tok[r] == k, (r, tok[r], k)
+            tol = U * abs(l) + 1e-11 + (0.0 if u is not None else log_z_tol(case, y, t)) if math.isfinite(l) else 0.0
+            same_or_close(lps[r], l, tol, "row %d" % r)
+            if st is not None:
+                s = int(case.state[r])
+                assert st[r] == (int(case.next[s, k]) if k >= 0 and 0 <= s < case.next.shape[0] else s)
+    check_logprob(cuda, case, x, None, lp, dx, None, case.g, some)
 
 
 def test_gradient_against_differences(cuda):
