@@ -50,20 +50,19 @@ class Grammar:
         if not 0 <= int(start) < self.states:
             raise ValueError("Grammar: start state %d of %d" % (int(start), self.states))
         self.start = int(start)
-        words = (self.vocab + 31) // 32
-        bits = torch.zeros(self.states, words * 32, dtype=torch.int64, device=allowed.device)
-        bits[:, :self.vocab] = allowed
-        weight = torch.ones((), dtype=torch.int64, device=allowed.device) << torch.arange(32, device=allowed.device)
-        packed = (bits.view(self.states, words, 32) * weight).sum(2)
-        # two's complement: the 32 bits of an unsigned word in an int32
-        self.masks = torch.where(packed >= 1 << 31, packed - (1 << 32), packed).to(torch.int32).contiguous()
+        # 32 tokens a word; as int32, where bit 31 is the sign: the sum of distinct powers of two wraps to the right word
+        bits = torch.nn.functional.pad(allowed.int(), (0, -self.vocab % 32)).view(self.states, -1, 32)
+        weight = torch.bitwise_left_shift(1, torch.arange(32, dtype=torch.int32, device=allowed.device))
+        self.masks = (bits * weight).sum(2, dtype=torch.int32)
         self.next_state = None
         if next_state is not None:
             if not torch.is_tensor(next_state) or next_state.dtype not in _INDEX or next_state.shape != allowed.shape:
                 raise ValueError("Grammar: next_state must be an int32 / int64 tensor [states, vocab]")
             if next_state.device != allowed.device:
                 raise ValueError("Grammar: next_state is on %s, allowed on %s" % (next_state.device, allowed.device))
-            self.next_state = next_state.clamp(-1, self.states).to(torch.int32).contiguous()
+            if next_state.dtype != torch.int32:
+                next_state = next_state.clamp(-1, self.states).to(torch.int32)
+            self.next_state = next_state.contiguous()
 
     def to(self, device):
         g = object.__new__(Grammar)

@@ -28,7 +28,10 @@ def test_next_states_outside_the_table_stay_outside():
     allowed = torch.ones(3, 4, dtype=torch.bool)
     nxt = torch.tensor([[0, 1, 2, 3], [-7, 2 ** 40, -2 ** 40, 1], [0, 0, 0, 0]])
     g = Grammar(allowed, nxt)
+    assert g.next_state.dtype == torch.int32
     assert g.next_state.tolist() == [[0, 1, 2, 3], [-1, 3, -1, 1], [0, 0, 0, 0]]
+    small = torch.tensor([[0, -5, 7, 1]] * 3, dtype=torch.int32)
+    assert Grammar(allowed, small).next_state.tolist() == small.tolist()
 
 
 def test_grammar_refusals():
