@@ -16,7 +16,7 @@
 // Numbers.  A token the history does not hold has the value x + b, one fp32 rounding; a counted one is computed in
 // double and rounded once.  Decisions do not rest on that rounding: rounding is monotone, so the largest exact value is
 // among the elements whose rounded value is the largest; those few are compared by the part the rounding dropped
-// (two-sum; for counted ones double minus the rounded value).  A drawn token is decided where a running sum over the
+// (the double minus the rounded value).  A drawn token is decided where a running sum over the
 // whole vocabulary crosses u Z, and with thousands of probable tokens a border of fp32 sums lies within their rounding of
 // u Z for a few percent of the rows: its weights and sums are doubles, with an exp2 of 4e-14.
 #include <algorithm>
@@ -30,6 +30,7 @@ namespace {
 
 constexpr double LOG2E = 1.4426950408889634074;
 constexpr double LN2 = 0.69314718055994530942;
+constexpr double TEMP_MIN = 1e-37, TEMP_MAX = 1e37;       // k and 1 / k are ordinary floats
 
 // what a wave knows about its row
 struct RowP {
@@ -38,10 +39,10 @@ struct RowP {
   const float* bias;              // or NULL
   const char* hist;               // the row's history
   int n_hist;
+  bool fine;                      // the temperature is one (TEMP_MIN .. TEMP_MAX); else the row is NaN, as for a NaN logit
 };
 
-// 1 / v to the last bits: the hardware's approximation and two Newton steps (no infinities or zeros inside: those rows
-// are refused by their k)
+// 1 / v to the last bits for an ordinary v: the hardware's approximation and two Newton steps
 __device__ __forceinline__ double reciprocal(double v) {
   double r = __builtin_amdgcn_rcp(v);
   r = fma(fma(-v, r, 1.0), r, r);
@@ -69,6 +70,7 @@ __device__ __forceinline__ RowP row_params(const Rules& q, long long r) {
     p.temp = q.temperature_rows[r];
     p.k = LOG2E * reciprocal(p.temp);
   }
+  p.fine = p.temp >= TEMP_MIN && p.temp <= TEMP_MAX;
   p.bias = q.bias ? q.bias + r * q.bias_ld : nullptr;
   p.mask = nullptr;
   if (q.mask) {
@@ -138,7 +140,8 @@ __device__ __forceinline__ double wave_sum(double v) {
 
 // 2^(d k) in double for d k from -1000 (`low` = -1000 / k; what lies below counts as 2^-1000) to 1000: a = d k = n + f,
 // |f| <= 1/2; n by adding 1.5 2^52, which leaves it in the low bits; 2^f as 1 + f q(f), q the polynomial that
-// meets (2^f - 1) / f in the nine Chebyshev nodes of [-1/2, 1/2] (off by at most 3.7e-14 of the result, exact at 0); n goes into the exponent by an integer addition.
+// meets (2^f - 1) / f in the nine Chebyshev nodes of [-1/2, 1/2] (off by at most 3.7e-14 of the result, exact at 0);
+// n goes into the exponent by an integer addition.
 // 15 operations of full rate: the accurate exp of the math library and its branches took three times as long.
 __device__ __forceinline__ double exp2_fast(double d, double k, double low) {
   constexpr double SHIFT = 6755399441055744.0;
@@ -566,7 +569,7 @@ __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
   constexpr bool DRAW = MODE == M_DRAW;
   typedef Elem<T> E;
   constexpr int EV = E::EV;
-  extern __shared__ uint32_t lds[];          // counts of the workgroup's 4 segments, a bit for each token, and the lists of counted ones
+  extern __shared__ uint32_t lds[];          // counts of the 4 segments, a bit for each token, lists of the counted ones
   const Rules& q = a.q;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -731,7 +734,7 @@ __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
     return;
   }
   // a row of one segment: its wave decides it
-  const bool ok = m > -INFINITY && m < INFINITY && p.k > 0.0 && p.k < INFINITY;
+  const bool ok = m > -INFINITY && m < INFINITY && p.fine;
   long long tok = -1;
   const auto count = [&](int v) { return HIST ? count_at<HIST ? HIST : 1>(cnt, v) : 0u; };
   // values of EV tokens, -inf where there is none
@@ -905,8 +908,7 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
   float m = mine.m;
   for (int i = i0 + 1; i < i1; ++i) m = max_nan(m, seg[i].m);
   m = block_reduce(m, shf, [](float x, float y) { return max_nan(x, y); });
-  // a temperature that is not positive and finite makes the row NaN, as a NaN logit does
-  const bool ok = m > -INFINITY && m < INFINITY && p.k > 0.0 && p.k < INFINITY;
+  const bool ok = m > -INFINITY && m < INFINITY && p.fine;
   const auto scaled = [&](const Seg& s) { return s.m > -INFINITY ? s.s * exp2_64((double)s.ref - (double)m, p.k) : 0.0; };
   double z0 = 0.0, z = 0.0;
   if (ok) {
@@ -1191,7 +1193,7 @@ __global__ __launch_bounds__(256) void rules_tiny_kernel(SmallArgs a) {
     float m = (float)y[0];
 #pragma unroll
     for (int v = 1; v < VM; ++v) m = max_nan(m, (float)y[v]);
-    const bool ok = m > -INFINITY && m < INFINITY && p.k > 0.0 && p.k < INFINITY;
+    const bool ok = m > -INFINITY && m < INFINITY && p.fine;
     double w[VM], Z = 0.0;
 #pragma unroll
     for (int v = 0; v < VM; ++v) {
@@ -1289,7 +1291,7 @@ __global__ __launch_bounds__(256) void rules_small_kernel(SmallArgs a) {
     }
     float m = (float)y;
     for (int o = W >> 1; o > 0; o >>= 1) m = max_nan(m, __shfl_xor(m, o));
-    const bool ok = m > -INFINITY && m < INFINITY && p.k > 0.0 && p.k < INFINITY;
+    const bool ok = m > -INFINITY && m < INFINITY && p.fine;
     const double w = kept && ok ? exp2_64(y - (double)m, p.k) : 0.0;
     double run = w;                                   // running sum in the vocabulary's order
     for (int o = 1; o < W; o <<= 1) {
@@ -1570,11 +1572,11 @@ int rules_check(const dvae_rules& q, const char* who) {
   DVAE_REQUIRE(q.dtype == DVAE_F32 || q.dtype == DVAE_BF16 || q.dtype == DVAE_F16, "%s: dtype %d", who, q.dtype);
   DVAE_REQUIRE(q.logits || q.rows == 0, "%s: null logits", who);
   DVAE_REQUIRE(q.rows <= 1 || q.ld >= q.vocab, "%s: rows of logits overlap (ld %lld < vocab %d)", who, q.ld, q.vocab);
-  DVAE_REQUIRE(q.vocab <= (1 << 30), "%s: vocab %d above 2^30", who, q.vocab);
+  DVAE_REQUIRE(q.vocab <= (1 << 27), "%s: vocab %d above 2^27", who, q.vocab);
   DVAE_REQUIRE(q.repetition_rows || (q.repetition > 0.0 && std::isfinite(q.repetition)), "%s: repetition must be positive", who);
   DVAE_REQUIRE(q.frequency_rows || std::isfinite(q.frequency), "%s: frequency must be finite", who);
   DVAE_REQUIRE(q.presence_rows || q.presence > -INFINITY, "%s: presence must be above -inf", who);
-  DVAE_REQUIRE(q.temperature_rows || (q.temperature > 0.0 && std::isfinite(q.temperature)), "%s: temperature must be positive", who);
+  DVAE_REQUIRE(q.temperature_rows || (q.temperature >= TEMP_MIN && q.temperature <= TEMP_MAX), "%s: temperature must be in [1e-37, 1e37]", who);
   if (q.history) {
     DVAE_REQUIRE(q.history_len >= 0 && q.history_ld >= 0, "%s: negative history length", who);
     DVAE_REQUIRE(q.rows_per_history >= 1, "%s: rows_per_history must be at least 1", who);

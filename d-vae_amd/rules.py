@@ -20,7 +20,7 @@ all rows or an fp32 tensor with one per row.  Rows may lie anywhere in memory as
 layouts are copied).  Everything is queued on the current stream of the logits' device.
 
 A row whose rules leave nothing: token -1, log-probability -inf, no gradient.  A row that allows a NaN or a +inf, or whose
-own temperature is not positive and finite: token -1, log-probability NaN.
+own temperature is not in [1e-37, 1e37]: token -1, log-probability NaN.
 """
 import collections
 import math
@@ -226,8 +226,8 @@ class _Call:
         q.frequency = self._setting(q, "frequency", rules.frequency)
         q.presence = self._setting(q, "presence", rules.presence)
         q.temperature = t = self._setting(q, "temperature", temperature)
-        if not (t > 0.0 and t < math.inf):
-            raise ValueError("temperature must be positive and finite, got %r" % t)
+        if not 1e-37 <= t <= 1e37:
+            raise ValueError("temperature must be in [1e-37, 1e37], got %r" % t)
         if index < 0:
             E._require_cuda(logits, "logits")
         self.q = q

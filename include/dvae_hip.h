@@ -504,8 +504,8 @@ int dvae_clip_grads(const dvae_tensor* tensors, int n, double max_norm, float* n
  *   x3 = x2 + bias[v]
  *   x4 = the row's grammar state allows v ? x3 : -inf;  p = softmax(x4 / temperature)
  * Each setting is one double for all rows, or an array of one float per row (the *_rows pointers) where that is not NULL.
- * repetition and temperature are positive, temperature finite; a row whose own temperature is not, or that allows a NaN or
- * +inf logit, has token -1 and a NaN log-probability.
+ * repetition is positive and finite, temperature in [1e-37, 1e37], vocab at most 2^27; a row whose own temperature is not,
+ * or that allows a NaN or +inf logit, has token -1 and a NaN log-probability.
  * ---------------------------------------------------------------------- */
 typedef struct dvae_rules {
   const void* logits;         /* [rows][ld], ld >= vocab, any alignment of the type                                   */

@@ -443,6 +443,29 @@ def test_temperatures_of_rows_that_are_no_temperatures(cuda):
         assert torch.isnan(lp[:4]).all() and torch.isfinite(lp[4])
 
 
+def test_temperatures_at_the_ends(cuda):
+    """1e37: every allowed token alike; 1e-37: only the largest has a probability (a tie: two halves)."""
+    from dvae_amd.rules import Grammar, TokenRules, choose, token_logprob
+    for vocab in (6, 500, 9000):
+        x = torch.randn(3, vocab, generator=torch.Generator().manual_seed(0)).to(cuda)
+        x[1] = torch.finfo(torch.float32).min
+        x[2, :2] = 50.0
+        allowed = torch.ones(1, vocab, dtype=torch.bool, device=cuda)
+        allowed[0, vocab - 1] = False
+        r, st = TokenRules(grammar=Grammar(allowed)), torch.zeros(3, dtype=torch.int32, device=cuda)
+        flat = choose(x, r, state=st, temperature=1e37, uniforms=torch.full((3,), 0.999999, device=cuda))
+        assert flat.tokens.tolist()[0] == vocab - 2 and flat.tokens.tolist()[2] == vocab - 2
+        assert torch.allclose(flat.logprob[[0, 2]].double(), torch.full((2,), -math.log(vocab - 1), dtype=torch.float64, device=cuda),
+                              rtol=2 * U, atol=0)
+        cold = choose(x, r, state=st, temperature=1e-37, uniforms=torch.full((3,), 0.75, device=cuda))
+        best = int(x[0, :vocab - 1].argmax())
+        assert cold.tokens.tolist() == [best, (3 * (vocab - 1)) // 4, 1] and abs(float(cold.logprob[0])) <= 1e-13
+        assert abs(float(cold.logprob[2]) + math.log(2)) <= 2 * U
+        t = torch.tensor([best, 0, 1], device=cuda)
+        lp = token_logprob(x, t, r, state=st, temperature=1e-37)
+        assert abs(lp[0].item()) <= U and abs(lp[1].item() + math.log(vocab - 1)) <= 1e-5 and abs(lp[2].item() + math.log(2)) <= 2 * U
+
+
 def test_ties_go_to_the_lowest_index(cuda):
     from dvae_amd.rules import TokenRules, choose
     for vocab in (8, 600, 20000):

@@ -99,7 +99,7 @@ def test_refused_arguments(i):
 
 
 def test_refused_temperatures_uniforms_tokens_and_outputs():
-    for t in (0.0, -1.0, math.inf, math.nan, torch.ones(3), torch.ones(4, dtype=torch.float64),
+    for t in (0.0, -1.0, math.inf, math.nan, 1e-38, 1e38, torch.ones(3), torch.ones(4, dtype=torch.float64),
               torch.ones(4, requires_grad=True)):
         with pytest.raises(ValueError):
             rules.choose(X, TokenRules(), temperature=t)
@@ -144,6 +144,7 @@ BAD_RULES = [dict(rows=-1), dict(vocab=0), dict(vocab=(1 << 30) + 1, ld=1 << 31)
              dict(ld=15), dict(repetition=0.0),
              dict(repetition=float("inf")), dict(frequency=float("nan")), dict(presence=float("nan")),
              dict(presence=float("-inf")), dict(temperature=0.0), dict(temperature=float("inf")),
+             dict(temperature=9e-38), dict(temperature=1.1e37), dict(vocab=(1 << 27) + 1, ld=1 << 28),
              dict(history=4096, history_len=-1), dict(history=4096, history_len=2, history_ld=-1),
              dict(history=4096, history_len=2, rows_per_history=0), dict(mask=4096, states=1, mask_words=1),
              dict(mask=4096, states=0, mask_words=1, state=4096), dict(mask=4096, states=1, mask_words=0, state=4096),
