@@ -5,13 +5,20 @@
 //   x1 = c > 0 ? (x > 0 ? x / rho : x * rho) : x;  x2 = x1 - frequency c - presence [c > 0];  x3 = x2 + bias[v]
 //   x4 = allowed(state, v) ? x3 : -inf;            p = softmax(x4 / T)
 //
-// The operations are one pass over the logits.  A row is cut into segments, one wave each (64 lanes x 16 bytes a step); a
-// lane keeps a running sum of exp against a reference of its own that moves only when a value exceeds it by 2^8 -- no
-// rescaling in the common step, no block barrier.  Segments of one row leave (maximum, sum) pairs that a second, small
-// launch joins: sum_r = sum_seg s_seg 2^((m_seg - m) k), k = log2(e) / T; the token is then looked for in ONE segment.
+// Kernels, by size.
+//   map    (apply, gradients) and sum (what a softmax needs): a row is cut into segments of up to 2048 tokens, one wave each,
+//          64 lanes x 16 bytes a step, four steps in flight.  Rows of one segment are decided by their wave on the spot.
+//   join   the other rows: segments leave (sum, reference, maximum); a workgroup a row adds them, finds the ONE segment the
+//          token is in and searches it again.
+//   small  up to 64 tokens: a group of lanes a row, everything in one launch; tiny: up to 16 tokens and many rows, a lane a row.
+//   col    gradients with a bias shared by the rows: its sum over rows in registers.
+// Counts: a workgroup counts the history's tokens that fall into its segments in LDS (integer atomics: their order does not
+// matter).
 //
-// Counts: a workgroup counts the history's tokens that fall into its 4 segments in LDS (integer atomics: the order does
-// not matter).
+// Bounds.  apply and log p move the logits once each way and are bound by memory: 256 x 131072 bf16 under all rules 31 us (137
+// MB, 4.4 TB/s), log p of 4096 x 65536 bf16 100 + 10 us, its gradients 175 us (1.07 GB, 6.1 TB/s).  A drawn batch is bound by
+// its sums of doubles: 512 x 131072 bf16 under all rules 105 us for 41 M wave instructions -- 39 per element, 15 of them the exp, 15 its value and
+// masks, the rest counting and reductions -- where the bytes alone would take 29 us; + 17 us join.
 //
 // Numbers.  A token the history does not hold has the value x + b, one fp32 rounding; a counted one is computed in
 // double and rounded once.  Decisions do not rest on that rounding: rounding is monotone, so the largest exact value is
@@ -259,8 +266,7 @@ __device__ __forceinline__ Loaded load_step(const RowP& p, const char* lrow, int
   Loaded l;
   l.keep = (1u << EV) - 1;
   if (WHOLE || v + EV <= V) {
-    // read once: not to push out what is read again
-    l.raw = __builtin_nontemporal_load(reinterpret_cast<const u32x4_u*>(lrow + (size_t)v * BYTES));
+    l.raw = *reinterpret_cast<const u32x4_u*>(lrow + (size_t)v * BYTES);
   } else {
     l.raw = u32x4{0, 0, 0, 0};
     l.keep = v < V ? (1u << (V - v)) - 1 : 0u;
@@ -302,6 +308,8 @@ __device__ __forceinline__ void store_step(typename Elem<T>::type* orow, int v, 
   if (WHOLE || v + EV <= V) {
     u32x4 w;
     __builtin_memcpy(&w, o, 16);
+    // streamed: results do not push logits out of the cache (a training pass over 4096 x 65536 bf16 299 -> 289 us; streamed
+    // loads as well 282, but where logits fit the cache they cost: 301 x 50021 fp32 kernels 66 -> 83 us)
     __builtin_nontemporal_store(w, reinterpret_cast<u32x4_u*>(orow + v));
   } else {
 #pragma unroll
