@@ -550,7 +550,7 @@ __device__ __forceinline__ Counted load_counted(const Rules& q, const RowP& p, c
   t.x = Elem<T>::one(lrow, v);
   t.b = p.bias ? p.bias[v] : 0.f;
   t.kept = !p.mask || ((p.mask[v >> 3] >> (v & 7)) & 1);
-  t.c = count_at<HIST ? HIST : 1>(cnt, d);
+  t.c = HIST ? count_at<HIST ? HIST : 1>(cnt, d) : 0u;
   return t;
 }
 template <int T>
@@ -570,7 +570,7 @@ constexpr int LIST = 512;       // counted tokens of a segment that are listed; 
 // A segment's maximum and sum of weights.  Tokens that the history holds are left out of the steps (one more bit mask) and
 // taken afterwards, a lane each: they are few, and the steps stay free of branches.
 // DRAW: sums of doubles, against 0 as reference -- an exponent of a double has room for every ordinary row; where the
-// maximum is no ordinary one (beyond 2^-400 .. 2^900) the segment is summed again against it.  Else fp32 sums, against a
+// maximum is no ordinary one (beyond 2^-400 .. 2^900) the segment is summed again against it, token by token.  Else fp32 sums, against a
 // reference of the lane's own that moves when a value exceeds it by 2^8 (an exponent of 8 is still exact to 2^-20).
 template <int T, int HIST, int MODE, bool ROWWAVE>
 __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
@@ -648,77 +648,74 @@ __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
       lim = ref + room;
     }
   };
-  const auto scan = [&](auto shifted, double base) {
-    const auto weigh = [&](double y) { zd += exp2_fast(decltype(shifted)::value ? y - base : y, p.k, low); };
-    steps.run(p, lrow, V, [&](Loaded in, int v, auto whole) {
-      constexpr bool WHOLE = decltype(whole)::value;
-      if (HIST) {
-        const uint32_t byte = reinterpret_cast<const uint8_t*>(seen)[(v - v0) >> 3];
-        in.keep &= ~(EV == 8 ? byte : byte >> (v & 4));
-      }
-      float x[EV], s[EV];
-#pragma unroll
-      for (int e = 0; e < EV; ++e) x[e] = E::at(in.raw, e);
-      const auto on = [&](int e) { return (uint32_t)((int)(in.keep << (31 - e)) >> 31); };
-      if (HIST || p.mask || !WHOLE) {
-#pragma unroll
-        for (int e = 0; e < EV; ++e) x[e] = __uint_as_float((__float_as_uint(x[e]) & on(e)) | (0xff800000u & ~on(e)));
-      }
-      if (p.bias) {
-        float b[EV];
-        load_bias<EV, WHOLE>(p.bias, v, V, b);
-        if (HIST || p.mask) {
-#pragma unroll
-          for (int e = 0; e < EV; ++e) b[e] = __uint_as_float(__float_as_uint(b[e]) & on(e));
-        }
-#pragma unroll
-        for (int e = 0; e < EV; ++e) s[e] = x[e] + b[e];
-        if (DRAW) {
-#pragma unroll
-          for (int e = 0; e < EV; ++e) weigh((double)x[e] + (double)b[e]);
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < EV; ++e) s[e] = x[e];
-        if (DRAW) {
-#pragma unroll
-          for (int e = 0; e < EV; ++e) weigh((double)x[e]);
-        }
-      }
-      float mx = s[0];
-#pragma unroll
-      for (int e = 1; e < EV; ++e) mx = max_nan(mx, s[e]);
-      take(mx);
-      if (!DRAW) {
-#pragma unroll
-        for (int e = 0; e < EV; ++e) z += __builtin_amdgcn_exp2f((s[e] - ref) * kf);
-      }
-    });
+  const auto weigh = [&](double y) { zd += exp2_fast(y, p.k, low); };
+  steps.run(p, lrow, V, [&](Loaded in, int v, auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value;
     if (HIST) {
-      const auto one = [&](double y) {
-        take((float)y);
-        if (DRAW) weigh(y);
-        else z += __builtin_amdgcn_exp2f(((float)y - ref) * kf);
-      };
-      if (held <= LIST) {
-        if (lane < held) one(counted_value<T>(p, first_held));
-        for (int i = lane + 64; i < held; i += 256) {          // four in flight
-          Counted t[4];
+      const uint32_t byte = reinterpret_cast<const uint8_t*>(seen)[(v - v0) >> 3];
+      in.keep &= ~(EV == 8 ? byte : byte >> (v & 4));
+    }
+    float x[EV], s[EV];
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (i + 64 * u < held) t[u] = load_counted<T, HIST>(q, p, lrow, cnt, v0, list[i + 64 * u]);
+    for (int e = 0; e < EV; ++e) x[e] = E::at(in.raw, e);
+    const auto on = [&](int e) { return (uint32_t)((int)(in.keep << (31 - e)) >> 31); };
+    if (HIST || p.mask || !WHOLE) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (i + 64 * u < held) one(counted_value<T>(p, t[u]));
-        }
-      } else {
-        for (int w = lane; w < a.seg_len / 32; w += 64)
-          for (uint32_t left = seen[w]; left; left &= left - 1)
-            one(counted_value<T>(p, load_counted<T, HIST>(q, p, lrow, cnt, v0, w * 32 + __ffs(left) - 1)));
+      for (int e = 0; e < EV; ++e) x[e] = __uint_as_float((__float_as_uint(x[e]) & on(e)) | (0xff800000u & ~on(e)));
+    }
+    if (p.bias) {
+      float b[EV];
+      load_bias<EV, WHOLE>(p.bias, v, V, b);
+      if (HIST || p.mask) {
+#pragma unroll
+        for (int e = 0; e < EV; ++e) b[e] = __uint_as_float(__float_as_uint(b[e]) & on(e));
+      }
+#pragma unroll
+      for (int e = 0; e < EV; ++e) s[e] = x[e] + b[e];
+      if (DRAW) {
+#pragma unroll
+        for (int e = 0; e < EV; ++e) weigh((double)x[e] + (double)b[e]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < EV; ++e) s[e] = x[e];
+      if (DRAW) {
+#pragma unroll
+        for (int e = 0; e < EV; ++e) weigh((double)x[e]);
       }
     }
-  };
-  scan(std::false_type{}, 0.0);
+    float mx = s[0];
+#pragma unroll
+    for (int e = 1; e < EV; ++e) mx = max_nan(mx, s[e]);
+    take(mx);
+    if (!DRAW) {
+#pragma unroll
+      for (int e = 0; e < EV; ++e) z += __builtin_amdgcn_exp2f((s[e] - ref) * kf);
+    }
+  });
+  if (HIST) {
+    const auto one = [&](double y) {
+      take((float)y);
+      if (DRAW) weigh(y);
+      else z += __builtin_amdgcn_exp2f(((float)y - ref) * kf);
+    };
+    if (held <= LIST) {
+      if (lane < held) one(counted_value<T>(p, first_held));
+      for (int i = lane + 64; i < held; i += 256) {          // four in flight
+        Counted t[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (i + 64 * u < held) t[u] = load_counted<T, HIST>(q, p, lrow, cnt, v0, list[i + 64 * u]);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (i + 64 * u < held) one(counted_value<T>(p, t[u]));
+      }
+    } else {
+      for (int w = lane; w < a.seg_len / 32; w += 64)
+        for (uint32_t left = seen[w]; left; left &= left - 1)
+          one(counted_value<T>(p, load_counted<T, HIST>(q, p, lrow, cnt, v0, w * 32 + __ffs(left) - 1)));
+    }
+  }
   m = wave_max_nan(m);
   Seg r;
   r.s = 0.0; r.m = m; r.ref = m;
@@ -726,11 +723,11 @@ __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
     if (DRAW) {
       const double top = (double)m * p.k;
       r.ref = 0.f;
-      if (!(top > -400.0 && top < 900.0)) {
+      if (!(top > -400.0 && top < 900.0)) {       // no ordinary row: token by token
         r.ref = m;
         zd = 0.0;
-        steps.begin(p, lrow, v0, end, lane, V);
-        scan(std::true_type{}, (double)m);
+        for (int d = lane; d < end - v0; d += 64)
+          zd += exp2_64(any_value<T>(p, load_counted<T, HIST>(q, p, lrow, cnt, v0, d)) - (double)m, p.k);
       }
       r.s = wave_sum(zd);
     } else {

@@ -466,6 +466,25 @@ def test_temperatures_at_the_ends(cuda):
         assert abs(lp[0].item()) <= U and abs(lp[1].item() + math.log(vocab - 1)) <= 1e-5 and abs(lp[2].item() + math.log(2)) <= 2 * U
 
 
+@pytest.mark.parametrize("shift", [4096.0, -4096.0])
+def test_rows_far_from_zero(cuda, shift):
+    """A softmax does not see a shift (exact here: multiples of 2^-6): exponents of +-12000 and more."""
+    from dvae_amd.rules import choose, token_logprob
+    for vocab in (7, 500, 9000):
+        g = torch.Generator().manual_seed(3)
+        x = (torch.randn(8, vocab, generator=g) * 3 * 64).round().div(64).to(cuda)
+        u, tok = torch.rand(8, generator=g).to(cuda), torch.randint(0, vocab, (8,), generator=g).to(cuda)
+        hist = torch.randint(0, vocab, (8, 5), generator=g).to(cuda)
+        for kw in (dict(), dict(history=hist)):
+            for uu in (u, None):
+                a, b = choose(x, uniforms=uu, temperature=0.5, **kw), choose(x + shift, uniforms=uu, temperature=0.5, **kw)
+                assert torch.equal(a.tokens, b.tokens)
+                assert float((a.logprob - b.logprob).abs().max()) <= 4 * U * (float(a.logprob.abs().max()) + 100)
+            a, b = token_logprob(x, tok, temperature=0.5, **kw), token_logprob(x + shift, tok, temperature=0.5, **kw)
+            # both sums are of the same differences x4 - ref: they differ by the segments' joins only
+            assert float((a - b).abs().max()) <= 4 * U * (float(a.abs().max()) + 100)
+
+
 def test_ties_go_to_the_lowest_index(cuda):
     from dvae_amd.rules import TokenRules, choose
     for vocab in (8, 600, 20000):
