@@ -10,7 +10,7 @@
 //          64 lanes x 16 bytes a step, four steps in flight.  Rows of one segment are decided by their wave on the spot.
 //   join   the other rows: segments leave (sum, reference, maximum); a workgroup a row adds them, finds the ONE segment the
 //          token is in and searches it again.
-//   small  up to 64 tokens: a group of lanes a row, everything in one launch; tiny: up to 16 tokens and many rows, a lane a row.
+//   group  up to 128 tokens: a group of lanes a row, eight tokens a lane, everything in one launch.
 //   col    gradients with a bias shared by the rows: its sum over rows in registers.
 // Counts: a workgroup counts the history's tokens that fall into its segments in LDS (integer atomics: their order does not
 // matter).
@@ -1085,261 +1085,175 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// small vocabularies: W lanes a row (W the power of two from the vocabulary on, up to a wave), one token a lane, one
-// launch that ends each row -- everything in double, sums and searches by shuffles inside the group
+// vocabularies of up to 128 tokens: a group of W lanes a row (a power of two), eight tokens a lane, one launch that ends each
+// row -- everything in double, sums and searches by shuffles inside the group.  Eight tokens a lane, because what a row costs
+// once (its settings, log, decision) takes a whole wave's time however few lanes share it: 100000 x 8 drawn after seven tokens
+// of history 8.5 us with a lane a row, 15.6 us with eight.  Against a wave a row: 100000 x 65 bf16 drawn 43 / 160 us, applied 45 /
+// 59 us, but 20000 x 300 fp32 40 / 32 and 37 / 15 us.
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int SMALL_VOCAB = 64, SMALL_HISTORY = 256;
+constexpr int GROUP_TOKENS = 8, GROUP_VOCAB = 128;
 
-struct SmallArgs {
+struct GroupArgs {
   Rules q;
   RowOut o;
   int w;                          // lanes of a row
   const float* d_logprob; void* out; long long out_ld; float* d_bias; float* part;             // APPLY, BWD
 };
 
-template <typename X>
-__device__ __forceinline__ X group_sum(X v, int w) {
-  for (int o = w >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  return v;
-}
-
-// Vocabularies of up to VM = 8 or 16 tokens with many rows: a lane a row.  No sums or searches across lanes, and an eighth of
-// the operations of a group of lanes, whose single exp, log and decision each take a whole wave's time: 100000 x 8 drawn with
-// seven tokens of history 8.6 us (15.6 in groups).  But 64 rows a wave make few waves: at 32768 x 8 the two are even
-// (log p 5.2 / 6.1, gradients 5.4 / 4.4 us), so fewer rows take the groups.
-constexpr int TINY_VOCAB = 16, TINY_ROWS = 32768, TINY_HISTORY = 255;      // counts are bytes of a register
-
-template <int T, int VM, int MODE>
-__global__ __launch_bounds__(256) void rules_tiny_kernel(SmallArgs a) {
+template <int T, int MODE>
+__global__ __launch_bounds__(256) void rules_group_kernel(GroupArgs a) {
   typedef Elem<T> E;
-  constexpr int EV = E::EV;
-  __shared__ float acc_sh[4][VM];
+  constexpr int EV = E::EV, K = GROUP_TOKENS;
+  __shared__ float acc_sh[MODE == M_BWD ? 4 : 1][MODE == M_BWD ? GROUP_VOCAB : 1];
   const Rules& q = a.q;
-  const int V = q.vocab;
-  float acc[VM];
+  const int W = a.w, V = q.vocab;
+  const int lane = threadIdx.x & (W - 1), v0 = lane * K;
+  const int groups = 256 / W;
+  float acc[K];
 #pragma unroll
-  for (int v = 0; v < VM; ++v) acc[v] = 0.f;
-  for (long long row = (long long)blockIdx.x * 256 + threadIdx.x; row < q.rows; row += (long long)gridDim.x * 256) {
+  for (int j = 0; j < K; ++j) acc[j] = 0.f;
+  for (long long row = (long long)blockIdx.x * groups + threadIdx.x / W; row < q.rows; row += (long long)gridDim.x * groups) {
     const RowP p = row_params(q, row);
     const char* lrow = static_cast<const char*>(q.logits) + row * q.ld * (long long)sizeof(typename E::type);
-    float x[VM];
-    if (V == VM) {
+    float x[K], b[K];
+    uint32_t keep = v0 >= V ? 0u : v0 + K <= V ? 0xffu : (1u << (V - v0)) - 1;
+    if (v0 + K <= V) {
 #pragma unroll
-      for (int i = 0; i < VM / EV; ++i) {
-        const u32x4 raw = *reinterpret_cast<const u32x4_u*>(lrow + 16 * i);
+      for (int i = 0; i < K / EV; ++i) {
+        const u32x4 raw = *reinterpret_cast<const u32x4_u*>(lrow + (size_t)v0 * sizeof(typename E::type) + 16 * i);
 #pragma unroll
         for (int e = 0; e < EV; ++e) x[i * EV + e] = E::at(raw, e);
       }
     } else {
 #pragma unroll
-      for (int v = 0; v < VM; ++v) x[v] = v < V ? E::one(lrow, v) : 0.f;
+      for (int j = 0; j < K; ++j) x[j] = v0 + j < V ? E::one(lrow, v0 + j) : 0.f;
     }
-    uint32_t keep = p.mask ? *reinterpret_cast<const uint32_t*>(p.mask) : 0xffffffffu;
-    keep &= (1u << V) - 1;
-    uint64_t c0 = 0, c1 = 0;
-    const auto add = [&](long long t) {
-      const uint64_t one = (unsigned long long)t < (unsigned long long)V ? 1ull << (8 * (t & 7)) : 0ull;
-      if (VM == 8 || t < 8) c0 += one;
-      else c1 += one;
-    };
-    int i = 0;
-    for (; i + 3 < p.n_hist; i += 4) {
-      long long t[4];
+    if (p.mask && v0 < V) keep &= p.mask[lane];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) t[u] = hist_at(p, q.history_i64, i + u);
+    for (int j = 0; j < K; ++j) b[j] = p.bias && v0 + j < V ? p.bias[v0 + j] : 0.f;
+    // counts: bytes of a register (a history has at most 255 tokens here)
+    uint64_t c = 0;
+    for_history<4>(p, q.history_i64, 0, 0, 1, [&](long long t) {
+      const unsigned long long d = (unsigned long long)(t - v0);
+      c += d < K ? 1ull << (8 * (d & 7)) : 0ull;
+    });
+    const auto count = [&](int j) { return (uint32_t)(c >> (8 * j)) & 0xffu; };
+    double y[K];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) add(t[u]);
-    }
-    for (; i < p.n_hist; ++i) add(hist_at(p, q.history_i64, i));
-    const auto count = [&](int v) { return (uint32_t)((v < 8 ? c0 : c1) >> (8 * (v & 7))) & 0xffu; };
-    double y[VM];
-#pragma unroll
-    for (int v = 0; v < VM; ++v) {
-      const float b = p.bias && v < V ? p.bias[v] : 0.f;
-      y[v] = -INFINITY;
-      if ((keep >> v) & 1) y[v] = count(v) ? counted64(p, x[v], count(v), b) : (double)x[v] + (double)b;
+    for (int j = 0; j < K; ++j) {
+      y[j] = -INFINITY;
+      if ((keep >> j) & 1) y[j] = count(j) ? counted64(p, x[j], count(j), b[j]) : (double)x[j] + (double)b[j];
     }
     if (MODE == M_APPLY || MODE == M_BWD) {
-      typename E::type o[VM];
+      float out[K];
       if (MODE == M_BWD) {
         const float m = a.o.stat[2 * row];
         const long long tok = a.o.given[row];
         const bool zero = tok < 0 || tok >= V || m == -INFINITY;
         const double coef = (double)a.d_logprob[row] * (p.k * LN2), iz = a.o.stat[2 * row + 1];
 #pragma unroll
-        for (int v = 0; v < VM; ++v) {
+        for (int j = 0; j < K; ++j) {
           double g = 0.0;
-          if (!zero && ((keep >> v) & 1)) g = coef * ((v == tok ? 1.0 : 0.0) - exp2_64(y[v] - (double)m, p.k) * iz);
+          if (!zero && ((keep >> j) & 1)) g = coef * ((v0 + j == tok ? 1.0 : 0.0) - exp2_64(y[j] - (double)m, p.k) * iz);
           const float gf = (float)g;
-          if (a.part) acc[v] += gf;
-          else if (a.d_bias && v < V) a.d_bias[row * V + v] = gf;
-          if (count(v)) g *= x[v] > 0.f ? p.inv_rho : p.rho;
-          o[v] = E::cast((float)g);
+          if (a.part) acc[j] += gf;
+          else if (a.d_bias && v0 + j < V) a.d_bias[row * V + v0 + j] = gf;
+          if (count(j)) g *= x[j] > 0.f ? p.inv_rho : p.rho;
+          out[j] = (float)g;
         }
       } else {
 #pragma unroll
-        for (int v = 0; v < VM; ++v) o[v] = E::cast((float)y[v]);
+        for (int j = 0; j < K; ++j) out[j] = (float)y[j];
       }
       typename E::type* orow = static_cast<typename E::type*>(a.out) + row * a.out_ld;
-      if (V == VM) {
+      typename E::type o[K];
 #pragma unroll
-        for (int j = 0; j < VM / EV; ++j) {
+      for (int j = 0; j < K; ++j) o[j] = E::cast(out[j]);
+      if (v0 + K <= V) {
+#pragma unroll
+        for (int i = 0; i < K / EV; ++i) {
           u32x4 w;
-          __builtin_memcpy(&w, o + j * EV, 16);
-          *reinterpret_cast<u32x4_u*>(orow + j * EV) = w;
+          __builtin_memcpy(&w, o + i * EV, 16);
+          *reinterpret_cast<u32x4_u*>(orow + v0 + i * EV) = w;
         }
       } else {
 #pragma unroll
-        for (int v = 0; v < VM; ++v)
-          if (v < V) orow[v] = o[v];
+        for (int j = 0; j < K; ++j)
+          if (v0 + j < V) orow[v0 + j] = o[j];
       }
       continue;
     }
     float m = (float)y[0];
 #pragma unroll
-    for (int v = 1; v < VM; ++v) m = max_nan(m, (float)y[v]);
+    for (int j = 1; j < K; ++j) m = max_nan(m, (float)y[j]);
+    for (int o = W >> 1; o > 0; o >>= 1) m = max_nan(m, __shfl_xor(m, o));
     const bool ok = m > -INFINITY && m < INFINITY && p.fine;
-    double w[VM], Z = 0.0;
+    double w[K], sum = 0.0;
 #pragma unroll
-    for (int v = 0; v < VM; ++v) {
-      w[v] = ok && ((keep >> v) & 1) ? exp2_64(y[v] - (double)m, p.k) : 0.0;
-      Z += w[v];
+    for (int j = 0; j < K; ++j) {
+      w[j] = ok && ((keep >> j) & 1) ? exp2_64(y[j] - (double)m, p.k) : 0.0;
+      sum += w[j];
     }
+    double run = sum;                                 // running sum of the lanes, in the vocabulary's order
+    for (int o = 1; o < W; o <<= 1) {
+      const double t = __shfl_up(run, o, W);
+      if (lane >= o) run += t;
+    }
+    const double Z = __shfl(run, W - 1, W);
     int tok = -1;
     if (MODE == M_SUM) {
       const long long t = a.o.given[row];
       tok = t >= 0 && t < V ? (int)t : -1;
     } else if (ok && MODE == M_GREEDY) {
       double best = -INFINITY;
+      int idx = INT32_MAX;
 #pragma unroll
-      for (int v = 0; v < VM; ++v)
-        if (y[v] > best) { best = y[v]; tok = v; }
-    } else if (ok && MODE == M_DRAW) {
-      const float u = a.o.uniforms[row];
-      const double edge = fmax((double)u, 0.0) * Z;
-      double run = 0.0;
-      int last = -1;
-#pragma unroll
-      for (int v = 0; v < VM; ++v) {
-        run += w[v];
-        if (w[v] > 0.0) {
-          last = v;
-          if (run > edge && tok < 0) tok = v;
-        }
-      }
-      if (tok < 0) tok = last;
-      if (u != u) tok = -1;
-    }
-    double at = 0.0;
-#pragma unroll
-    for (int v = 0; v < VM; ++v)
-      if (v == tok) at = y[v];
-    end_row<MODE>(q, a.o, p, row, tok, at, m, ok, Z);
-  }
-  if (MODE == M_BWD) {
-    if (!a.part) return;
-    // the workgroup's share of the bias gradient, summed in a fixed order
-#pragma unroll
-    for (int v = 0; v < VM; ++v) {
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) acc[v] += __shfl_xor(acc[v], o);
-      if ((threadIdx.x & 63) == 0) acc_sh[threadIdx.x >> 6][v] = acc[v];
-    }
-    __syncthreads();
-    const int v = threadIdx.x;
-    if (v < V) a.part[(size_t)blockIdx.x * V + v] = (acc_sh[0][v] + acc_sh[1][v]) + (acc_sh[2][v] + acc_sh[3][v]);
-  }
-}
-
-template <int T, int MODE>
-__global__ __launch_bounds__(256) void rules_small_kernel(SmallArgs a) {
-  typedef Elem<T> E;
-  __shared__ float acc_sh[256];
-  const Rules& q = a.q;
-  const int W = a.w, V = q.vocab;
-  const int v = threadIdx.x & (W - 1);
-  const int groups = 256 / W;
-  float acc = 0.f;
-  for (long long row = (long long)blockIdx.x * groups + threadIdx.x / W; row < q.rows; row += (long long)gridDim.x * groups) {
-    const RowP p = row_params(q, row);
-    const bool in = v < V;
-    const float x = in ? E::one(q.logits, row * q.ld + v) : 0.f;
-    uint32_t c = 0;
-    int i = 0;
-    for (; i + 3 < p.n_hist; i += 4) {
-      long long t[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) t[u] = hist_at(p, q.history_i64, i + u);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) c += t[u] == v;
-    }
-    for (; i < p.n_hist; ++i) c += hist_at(p, q.history_i64, i) == v;
-    const bool kept = in && !(p.mask && !((p.mask[v >> 3] >> (v & 7)) & 1));
-    const float b = p.bias && in ? p.bias[v] : 0.f;
-    const double y = !kept ? -INFINITY : c ? counted64(p, x, c, b) : (double)x + (double)b;
-    if (MODE == M_APPLY) {
-      if (in) static_cast<typename E::type*>(a.out)[row * a.out_ld + v] = E::cast((float)y);
-      continue;
-    }
-    if (MODE == M_BWD) {
-      const float m = a.o.stat[2 * row];
-      const long long tok = a.o.given[row];
-      double g = 0.0;
-      if (kept && tok >= 0 && tok < V && m != -INFINITY)
-        g = (double)a.d_logprob[row] * (p.k * LN2) * ((v == tok ? 1.0 : 0.0) - exp2_64(y - (double)m, p.k) * (double)a.o.stat[2 * row + 1]);
-      const float gf = (float)g;
-      if (a.part) acc += gf;
-      else if (a.d_bias && in) a.d_bias[row * V + v] = gf;
-      if (c) g *= x > 0.f ? p.inv_rho : p.rho;
-      if (in) static_cast<typename E::type*>(a.out)[row * a.out_ld + v] = E::cast((float)g);
-      continue;
-    }
-    float m = (float)y;
-    for (int o = W >> 1; o > 0; o >>= 1) m = max_nan(m, __shfl_xor(m, o));
-    const bool ok = m > -INFINITY && m < INFINITY && p.fine;
-    const double w = kept && ok ? exp2_64(y - (double)m, p.k) : 0.0;
-    double run = w;                                   // running sum in the vocabulary's order
-    for (int o = 1; o < W; o <<= 1) {
-      const double t = __shfl_up(run, o, W);
-      if (v >= o) run += t;
-    }
-    const double Z = __shfl(run, W - 1, W);
-    long long tok = -1;
-    if (MODE == M_SUM) {
-      tok = a.o.given[row];
-    } else if (ok && MODE == M_GREEDY) {
-      double best = y;
-      int idx = v;
+      for (int j = 0; j < K; ++j)
+        if (y[j] > best) { best = y[j]; idx = v0 + j; }
       for (int o = W >> 1; o > 0; o >>= 1) {
         const double b2 = __shfl_xor(best, o);
         const int i2 = __shfl_xor(idx, o);
         if (b2 > best || (b2 == best && i2 < idx)) { best = b2; idx = i2; }
       }
-      tok = idx;
+      tok = idx < V ? idx : -1;
     } else if (ok && MODE == M_DRAW) {
       const float u = a.o.uniforms[row];
-      if (u == u) {
-        int hit = w > 0.0 && run > fmax((double)u, 0.0) * Z ? v : INT32_MAX;
-        int last = w > 0.0 ? v : -1;
-        for (int o = W >> 1; o > 0; o >>= 1) {
-          hit = min(hit, __shfl_xor(hit, o));
-          last = max(last, __shfl_xor(last, o));
+      const double edge = fmax((double)u, 0.0) * Z;
+      double at = run - sum;
+      int hit = INT32_MAX, last = -1;
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        at += w[j];
+        if (w[j] > 0.0) {
+          last = v0 + j;
+          if (at > edge && hit == INT32_MAX) hit = v0 + j;
         }
-        tok = hit != INT32_MAX ? hit : last;
       }
+      for (int o = W >> 1; o > 0; o >>= 1) {
+        hit = min(hit, __shfl_xor(hit, o));
+        last = max(last, __shfl_xor(last, o));
+      }
+      tok = u != u ? -1 : hit != INT32_MAX ? hit : last;      // beyond the end (u >= 1): the last token with a weight
     }
-    const double at = __shfl(y, tok >= 0 && tok < V ? (int)tok : 0, W);
-    if (v == 0) end_row<MODE>(q, a.o, p, row, tok, at, m, ok, Z);
+    double at = 0.0;
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+      if (v0 + j == tok) at = y[j];
+    at = __shfl(at, tok >= 0 ? tok / K : 0, W);
+    if (lane == 0) end_row<MODE>(q, a.o, p, row, tok, at, m, ok, Z);
   }
   if (MODE == M_BWD) {
     if (!a.part) return;
-    // the workgroup's share of the bias gradient: its groups in order
-    acc_sh[threadIdx.x] = acc;
+    // the workgroup's share of the bias gradient, in a fixed order: the wave's groups, then the waves
+    const int wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      for (int o = W; o < 64; o <<= 1) acc[j] += __shfl_xor(acc[j], o);
+      if ((threadIdx.x & 63) < W) acc_sh[wave][v0 + j] = acc[j];
+    }
     __syncthreads();
-    if (threadIdx.x >= V) return;
-    float s = 0.f;
-    for (int g = 0; g < groups; ++g) s += acc_sh[g * W + threadIdx.x];
-    a.part[(size_t)blockIdx.x * V + threadIdx.x] = s;
+    for (int v = threadIdx.x; v < V; v += 256)
+      a.part[(size_t)blockIdx.x * V + v] = (acc_sh[0][v] + acc_sh[1][v]) + (acc_sh[2][v] + acc_sh[3][v]);
   }
 }
 
@@ -1519,52 +1433,40 @@ int run_join(SegArgs& s, hipStream_t st) {
   return DVAE_OK;
 }
 
-// a lane a token and its history read by every lane of the group: pays while both are short
+// every lane of a group reads the whole history: short ones, the shorter the more lanes do (a wave that counts in LDS reads it
+// once; bytes hold counts up to 255)
 bool is_small(const dvae_rules& q) {
-  return q.vocab <= SMALL_VOCAB && (!q.history || q.history_len <= SMALL_HISTORY);
+  return q.vocab <= GROUP_VOCAB && (!q.history || q.history_len <= (q.vocab <= 64 ? 255 : 32));
 }
 
 bool needs_segments(const dvae_rules& q) { return !is_small(q) && !plan_of(q).row_wave; }
 
-int small_lanes(const dvae_rules& q) {
+int group_lanes(const dvae_rules& q) {
   int w = 1;
-  while (w < q.vocab) w <<= 1;
+  while (w * GROUP_TOKENS < q.vocab) w <<= 1;
   return w;
 }
 
-bool is_tiny(const dvae_rules& q) {
-  return q.vocab <= TINY_VOCAB && q.rows >= TINY_ROWS && (!q.history || q.history_len <= TINY_HISTORY);
-}
-
-long long small_blocks(const dvae_rules& q) {
-  if (is_tiny(q)) return (q.rows + 255) / 256;
-  const int groups = 256 / small_lanes(q);
-  return std::min<long long>((q.rows + groups - 1) / groups, MAX_BLOCKS);
+long long group_blocks(const dvae_rules& q) {
+  const int groups = 256 / group_lanes(q);
+  return (q.rows + groups - 1) / groups;
 }
 
 template <int MODE>
-int run_small(SmallArgs& a, long long blocks, hipStream_t st) {
-  a.w = small_lanes(a.q);
+int run_group(GroupArgs& a, long long blocks, hipStream_t st) {
+  a.w = group_lanes(a.q);
   const dim3 grid((unsigned)blocks), block(256);
-  const bool tiny = is_tiny(a.q), eight = a.q.vocab <= 8;
-#define SMALL(T)                                                                                                  \
-  do {                                                                                                            \
-    if (tiny && eight) hipLaunchKernelGGL((rules_tiny_kernel<T, 8, MODE>), grid, block, 0, st, a);                \
-    else if (tiny) hipLaunchKernelGGL((rules_tiny_kernel<T, 16, MODE>), grid, block, 0, st, a);                   \
-    else hipLaunchKernelGGL((rules_small_kernel<T, MODE>), grid, block, 0, st, a);                                \
-  } while (0)
   switch (a.q.dtype) {
-    case DVAE_F32: SMALL(DVAE_F32); break;
-    case DVAE_BF16: SMALL(DVAE_BF16); break;
-    default: SMALL(DVAE_F16);
+    case DVAE_F32: hipLaunchKernelGGL((rules_group_kernel<DVAE_F32, MODE>), grid, block, 0, st, a); break;
+    case DVAE_BF16: hipLaunchKernelGGL((rules_group_kernel<DVAE_BF16, MODE>), grid, block, 0, st, a); break;
+    default: hipLaunchKernelGGL((rules_group_kernel<DVAE_F16, MODE>), grid, block, 0, st, a);
   }
-#undef SMALL
   DVAE_LAUNCH_CHECK();
   return DVAE_OK;
 }
 
 int bias_shares(const dvae_rules& q) {
-  if (is_small(q)) return (int)std::min<long long>(small_blocks(q), 1024);
+  if (is_small(q)) return (int)std::min<long long>(group_blocks(q), 1024);
   const int span = 64 * COL_STEPS * (16 / elem_bytes(q.dtype));
   const long long cols = ((long long)q.vocab + span - 1) / span;
   return (int)std::min<long long>((q.rows + 3) / 4, std::max<long long>(1, 1024 / cols));
@@ -1611,9 +1513,9 @@ extern "C" int dvae_rules_apply(const dvae_rules* q, void* out, long long out_ld
   DVAE_REQUIRE(out, "rules_apply: null pointer");
   DVAE_REQUIRE(q->rows <= 1 || out_ld >= q->vocab, "rules_apply: rows of out overlap (ld %lld < vocab %d)", out_ld, q->vocab);
   if (is_small(*q)) {
-    SmallArgs m{};
+    GroupArgs m{};
     m.q = with_constants(*q); m.out = out; m.out_ld = out_ld;
-    return run_small<M_APPLY>(m, small_blocks(*q), (hipStream_t)stream);
+    return run_group<M_APPLY>(m, group_blocks(*q), (hipStream_t)stream);
   }
   SegArgs a{};
   a.q = with_constants(*q);
@@ -1634,9 +1536,9 @@ extern "C" int dvae_rules_choose(const dvae_rules* q, const float* uniforms, con
   o.uniforms = uniforms; o.next = next; o.tokens = tokens; o.logprob = logprob; o.state_out = state_out;
   hipStream_t st = (hipStream_t)stream;
   if (is_small(*q)) {
-    SmallArgs m{};
+    GroupArgs m{};
     m.q = with_constants(*q); m.o = o;
-    return uniforms ? run_small<M_DRAW>(m, small_blocks(*q), st) : run_small<M_GREEDY>(m, small_blocks(*q), st);
+    return uniforms ? run_group<M_DRAW>(m, group_blocks(*q), st) : run_group<M_GREEDY>(m, group_blocks(*q), st);
   }
   SegArgs a{};
   a.q = with_constants(*q); a.o = o; a.seg = (Seg*)ws;
@@ -1652,9 +1554,9 @@ extern "C" int dvae_rules_logprob(const dvae_rules* q, const long long* tokens, 
   RowOut o{};
   o.given = tokens; o.logprob = logprob; o.stat = stat;
   if (is_small(*q)) {
-    SmallArgs m{};
+    GroupArgs m{};
     m.q = with_constants(*q); m.o = o;
-    return run_small<M_SUM>(m, small_blocks(*q), (hipStream_t)stream);
+    return run_group<M_SUM>(m, group_blocks(*q), (hipStream_t)stream);
   }
   SegArgs a{};
   a.q = with_constants(*q); a.o = o; a.seg = (Seg*)ws;
@@ -1685,10 +1587,10 @@ extern "C" int dvae_rules_logprob_bwd(const dvae_rules* q, const long long* toke
     return DVAE_OK;
   };
   if (is_small(*q)) {
-    SmallArgs m{};
+    GroupArgs m{};
     m.q = with_constants(*q); m.o.given = tokens; m.o.stat = const_cast<float*>(stat); m.d_logprob = d_logprob;
     m.out = d_logits; m.out_ld = d_ld; m.d_bias = shared ? nullptr : d_bias; m.part = shared ? (float*)ws : nullptr;
-    DVAE_TRY(run_small<M_BWD>(m, shared ? shares : small_blocks(*q), st));
+    DVAE_TRY(run_group<M_BWD>(m, shared ? shares : group_blocks(*q), st));
     return shared ? sum_shares() : DVAE_OK;
   }
   const Plan p = plan_of(*q);

@@ -244,9 +244,10 @@ def test_many_rows_share_one_bias(cuda):
                                    dict(vocab=5, L=200, ragged=True, dtype="bf16", bias="shared", per_row=True, junk=True),
                                    dict(vocab=16, L=9, dtype="fp16", bias="rows", states=3, per_row=True, pad=1),
                                    dict(vocab=11, L=3, states=4), dict(vocab=1), dict(vocab=8, L=255),
-                                   dict(vocab=13, L=256, states=2)], ids=ident)
+                                   dict(vocab=100, L=32, dtype="bf16", states=3, per_row=True),
+                                   dict(vocab=128, dtype="fp16", bias="rows"), dict(vocab=33, L=40, pad=2)], ids=ident)
 def test_many_rows_of_a_few_tokens(cuda, shape):
-    """32800 rows: a lane a row.  The oracle sees 200 rows spread over them (the bias gradient: all)."""
+    """32800 rows, histories short enough for groups of lanes, which compute in doubles.  The oracle sees 200 rows spread over them (the bias gradient: all)."""
     from dvae_amd.rules import apply_rules, choose, token_logprob
     rows = 32800
     case = Case(rows=rows, seed=12, drawn=True, **shape)
@@ -291,9 +292,10 @@ def test_many_rows_of_a_few_tokens(cuda, shape):
 
 @pytest.mark.parametrize("shape", [dict(vocab=700, L=40, ragged=True, states=4, free=True, per_row=True),
                                    dict(vocab=1900, dtype="bf16", L=9, bias="rows", index=torch.int32, pad=3),
-                                   dict(vocab=2048, dtype="fp16", states=3), dict(vocab=1025, L=600, junk=True)], ids=ident)
+                                   dict(vocab=2048, dtype="fp16", states=3), dict(vocab=1025, L=600, junk=True),
+                                   dict(vocab=13, L=256, states=2), dict(vocab=90, L=33, dtype="bf16")], ids=ident)
 def test_many_rows_of_a_middle_vocabulary(cuda, shape):
-    """4200 rows: a wave a row, all in one launch.  The oracle sees 60 of them."""
+    """4200 rows, more tokens or history than groups of lanes take: a wave a row, fp32 sums.  The oracle sees 60 of them."""
     from dvae_amd.rules import apply_rules, choose, token_logprob
     rows = 4200
     case = Case(rows=rows, seed=13, drawn=True, **shape)
