@@ -15,17 +15,19 @@
 // Counts: a workgroup counts the history's tokens that fall into its segments in LDS (integer atomics: their order does not
 // matter).
 //
-// Bounds.  apply and log p move the logits once each way and are bound by memory: 256 x 131072 bf16 under all rules 31 us (137
-// MB, 4.4 TB/s), log p of 4096 x 65536 bf16 100 + 10 us, its gradients 175 us (1.07 GB, 6.1 TB/s).  A drawn batch is bound by
-// its sums of doubles: 512 x 131072 bf16 under all rules 105 us for 41 M wave instructions -- 39 per element, 15 of them the exp, 15 its value and
-// masks, the rest counting and reductions -- where the bytes alone would take 29 us; + 17 us join.
+// Bounds.  apply and log p move the logits once each way and are bound by memory: 256 x 131072 bf16 under all rules 31 us
+// (137 MB, 4.4 TB/s), log p of 4096 x 65536 bf16 105 + 10 us, its gradients 175 us (1.07 GB, 6.1 TB/s).  A drawn batch is
+// bound by its sums of doubles: 512 x 131072 bf16 under all rules 105 us for 41 M wave instructions -- 39 per element, 15 of
+// them the exp, 10 its value and masks, the rest counting and reductions -- where the bytes alone would take 29 us; + 17 us
+// join.
 //
-// Numbers.  A token the history does not hold has the value x + b, one fp32 rounding; a counted one is computed in
-// double and rounded once.  Decisions do not rest on that rounding: rounding is monotone, so the largest exact value is
-// among the elements whose rounded value is the largest; those few are compared by the part the rounding dropped
-// (the double minus the rounded value).  A drawn token is decided where a running sum over the
-// whole vocabulary crosses u Z, and with thousands of probable tokens a border of fp32 sums lies within their rounding of
-// u Z for a few percent of the rows: its weights and sums are doubles, with an exp2 of 4e-14.
+// Numbers.  A token the history does not hold has the value x + b, one fp32 rounding; a counted one is computed in double
+// and rounded once.  Decisions do not rest on that rounding: rounding is monotone, so the largest exact value is among the
+// elements whose rounded value is the largest; those few are compared by the part the rounding dropped (the double minus
+// the rounded value).  A drawn token is decided where a running sum over the whole vocabulary crosses u Z.  With thousands of
+// probable tokens fp32 weights (off by 5e-8) would decide 3 to 6 rows in a thousand otherwise (131072 tokens, normal logits of
+// deviation 2.7, T 0.75 to 1.5), and a bound of their error flags 8 to 37 % of the rows: so weights and sums are doubles, with
+// an exp2 of 4e-14.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
