@@ -169,7 +169,7 @@ class _Call:
         self.logits = x = _rows2d(logits)
         q = _lib.DvaeRules(logits=x.data_ptr(), rows=rows, ld=x.stride(0) if rows > 1 else V, vocab=V,
                            dtype=_DTYPES[x.dtype], rows_per_history=1)
-        self.tensors = keep = []                           # behind q's pointers, besides logits and bias
+        self.tensors, self.fields = keep, fields = [], []  # behind q's pointers, besides logits and bias, and q's names for them
         if history is not None:
             if not isinstance(history, torch.Tensor) or history.dtype not in _INDEX or history.dim() < 1:
                 raise ValueError("history must be an int32 / int64 tensor [..., L]")
@@ -186,6 +186,7 @@ class _Call:
                 q.history_i64 = h.dtype == torch.int64
                 q.rows_per_history = rows // n
                 keep.append(h)
+                fields.append("history")
             if lengths is not None:
                 self._per_row(lengths, "lengths", _INDEX)
                 if lengths.dtype != torch.int32:
@@ -193,6 +194,7 @@ class _Call:
                 lengths = lengths.contiguous()
                 q.lengths = lengths.data_ptr()
                 keep.append(lengths)
+                fields.append("lengths")
         elif lengths is not None:
             raise ValueError("lengths without a history")
         grammar = rules.grammar
@@ -207,8 +209,8 @@ class _Call:
                 state = state.clamp(-1, grammar.states).to(torch.int32)
             state = state.contiguous()
             q.mask, q.mask_words, q.states, q.state = masks.data_ptr(), masks.shape[1], masks.shape[0], state.data_ptr()
-            keep.append(masks)
-            keep.append(state)
+            keep.extend((masks, state))
+            fields.extend(("mask", "state"))
         elif state is not None:
             raise ValueError("state without a grammar")
         self.bias = None
@@ -239,6 +241,7 @@ class _Call:
         v = self._per_row(v, name, (torch.float32,)).contiguous()
         setattr(q, name + "_rows", v.data_ptr())
         self.tensors.append(v)
+        self.fields.append(name + "_rows")
         return 1.0
 
     def _here(self, t, name):
@@ -263,6 +266,27 @@ class _Call:
     def launch(self, fn, *args):
         E._on_device(self.index, fn, self.q, *args)
 
+    def elsewhere(self, logits, bias, *others):
+        """-> (descriptor, tensors behind it) of the same call on copies of its tensors."""
+        q = _lib.DvaeRules.from_buffer_copy(self.q)
+        x = _rows2d(self._here(logits, "logits"))
+        q.logits, q.ld = x.data_ptr(), x.stride(0) if self.rows > 1 else self.V
+        keep = [x]
+        if bias is not None:
+            b = self._here(bias, "bias")
+            b = b.contiguous() if b.dim() == 1 else _rows2d(b)
+            q.bias = b.data_ptr()
+            if b.dim() > 1:
+                q.bias_ld = b.stride(0) if self.rows > 1 else self.V
+            keep.append(b)
+        for name, t in zip(self.fields, others):
+            t = self._here(t, name).contiguous()
+            setattr(q, name, t.data_ptr())
+            if name == "history":
+                q.history_ld = t.shape[1] if t.shape[0] > 1 else 0
+            keep.append(t)
+        return q, keep
+
 
 def _address(t):
     return None if t is None else t.data_ptr()
@@ -276,6 +300,8 @@ def apply_rules(logits, rules, history=None, lengths=None, state=None, out=None)
     themselves; its rows must have adjacent elements.  No gradient: see ``token_logprob``."""
     if torch.is_grad_enabled() and torch.is_tensor(logits) and logits.requires_grad:
         raise ValueError("apply_rules has no gradient: detach the logits, or use token_logprob")
+    if torch.is_grad_enabled() and isinstance(rules, TokenRules) and rules.bias is not None and rules.bias.requires_grad:
+        raise ValueError("apply_rules has no gradient: detach the bias, or use token_logprob")
     c = _Call(logits, rules, history, lengths, state, 1.0)
     if out is None:
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
@@ -333,8 +359,10 @@ def choose(logits, rules=None, history=None, lengths=None, state=None, temperatu
 
 
 class _LogprobFn(torch.autograd.Function):
-    # Every tensor behind a pointer goes through save_for_backward: a change between forward and backward is an error.  The
-    # backward pass runs on autograd's own thread, where Python is slowest: what it needs is at hand when the forward pass ends.
+    # Every tensor behind a pointer goes through save_for_backward: a change between forward and backward is an error, and
+    # hooks of saved tensors (stored on the host, computed again by a checkpoint) see them.  The call holds them too, so that
+    # equal addresses mean equal tensors.  The backward pass runs on autograd's own thread, where Python is slowest: what it
+    # needs is at hand when the forward pass ends.
     @staticmethod
     def forward(ctx, call, logits, bias, tokens, *others):
         lib = load()
@@ -344,6 +372,7 @@ class _LogprobFn(torch.autograd.Function):
         at = tokens.data_ptr(), stat.data_ptr()
         call.launch(lib.dvae_rules_logprob, at[0], logprob.data_ptr(), at[1], ws)
         ctx.call, ctx.stat, ctx.at, ctx.fn = call, stat, at, lib.dvae_rules_logprob_bwd
+        ctx.where = [t.data_ptr() for t in (logits, tokens, *others)], _address(bias)
         ctx.save_for_backward(logits, bias, tokens, *others)
         return logprob
 
@@ -356,29 +385,48 @@ class _LogprobFn(torch.autograd.Function):
     @staticmethod
     def _gradients(ctx, d_logprob):
         call = ctx.call
-        saved = ctx.saved_tensors                             # checks every saved tensor's version
-        logits = saved[0]
+        logits, bias, tokens, *others = ctx.saved_tensors     # checks every saved tensor's version
+        q, at = call.q, ctx.at
+        if ctx.where != ([t.data_ptr() for t in (logits, tokens, *others)], _address(bias)):
+            q, held = call.elsewhere(logits, bias, *others)
+            tokens = call._here(tokens, "tokens").contiguous()
+            at = tokens.data_ptr(), at[1]
         if d_logprob.dtype != torch.float32 or not d_logprob.is_contiguous():
             d_logprob = d_logprob.to(torch.float32).contiguous()
         d_logits = torch.empty_like(logits, memory_format=torch.contiguous_format)
         d_bias = ws = None
         _, want_logits, want_bias, *rest = ctx.needs_input_grad
         if want_bias:
-            d_bias = torch.empty_like(saved[1], memory_format=torch.contiguous_format)
+            d_bias = torch.empty_like(bias, memory_format=torch.contiguous_format)
             ws, keep = call.workspace()
-        call.launch(ctx.fn, *ctx.at, d_logprob.data_ptr(), d_logits.data_ptr(), call.V,
-                    None if d_bias is None else d_bias.data_ptr(), ws)
+        E._on_device(call.index, ctx.fn, q, *at, d_logprob.data_ptr(), d_logits.data_ptr(), call.V, _address(d_bias), ws)
         return None, d_logits if want_logits else None, d_bias, *([None] * len(rest))
+
+
+def _made_elsewhere(node, index):
+    """Whether a capture's backward pass would reach nodes (of the logits, of the bias) made on another stream."""
+    stream, found = torch._C._cuda_getCurrentRawStream(index), False
+    for made, _ in node.next_functions[:2]:
+        if made is not None and made.metadata.setdefault("dvae_stream", stream) != stream:
+            found = True
+    return found and torch.cuda.is_current_stream_capturing()
 
 
 def token_logprob(logits, tokens, rules=None, history=None, lengths=None, state=None, temperature=1.0):
     """log p of ``tokens`` (int32 / int64, one per row) under the rules, fp32, one per row; differentiable once with respect
     to the logits and the rules' bias.  A token outside [0, V) marks a row to ignore: 0 and no gradient.  A token the
-    grammar forbids has -inf (and still the gradient -p / temperature of the allowed ones)."""
+    grammar forbids has -inf (and still the gradient -p / temperature of the allowed ones).
+
+    Under capture into a HIP graph: autograd runs a leaf's accumulation on the stream where its first living graph was made,
+    and a captured backward pass must not wait for a stream outside.  Where this function made that graph, it refuses; end
+    the eager graph before the capture, or use ``torch.no_grad()`` for a forward pass alone."""
     c = _Call(logits, rules, history, lengths, state, temperature)
     c._per_row(tokens, "tokens", _INDEX)
     tokens = (tokens if tokens.dtype == torch.int64 else tokens.to(torch.int64)).contiguous()
     x, b = c.logits, c.bias
-    c.logits, c.bias = x.detach(), None                   # the graph holds what needs a gradient, not the call
+    c.logits, c.bias, c.given = x.detach(), None if b is None else b.detach(), tokens
     lp = _LogprobFn.apply(c, x, b, tokens, *c.tensors)
+    if lp.requires_grad and _made_elsewhere(lp.grad_fn, c.index):
+        lp = x = b = c = None                             # the error's traceback is not to keep this graph alive as well
+        raise _lib.DvaeError("token_logprob: captured while a graph of the same tensor, made on another stream, is alive")
     return lp if len(c.lead) == 1 else lp.view(c.lead)

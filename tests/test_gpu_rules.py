@@ -17,6 +17,7 @@ import math
 import numpy as np
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from oracle import rules_ref as R
 
@@ -664,6 +665,34 @@ def test_captured_and_replayed(cuda):
             assert torch.equal(a.nan_to_num(3.0), e.nan_to_num(3.0)), i
 
 
+@pytest.mark.parametrize("shared", ["logits", "bias"])
+def test_capture_beside_a_living_graph_is_refused(cuda, shared):
+    """Of the same leaf, made on another stream; on the capture's own stream, without a gradient or after its end it is none."""
+    from dvae_amd._lib import DvaeError
+    from dvae_amd.rules import TokenRules, token_logprob
+    x, b = torch.randn(4, 300, device=cuda, requires_grad=True), torch.randn(300, device=cuda, requires_grad=True)
+    y, c = torch.randn(4, 300, device=cuda, requires_grad=True), torch.randn(300, device=cuda, requires_grad=True)
+    t = torch.tensor([0, 5, 299, -1], device=cuda)
+    want = torch.autograd.grad(token_logprob(x, t, TokenRules(bias=b)).sum(), [x, b])
+    alive = token_logprob(x if shared == "logits" else y, t, TokenRules(bias=b if shared == "bias" else c))
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        with pytest.raises(DvaeError, match="alive"):
+            token_logprob(x, t, TokenRules(bias=b))
+        with torch.no_grad():
+            token_logprob(x, t, TokenRules(bias=b))
+    torch.cuda.synchronize()
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(token_logprob(x, t, TokenRules(bias=b)), [x, b], torch.ones(4, device=cuda))
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for u, v in zip(got, want):
+            assert torch.equal(u, v)
+
+
 def test_changed_inputs_are_refused_by_the_backward_pass(cuda):
     from dvae_amd.rules import TokenRules, token_logprob
     x = torch.randn(3, 40, device=cuda, requires_grad=True)
@@ -688,6 +717,63 @@ def _dvae(cuda, N=7, C=6, mod=None):
     torch.manual_seed(3)
     m = dvae_amd.Dvae(Namespace(dataset_file=None, mod=mod, bidirectional=False, num_classes=C, max_seq=N, hidden_state_size=48))
     return m.to(cuda)
+
+
+def _saved_elsewhere(cuda, bias_rows):
+    """-> (leaves, call, junk): a call whose every argument is copied on the way in, its leaves, and what spoils its inputs."""
+    from dvae_amd.rules import Grammar, TokenRules, token_logprob
+    g = torch.Generator().manual_seed(17)
+    rows, vocab, states = 6, 700, 3
+    big = torch.randn(rows, vocab + 5, generator=g).to(cuda)
+    history = torch.randint(0, vocab, (1, 40), generator=g, dtype=torch.int32).to(cuda).expand(rows, 40)
+    lengths = torch.tensor([0, 1, 7, 39, 40, 90]).to(cuda)
+    state = torch.tensor([0, 1, 2, 0, 1, 2]).to(cuda)
+    tokens = torch.randint(0, vocab, (rows,), generator=g, dtype=torch.int32).to(cuda)
+    temperature = (0.5 + torch.rand(2 * rows, generator=g)).to(cuda)[::2]
+    grammar = Grammar((torch.rand(states, vocab, generator=g) < 0.7).to(cuda))
+    bias = torch.randn(*((rows,) if bias_rows else ()), 2 * vocab, generator=g).to(cuda).requires_grad_()
+    big.requires_grad_()
+
+    def call(big, bias):
+        rules = TokenRules(1.2, 0.1, 0.2, bias[..., ::2], grammar)
+        return token_logprob(big[:, :vocab] * 1.5, tokens, rules, history, lengths, state, temperature)
+
+    def junk():                                     # temporaries that the call left behind are given out again
+        for n in (rows, 2 * rows, vocab, rows * vocab, 40, 240):
+            for t in (torch.float32, torch.int32, torch.int64):
+                torch.full((n,), 3, dtype=t, device=cuda)
+    return (big, bias), call, junk
+
+
+@pytest.mark.parametrize("bias_rows", [False, True])
+def test_hooks_of_saved_tensors(cuda, bias_rows):
+    """Saved tensors that a hook stores on the host, or a checkpoint computes again, give the same bits."""
+    leaves, call, junk = _saved_elsewhere(cuda, bias_rows)
+    weight = torch.linspace(-1, 2, 6, device=cuda)
+    lp = call(*leaves)
+    want = torch.autograd.grad((lp * weight).sum(), leaves)
+    with torch.autograd.graph.save_on_cpu():
+        held = call(*leaves)
+    junk()
+    again = torch.utils.checkpoint.checkpoint(call, *leaves, use_reentrant=False)
+    junk()
+    for other in (held, again):
+        assert torch.equal(other, lp)
+        for a, b in zip(torch.autograd.grad((other * weight).sum(), leaves), want):
+            assert torch.equal(a, b)
+
+
+def test_a_hook_that_stored_the_logits_keeps_their_values(cuda):
+    from dvae_amd.rules import token_logprob
+    x = torch.linspace(-2, 2, 2 * 600, device=cuda).view(2, 600)
+    t = torch.tensor([3, 599], device=cuda)
+    want, = torch.autograd.grad(token_logprob(x.requires_grad_(), t).sum(), x)
+    y = x.detach().clone().requires_grad_()
+    with torch.autograd.graph.save_on_cpu():
+        lp = token_logprob(y, t)
+    with torch.no_grad():
+        y.mul_(3.0)
+    assert torch.equal(torch.autograd.grad(lp.sum(), y)[0], want)
 
 
 @pytest.mark.parametrize("mod", [None, "bn"])
