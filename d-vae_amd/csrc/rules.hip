@@ -546,7 +546,8 @@ __device__ __forceinline__ void end_row(const Rules& q, const RowOut& o, const R
 // a counted token's loads (none waits for another), and its value
 struct Counted { float x, b; uint32_t c; bool kept; };
 template <int T, int HIST>
-__device__ __forceinline__ Counted load_counted(const Rules& q, const RowP& p, const char* lrow, const uint32_t* cnt, int v0, int d) {
+__device__ __forceinline__ Counted load_counted(const Rules& q, const RowP& p, const char* lrow, const uint32_t* cnt, int v0,
+                                                int d) {
   const int v = v0 + d;
   Counted t;
   t.x = Elem<T>::one(lrow, v);
@@ -619,7 +620,8 @@ __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
   const double low = -1000.0 * LN2 * p.temp;        // -1000 / k
 
   // the segment's counted tokens as a list (in a fixed order); the first 64 are loaded ahead of the steps, which hide the way
-  uint16_t* list = reinterpret_cast<uint16_t*>(lds + (HIST ? 4 * a.seg_len / Counts<HIST ? HIST : 1>::PER_WORD + a.seg_len / 8 : 0)) + wave * LIST;
+  const int counts = HIST ? 4 * a.seg_len / Counts<HIST ? HIST : 1>::PER_WORD + a.seg_len / 8 : 0;
+  uint16_t* list = reinterpret_cast<uint16_t*>(lds + counts) + wave * LIST;
   int held = 0;
   Counted first_held{};
   if (HIST) {
@@ -1485,7 +1487,8 @@ int rules_check(const dvae_rules& q, const char* who) {
   DVAE_REQUIRE(q.repetition_rows || (q.repetition > 0.0 && std::isfinite(q.repetition)), "%s: repetition must be positive", who);
   DVAE_REQUIRE(q.frequency_rows || std::isfinite(q.frequency), "%s: frequency must be finite", who);
   DVAE_REQUIRE(q.presence_rows || q.presence > -INFINITY, "%s: presence must be above -inf", who);
-  DVAE_REQUIRE(q.temperature_rows || (q.temperature >= TEMP_MIN && q.temperature <= TEMP_MAX), "%s: temperature must be in [1e-37, 1e37]", who);
+  DVAE_REQUIRE(q.temperature_rows || (q.temperature >= TEMP_MIN && q.temperature <= TEMP_MAX),
+               "%s: temperature must be in [1e-37, 1e37]", who);
   if (q.history) {
     DVAE_REQUIRE(q.history_len >= 0 && q.history_ld >= 0, "%s: negative history length", who);
     DVAE_REQUIRE(q.rows_per_history >= 1, "%s: rows_per_history must be at least 1", who);
@@ -1574,7 +1577,8 @@ extern "C" int dvae_rules_logprob_bwd(const dvae_rules* q, const long long* toke
   DVAE_REQUIRE(!d_bias || q->bias, "rules_logprob_bwd: d_bias without a bias");
   const bool shared = d_bias && q->bias_ld == 0;
   if (q->rows == 0) {
-    if (shared) hipLaunchKernelGGL(rules_bias_sum_kernel, dim3(cdiv(q->vocab, 16)), dim3(256), 0, st, nullptr, 0, q->vocab, d_bias);
+    if (shared) hipLaunchKernelGGL(rules_bias_sum_kernel, dim3(cdiv(q->vocab, 16)), dim3(256), 0, st, nullptr, 0, q->vocab,
+                                   d_bias);
     DVAE_LAUNCH_CHECK();
     return DVAE_OK;
   }

@@ -91,9 +91,9 @@ def grad_norm(grads, max_norm=math.inf):
 def clip_grads(grads, max_norm, out=None):
     """Scales the gradients so that their norm (see ``grad_norm``) is at most ``max_norm``, in place or, with ``out`` (a
     tensor for each, of any of the three types: contiguous as the gradient is, or of its shape and strides), into other
-    tensors -- flat buffers, or single-precision copies of half-precision gradients.  Returns the norm before clipping, a scalar on the device.
-    The reference's Lightning Trainer has this as ``gradient_clip_val`` (train.py:41-47).  A NaN norm makes the gradients
-    NaN; an infinite one makes them 0 (NaN where they were infinite)."""
+    tensors -- flat buffers, or single-precision copies of half-precision gradients.  Returns the norm before clipping, a
+    scalar on the device.  The reference's Lightning Trainer has this as ``gradient_clip_val`` (train.py:41-47).  A NaN norm
+    makes the gradients NaN; an infinite one makes them 0 (NaN where they were infinite)."""
     m = _limit(max_norm, "clip_grads")
     ts = _as_list(grads)
     ins = _flat_list(ts, "clip_grads", "gradient")
