@@ -34,7 +34,10 @@ def _on_device(index, fn, *args):
 
 def _written(tensors):
     """Tells autograd that a kernel wrote these tensors in place."""
-    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+    try:
+        torch.autograd.graph.increment_version(tensors)
+    except RuntimeError:                                  # tensors of inference mode have no version
+        torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
 
 
 def _side(side):

@@ -33,11 +33,9 @@ def _flat_list(ts, what, name):
     """Dense fp32 / bf16 / fp16 tensors on one device -> (addresses, sizes, types); each is one stretch of memory."""
     try:
         types = [_TYPES[t.dtype] for t in ts]
-        fine = all([t.layout is torch.strided and (t.is_contiguous() or _flat_order(t)) for t in ts]) and \
-            len({t.get_device() for t in ts}) <= 1
-        if fine:
+        if all([t.is_contiguous() or _flat_order(t) for t in ts]) and len({t.get_device() for t in ts}) <= 1:
             return [t.data_ptr() for t in ts], [t.numel() for t in ts], types
-    except (AttributeError, KeyError):
+    except (AttributeError, KeyError, RuntimeError):         # (a sparse tensor has no is_contiguous and no address)
         pass
     for i, t in enumerate(ts):           # which one it is
         if not isinstance(t, torch.Tensor) or t.layout != torch.strided or t.dtype not in _TYPES:
@@ -53,10 +51,11 @@ def _flat_list(ts, what, name):
 def _table(ins, outs):
     """An array of struct dvae_tensor: per tensor its two addresses, its size and (in one word) its two types."""
     (pi, n, ti), (po, _, to) = ins, outs
-    flat = [0] * (4 * len(pi))
-    flat[0::4], flat[1::4], flat[2::4] = pi, po, n
-    flat[3::4] = [a | b << 32 for a, b in zip(ti, to)]
-    return array.array('q', flat or [0])
+    table, types = array.array('q', bytes(32 * len(pi))), array.array('i', bytes(8 * len(pi)))
+    types[0::2], types[1::2] = array.array('i', ti), array.array('i', to)
+    table[0::4], table[1::4], table[2::4] = array.array('q', pi), array.array('q', po), array.array('q', n)
+    table[3::4] = array.array('q', types.tobytes())
+    return table
 
 
 def _as_list(ts):
