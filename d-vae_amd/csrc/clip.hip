@@ -5,8 +5,8 @@
 // gradients of 1e-30 or 1e30 neither vanish nor overflow, and no order of summation shows in the fp32 result.
 // Tensors are described in the kernel's arguments (no table in device memory to keep or upload): a launch covers up to
 // CLIP_BATCH of them, cut into chunks of CHUNK elements, each loaded whole before its first value is used.
-// Bound by memory: 400 M bf16 / fp32 gradients into fp32 190 + 500 us (4.2 and 4.8 TB/s; element by element it took 1285); the
-// 40 tensors of a model with 6.9 M parameters 13 + 17 us, most of it the way to the memory and back.
+// Bound by memory: 400 M bf16 / fp32 gradients into fp32 194 + 535 us (4.1 and 4.5 TB/s; element by element it took 1285); the
+// 40 tensors of a model with 6.9 M parameters 10 + 15 us, most of it the way to the memory and back.
 #include <algorithm>
 #include <cmath>
 #include <new>
@@ -17,7 +17,9 @@
 namespace {
 
 constexpr int CLIP_BATCH = 96;          // 96 descriptors of 32 bytes and their chunk starts: under the 4 KB of arguments
-constexpr int CHUNK = 8192;             // elements of a workgroup's step: 256 threads x 4 loads of 8, or 8 of 4
+// elements of a workgroup's step: 256 threads x 2 loads of 8, or 4 of 4.  Twice as many per step leave fewer workgroups: 13 + 17 us
+// for a model's 28 MB instead of 10 + 15, and 212 + 524 for 2.4 GB instead of 194 + 535.
+constexpr int CHUNK = 4096;
 constexpr int MAX_GRID = 2048;
 
 struct Batch {
