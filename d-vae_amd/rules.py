@@ -166,6 +166,7 @@ class _Call:
         self.lead, self.V = lead, V = shape[:-1], shape[-1]
         self.rows = rows = math.prod(lead)
         self.index = index = logits.get_device()           # -1: the CPU
+        self.device = logits.device
         self.logits = x = _rows2d(logits)
         q = _lib.DvaeRules(logits=x.data_ptr(), rows=rows, ld=x.stride(0) if rows > 1 else V, vocab=V,
                            dtype=_DTYPES[x.dtype], rows_per_history=1)
@@ -246,7 +247,7 @@ class _Call:
 
     def _here(self, t, name):
         if t.get_device() != self.index:
-            raise _lib.DvaeError("%s is on %s, the logits on %s" % (name, t.device, self.logits.device))
+            raise _lib.DvaeError("%s is on %s, the logits on %s" % (name, t.device, self.device))
         return t
 
     def _per_row(self, t, name, dtypes):
@@ -260,7 +261,7 @@ class _Call:
         n = load().dvae_rules_ws_bytes(self.q)
         if not n:
             return None, None
-        ws = E._workspace(n, self.logits.device)
+        ws = E._workspace(n, self.device)
         return ws.data_ptr(), ws
 
     def launch(self, fn, *args):
@@ -359,10 +360,9 @@ def choose(logits, rules=None, history=None, lengths=None, state=None, temperatu
 
 
 class _LogprobFn(torch.autograd.Function):
-    # Every tensor behind a pointer goes through save_for_backward: a change between forward and backward is an error, and
-    # hooks of saved tensors (stored on the host, computed again by a checkpoint) see them.  The call holds them too, so that
-    # equal addresses mean equal tensors.  The backward pass runs on autograd's own thread, where Python is slowest: what it
-    # needs is at hand when the forward pass ends.
+    # Every tensor behind a pointer goes through save_for_backward: a change between forward and backward is an error.  Where
+    # hooks take saved tensors (stored on the host, computed again by a checkpoint), what they give back is read instead.  The
+    # backward pass runs on autograd's own thread, where Python is slowest: what it needs is at hand when the forward pass ends.
     @staticmethod
     def forward(ctx, call, logits, bias, tokens, *others):
         lib = load()
@@ -372,7 +372,10 @@ class _LogprobFn(torch.autograd.Function):
         at = tokens.data_ptr(), stat.data_ptr()
         call.launch(lib.dvae_rules_logprob, at[0], logprob.data_ptr(), at[1], ws)
         ctx.call, ctx.stat, ctx.at, ctx.fn = call, stat, at, lib.dvae_rules_logprob_bwd
-        ctx.where = [t.data_ptr() for t in (logits, tokens, *others)], _address(bias)
+        ctx.hooks = torch._C._autograd._top_saved_tensors_default_hooks(False) is not None
+        if ctx.hooks:                                         # theirs to keep
+            call.logits = call.bias = call.given = None
+            call.tensors = ()
         ctx.save_for_backward(logits, bias, tokens, *others)
         return logprob
 
@@ -387,7 +390,7 @@ class _LogprobFn(torch.autograd.Function):
         call = ctx.call
         logits, bias, tokens, *others = ctx.saved_tensors     # checks every saved tensor's version
         q, at = call.q, ctx.at
-        if ctx.where != ([t.data_ptr() for t in (logits, tokens, *others)], _address(bias)):
+        if ctx.hooks:
             q, held = call.elsewhere(logits, bias, *others)
             tokens = call._here(tokens, "tokens").contiguous()
             at = tokens.data_ptr(), at[1]

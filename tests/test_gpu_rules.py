@@ -776,6 +776,19 @@ def test_a_hook_that_stored_the_logits_keeps_their_values(cuda):
     assert torch.equal(torch.autograd.grad(lp.sum(), y)[0], want)
 
 
+def test_a_hook_that_stored_the_logits_frees_their_memory(cuda):
+    from dvae_amd.rules import token_logprob
+    x = torch.randn(64, 1 << 16, device=cuda, requires_grad=True)
+    t = torch.arange(64, device=cuda)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    with torch.autograd.graph.save_on_cpu():
+        lp = token_logprob(x + 1.0, t)
+    assert torch.cuda.memory_allocated() - before < x.numel() * 4
+    want, = torch.autograd.grad(token_logprob(x + 1.0, t).sum(), x)
+    assert torch.equal(torch.autograd.grad(lp.sum(), x)[0], want)
+
+
 @pytest.mark.parametrize("mod", [None, "bn"])
 def test_decoder_without_effective_rules_decides_as_before(cuda, mod):
     from dvae_amd.rules import TokenRules
