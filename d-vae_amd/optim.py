@@ -30,11 +30,13 @@ def _flat_order(t):
 
 
 def _flat_list(ts, what, name):
-    """Dense fp32 / bf16 / fp16 tensors on one device -> (addresses, sizes, types); each is one stretch of memory."""
+    """Dense fp32 / bf16 / fp16 tensors on one device -> (addresses, sizes, types, whether all are contiguous); each
+    is one stretch of memory."""
     try:
         types = [_TYPES[t.dtype] for t in ts]
-        if all([t.is_contiguous() or _flat_order(t) for t in ts]) and len({t.get_device() for t in ts}) <= 1:
-            return [t.data_ptr() for t in ts], [t.numel() for t in ts], types
+        plain = all([t.is_contiguous() for t in ts])
+        if (plain or all([_flat_order(t) for t in ts])) and len({t.get_device() for t in ts}) <= 1:
+            return [t.data_ptr() for t in ts], [t.numel() for t in ts], types, plain
     except (AttributeError, KeyError, RuntimeError):         # (a sparse tensor has no is_contiguous and no address)
         pass
     for i, t in enumerate(ts):           # which one it is
@@ -50,7 +52,7 @@ def _flat_list(ts, what, name):
 
 def _table(ins, outs):
     """An array of struct dvae_tensor: per tensor its two addresses, its size and (in one word) its two types."""
-    (pi, n, ti), (po, _, to) = ins, outs
+    (pi, n, ti, _), (po, _, to, _) = ins, outs
     table, types = array.array('q', bytes(32 * len(pi))), array.array('i', bytes(8 * len(pi)))
     types[0::2], types[1::2] = array.array('i', ti), array.array('i', to)
     table[0::4], table[1::4], table[2::4] = array.array('q', pi), array.array('q', po), array.array('q', n)
@@ -104,7 +106,7 @@ def clip_grads(grads, max_norm, out=None):
         outs = _flat_list(os_, "clip_grads", "output")
         if outs[1] != ins[1] or (ts and os_[0].get_device() != ts[0].get_device()):
             raise ValueError("clip_grads: outputs unlike the gradients: sizes %s for %s" % (outs[1], ins[1]))
-        for i, (t, o) in enumerate(zip(ts, os_)):
+        for i, (t, o) in enumerate(() if ins[3] and outs[3] else zip(ts, os_)):
             if not (t.is_contiguous() and o.is_contiguous()) and (t.shape != o.shape or any(
                     n > 1 and a != b for n, a, b in zip(t.shape, t.stride(), o.stride()))):
                 raise ValueError("clip_grads: output %d is laid out unlike its gradient" % i)
