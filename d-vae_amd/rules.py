@@ -305,7 +305,7 @@ def apply_rules(logits, rules, history=None, lengths=None, state=None, out=None)
         raise ValueError("apply_rules has no gradient: detach the bias, or use token_logprob")
     c = _Call(logits, rules, history, lengths, state, 1.0)
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        out = logits.new_empty(logits.shape)
         c.launch(load().dvae_rules_apply, out.data_ptr(), c.V)
         return out
     if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
@@ -406,13 +406,14 @@ class _LogprobFn(torch.autograd.Function):
         return None, d_logits if want_logits else None, d_bias, *([None] * len(rest))
 
 
-def _made_elsewhere(node, index):
-    """Whether a capture's backward pass would reach nodes (of the logits, of the bias) made on another stream."""
+def _on_default_stream(node, index):
+    """Whether the stream is capturing and its backward pass would reach nodes (of the logits, of the bias) that this module
+    first met on the default stream, which no capture can join (other streams it can)."""
     stream, found = torch._C._cuda_getCurrentRawStream(index), False
     for made, _ in node.next_functions[:2]:
-        if made is not None and made.metadata.setdefault("dvae_stream", stream) != stream:
+        if made is not None and made.metadata.setdefault("dvae_stream", stream) == 0:
             found = True
-    return found and torch.cuda.is_current_stream_capturing()
+    return found and stream != 0 and torch.cuda.is_current_stream_capturing()
 
 
 def token_logprob(logits, tokens, rules=None, history=None, lengths=None, state=None, temperature=1.0):
@@ -421,15 +422,15 @@ def token_logprob(logits, tokens, rules=None, history=None, lengths=None, state=
     grammar forbids has -inf (and still the gradient -p / temperature of the allowed ones).
 
     Under capture into a HIP graph: autograd runs a leaf's accumulation on the stream where its first living graph was made,
-    and a captured backward pass must not wait for a stream outside.  Where this function made that graph, it refuses; end
-    the eager graph before the capture, or use ``torch.no_grad()`` for a forward pass alone."""
+    and a capture cannot wait for the default stream.  Where this function made that graph, it refuses: warm up on a side
+    stream, end the eager graph before the capture, or use ``torch.no_grad()`` for a forward pass alone."""
     c = _Call(logits, rules, history, lengths, state, temperature)
     c._per_row(tokens, "tokens", _INDEX)
     tokens = (tokens if tokens.dtype == torch.int64 else tokens.to(torch.int64)).contiguous()
     x, b = c.logits, c.bias
     c.logits, c.bias, c.given = x.detach(), None if b is None else b.detach(), tokens
     lp = _LogprobFn.apply(c, x, b, tokens, *c.tensors)
-    if lp.requires_grad and _made_elsewhere(lp.grad_fn, c.index):
+    if lp.requires_grad and _on_default_stream(lp.grad_fn, c.index):
         lp = x = b = c = None                             # the error's traceback is not to keep this graph alive as well
-        raise _lib.DvaeError("token_logprob: captured while a graph of the same tensor, made on another stream, is alive")
+        raise _lib.DvaeError("token_logprob: captured while a graph of the same tensor, made on the default stream, is alive")
     return lp if len(c.lead) == 1 else lp.view(c.lead)

@@ -667,7 +667,7 @@ def test_captured_and_replayed(cuda):
 
 @pytest.mark.parametrize("shared", ["logits", "bias"])
 def test_capture_beside_a_living_graph_is_refused(cuda, shared):
-    """Of the same leaf, made on another stream; on the capture's own stream, without a gradient or after its end it is none."""
+    """Of the same leaf, made on the default stream; without a gradient or after the graph's end a capture is none."""
     from dvae_amd._lib import DvaeError
     from dvae_amd.rules import TokenRules, token_logprob
     x, b = torch.randn(4, 300, device=cuda, requires_grad=True), torch.randn(300, device=cuda, requires_grad=True)
@@ -691,6 +691,33 @@ def test_capture_beside_a_living_graph_is_refused(cuda, shared):
         torch.cuda.synchronize()
         for u, v in zip(got, want):
             assert torch.equal(u, v)
+
+
+def test_capture_after_a_side_streams_living_graph(cuda):
+    """A training step warmed up on a side stream, its last graph still alive, then captured: a trained bias accumulates."""
+    from dvae_amd.rules import TokenRules, token_logprob
+    x, b = torch.randn(4, 300, device=cuda), torch.randn(300, device=cuda, requires_grad=True)
+    t = torch.tensor([0, 5, 299, -1], device=cuda)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            b.grad = None
+            loss = token_logprob(x, t, TokenRules(bias=b)).sum()
+            loss.backward()
+    torch.cuda.current_stream().wait_stream(side)
+    want = b.grad.clone()
+    torch.cuda.synchronize()
+    b.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        token_logprob(x, t, TokenRules(bias=b)).sum().backward()
+    for _ in range(3):
+        b.grad.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(b.grad, want)
+    assert loss.grad_fn is not None
 
 
 def test_changed_inputs_are_refused_by_the_backward_pass(cuda):
