@@ -8,7 +8,7 @@
 // Kernels, by size.
 //   map    (apply, gradients) and sum (what a softmax needs): a row is cut into segments of up to 2048 tokens, one wave each,
 //          64 lanes x 16 bytes a step, four steps in flight.  Rows of one segment are decided by their wave on the spot.
-//   join   the other rows: segments leave (sum, reference, maximum); a workgroup a row adds them, finds the ONE segment the
+//   join   the other rows: segments leave (sum, maximum); a workgroup a row adds them, finds the ONE segment the
 //          token is in and searches it again.
 //   group  up to 128 tokens: a group of lanes a row, eight tokens a lane, everything in one launch.
 //   col    gradients with a bias shared by the rows: its sum over rows in registers.
@@ -23,11 +23,14 @@
 //
 // Numbers.  A token the history does not hold has the value x + b, one fp32 rounding; a counted one is computed in double
 // and rounded once.  Decisions do not rest on that rounding: rounding is monotone, so the largest exact value is among the
-// elements whose rounded value is the largest; those few are compared by the part the rounding dropped (the double minus
-// the rounded value).  A drawn token is decided where a running sum over the whole vocabulary crosses u Z.  With thousands of
-// probable tokens fp32 weights (off by 5e-8) would decide 3 to 6 rows in a thousand otherwise (131072 tokens, normal logits of
-// deviation 2.7, T 0.75 to 1.5), and a bound of their error flags 8 to 37 % of the rows: so weights and sums are doubles, with
-// an exp2 of 4e-14.
+// elements whose rounded value is the largest; those few are compared as doubles.  A drawn token is decided where a running
+// sum over the whole vocabulary crosses u Z.  With thousands of probable tokens fp32 weights (off by 5e-8) would decide 3 to 6
+// rows in a thousand otherwise (131072 tokens, normal logits of deviation 2.7, T 0.75 to 1.5), and a bound of their error flags
+// 8 to 37 % of the rows: so weights and sums are doubles, with an exp2 of 4e-14.
+// A low temperature magnifies what the rounding dropped: against the largest value as rounded, a weight 2^((x4 - ref) k) may
+// be 2^1000 or 0 where it is 1.  So doubles are summed against the exact largest value, and a segment whose largest |x4| k is
+// no ordinary one (`ordinary`: beyond 2^-400 .. 2^900, a T below 0.02 for a logit of 13) is summed in doubles throughout, token
+// by token, as is its gradient; within these bounds the rounding moves a log p of fp32 sums by at most 900 ln2 2^-24 = 4e-5.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -130,6 +133,7 @@ __device__ __forceinline__ double counted64(const RowP& p, float x, uint32_t c, 
 
 // NaN if either is: a NaN among the allowed values has to reach the result
 __device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ __forceinline__ double max_nan(double a, double b) { return a > b || a != a ? a : b; }
 
 __device__ __forceinline__ float wave_max_nan(float v) {
 #pragma unroll
@@ -144,6 +148,11 @@ __device__ __forceinline__ float wave_sum(float v) {
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+__device__ __forceinline__ double wave_max(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o));
   return v;
 }
 
@@ -177,6 +186,21 @@ __device__ __forceinline__ double exp2_64(double d, double k) {
   return a != a ? a : a < -1000.0 ? 0.0 : w;
 }
 
+// exp2_64 for loops that hardly ever run: the coefficients come from memory one by one, so that the kernel's ordinary steps
+// do not pay for their registers
+__constant__ double EXP2_C[] = {1.0203121138901363e-07, 1.325522487892511e-06, 1.525268684597521e-05, 0.00015403455852451678,
+                                0.0013333558179043376, 0.009618129159402562, 0.055504108664760424, 0.2402265069581299,
+                                0.6931471805599453, 1.0};
+__device__ __forceinline__ double exp2_rare(double d, double k) {
+  const double a = d * k;
+  if (!(a >= -1000.0)) return a != a ? a : 0.0;
+  const double n = rint(a), f = fma(d, k, -n);
+  double y = EXP2_C[0];
+#pragma unroll 1
+  for (int i = 1; i < 10; ++i) y = fma(y, f, EXP2_C[i]);
+  return ldexp(y, (int)n);
+}
+
 // log Z for Z > 0 in double: Z = 2^n c, c in [sqrt 1/2, sqrt 2), log c = 2 atanh t, t = (c - 1) / (c + 1), |t| < 0.172; the
 // first term left out of the series is t^18 / 19 of the result (9e-16).  A third of the math library's operations.
 __device__ __forceinline__ double log_64(double z) {
@@ -196,14 +220,28 @@ __device__ __forceinline__ double log_64(double z) {
   return fma((double)n, LN2, 2.0 * t * s);
 }
 
+// whether 2^(m k) and what is near it have their places in the exponents of a double, and the part of m that a rounding to fp32
+// drops does not show in it
+__device__ __forceinline__ bool ordinary(float m, double k) {
+  const double a = (double)m * k;
+  return a > -400.0 && a < 900.0;
+}
+
+// whether the row's values may lie between two floats: those of a bias or a history
+__device__ __forceinline__ bool inexact(const Rules& q, const RowP& p) { return p.bias || (q.history && q.history_len); }
+
 // what a segment leaves for the join
 struct Seg {
-  double s;       // sum of 2^((x4 - ref) k)
-  float m;        // maximum (NaN when an allowed value is)
-  float ref;
+  double s;       // sum of 2^((x4 - ref) k); ref: 0 for an ordinary maximum of a draw (reference()), else top
+  double top;     // maximum (NaN when an allowed value is): as rounded to fp32, but exact where it is no ordinary one
 };
 
 enum { M_APPLY = 0, M_SUM = 1, M_GREEDY = 2, M_DRAW = 3, M_BWD = 4 };
+
+template <int MODE>
+__device__ __forceinline__ double reference(double top, double k) {
+  return MODE == M_DRAW && ordinary((float)top, k) ? 0.0 : top;
+}
 
 constexpr int SEG_MAX = 4096;   // tokens of a segment at most: the counts of a workgroup's 4 segments are 32 KB of 16 bits
 
@@ -214,7 +252,7 @@ struct RowOut {
   const long long* given;        // SUM, BWD: the given tokens
   long long* tokens;             // GREEDY / DRAW
   float* logprob;
-  float* stat;                   // SUM, BWD: [rows][2] = maximum and 1 / Z, kept for the backward pass
+  double* stat;                  // SUM, BWD: [rows][2] = the reference of Z and 1 / Z, kept for the backward pass
   int* state_out;
 };
 
@@ -415,17 +453,19 @@ struct Bwd {
   float m, coef, spread, kf, up, down;
   int tok;
   bool zero;                      // an ignored row, or one whose rules leave nothing
+  bool far;                       // no ordinary maximum: far_gradient instead
   __device__ __forceinline__ Bwd() {}
   __device__ __forceinline__ Bwd(const SegArgs& a, const RowP& p, long long row) {
     const long long t = a.o.given[row];
-    m = a.o.stat[2 * row];
+    m = (float)a.o.stat[2 * row];
     kf = (float)p.k;
     coef = (float)((double)a.d_logprob[row] * (p.k * LN2));
-    spread = -coef * a.o.stat[2 * row + 1];
+    spread = -coef * (float)a.o.stat[2 * row + 1];
     up = (float)p.rho;
     down = (float)p.inv_rho;
     zero = t < 0 || t >= a.q.vocab || m == -INFINITY;
     tok = zero ? 0 : (int)t;
+    far = inexact(a.q, p) && fabsf(m) < INFINITY && !ordinary(m, p.k);
   }
   // d values of the step's tokens, from v on
   template <typename R, int EV>
@@ -454,6 +494,45 @@ struct Bwd {
     }
   }
 };
+
+// a counted token's loads (none waits for another), and its value
+struct Counted { float x, b; uint32_t c; bool kept; };
+template <int T, int HIST>
+__device__ __forceinline__ Counted load_counted(const Rules& q, const RowP& p, const char* lrow, const uint32_t* cnt, int v0,
+                                                int d) {
+  const int v = v0 + d;
+  Counted t;
+  t.x = Elem<T>::one(lrow, v);
+  t.b = p.bias ? p.bias[v] : 0.f;
+  t.kept = !p.mask || ((p.mask[v >> 3] >> (v & 7)) & 1);
+  t.c = HIST ? count_at<HIST ? HIST : 1>(cnt, d) : 0u;
+  return t;
+}
+template <int T>
+__device__ __forceinline__ double counted_value(const RowP& p, const Counted& t) {
+  return t.kept ? counted64(p, t.x, t.c, t.b) : -INFINITY;
+}
+
+// the value of a token, counted or not
+template <int T>
+__device__ __forceinline__ double any_value(const RowP& p, const Counted& t) {
+  if (!t.kept) return -INFINITY;
+  return t.c ? counted64(p, t.x, t.c, t.b) : (double)t.x + (double)t.b;
+}
+
+// one token's gradient in a far row, in doubles: writes the logit's, returns the value's
+template <int T, int HIST>
+__device__ __forceinline__ float far_gradient(const SegArgs& a, const RowP& p, long long row, const Bwd& b, const char* lrow,
+                                              typename Elem<T>::type* orow, const uint32_t* cnt, int v0, int d) {
+  const Counted t = load_counted<T, HIST>(a.q, p, lrow, cnt, v0, d);
+  float y = 0.f;
+  if (t.kept && !b.zero) {
+    const double w = exp2_rare(any_value<T>(p, t) - a.o.stat[2 * row], p.k) * a.o.stat[2 * row + 1];
+    y = (float)((double)a.d_logprob[row] * (p.k * LN2) * ((v0 + d == b.tok ? 1.0 : 0.0) - w));
+  }
+  orow[v0 + d] = Elem<T>::cast(t.c ? y * (t.x > 0.f ? b.down : b.up) : y);
+  return y;
+}
 
 // APPLY and BWD: a value written for every logit
 template <int T, int HIST, int MODE, bool ROWWAVE>
@@ -493,7 +572,17 @@ __global__ __launch_bounds__(256) void rules_map_kernel(SegArgs a) {
 
   typename E::type* orow = static_cast<typename E::type*>(a.out) + row * a.out_ld;
   Bwd b;
-  if (MODE == M_BWD) b = Bwd(a, p, row);
+  if (MODE == M_BWD) {
+    b = Bwd(a, p, row);
+    if (b.far) {
+#pragma unroll 1
+      for (int d = lane; d < end - v0; d += 64) {
+        const float y = far_gradient<T, HIST>(a, p, row, b, lrow, orow, cnt, v0, d);
+        if (a.d_bias_rows) a.d_bias_rows[row * V + v0 + d] = y;
+      }
+      return;
+    }
+  }
   steps.run(p, lrow, V, [&](const Loaded& in, int v, auto whole) {
     const Ruled<T, HIST> r(p, in, cnt + (v - v0) / PER, v, V, whole);
     float y[EV];
@@ -520,20 +609,20 @@ __device__ __forceinline__ double token_value(const Rules& q, const RowP& p, lon
   return c ? counted64(p, x, c, b) : (double)x + (double)b;
 }
 
-// a row's results: its token, `at` the token's value, m and Z the row's maximum and sum
+// a row's results: its token, `at` the token's value, Z the row's sum against the reference `top` (its maximum)
 template <int MODE>
 __device__ __forceinline__ void end_row(const Rules& q, const RowOut& o, const RowP& p, long long row, long long tok,
-                                        double at, float m, bool ok, double Z) {
+                                        double at, double top, bool ok, double Z) {
   const bool have = tok >= 0 && tok < q.vocab;
   float lp;
   if (MODE == M_SUM && !have) lp = 0.f;                   // an ignored row
-  else if (m == -INFINITY) lp = -INFINITY;                // the rules leave nothing
+  else if (top == -INFINITY) lp = -INFINITY;              // the rules leave nothing
   else if (!ok || !have) lp = NAN;                        // NaN or +inf among the allowed values (or a NaN u)
-  else lp = (float)((at - (double)m) * (p.k * LN2) - log_64(Z));
+  else lp = (float)((at - top) * (p.k * LN2) - log_64(Z));
   o.logprob[row] = lp;
   if (MODE == M_SUM) {
-    o.stat[2 * row] = m == -INFINITY || ok ? m : NAN;
-    o.stat[2 * row + 1] = ok ? (float)reciprocal(Z) : NAN;
+    o.stat[2 * row] = top == -INFINITY || ok ? top : NAN;
+    o.stat[2 * row + 1] = ok ? reciprocal(Z) : NAN;
   } else {
     o.tokens[row] = tok;
     if (o.state_out) {
@@ -543,38 +632,14 @@ __device__ __forceinline__ void end_row(const Rules& q, const RowOut& o, const R
   }
 }
 
-// a counted token's loads (none waits for another), and its value
-struct Counted { float x, b; uint32_t c; bool kept; };
-template <int T, int HIST>
-__device__ __forceinline__ Counted load_counted(const Rules& q, const RowP& p, const char* lrow, const uint32_t* cnt, int v0,
-                                                int d) {
-  const int v = v0 + d;
-  Counted t;
-  t.x = Elem<T>::one(lrow, v);
-  t.b = p.bias ? p.bias[v] : 0.f;
-  t.kept = !p.mask || ((p.mask[v >> 3] >> (v & 7)) & 1);
-  t.c = HIST ? count_at<HIST ? HIST : 1>(cnt, d) : 0u;
-  return t;
-}
-template <int T>
-__device__ __forceinline__ double counted_value(const RowP& p, const Counted& t) {
-  return t.kept ? counted64(p, t.x, t.c, t.b) : -INFINITY;
-}
-
-// the value of a token, counted or not
-template <int T>
-__device__ __forceinline__ double any_value(const RowP& p, const Counted& t) {
-  if (!t.kept) return -INFINITY;
-  return t.c ? counted64(p, t.x, t.c, t.b) : (double)t.x + (double)t.b;
-}
-
 constexpr int LIST = 512;       // counted tokens of a segment that are listed; more are looked up bit by bit
 
 // A segment's maximum and sum of weights.  Tokens that the history holds are left out of the steps (one more bit mask) and
 // taken afterwards, a lane each: they are few, and the steps stay free of branches.
-// DRAW: sums of doubles, against 0 as reference -- an exponent of a double has room for every ordinary row; where the
-// maximum is no ordinary one (beyond 2^-400 .. 2^900) the segment is summed again against it, token by token.  Else fp32 sums, against a
-// reference of the lane's own that moves when a value exceeds it by 2^8 (an exponent of 8 is still exact to 2^-20).
+// DRAW: sums of doubles, against 0 as reference -- an exponent of a double has room for every ordinary row.  Else fp32 sums,
+// against a reference of the lane's own that moves when a value exceeds it by 2^8 (an exponent of 8 is still exact to 2^-20).
+// Where the maximum is no ordinary one and either kind of sum would show it, the segment is summed again in doubles, token by
+// token, against its exact maximum.
 template <int T, int HIST, int MODE, bool ROWWAVE>
 __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
   constexpr bool DRAW = MODE == M_DRAW;
@@ -721,29 +786,29 @@ __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
     }
   }
   m = wave_max_nan(m);
+  const bool ok = m > -INFINITY && m < INFINITY && p.fine;
+  const bool far = ok && (DRAW || inexact(q, p)) && !ordinary(m, p.k);
   Seg r;
-  r.s = 0.0; r.m = m; r.ref = m;
-  if (m > -INFINITY && m < INFINITY) {
-    if (DRAW) {
-      const double top = (double)m * p.k;
-      r.ref = 0.f;
-      if (!(top > -400.0 && top < 900.0)) {       // no ordinary row: token by token
-        r.ref = m;
-        zd = 0.0;
-        for (int d = lane; d < end - v0; d += 64)
-          zd += exp2_64(any_value<T>(p, load_counted<T, HIST>(q, p, lrow, cnt, v0, d)) - (double)m, p.k);
-      }
-      r.s = wave_sum(zd);
-    } else {
-      r.s = (double)wave_sum(z * __builtin_amdgcn_exp2f((ref - m) * kf));
-    }
+  r.s = 0.0; r.top = m;
+  if (far) {
+    const auto value = [&](int d) { return any_value<T>(p, load_counted<T, HIST>(q, p, lrow, cnt, v0, d)); };
+    double top = -INFINITY;
+#pragma unroll 1
+    for (int d = lane; d < end - v0; d += 64) top = fmax(top, value(d));
+    r.top = top = wave_max(top);
+    zd = 0.0;
+#pragma unroll 1
+    for (int d = lane; d < end - v0; d += 64) zd += exp2_rare(value(d) - top, p.k);
+    r.s = wave_sum(zd);
+  } else if (ok) {
+    r.s = DRAW ? wave_sum(zd) : (double)wave_sum(z * __builtin_amdgcn_exp2f((ref - m) * kf));
   }
   if (!ROWWAVE) {
     if (lane == 0) a.seg[row * a.nseg + seg] = r;
     return;
   }
   // a row of one segment: its wave decides it
-  const bool ok = m > -INFINITY && m < INFINITY && p.fine;
+  const double base = reference<MODE>(r.top, p.k);
   long long tok = -1;
   const auto count = [&](int v) { return HIST ? count_at<HIST ? HIST : 1>(cnt, v) : 0u; };
   // values of EV tokens, -inf where there is none
@@ -763,22 +828,20 @@ __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
   if (MODE == M_SUM) {
     tok = a.o.given[row];
   } else if (ok && MODE == M_GREEDY) {
-    float lo = -INFINITY;
+    double best = -INFINITY;
     int idx = INT32_MAX;
     for (int v = lane * EV; v < end; v += 64 * EV) {
       double y[EV];
       values(v, y);
 #pragma unroll
-      for (int e = 0; e < EV; ++e) {
-        const float l = (float)y[e] == m ? (float)(y[e] - (double)m) : -INFINITY;
-        if (l > lo) { lo = l; idx = v + e; }
-      }
+      for (int e = 0; e < EV; ++e)
+        if (y[e] > best) { best = y[e]; idx = v + e; }
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
-      const float l2 = __shfl_xor(lo, o);
+      const double b2 = __shfl_xor(best, o);
       const int i2 = __shfl_xor(idx, o);
-      if (l2 > lo || (l2 == lo && i2 < idx)) { lo = l2; idx = i2; }
+      if (b2 > best || (b2 == best && i2 < idx)) { best = b2; idx = i2; }
     }
     if (idx < V) tok = idx;
   } else if (ok && MODE == M_DRAW) {
@@ -793,7 +856,7 @@ __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
         if (v < end) values(v, w);
 #pragma unroll
         for (int e = 0; e < EV; ++e) {
-          w[e] = v < end ? exp2_64(w[e] - (double)r.ref, p.k) : 0.0;
+          w[e] = v < end ? exp2_64(w[e] - base, p.k) : 0.0;
           sum += w[e];
           if (w[e] > 0.0) last = v + e;
         }
@@ -825,7 +888,7 @@ __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
   if (lane) return;
   const bool have = tok >= 0 && tok < V;
   const double at = have ? token_value<T>(q, p, row, (int)tok, count((int)tok)) : 0.0;
-  end_row<MODE>(q, a.o, p, row, tok, at, m, ok, ok ? r.s * exp2_64((double)r.ref - (double)m, p.k) : 0.0);
+  end_row<MODE>(q, a.o, p, row, tok, at, r.top, ok, ok ? r.s * exp2_64(base - r.top, p.k) : 0.0);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -874,7 +937,6 @@ template <int T, int MODE>
 __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
   constexpr bool SEARCH = MODE != M_SUM;
   __shared__ double shd[4];
-  __shared__ float shf[4];
   __shared__ int shi[4];
   __shared__ double pick_before;
   __shared__ int hist[SEARCH ? HIST_STAGE : 1];
@@ -890,7 +952,7 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
   const int per = (a.nseg + 255) / 256;
   const int i0 = min(tid * per, a.nseg), i1 = min(i0 + per, a.nseg);
   Seg mine;
-  mine.s = 0.0; mine.m = -INFINITY; mine.ref = 0.f;
+  mine.s = 0.0; mine.top = -INFINITY;
   if (i0 < i1) mine = seg[i0];
 
   const float uf = MODE == M_DRAW ? a.o.uniforms[row] : 0.f;
@@ -914,11 +976,13 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
     }
   }
 
-  float m = mine.m;
-  for (int i = i0 + 1; i < i1; ++i) m = max_nan(m, seg[i].m);
-  m = block_reduce(m, shf, [](float x, float y) { return max_nan(x, y); });
-  const bool ok = m > -INFINITY && m < INFINITY && p.fine;
-  const auto scaled = [&](const Seg& s) { return s.m > -INFINITY ? s.s * exp2_64((double)s.ref - (double)m, p.k) : 0.0; };
+  double top = mine.top;
+  for (int i = i0 + 1; i < i1; ++i) top = max_nan(top, seg[i].top);
+  top = block_reduce(top, shd, [](double x, double y) { return max_nan(x, y); });
+  const bool ok = top > -INFINITY && top < INFINITY && p.fine;
+  const auto scaled = [&](const Seg& s) {
+    return s.top > -INFINITY ? s.s * exp2_64(reference<MODE>(s.top, p.k) - top, p.k) : 0.0;
+  };
   double z0 = 0.0, z = 0.0;
   if (ok) {
     z0 = scaled(mine);
@@ -928,7 +992,7 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
   double Z;
   const double before = block_prefix(z, shd, Z);
 
-  const auto finish = [&](long long t, double y) { end_row<MODE>(q, a.o, p, row, t, y, m, ok, Z); };
+  const auto finish = [&](long long t, double y) { end_row<MODE>(q, a.o, p, row, t, y, top, ok, Z); };
   if (MODE == M_SUM) {
     if (tid == 0) finish(tok, given_y);
     return;
@@ -955,16 +1019,16 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
   };
 
   if (MODE == M_GREEDY) {
-    // the largest value's segments (hardly ever more than one), and in them the elements that round to it: among those
-    // the largest dropped part, then the lowest index
-    float lo = -INFINITY;
+    // the segments whose maximum rounds to the row's (hardly ever more than one), and in them the elements that do: among
+    // those the largest one, then the lowest index
+    const float m = (float)top;
+    double best = -INFINITY;
     int idx = INT32_MAX;
-    double best_y = 0.0;
     int from = 0;
     while (true) {
-      int g = mine.m == m && i0 >= from ? i0 : INT32_MAX;
+      int g = (float)mine.top == m && i0 >= from ? i0 : INT32_MAX;
       for (int i = i0 + 1; i < i1; ++i)
-        if (i >= from && i < g && seg[i].m == m) g = i;
+        if (i >= from && i < g && (float)seg[i].top == m) g = i;
       g = block_reduce(g, shi, [](int x, int y) { return min(x, y); });
       if (g == INT32_MAX) break;
       from = g + 1;
@@ -981,18 +1045,17 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
           if (e + 256 * u >= n || v >= V) continue;
           const double y = any_value<T>(p, t[u]);
           if ((float)y != m) continue;
-          const float l = (float)(y - (double)m);
-          if (l > lo || (l == lo && v < idx)) { lo = l; idx = v; best_y = y; }
+          if (y > best || (y == best && v < idx)) { best = y; idx = v; }
         }
       }
       __syncthreads();
     }
-    const float best = block_reduce(lo, shf, [](float x, float y) { return fmaxf(x, y); });
-    const int t = block_reduce(lo == best ? idx : INT32_MAX, shi, [](int x, int y) { return min(x, y); });
+    const double most = block_reduce(best, shd, [](double x, double y) { return fmax(x, y); });
+    const int t = block_reduce(best == most ? idx : INT32_MAX, shi, [](int x, int y) { return min(x, y); });
     if (t == INT32_MAX) {                // (the sum pass computed the same values: one of them is the maximum)
       if (tid == 0) finish(-1, 0.0);
     } else if (idx == t) {
-      finish(t, best_y);
+      finish(t, best);
     }
     return;
   }
@@ -1031,7 +1094,7 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
 #pragma unroll
   for (int e = 0; e < STRIPS; ++e) {
     w[e] = 0.0;
-    if (e < strips && v0 + d0 + e * 64 < V) w[e] = exp2_64(any_value<T>(p, tokens[e]) - (double)m, p.k);
+    if (e < strips && v0 + d0 + e * 64 < V) w[e] = exp2_64(any_value<T>(p, tokens[e]) - top, p.k);
     sum += w[e];
   }
 #pragma unroll
@@ -1151,14 +1214,14 @@ __global__ __launch_bounds__(256) void rules_group_kernel(GroupArgs a) {
     if (MODE == M_APPLY || MODE == M_BWD) {
       float out[K];
       if (MODE == M_BWD) {
-        const float m = a.o.stat[2 * row];
+        const double top = a.o.stat[2 * row];
         const long long tok = a.o.given[row];
-        const bool zero = tok < 0 || tok >= V || m == -INFINITY;
+        const bool zero = tok < 0 || tok >= V || top == -INFINITY;
         const double coef = (double)a.d_logprob[row] * (p.k * LN2), iz = a.o.stat[2 * row + 1];
 #pragma unroll
         for (int j = 0; j < K; ++j) {
           double g = 0.0;
-          if (!zero && ((keep >> j) & 1)) g = coef * ((v0 + j == tok ? 1.0 : 0.0) - exp2_64(y[j] - (double)m, p.k) * iz);
+          if (!zero && ((keep >> j) & 1)) g = coef * ((v0 + j == tok ? 1.0 : 0.0) - exp2_64(y[j] - top, p.k) * iz);
           const float gf = (float)g;
           if (a.part) acc[j] += gf;
           else if (a.d_bias && v0 + j < V) a.d_bias[row * V + v0 + j] = gf;
@@ -1187,15 +1250,15 @@ __global__ __launch_bounds__(256) void rules_group_kernel(GroupArgs a) {
       }
       continue;
     }
-    float m = (float)y[0];
+    double top = y[0];
 #pragma unroll
-    for (int j = 1; j < K; ++j) m = max_nan(m, (float)y[j]);
-    for (int o = W >> 1; o > 0; o >>= 1) m = max_nan(m, __shfl_xor(m, o));
-    const bool ok = m > -INFINITY && m < INFINITY && p.fine;
+    for (int j = 1; j < K; ++j) top = max_nan(top, y[j]);
+    for (int o = W >> 1; o > 0; o >>= 1) top = max_nan(top, __shfl_xor(top, o));
+    const bool ok = top > -INFINITY && (float)top < INFINITY && p.fine;
     double w[K], sum = 0.0;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-      w[j] = ok && ((keep >> j) & 1) ? exp2_64(y[j] - (double)m, p.k) : 0.0;
+      w[j] = ok && ((keep >> j) & 1) ? exp2_64(y[j] - top, p.k) : 0.0;
       sum += w[j];
     }
     double run = sum;                                 // running sum of the lanes, in the vocabulary's order
@@ -1244,7 +1307,7 @@ __global__ __launch_bounds__(256) void rules_group_kernel(GroupArgs a) {
     for (int j = 0; j < K; ++j)
       if (v0 + j == tok) at = y[j];
     at = __shfl(at, tok >= 0 ? tok / K : 0, W);
-    if (lane == 0) end_row<MODE>(q, a.o, p, row, tok, at, m, ok, Z);
+    if (lane == 0) end_row<MODE>(q, a.o, p, row, tok, at, top, ok, Z);
   }
   if (MODE == M_BWD) {
     if (!a.part) return;
@@ -1275,7 +1338,7 @@ struct ColArgs {
 constexpr int COL_STEPS = 4;
 
 template <int T, int HIST>
-__global__ __launch_bounds__(256) void rules_bwd_col_kernel(ColArgs ca) {
+__global__ __launch_bounds__(256, T == DVAE_F32 ? 4 : 2) void rules_bwd_col_kernel(ColArgs ca) {
   typedef Elem<T> E;
   constexpr int EV = E::EV, STEP = 64 * EV, SPAN = COL_STEPS * STEP, PER = HIST ? Counts<HIST ? HIST : 1>::PER_WORD : 1;
   __shared__ uint32_t lds[4 * SPAN];              // counts of each wave's row, then each wave's sums
@@ -1310,6 +1373,18 @@ __global__ __launch_bounds__(256) void rules_bwd_col_kernel(ColArgs ca) {
       count_history<HIST>(p, q.history_i64, v0, min(SPAN, V - v0), cnt, nullptr, lane, 64);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
+    }
+    if (b.far) {
+#pragma unroll 1
+      for (int i = 0; i < COL_STEPS * EV; ++i) {
+        const int d = i / EV * STEP + lane * EV + i % EV;
+        const float y = v0 + d < V ? far_gradient<T, HIST>(a, p, row, b, lrow, orow, cnt, v0, d) : 0.f;
+#pragma unroll
+        for (int j = 0; j < COL_STEPS; ++j)
+#pragma unroll
+          for (int e = 0; e < EV; ++e) acc[j][e] += i == j * EV + e ? y : 0.f;
+      }
+      continue;
     }
 #pragma unroll
     for (int j = 0; j < COL_STEPS; ++j) {
@@ -1550,7 +1625,7 @@ extern "C" int dvae_rules_choose(const dvae_rules* q, const float* uniforms, con
   return uniforms ? run_join<M_DRAW>(a, st) : run_join<M_GREEDY>(a, st);
 }
 
-extern "C" int dvae_rules_logprob(const dvae_rules* q, const long long* tokens, float* logprob, float* stat, void* ws,
+extern "C" int dvae_rules_logprob(const dvae_rules* q, const long long* tokens, float* logprob, double* stat, void* ws,
                                   void* stream) {
   DVAE_REQUIRE(q, "rules_logprob: null pointer");
   DVAE_TRY(rules_check(*q, "rules_logprob"));
@@ -1568,7 +1643,7 @@ extern "C" int dvae_rules_logprob(const dvae_rules* q, const long long* tokens, 
   return run_join<M_SUM>(a, (hipStream_t)stream);
 }
 
-extern "C" int dvae_rules_logprob_bwd(const dvae_rules* q, const long long* tokens, const float* stat,
+extern "C" int dvae_rules_logprob_bwd(const dvae_rules* q, const long long* tokens, const double* stat,
                                       const float* d_logprob, void* d_logits, long long d_ld, float* d_bias, void* ws,
                                       void* stream) {
   DVAE_REQUIRE(q, "rules_logprob_bwd: null pointer");
@@ -1594,7 +1669,7 @@ extern "C" int dvae_rules_logprob_bwd(const dvae_rules* q, const long long* toke
   };
   if (is_small(*q)) {
     GroupArgs m{};
-    m.q = with_constants(*q); m.o.given = tokens; m.o.stat = const_cast<float*>(stat); m.d_logprob = d_logprob;
+    m.q = with_constants(*q); m.o.given = tokens; m.o.stat = const_cast<double*>(stat); m.d_logprob = d_logprob;
     m.out = d_logits; m.out_ld = d_ld; m.d_bias = shared ? nullptr : d_bias; m.part = shared ? (float*)ws : nullptr;
     DVAE_TRY(run_group<M_BWD>(m, shared ? shares : group_blocks(*q), st));
     return shared ? sum_shares() : DVAE_OK;
@@ -1602,7 +1677,7 @@ extern "C" int dvae_rules_logprob_bwd(const dvae_rules* q, const long long* toke
   const Plan p = plan_of(*q);
   SegArgs a{};
   a.q = with_constants(*q); a.out = d_logits; a.out_ld = d_ld; a.o.given = tokens;
-  a.o.stat = const_cast<float*>(stat); a.d_logprob = d_logprob;
+  a.o.stat = const_cast<double*>(stat); a.d_logprob = d_logprob;
   a.d_bias_rows = shared ? nullptr : d_bias;
   if (!shared) return run_seg<M_BWD>(a, p, st);
   ColArgs c{};

@@ -368,7 +368,7 @@ class _LogprobFn(torch.autograd.Function):
         lib = load()
         ws, keep = call.workspace()
         logprob = logits.new_empty(call.rows, dtype=torch.float32)
-        stat = logits.new_empty((call.rows, 2), dtype=torch.float32)
+        stat = logits.new_empty((call.rows, 2), dtype=torch.float64)
         at = tokens.data_ptr(), stat.data_ptr()
         call.launch(lib.dvae_rules_logprob, at[0], logprob.data_ptr(), at[1], ws)
         ctx.call, ctx.stat, ctx.at, ctx.fn = call, stat, at, lib.dvae_rules_logprob_bwd

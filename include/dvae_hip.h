@@ -538,13 +538,13 @@ int dvae_rules_choose(const dvae_rules* rules, const float* uniforms, const int*
                       int* state_out, void* ws, void* stream);
 /* log p of the given tokens [rows]; a token outside [0, vocab) makes an ignored row (0).  stat [rows][2]: kept by the
  * caller for the backward call. */
-int dvae_rules_logprob(const dvae_rules* rules, const long long* tokens, float* logprob, float* stat, void* ws,
+int dvae_rules_logprob(const dvae_rules* rules, const long long* tokens, float* logprob, double* stat, void* ws,
                        void* stream);
 /* d_logits [rows][d_ld] (the logits' type) = slope * d_logprob[r] / temperature * ([v = token] - p), slope the derivative
  * of x2 (1, 1 / repetition or repetition), 0 where the grammar forbids v, in ignored rows and in rows with nothing
  * allowed.  d_bias (or NULL): the same without the slope, summed over the rows in a fixed order for a shared bias
  * ([vocab]), else [rows][vocab].  d_logits may be the logits. */
-int dvae_rules_logprob_bwd(const dvae_rules* rules, const long long* tokens, const float* stat, const float* d_logprob,
+int dvae_rules_logprob_bwd(const dvae_rules* rules, const long long* tokens, const double* stat, const float* d_logprob,
                            void* d_logits, long long d_ld, float* d_bias, void* ws, void* stream);
 
 /* dvae_decoder_predict with its type decisions (dvae_model.py:282-291) under rules: repetition .. temperature (and their

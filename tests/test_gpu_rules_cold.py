@@ -1,0 +1,189 @@
+"""GPU: token rules at low temperatures, where the part of a value that fp32 drops decides -- against oracle/rules_ref.py.
+
+Values there are doubles: y of the kernel and of the oracle are sums, products and quotients of the same doubles in the same
+order (x rho, x / rho, - frequency c, - presence, + bias: 5 roundings, the kernel's division off by one step more), so they differ by
+at most 6 steps of 2^-52 relative to the largest intermediate value A: E = 6 2^-52 A.  An exponent (y - top) / T is then off by 2 E / T plus
+3 roundings of a double, log Z by no more than the exponents of the weights that matter.
+* log p: 4 E / T + 2^-24 |log p| (one rounding to fp32) + 1e-11 (exp2 and log of the kernel).
+* gradients g / T ([v = t] - p) times the slope: p off by p (4 E / T + 1e-11), the difference rounded to fp32, then times the
+  slope's rounding, the product's, and the one to the type.
+Where |x4| / T is ordinary (below 277), sums over more than 128 tokens are fp32 ones: the bounds of test_gpu_rules.py."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import rules_ref as R
+from test_gpu_rules import TINY, TYPES, U, half, log_z_tol, same_or_close
+
+pytestmark = pytest.mark.gpu
+
+COLD = [1e-2, 1e-4, 1e-6, 1e-9, 1e-10, 1e-37]
+
+
+class Cold:
+    """Rows whose largest values lie between two floats: 0, 1 a counted token on top (7.3 / 1.3 lies below its float, 13.7 / 1.3
+    above); 2 a biased one; 3, 4 two tokens that round alike, the larger one first / last; 5 several a few ulps apart;
+    6, 7 negative values only, penalised."""
+    nrows = 8
+
+    def __init__(self, vocab, dtype, history=True, bias=True):
+        g = torch.Generator().manual_seed(vocab)
+        self.vocab, self.dtype = vocab, TYPES[dtype]
+        x = torch.randn(8, vocab, generator=g).clamp_(-3, 3)
+        b = torch.zeros(8, vocab)
+        h = torch.full((8, 3), -1, dtype=torch.int64)
+        lo, hi = 1, vocab - 2
+        x[0, hi], x[1, hi] = 7.3, 13.7
+        h[0, 1] = h[1, 0] = hi
+        x[2, lo], b[2, lo] = 9.0, 0.1234567
+        for r, (first, last) in ((3, (2.0 ** -25, 2.0 ** -26)), (4, (2.0 ** -26, 2.0 ** -25))):
+            x[r, lo] = x[r, hi] = 5.0
+            b[r, lo], b[r, hi] = first, last
+        for i in range(min(4, vocab - 2)):
+            x[5, 1 + i], b[5, 1 + i] = 8.0, 1.0 + 1e-7 * i
+        h[5, 2] = 1
+        x[6] = -9.0 - x[6].abs()
+        x[7] = -5.0
+        h[6] = h[7] = torch.tensor([0, 2, 2])
+        b[6:] = torch.randn(2, vocab, generator=g) * 1e-3
+        self.x = x.to(self.dtype)
+        self.b = b if bias else None
+        self.h = h if history else None
+        self.rho, self.freq, self.pres = 1.3, 0.03, 0.01
+        self.u = torch.tensor([0.5, 0.999, 0.0, 0.4, 0.6, 0.7, 0.3, 0.9])
+        self.g = torch.tensor([1.0, -2.0, 0.5, 1.0, -1.0, 3.0, 0.25, 1.0])
+        self.tokens = torch.tensor([hi, hi, lo, lo, hi, 2, 0, hi])
+
+    def rounded(self):
+        return True
+
+    def rules(self, dev, bias=None):
+        from dvae_amd.rules import TokenRules
+        return TokenRules(self.rho, self.freq, self.pres, bias if bias is not None else None if self.b is None else self.b.to(dev))
+
+    def history(self, dev):
+        return None if self.h is None else self.h.to(dev)
+
+    def row(self, r):
+        c = R.counts(None if self.h is None else self.h[r].tolist(), 3, self.vocab)
+        return R.ruled_row(self.x[r].double().numpy(), c, self.rho, self.freq, self.pres, None if self.b is None else self.b[r].numpy())
+
+    def steps(self, y):
+        """E: how far the kernel's value may be from the oracle's."""
+        return 6 * 2.0 ** -52 * (np.abs(y).max() + 20.0)
+
+    def doubles(self, y, temp):
+        """Whether the row is computed in doubles whatever its vocabulary (away from the rule's borders)."""
+        top = abs(y.max()) / temp
+        return self.vocab <= 128 or top > 1000
+
+
+def tolerance(case, y, lp, temp, drawn):
+    tol = 4 * case.steps(y) / temp + U * abs(lp) + 1e-11
+    return tol if drawn or case.doubles(y, temp) else tol + log_z_tol(case, y, temp)
+
+
+VOCABS = [6, 128, 200, 500, 9000]
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("temp", COLD)
+@pytest.mark.parametrize("vocab", VOCABS)
+def test_decisions_and_their_log_probability(cuda, vocab, temp, dtype):
+    from dvae_amd.rules import choose
+    case = Cold(vocab, dtype)
+    for u in (None, case.u):
+        got = choose(case.x.to(cuda), case.rules(cuda), case.history(cuda), temperature=temp, uniforms=None if u is None else u.to(cuda))
+        for r in range(case.nrows):
+            y, _ = case.row(r)
+            t, lp = R.choose_row(y, temp, None if u is None else float(u[r]))
+            assert int(got.tokens[r]) == t, (r, int(got.tokens[r]), t)
+            same_or_close(float(got.logprob[r]), lp, tolerance(case, y, lp, temp, u is not None), "row %d" % r)
+
+
+def check_gradients(cuda, case, temp, bias_kind):
+    from dvae_amd.rules import token_logprob
+    x = case.x.to(cuda).requires_grad_(True)
+    b = case.b.to(cuda).requires_grad_(True) if case.b is not None else None
+    lp = token_logprob(x, case.tokens.to(cuda), case.rules(cuda, b), case.history(cuda), temperature=temp)
+    grads = torch.autograd.grad(lp, [x] + ([] if b is None else [b]), case.g.to(cuda))
+    total, off = np.zeros(case.vocab), np.zeros(case.vocab)
+    for r in range(case.nrows):
+        y, slope = case.row(r)
+        want, d, dv = R.logprob_row(y, slope, int(case.tokens[r]), temp, float(case.g[r]))
+        same_or_close(lp[r].item(), np.float32(want) if abs(want) > 3.4e38 else want, tolerance(case, y, want, temp, False), "log p of row %d" % r)
+        p = np.exp(R.log_softmax(y, temp)[0])
+        scale = abs(float(case.g[r])) / temp
+        err = scale * p * (4 * case.steps(y) / temp + 1e-11) + U * np.abs(dv) + 2.0 ** -150
+        if not case.doubles(y, temp):
+            err = err + scale * (U * LN2_3 + p * (U * np.abs(y) / temp + 4 * U + log_z_tol(case, y, temp))) + 3 * U * np.abs(dv)
+        same_or_close(grads[0][r].double().cpu().numpy(), d, err * slope + (half(case.dtype) + 2 * U) * np.abs(d) + TINY[case.dtype],
+                      "d logits of row %d" % r)
+        total, off = total + dv, off + err
+        if bias_kind == "rows":
+            same_or_close(grads[1][r].double().cpu().numpy(), dv, err, "d bias of row %d" % r)
+    if bias_kind == "shared":
+        same_or_close(grads[1].double().cpu().numpy(), total, off + case.nrows * U * (np.abs(total) + off), "d bias")
+
+
+LN2_3 = 3 * math.log(2.0)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("temp", COLD)
+@pytest.mark.parametrize("vocab", VOCABS)
+def test_log_probability_and_gradients(cuda, vocab, temp, dtype):
+    check_gradients(cuda, Cold(vocab, dtype), temp, "rows")
+
+
+@pytest.mark.parametrize("temp", [1e-4, 1e-9, 1e-37])
+@pytest.mark.parametrize("vocab", VOCABS)
+def test_gradients_without_a_bias(cuda, vocab, temp):
+    check_gradients(cuda, Cold(vocab, "fp32", bias=False), temp, None)
+
+
+class Shared(Cold):
+    """The same rows under one bias, which is not exact beside any logit of the top."""
+
+    def __init__(self, vocab, dtype, history):
+        super().__init__(vocab, dtype, history)
+        g = torch.Generator().manual_seed(7)
+        self.b = torch.randn(vocab, generator=g) * 1e-3
+
+    def row(self, r):
+        c = R.counts(None if self.h is None else self.h[r].tolist(), 3, self.vocab)
+        return R.ruled_row(self.x[r].double().numpy(), c, self.rho, self.freq, self.pres, self.b.numpy())
+
+
+@pytest.mark.parametrize("history", [False, True])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("temp", [1e-4, 1e-9, 1e-30])
+@pytest.mark.parametrize("vocab", VOCABS)
+def test_gradients_of_a_shared_bias(cuda, vocab, temp, dtype, history):
+    check_gradients(cuda, Shared(vocab, dtype, history), temp, "shared")
+
+
+@pytest.mark.parametrize("vocab", [200, 500, 9000])
+def test_many_cold_rows(cuda, vocab):
+    """Rows of one segment each (a wave decides them) and rows of several: 600 copies of the eight, every copy alike."""
+    from dvae_amd.rules import choose, token_logprob
+    case = Cold(vocab, "fp32")
+    n = 600
+    x, b, h = (t.repeat(n, 1).to(cuda) for t in (case.x, case.b, case.h))
+    from dvae_amd.rules import TokenRules
+    rules = TokenRules(case.rho, case.freq, case.pres, b)
+    few = choose(case.x.to(cuda), case.rules(cuda), case.history(cuda), temperature=1e-10, uniforms=case.u.to(cuda))
+    many = choose(x, rules, h, temperature=1e-10, uniforms=case.u.repeat(n).to(cuda))
+    assert torch.equal(many.tokens, few.tokens.repeat(n))
+    best = choose(x, rules, h, temperature=1e-10)
+    lp = token_logprob(x, case.tokens.repeat(n).to(cuda), rules, h, temperature=1e-10)
+    for r in range(8):
+        y, _ = case.row(r)
+        t, want = R.choose_row(y, 1e-10)
+        assert (best.tokens[r::8] == t).all()
+        tol = tolerance(case, y, want, 1e-10, True)
+        assert (best.logprob[r::8] - want).abs().max() <= tol
+        want = R.log_softmax(y, 1e-10)[0][int(case.tokens[r])]
+        assert ((lp[r::8] - want).abs() <= tolerance(case, y, want, 1e-10, True)).all()
