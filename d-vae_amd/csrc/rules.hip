@@ -30,7 +30,8 @@
 // A low temperature magnifies what the rounding dropped: against the largest value as rounded, a weight 2^((x4 - ref) k) may
 // be 2^1000 or 0 where it is 1.  So doubles are summed against the exact largest value, and a segment whose largest |x4| k is
 // no ordinary one (`ordinary`: beyond 2^-400 .. 2^900, a T below 0.02 for a logit of 13) is summed in doubles throughout, token
-// by token, as is its gradient; within these bounds the rounding moves a log p of fp32 sums by at most 900 ln2 2^-24 = 4e-5.
+// by token, as is its gradient; within these bounds the rounding of the other tokens moves a log p of fp32 sums by at most
+// 900 ln2 2^-24 = 4e-5.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -609,16 +610,24 @@ __device__ __forceinline__ double token_value(const Rules& q, const RowP& p, lon
   return c ? counted64(p, x, c, b) : (double)x + (double)b;
 }
 
-// a row's results: its token, `at` the token's value, Z the row's sum against the reference `top` (its maximum)
+// a row's results: its token, `at` the token's value, Z the row's sum against the reference `top` (its maximum); `rounded`: the
+// weights in Z are those of values rounded to fp32
 template <int MODE>
 __device__ __forceinline__ void end_row(const Rules& q, const RowOut& o, const RowP& p, long long row, long long tok,
-                                        double at, double top, bool ok, double Z) {
+                                        double at, double top, bool ok, double Z, bool rounded) {
   const bool have = tok >= 0 && tok < q.vocab;
   float lp;
   if (MODE == M_SUM && !have) lp = 0.f;                   // an ignored row
   else if (top == -INFINITY) lp = -INFINITY;              // the rules leave nothing
   else if (!ok || !have) lp = NAN;                        // NaN or +inf among the allowed values (or a NaN u)
-  else lp = (float)((at - top) * (p.k * LN2) - log_64(Z));
+  else {
+    // the token's own weight as its value has it (where it is most of Z, log p is that of the others' share and never above 0):
+    // w e^d - w = w (d + d^2 / 2), |d| <= 4e-5
+    const double near = (float)at, d = (at - near) * (p.k * LN2);
+    double z = Z;
+    if (rounded && at != near) z += exp2_64(near - top, p.k) * fma(0.5 * d, d, d);
+    lp = (float)((at - top) * (p.k * LN2) - log_64(z));
+  }
   o.logprob[row] = lp;
   if (MODE == M_SUM) {
     o.stat[2 * row] = top == -INFINITY || ok ? top : NAN;
@@ -888,7 +897,7 @@ __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
   if (lane) return;
   const bool have = tok >= 0 && tok < V;
   const double at = have ? token_value<T>(q, p, row, (int)tok, count((int)tok)) : 0.0;
-  end_row<MODE>(q, a.o, p, row, tok, at, r.top, ok, ok ? r.s * exp2_64(base - r.top, p.k) : 0.0);
+  end_row<MODE>(q, a.o, p, row, tok, at, r.top, ok, ok ? r.s * exp2_64(base - r.top, p.k) : 0.0, !DRAW && !far);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -937,6 +946,7 @@ template <int T, int MODE>
 __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
   constexpr bool SEARCH = MODE != M_SUM;
   __shared__ double shd[4];
+  __shared__ float shf[4];
   __shared__ int shi[4];
   __shared__ double pick_before;
   __shared__ int hist[SEARCH ? HIST_STAGE : 1];
@@ -976,10 +986,16 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
     }
   }
 
-  double top = mine.top;
-  for (int i = i0 + 1; i < i1; ++i) top = max_nan(top, seg[i].top);
-  top = block_reduce(top, shd, [](double x, double y) { return max_nan(x, y); });
-  const bool ok = top > -INFINITY && top < INFINITY && p.fine;
+  float m = (float)mine.top;
+  for (int i = i0 + 1; i < i1; ++i) m = max_nan(m, (float)seg[i].top);
+  m = block_reduce(m, shf, [](float x, float y) { return max_nan(x, y); });
+  const bool ok = m > -INFINITY && m < INFINITY && p.fine, plain = ordinary(m, p.k);
+  double top = m;
+  if (ok && !plain) {                  // the exact one (a reduction of doubles takes half a microsecond more)
+    top = mine.top;
+    for (int i = i0 + 1; i < i1; ++i) top = fmax(top, seg[i].top);
+    top = block_reduce(top, shd, [](double x, double y) { return fmax(x, y); });
+  }
   const auto scaled = [&](const Seg& s) {
     return s.top > -INFINITY ? s.s * exp2_64(reference<MODE>(s.top, p.k) - top, p.k) : 0.0;
   };
@@ -992,7 +1008,8 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
   double Z;
   const double before = block_prefix(z, shd, Z);
 
-  const auto finish = [&](long long t, double y) { end_row<MODE>(q, a.o, p, row, t, y, top, ok, Z); };
+  const bool rounded = MODE != M_DRAW && plain;
+  const auto finish = [&](long long t, double y) { end_row<MODE>(q, a.o, p, row, t, y, top, ok, Z, rounded); };
   if (MODE == M_SUM) {
     if (tid == 0) finish(tok, given_y);
     return;
@@ -1021,7 +1038,6 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
   if (MODE == M_GREEDY) {
     // the segments whose maximum rounds to the row's (hardly ever more than one), and in them the elements that do: among
     // those the largest one, then the lowest index
-    const float m = (float)top;
     double best = -INFINITY;
     int idx = INT32_MAX;
     int from = 0;
@@ -1307,7 +1323,7 @@ __global__ __launch_bounds__(256) void rules_group_kernel(GroupArgs a) {
     for (int j = 0; j < K; ++j)
       if (v0 + j == tok) at = y[j];
     at = __shfl(at, tok >= 0 ? tok / K : 0, W);
-    if (lane == 0) end_row<MODE>(q, a.o, p, row, tok, at, top, ok, Z);
+    if (lane == 0) end_row<MODE>(q, a.o, p, row, tok, at, top, ok, Z, false);
   }
   if (MODE == M_BWD) {
     if (!a.part) return;

@@ -187,3 +187,28 @@ def test_many_cold_rows(cuda, vocab):
         assert (best.logprob[r::8] - want).abs().max() <= tol
         want = R.log_softmax(y, 1e-10)[0][int(case.tokens[r])]
         assert ((lp[r::8] - want).abs() <= tolerance(case, y, want, 1e-10, True)).all()
+
+
+@pytest.mark.parametrize("temp", [0.02, 0.05, 0.2])
+@pytest.mark.parametrize("vocab", [8, 200, 500, 9000])
+@pytest.mark.parametrize("rows", [1, 600])
+def test_a_token_that_is_nearly_everything(cuda, vocab, temp, rows):
+    """Its log p is that of what the others leave, however its value rounds: rows 0 .. 2 of Cold, whose top stands 2.5 and more
+    above values of at most 3 (T 0.02 .. 0.2: the others' share S is at most V e^-12.5).  Its weight is 1 exactly; the fp32 sum of 1 and S is
+    rounded at most 8 + 6 times near 1 (a vector of 8 in the lane it is in, 6 steps of the wave), S itself is off by 2^-17 S (a
+    thousandth of the bound on the weights of test_gpu_rules.py would do); doubles: 1e-11."""
+    from dvae_amd.rules import TokenRules, choose, token_logprob
+    case = Cold(vocab, "fp32")
+    x, b, h = (t[:3].repeat(rows, 1).to(cuda) for t in (case.x, case.b, case.h))
+    tokens = case.tokens[:3].repeat(rows).to(cuda)
+    rules = TokenRules(case.rho, case.freq, case.pres, b)
+    best = choose(x, rules, h, temperature=temp)
+    assert torch.equal(best.tokens, tokens)
+    lp = token_logprob(x, tokens, rules, h, temperature=temp)
+    for r in range(3):
+        y, _ = case.row(r)
+        want = R.log_softmax(y, temp)[0][int(case.tokens[r])]
+        assert want > -0.04
+        tol = U * abs(want) + (14 * U + 2.0 ** -17 * abs(want) if vocab > 128 else 1e-11)
+        for got in (best.logprob[r::3], lp[r::3]):
+            assert (got.double() - want).abs().max() <= tol, (r, float(got[0]), want, tol)
