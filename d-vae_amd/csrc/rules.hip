@@ -126,7 +126,7 @@ __device__ __forceinline__ double counted64(const RowP& p, float x, uint32_t c, 
   const double xd = x;
   double v = xd * p.inv_rho;
   v = fma(fma(-v, p.rho, xd), p.inv_rho, v);
-  v = x > 0.f ? v : xd * p.rho;
+  v = __builtin_amdgcn_classf(x, 0x180) ? v : xd * p.rho;      // positive and finite (+inf: the correction is inf - inf)
   v = fma(-p.freq, (double)c, v);        // one operation everywhere: two kernels compute a value and have to agree
   v -= p.pres;
   return v + (double)b;
@@ -1456,7 +1456,8 @@ struct Plan { int seg_len, nseg, wgs_per_row; bool row_wave; long long blocks; }
 Rules with_constants(const dvae_rules& q) {
   Rules r;
   static_cast<dvae_rules&>(r) = q;
-  r.inv_rho = 1.0 / q.repetition;
+  r.repetition = std::max(q.repetition, 1e-200);               // below it every quotient is beyond fp32, and 1 / rho has to be finite
+  r.inv_rho = 1.0 / r.repetition;
   r.k = LOG2E / q.temperature;
   return r;
 }

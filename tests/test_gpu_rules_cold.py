@@ -212,3 +212,35 @@ def test_a_token_that_is_nearly_everything(cuda, vocab, temp, rows):
         tol = U * abs(want) + (14 * U + 2.0 ** -17 * abs(want) if vocab > 128 else 1e-11)
         for got in (best.logprob[r::3], lp[r::3]):
             assert (got.double() - want).abs().max() <= tol, (r, float(got[0]), want, tol)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("vocab", [5, 100, 300, 9000])
+def test_infinities_that_the_history_holds(cuda, vocab, dtype):
+    """+-inf / 1.3 and +-inf * 1.3 are infinite, not NaN; in the other tokens nothing of them shows."""
+    from dvae_amd.rules import TokenRules, apply_rules, choose
+    g = torch.Generator().manual_seed(vocab)
+    x = torch.randn(3, vocab, generator=g).to(TYPES[dtype])
+    x[0, 1] = x[1, vocab - 1] = math.inf
+    x[1, 0] = x[2, 2] = -math.inf
+    h = torch.tensor([1, 0, vocab - 1, 2, 2])
+    b = torch.randn(vocab, generator=g)
+    for bias in (None, b):
+        r = TokenRules(1.3, 0.25, 0.5, None if bias is None else bias.to(cuda))
+        got = apply_rules(x.to(cuda), r, h.to(cuda)).double().cpu().numpy()
+        for i in range(3):
+            y, _ = R.ruled_row(x[i].double().numpy(), R.counts(h.tolist(), 5, vocab), 1.3, 0.25, 0.5, None if bias is None else bias.numpy())
+            same_or_close(got[i], y, (half(TYPES[dtype]) + U) * np.abs(np.where(np.isfinite(y), y, 0.0)) + TINY[TYPES[dtype]], "row %d" % i)
+        for u in (None, torch.full((3,), 0.5, device=cuda)):
+            picked = choose(x.to(cuda), r, h.to(cuda), uniforms=u)
+            assert picked.tokens[:2].tolist() == [-1, -1] and torch.isnan(picked.logprob[:2]).all() and int(picked.tokens[2]) >= 0
+
+
+def test_a_repetition_penalty_near_zero(cuda):
+    """x / 1e-310 is beyond every type: +inf, not NaN; 0 stays 0 and a negative value goes to 0."""
+    from dvae_amd.rules import TokenRules, apply_rules
+    for vocab in (5, 300):
+        x = torch.zeros(2, vocab, device=cuda)
+        x[:, 0], x[:, 1] = 2.0, -3.0
+        got = apply_rules(x, TokenRules(1e-310), torch.tensor([0, 1, 2], device=cuda))
+        assert torch.isinf(got[:, 0]).all() and (got[:, 0] > 0).all() and (got[:, 1:] == 0).all()
