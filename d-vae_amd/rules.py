@@ -2,7 +2,7 @@
 
 The reference decides node types by a plain argmax or draw (Decoder.predict, dvae_model.py:282-291;
 Svae._predict_from_logits, svae_model.py:112-131).  Here the same decision can be constrained, its log-probability read
-and differentiated, for any vocabulary and for fp32, bf16 and fp16 logits.  With c(v) how often the row's history holds v:
+and differentiated, for vocabularies of up to 2^27 tokens and fp32, bf16 and fp16 logits.  With c(v) how often the row's history holds v:
 
     x1 = x / repetition if x > 0 else x * repetition, where c > 0
     x2 = x1 - frequency * c - presence * [c > 0]
@@ -34,6 +34,7 @@ from ._lib import load
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # DVAE_F32 / DVAE_BF16 / DVAE_F16
 _INDEX = (torch.int32, torch.int64)
+_MAX_VOCAB, _INT_MAX = 2 ** 27, 2 ** 31 - 1                             # what csrc/rules.hip holds; what a C int does
 
 Choice = collections.namedtuple("Choice", "tokens logprob state")
 
@@ -47,6 +48,8 @@ class Grammar:
         if not torch.is_tensor(allowed) or allowed.dtype != torch.bool or allowed.dim() != 2 or 0 in allowed.shape:
             raise ValueError("Grammar: allowed must be a bool tensor [states, vocab]")
         self.states, self.vocab = (int(n) for n in allowed.shape)
+        if self.vocab > _MAX_VOCAB or self.states > _INT_MAX:
+            raise ValueError("Grammar: %d states of %d tokens are too many" % (self.states, self.vocab))
         if not 0 <= int(start) < self.states:
             raise ValueError("Grammar: start state %d of %d" % (int(start), self.states))
         self.start = int(start)
@@ -159,6 +162,8 @@ class _Call:
         shape = logits.shape
         if len(shape) < 1 or shape[-1] < 1:
             raise ValueError("logits must have a vocabulary axis, got %s" % (tuple(shape),))
+        if shape[-1] > _MAX_VOCAB:
+            raise ValueError("a vocabulary of %d tokens: at most 2^27" % shape[-1])
         if rules is None:
             rules = TokenRules()
         elif not isinstance(rules, TokenRules):
@@ -178,6 +183,8 @@ class _Call:
                 raise ValueError("history %s does not go with the rows %s" % (tuple(history.shape), tuple(lead)))
             self._here(history, "history")
             L = history.shape[-1]
+            if L > _INT_MAX:
+                raise ValueError("a history of %d tokens: at most 2^31 - 1" % L)
             if L > 0 and rows > 0:
                 h = history if history.dim() == 2 else history.reshape(-1, L)
                 if L > 1 and h.stride(1) != 1:

@@ -280,3 +280,23 @@ def test_decoder_arguments():
         sv._predict_from_logits(ts, es, temperature=0.5)
     with pytest.raises(ValueError):
         sv._predict_from_logits(ts[0], es[0], rules=TokenRules())
+
+
+def test_sizes_that_a_c_int_does_not_hold():
+    """Refused by the size alone: 2^32 + 5 is no 5 (views of one element: nothing is copied before)."""
+    one, tok = torch.zeros(1, 1, dtype=torch.float16), torch.zeros(1, dtype=torch.int64)
+    for vocab in (2 ** 27 + 1, 2 ** 31, 2 ** 32 + 5):
+        x = one.expand(1, vocab)
+        for call in (lambda: rules.apply_rules(x, TokenRules()), lambda: rules.choose(x), lambda: rules.token_logprob(x, tok)):
+            with pytest.raises(ValueError, match="vocabulary"):
+                call()
+    for length in (2 ** 31, 2 ** 32 + 1):
+        h = torch.zeros(1, 1, dtype=torch.int64).expand(1, length)
+        for call in (lambda: rules.apply_rules(X[:1], TokenRules(), h), lambda: rules.choose(X[:1], history=h),
+                     lambda: rules.token_logprob(X[:1], tok, history=h)):
+            with pytest.raises(ValueError, match="history"):
+                call()
+    yes = torch.ones(1, 1, dtype=torch.bool)
+    for shape in ((2 ** 31, 1), (1, 2 ** 27 + 1)):
+        with pytest.raises(ValueError, match="too many"):
+            Grammar(yes.expand(shape))
