@@ -367,9 +367,11 @@ def choose(logits, rules=None, history=None, lengths=None, state=None, temperatu
 
 
 class _LogprobFn(torch.autograd.Function):
-    # Every tensor behind a pointer goes through save_for_backward: a change between forward and backward is an error.  Where
-    # hooks take saved tensors (stored on the host, computed again by a checkpoint), what they give back is read instead.  The
-    # backward pass runs on autograd's own thread, where Python is slowest: what it needs is at hand when the forward pass ends.
+    # Every tensor behind a pointer goes through save_for_backward, and nothing else keeps it: a change between forward and
+    # backward is an error, and the backward pass (without retain_graph) frees it.  Logits and bias are saved as the call's
+    # detached views, which stay on their memory if the caller gives its tensor another one (x.data = y).  Where hooks take saved
+    # tensors (stored on the host, computed again by a checkpoint), what they give back is read instead.  The backward pass runs
+    # on autograd's own thread, where Python is slowest: what it needs is at hand when the forward pass ends.
     @staticmethod
     def forward(ctx, call, logits, bias, tokens, *others):
         lib = load()
@@ -380,10 +382,9 @@ class _LogprobFn(torch.autograd.Function):
         call.launch(lib.dvae_rules_logprob, at[0], logprob.data_ptr(), at[1], ws)
         ctx.call, ctx.stat, ctx.at, ctx.fn = call, stat, at, lib.dvae_rules_logprob_bwd
         ctx.hooks = torch._C._autograd._top_saved_tensors_default_hooks(False) is not None
-        if ctx.hooks:                                         # theirs to keep
-            call.logits = call.bias = call.given = None
-            call.tensors = ()
-        ctx.save_for_backward(logits, bias, tokens, *others)
+        ctx.save_for_backward(call.logits, call.bias, tokens, *others)
+        call.logits = call.bias = None
+        call.tensors = ()
         return logprob
 
     @staticmethod
@@ -435,7 +436,7 @@ def token_logprob(logits, tokens, rules=None, history=None, lengths=None, state=
     c._per_row(tokens, "tokens", _INDEX)
     tokens = (tokens if tokens.dtype == torch.int64 else tokens.to(torch.int64)).contiguous()
     x, b = c.logits, c.bias
-    c.logits, c.bias, c.given = x.detach(), None if b is None else b.detach(), tokens
+    c.logits, c.bias = x.detach(), None if b is None else b.detach()
     lp = _LogprobFn.apply(c, x, b, tokens, *c.tensors)
     if lp.requires_grad and _on_default_stream(lp.grad_fn, c.index):
         lp = x = b = c = None                             # the error's traceback is not to keep this graph alive as well
