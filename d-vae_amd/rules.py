@@ -26,6 +26,7 @@ import collections
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -310,6 +311,10 @@ def apply_rules(logits, rules, history=None, lengths=None, state=None, out=None)
         raise ValueError("apply_rules has no gradient: detach the logits, or use token_logprob")
     if torch.is_grad_enabled() and isinstance(rules, TokenRules) and rules.bias is not None and rules.bias.requires_grad:
         raise ValueError("apply_rules has no gradient: detach the bias, or use token_logprob")
+    if forward_ad._current_level >= 0:
+        for t in (logits, out, *(vars(rules).values() if isinstance(rules, TokenRules) else ())):
+            if torch.is_tensor(t) and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError("apply_rules has no gradient: its arguments must not be dual tensors")
     c = _Call(logits, rules, history, lengths, state, 1.0)
     if out is None:
         out = logits.new_empty(logits.shape)

@@ -300,3 +300,17 @@ def test_sizes_that_a_c_int_does_not_hold():
     for shape in ((2 ** 31, 1), (1, 2 ** 27 + 1)):
         with pytest.raises(ValueError, match="too many"):
             Grammar(yes.expand(shape))
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor would come back without its tangent: a derivative of 0 that nobody asked for."""
+    import torch.autograd.forward_ad as fw
+    with fw.dual_level():
+        dual, bias = fw.make_dual(X.clone(), torch.ones_like(X)), fw.make_dual(torch.zeros(6), torch.ones(6))
+        for call in (lambda: rules.apply_rules(dual, TokenRules()), lambda: rules.apply_rules(X, TokenRules(bias=bias)),
+                     lambda: rules.apply_rules(X, TokenRules(frequency=fw.make_dual(torch.zeros(4), torch.ones(4)))),
+                     lambda: rules.apply_rules(X, TokenRules(), out=dual)):
+            with pytest.raises(ValueError, match="dual"):
+                call()
+        with pytest.raises(_lib.DvaeError):            # plain tensors inside the level: on to the next check
+            rules.apply_rules(X, TokenRules())
