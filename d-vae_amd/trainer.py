@@ -10,7 +10,7 @@ import os
 
 import torch
 
-from .optim import clip_grads
+from .optim import FlatAdam, clip_grads
 
 
 def save_checkpoint(path, model, optimizer=None, scheduler=None, epoch=0, extra=None):
@@ -92,11 +92,17 @@ class Trainer:
 
     def _step(self, opt):
         """The optimizer's step on gradients of at most gradient_clip_val."""
-        if self.gradient_clip_val > 0.0:
-            if hasattr(opt, 'max_norm'):        # FlatAdam scales the gradients inside its update
-                opt.max_norm = self.gradient_clip_val
-            else:
-                clip_grads([p.grad for g in opt.param_groups for p in g['params']], self.gradient_clip_val)
+        limit = self.gradient_clip_val
+        if limit > 0.0 and isinstance(opt, FlatAdam):       # it scales the gradients inside its update
+            own = opt.max_norm
+            opt.max_norm = limit if own is None else min(own, limit)
+            try:
+                opt.step()
+            finally:
+                opt.max_norm = own
+            return
+        if limit > 0.0:
+            clip_grads([p.grad for g in opt.param_groups for p in g['params']], limit)
         opt.step()
 
     def fit(self, model, resume_from=None):

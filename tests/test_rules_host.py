@@ -314,3 +314,28 @@ def test_forward_mode_derivatives_are_refused():
                 call()
         with pytest.raises(_lib.DvaeError):            # plain tensors inside the level: on to the next check
             rules.apply_rules(X, TokenRules())
+
+
+def test_trainer_leaves_an_optimizers_own_limit_alone(monkeypatch):
+    """FlatAdam clips inside its step, at most to its own limit, and keeps it; any other optimizer's gradients are clipped for
+    it, whatever attributes it has."""
+    from dvae_amd import trainer
+    clipped, seen = [], []
+    monkeypatch.setattr(trainer, "clip_grads", lambda grads, limit: clipped.append((len(grads), limit)))
+    flat = object.__new__(optim.FlatAdam)
+    flat.step = lambda: seen.append(flat.max_norm)
+    for own, want in ((None, 0.5), (0.1, 0.1), (3.0, 0.5)):
+        flat.max_norm = own
+        trainer.Trainer(gradient_clip_val=0.5)._step(flat)
+        assert seen.pop() == want and flat.max_norm == own and not clipped
+
+    class Other:
+        max_norm, param_groups = 7.0, [{'params': [torch.zeros(2), torch.zeros(3)]}]
+
+        def step(self):
+            seen.append(self.max_norm)
+    other = Other()
+    trainer.Trainer(gradient_clip_val=0.5)._step(other)
+    assert clipped == [(2, 0.5)] and seen == [7.0] and other.max_norm == 7.0
+    trainer.Trainer()._step(other)
+    assert len(clipped) == 1 and seen == [7.0, 7.0]
