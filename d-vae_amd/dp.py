@@ -4,6 +4,8 @@ losses are reduction='sum', dvae_model.py:405,429,431, so SUM -- not mean --
 reproduces the single-device big-batch gradient) plus 4 logged loss scalars."""
 import torch
 
+from .rules import check_rules
+
 
 def shard_range(n, rank, world):
     """Contiguous shard [lo, hi) of n items for `rank`; the first n % world ranks get one more."""
@@ -104,6 +106,7 @@ def predict_sharded(decoder, z, dist, is_stochastic=False, uniforms=None, group=
     order.  Stochastic decode without injected uniforms draws them per rank on the device.  `rules`
     (of one setting for all latents) and `temperature` are `Decoder.predict`'s."""
     kw = {}
+    check_rules(rules, temperature, "predict_sharded")
     if rules is not None:
         if (rules.per_row() or torch.is_tensor(temperature)) and dist is not None and dist.is_initialized() \
                 and dist.get_world_size(group) > 1:

@@ -170,6 +170,7 @@ class Decoder(nn.Module):
         grammar then has next states.  A node the rules leave nothing for has
         an all-zero one-hot row.  `temperature` goes with rules."""
         M = z.shape[0]
+        rules_mod.check_rules(rules, temperature, "predict")
         if rules is not None:
             if return_margin:
                 raise ValueError("predict: no margin under rules")
@@ -179,8 +180,6 @@ class Decoder(nn.Module):
             state = None if rules.grammar is None else torch.full((M,), start, dtype=torch.int32, device=z.device)
             # the checks of the decisions that the decode will take
             call = rules_mod._Call(torch.empty(M, self.num_classes, device=z.device), rules, None, None, state, temperature)
-        elif temperature != 1.0:
-            raise ValueError("predict: a temperature goes with rules")
         E._require_cuda(z, "z")
         dims = E._dims_for(self._dims, M, self.seq_len)
         u_type = u_edge = None

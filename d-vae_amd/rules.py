@@ -297,6 +297,15 @@ class _Call:
         return q, keep
 
 
+def check_rules(rules, temperature, what):
+    """For callers with optional rules, which decide plainly without them -- at temperature 1."""
+    if rules is None:
+        if torch.is_tensor(temperature) or temperature != 1.0:
+            raise ValueError("%s: a temperature goes with rules" % what)
+    elif not isinstance(rules, TokenRules):
+        raise ValueError("%s: rules must be a TokenRules" % what)
+
+
 def _address(t):
     return None if t is None else t.data_ptr()
 

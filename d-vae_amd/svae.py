@@ -20,7 +20,7 @@ from . import _lib
 from . import engine as E
 from ._lib import check, load
 from .engine import _f32c, _ptr, _stream
-from .rules import choose
+from .rules import check_rules, choose
 
 
 class GruWeights(nn.Module):
@@ -281,8 +281,7 @@ class Svae(nn.Module):
         inverse CDF (the reference draws with torch.multinomial / torch.bernoulli).  ``rules`` (an addition): a
         rules.TokenRules the types [B, T, C] are decided under, step by step with the string's earlier types as history
         (rules.dag_rules(..., start=1)); a step the rules leave nothing for has an all-zero one-hot row."""
-        if rules is None and temperature != 1.0:
-            raise ValueError("a temperature goes with rules")
+        check_rules(rules, temperature, "predict")
         if rules is not None and type_scores.dim() != 3:
             raise ValueError("rules need the strings' type scores [B, T, C]")
         ts, es = _f32c(type_scores), _f32c(edge_scores)

@@ -316,6 +316,22 @@ def test_forward_mode_derivatives_are_refused():
             rules.apply_rules(X, TokenRules())
 
 
+def test_a_temperature_without_rules():
+    """Refused wherever rules are optional: nothing would follow it."""
+    from argparse import Namespace
+    import dvae_amd
+    from dvae_amd import dp
+    m = dvae_amd.Dvae(Namespace(dataset_file=None, mod=None, bidirectional=False, num_classes=6, max_seq=5,
+                                hidden_state_size=32))
+    sv = dvae_amd.Svae(Namespace(dataset_file=None, bidirectional=False))
+    z, ts, es = torch.zeros(3, 56), torch.zeros(2, 7, 8), torch.zeros(2, 7, 8)
+    for kw in (dict(temperature=0.5), dict(temperature=torch.full((3,), 1.0)), dict(rules="dag")):
+        for call in (lambda: m.decoder.predict(z, **kw), lambda: dp.predict_sharded(m.decoder, z, None, **kw),
+                     lambda: m.generation_eval(z=z, **kw), lambda: sv._predict_from_logits(ts, es, **kw)):
+            with pytest.raises(ValueError, match="rules"):
+                call()
+
+
 def test_trainer_leaves_an_optimizers_own_limit_alone(monkeypatch):
     """FlatAdam clips inside its step, at most to its own limit, and keeps it; any other optimizer's gradients are clipped for
     it, whatever attributes it has."""
