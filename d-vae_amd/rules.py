@@ -2,7 +2,8 @@
 
 The reference decides node types by a plain argmax or draw (Decoder.predict, dvae_model.py:282-291;
 Svae._predict_from_logits, svae_model.py:112-131).  Here the same decision can be constrained, its log-probability read
-and differentiated, for vocabularies of up to 2^27 tokens and fp32, bf16 and fp16 logits.  With c(v) how often the row's history holds v:
+and differentiated, for vocabularies of up to 2^27 tokens and fp32, bf16 and fp16 logits.  With c(v) how often the row's
+history holds v:
 
     x1 = x / repetition if x > 0 else x * repetition, where c > 0
     x2 = x1 - frequency * c - presence * [c > 0]
@@ -315,7 +316,8 @@ def _address(t):
 # ---------------------------------------------------------------------------------------------------------------
 def apply_rules(logits, rules, history=None, lengths=None, state=None, out=None):
     """-> x4 in the logits' type (one rounding).  ``out``: a tensor like the logits to write, which may be the logits
-    themselves; its rows must have adjacent elements.  No gradient: see ``token_logprob``."""
+    themselves, but nothing else that the call reads; its rows must have adjacent elements.  No gradient: see
+    ``token_logprob``."""
     if torch.is_grad_enabled() and torch.is_tensor(logits) and logits.requires_grad:
         raise ValueError("apply_rules has no gradient: detach the logits, or use token_logprob")
     if torch.is_grad_enabled() and isinstance(rules, TokenRules) and rules.bias is not None and rules.bias.requires_grad:
@@ -341,6 +343,10 @@ def apply_rules(logits, rules, history=None, lengths=None, state=None, out=None)
         _apart(o2, c.logits, "out overlaps the logits")
     elif c.rows > 1 and ld != c.logits.stride(0):
         raise ValueError("out overlaps the logits")
+    memory = out.untyped_storage().data_ptr()
+    for t in (c.bias, *c.tensors):                            # read by every workgroup while others write
+        if c.rows and t is not None and t.untyped_storage().data_ptr() == memory:
+            _apart(o2, t, "out overlaps the bias, the history or a setting")
     c.launch(load().dvae_rules_apply, out.data_ptr(), ld)
     E._written([out])
     return out

@@ -527,7 +527,7 @@ typedef struct dvae_rules {
 } dvae_rules;
 /* ws of choose / logprob / logprob_bwd; 0: they take NULL (and for arguments they refuse) */
 size_t dvae_rules_ws_bytes(const dvae_rules* rules);
-/* out [rows][out_ld] (of the logits' type; may be the logits) = x4 */
+/* out [rows][out_ld] (of the logits' type; may be the logits, else apart from all that is read) = x4 */
 int dvae_rules_apply(const dvae_rules* rules, void* out, long long out_ld, void* stream);
 /* One token per row and its log-probability log p.  uniforms NULL: the largest x4, the lowest index of equal ones.
  * uniforms [rows] in [0, 1): the first v at which the running sum of p exceeds u (u below 0 counts as 0, from 1 on the

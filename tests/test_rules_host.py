@@ -316,6 +316,28 @@ def test_forward_mode_derivatives_are_refused():
             rules.apply_rules(X, TokenRules())
 
 
+def test_out_over_an_argument():
+    """A workgroup would read what another one has written.  (No GPU: the check of the device comes first, so stand in for it.)"""
+    flat = torch.zeros(40)
+    bias, rest = flat[10:16], flat[16:40].view(4, 6)
+    setting, apart = flat[:4], flat[4:10]
+    ids = torch.zeros(40, dtype=torch.int32)
+    floats = ids.view(torch.float32)
+    require, launch = rules.E._require_cuda, rules._Call.launch
+    try:
+        rules.E._require_cuda = lambda *a: None
+        rules._Call.launch = lambda *a: None
+        for out, r, kw in ((flat[:24].view(4, 6), TokenRules(bias=bias), {}), (flat[:24].view(4, 6), TokenRules(frequency=setting), {}),
+                           (floats[:24].view(4, 6), TokenRules(), dict(history=ids[8:16].view(4, 2))),
+                           (floats[:24].view(4, 6), TokenRules(), dict(history=ids[32:40].view(4, 2), lengths=ids[20:24])),
+                           (floats[:24].view(4, 6), TokenRules(grammar=G), dict(state=ids[23:27]))):
+            with pytest.raises(ValueError, match="out overlaps"):
+                rules.apply_rules(X, r, out=out, **kw)
+        assert rules.apply_rules(X, TokenRules(frequency=setting, bias=apart), out=rest) is rest          # neighbours
+    finally:
+        rules.E._require_cuda, rules._Call.launch = require, launch
+
+
 def test_a_temperature_without_rules():
     """Refused wherever rules are optional: nothing would follow it."""
     from argparse import Namespace
