@@ -102,6 +102,12 @@ __device__ __forceinline__ RowP row_params(const Rules& q, long long r) {
   return p;
 }
 
+// the same for a path that hardly ever runs, read there: the steps before it need no registers for what only it uses
+__device__ __forceinline__ RowP params_anew(const Rules& q, long long r) {
+  asm volatile("" : "+s"(r));
+  return row_params(q, r);
+}
+
 __device__ __forceinline__ long long hist_at(const RowP& p, int i64, int i) {
   return i64 ? reinterpret_cast<const long long*>(p.hist)[i] : (long long)reinterpret_cast<const int*>(p.hist)[i];
 }
@@ -223,9 +229,9 @@ __device__ __forceinline__ double log_64(double z) {
 
 // whether 2^(m k) and what is near it have their places in the exponents of a double, and the part of m that a rounding to fp32
 // drops does not show in it
-__device__ __forceinline__ bool ordinary(float m, double k) {
-  const double a = (double)m * k;
-  return a > -400.0 && a < 900.0;
+__device__ __forceinline__ bool ordinary(float m, float k) {
+  const float a = m * k;
+  return a > -400.f && a < 900.f;
 }
 
 // whether the row's values may lie between two floats: those of a bias or a history
@@ -241,7 +247,7 @@ enum { M_APPLY = 0, M_SUM = 1, M_GREEDY = 2, M_DRAW = 3, M_BWD = 4 };
 
 template <int MODE>
 __device__ __forceinline__ double reference(double top, double k) {
-  return MODE == M_DRAW && ordinary((float)top, k) ? 0.0 : top;
+  return MODE == M_DRAW && ordinary((float)top, (float)k) ? 0.0 : top;
 }
 
 constexpr int SEG_MAX = 4096;   // tokens of a segment at most: the counts of a workgroup's 4 segments are 32 KB of 16 bits
@@ -466,7 +472,7 @@ struct Bwd {
     down = (float)p.inv_rho;
     zero = t < 0 || t >= a.q.vocab || m == -INFINITY;
     tok = zero ? 0 : (int)t;
-    far = inexact(a.q, p) && fabsf(m) < INFINITY && !ordinary(m, p.k);
+    far = inexact(a.q, p) && fabsf(m) < INFINITY && !ordinary(m, kf);
   }
   // d values of the step's tokens, from v on
   template <typename R, int EV>
@@ -575,7 +581,7 @@ __global__ __launch_bounds__(256) void rules_map_kernel(SegArgs a) {
   Bwd b;
   if (MODE == M_BWD) {
     b = Bwd(a, p, row);
-    if (b.far) {
+    if (__builtin_expect(b.far, 0)) {
 #pragma unroll 1
       for (int d = lane; d < end - v0; d += 64) {
         const float y = far_gradient<T, HIST>(a, p, row, b, lrow, orow, cnt, v0, d);
@@ -649,8 +655,14 @@ constexpr int LIST = 512;       // counted tokens of a segment that are listed; 
 // against a reference of the lane's own that moves when a value exceeds it by 2^8 (an exponent of 8 is still exact to 2^-20).
 // Where the maximum is no ordinary one and either kind of sum would show it, the segment is summed again in doubles, token by
 // token, against its exact maximum.
+// Waves a SIMD: as many as the steps' registers leave without spilling (with the token-by-token sum left to itself the compiler
+// takes more registers for it than the steps do, a wave less: 512 x 131072 bf16 greedy under all rules 66.6 -> 69.3 us).
+constexpr int sum_waves(int T, int HIST, int MODE, bool ROWWAVE) {
+  if (MODE == M_DRAW) return T == DVAE_F32 && !ROWWAVE ? 5 : 4;
+  return HIST && ROWWAVE && T != DVAE_F32 ? 6 : 7;
+}
 template <int T, int HIST, int MODE, bool ROWWAVE>
-__global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
+__global__ __launch_bounds__(256, sum_waves(T, HIST, MODE, ROWWAVE)) void rules_sum_kernel(SegArgs a) {
   constexpr bool DRAW = MODE == M_DRAW;
   typedef Elem<T> E;
   constexpr int EV = E::EV;
@@ -772,13 +784,14 @@ __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
     }
   });
   if (HIST) {
+    const RowP late = DRAW ? p : params_anew(q, row);        // (5 to 9 registers less in the steps)
     const auto one = [&](double y) {
       take((float)y);
       if (DRAW) weigh(y);
       else z += __builtin_amdgcn_exp2f(((float)y - ref) * kf);
     };
     if (held <= LIST) {
-      if (lane < held) one(counted_value<T>(p, first_held));
+      if (lane < held) one(counted_value<T>(late, first_held));
       for (int i = lane + 64; i < held; i += 256) {          // four in flight
         Counted t[4];
 #pragma unroll
@@ -786,20 +799,21 @@ __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
           if (i + 64 * u < held) t[u] = load_counted<T, HIST>(q, p, lrow, cnt, v0, list[i + 64 * u]);
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-          if (i + 64 * u < held) one(counted_value<T>(p, t[u]));
+          if (i + 64 * u < held) one(counted_value<T>(late, t[u]));
       }
     } else {
       for (int w = lane; w < a.seg_len / 32; w += 64)
         for (uint32_t left = seen[w]; left; left &= left - 1)
-          one(counted_value<T>(p, load_counted<T, HIST>(q, p, lrow, cnt, v0, w * 32 + __ffs(left) - 1)));
+          one(counted_value<T>(late, load_counted<T, HIST>(q, p, lrow, cnt, v0, w * 32 + __ffs(left) - 1)));
     }
   }
   m = wave_max_nan(m);
-  const bool ok = m > -INFINITY && m < INFINITY && p.fine;
-  const bool far = ok && (DRAW || inexact(q, p)) && !ordinary(m, p.k);
+  const bool finite = m > -INFINITY && m < INFINITY;
+  const bool far = finite && (DRAW || inexact(q, p)) && !ordinary(m, DRAW ? (float)p.k : kf);
   Seg r;
   r.s = 0.0; r.top = m;
-  if (far) {
+  if (__builtin_expect(far, 0)) {
+    const RowP p = params_anew(q, row);
     const auto value = [&](int d) { return any_value<T>(p, load_counted<T, HIST>(q, p, lrow, cnt, v0, d)); };
     double top = -INFINITY;
 #pragma unroll 1
@@ -809,7 +823,7 @@ __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
 #pragma unroll 1
     for (int d = lane; d < end - v0; d += 64) zd += exp2_rare(value(d) - top, p.k);
     r.s = wave_sum(zd);
-  } else if (ok) {
+  } else if (finite) {
     r.s = DRAW ? wave_sum(zd) : (double)wave_sum(z * __builtin_amdgcn_exp2f((ref - m) * kf));
   }
   if (!ROWWAVE) {
@@ -817,6 +831,7 @@ __global__ __launch_bounds__(256) void rules_sum_kernel(SegArgs a) {
     return;
   }
   // a row of one segment: its wave decides it
+  const bool ok = finite && p.fine;
   const double base = reference<MODE>(r.top, p.k);
   long long tok = -1;
   const auto count = [&](int v) { return HIST ? count_at<HIST ? HIST : 1>(cnt, v) : 0u; };
@@ -989,7 +1004,7 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
   float m = (float)mine.top;
   for (int i = i0 + 1; i < i1; ++i) m = max_nan(m, (float)seg[i].top);
   m = block_reduce(m, shf, [](float x, float y) { return max_nan(x, y); });
-  const bool ok = m > -INFINITY && m < INFINITY && p.fine, plain = ordinary(m, p.k);
+  const bool ok = m > -INFINITY && m < INFINITY && p.fine, plain = ordinary(m, (float)p.k);
   double top = m;
   if (ok && !plain) {                  // the exact one (a reduction of doubles takes half a microsecond more)
     top = mine.top;
@@ -1390,7 +1405,7 @@ __global__ __launch_bounds__(256, T == DVAE_F32 ? 4 : 2) void rules_bwd_col_kern
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     }
-    if (b.far) {
+    if (__builtin_expect(b.far, 0)) {
 #pragma unroll 1
       for (int i = 0; i < COL_STEPS * EV; ++i) {
         const int d = i / EV * STEP + lane * EV + i % EV;
