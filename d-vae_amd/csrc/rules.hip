@@ -268,7 +268,7 @@ struct SegArgs {
   RowOut o;
   int nseg, seg_len;            // segments of a row, their tokens (a multiple of 64 x 16 bytes)
   int wgs_per_row;              // workgroups of a row (ROWWAVE: unused)
-  void* out; long long out_ld;  // APPLY / BWD
+  void* out; long long out_ld;  // APPLY / BWD (NULL: the bias gradient only)
   Seg* seg;                     // sums: a segment's (ROWWAVE: unused)
   const float* d_logprob;       // BWD
   float* d_bias_rows;           // BWD: gradient of a bias of its own per row, [rows][vocab], or NULL
@@ -537,7 +537,7 @@ __device__ __forceinline__ float far_gradient(const SegArgs& a, const RowP& p, l
     const double w = exp2_rare(any_value<T>(p, t) - a.o.stat[2 * row], p.k) * a.o.stat[2 * row + 1];
     y = (float)((double)a.d_logprob[row] * (p.k * LN2) * ((v0 + d == b.tok ? 1.0 : 0.0) - w));
   }
-  orow[v0 + d] = Elem<T>::cast(t.c ? y * (t.x > 0.f ? b.down : b.up) : y);
+  if (a.out) orow[v0 + d] = Elem<T>::cast(t.c ? y * (t.x > 0.f ? b.down : b.up) : y);
   return y;
 }
 
@@ -602,6 +602,7 @@ __global__ __launch_bounds__(256) void rules_map_kernel(SegArgs a) {
         for (int e = 0; e < EV; ++e)
           if (v + e < V) a.d_bias_rows[row * V + v + e] = y[e];
       }
+      if (!a.out) return;
       b.slope(r, y);
     }
     store_step<T, decltype(whole)::value>(orow, v, V, y);
@@ -1263,6 +1264,7 @@ __global__ __launch_bounds__(256) void rules_group_kernel(GroupArgs a) {
 #pragma unroll
         for (int j = 0; j < K; ++j) out[j] = (float)y[j];
       }
+      if (MODE == M_BWD && !a.out) continue;
       typename E::type* orow = static_cast<typename E::type*>(a.out) + row * a.out_ld;
       typename E::type o[K];
 #pragma unroll
@@ -1426,6 +1428,7 @@ __global__ __launch_bounds__(256, T == DVAE_F32 ? 4 : 2) void rules_bwd_col_kern
         b.values(r, in[j].keep, v, y);
 #pragma unroll
         for (int e = 0; e < EV; ++e) acc[j][e] += y[e];
+        if (!a.out) return;
         b.slope(r, y);
         store_step<T, decltype(whole)::value>(orow, v, V, y);
       };
@@ -1689,8 +1692,8 @@ extern "C" int dvae_rules_logprob_bwd(const dvae_rules* q, const long long* toke
     DVAE_LAUNCH_CHECK();
     return DVAE_OK;
   }
-  DVAE_REQUIRE(tokens && stat && d_logprob && d_logits && (ws || !shared), "rules_logprob_bwd: null pointer");
-  DVAE_REQUIRE(q->rows <= 1 || d_ld >= q->vocab, "rules_logprob_bwd: rows of d_logits overlap (ld %lld < vocab %d)", d_ld,
+  DVAE_REQUIRE(tokens && stat && d_logprob && (d_logits || d_bias) && (ws || !shared), "rules_logprob_bwd: null pointer");
+  DVAE_REQUIRE(!d_logits || q->rows <= 1 || d_ld >= q->vocab, "rules_logprob_bwd: rows of d_logits overlap (ld %lld < vocab %d)", d_ld,
                q->vocab);
   const int shares = bias_shares(*q);
   const auto sum_shares = [&]() -> int {

@@ -424,14 +424,15 @@ class _LogprobFn(torch.autograd.Function):
             at = tokens.data_ptr(), at[1]
         if d_logprob.dtype != torch.float32 or not d_logprob.is_contiguous():
             d_logprob = d_logprob.to(torch.float32).contiguous()
-        d_logits = torch.empty_like(logits, memory_format=torch.contiguous_format)
-        d_bias = ws = None
+        d_logits = d_bias = ws = None
         _, want_logits, want_bias, *rest = ctx.needs_input_grad
+        if want_logits:
+            d_logits = torch.empty_like(logits, memory_format=torch.contiguous_format)
         if want_bias:
             d_bias = torch.empty_like(bias, memory_format=torch.contiguous_format)
             ws, keep = call.workspace()
-        E._on_device(call.index, ctx.fn, q, *at, d_logprob.data_ptr(), d_logits.data_ptr(), call.V, _address(d_bias), ws)
-        return None, d_logits if want_logits else None, d_bias, *([None] * len(rest))
+        E._on_device(call.index, ctx.fn, q, *at, d_logprob.data_ptr(), _address(d_logits), call.V, _address(d_bias), ws)
+        return None, d_logits, d_bias, *([None] * len(rest))
 
 
 def _on_default_stream(node, index):

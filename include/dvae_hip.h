@@ -543,7 +543,8 @@ int dvae_rules_logprob(const dvae_rules* rules, const long long* tokens, float* 
 /* d_logits [rows][d_ld] (the logits' type) = slope * d_logprob[r] / temperature * ([v = token] - p), slope the derivative
  * of x2 (1, 1 / repetition or repetition), 0 where the grammar forbids v, in ignored rows and in rows with nothing
  * allowed.  d_bias (or NULL): the same without the slope, summed over the rows in a fixed order for a shared bias
- * ([vocab]), else [rows][vocab].  d_logits may be the logits. */
+ * ([vocab]), else [rows][vocab].  d_logits may be the logits, or NULL where there is a
+ * d_bias: then that alone is computed. */
 int dvae_rules_logprob_bwd(const dvae_rules* rules, const long long* tokens, const double* stat, const float* d_logprob,
                            void* d_logits, long long d_ld, float* d_bias, void* ws, void* stream);
 

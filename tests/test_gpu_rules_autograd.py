@@ -57,3 +57,39 @@ def test_changed_logits_bias_or_tokens_are_refused(cuda, which):
         {"logits": y, "bias": c, "tokens": t}[which].add_(1)
     with pytest.raises(RuntimeError, match="modified"):
         lp.sum().backward()
+
+
+@pytest.mark.parametrize("temperature", [0.7, 1e-9])
+@pytest.mark.parametrize("per_row", [False, True])
+@pytest.mark.parametrize("vocab,history,dtype", [(6, 4, torch.float32), (100, 20, torch.bfloat16), (300, 0, torch.float32),
+                                                 (3000, 0, torch.bfloat16), (9000, 30, torch.float32), (9001, 70000, torch.float16)])
+def test_a_learned_bias_over_frozen_logits(cuda, vocab, history, dtype, per_row, temperature):
+    """The bias gradient alone: the same bits as beside the logits' gradient, and no memory for that."""
+    from dvae_amd.rules import TokenRules, token_logprob
+    g = torch.Generator().manual_seed(vocab)
+    rows = 33
+    x = (torch.randn(rows, vocab, generator=g) * 2).to(dtype).to(cuda)
+    b = torch.randn(*((rows,) if per_row else ()), vocab, generator=g).to(cuda).requires_grad_()
+    h = torch.randint(0, vocab, (rows, history), generator=g).to(cuda) if history else None
+    t, w = torch.randint(-1, vocab, (rows,), generator=g).to(cuda), torch.randn(rows, generator=g).to(cuda)
+    r = TokenRules(1.2, 0.1, 0.2, b)
+    y = x.clone().requires_grad_()
+    want = torch.autograd.grad(token_logprob(y, t, r, h, temperature=temperature), [y, b], w)[1]
+    got, = torch.autograd.grad(token_logprob(x, t, r, h, temperature=temperature), b, w)
+    assert torch.equal(got, want) and torch.isfinite(got).all()
+    # beside frozen logits that do have a gradient elsewhere
+    part, = torch.autograd.grad(token_logprob(y, t, r, h, temperature=temperature), b, w)
+    assert torch.equal(part, want)
+
+
+def test_frozen_logits_cost_no_gradient(cuda):
+    from dvae_amd.rules import TokenRules, token_logprob
+    x = torch.zeros(256, 1 << 16, dtype=torch.bfloat16, device=cuda)
+    b = torch.zeros(1 << 16, device=cuda, requires_grad=True)
+    lp = token_logprob(x, torch.arange(256, device=cuda), TokenRules(bias=b)).sum()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    lp.backward()
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - before < x.numel() * 2 and abs(float(b.grad.sum())) < 1e-3
