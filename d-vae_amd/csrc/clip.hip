@@ -1,8 +1,9 @@
 // Global norm of many gradient tensors, and the gradients scaled down to a largest norm:
 //   norm = sqrt(sum over all tensors of g^2);  coef = min(1, max_norm / (norm + 1e-6));  out = coef g
 // Two streaming passes; every workgroup of the second adds the first one's partial sums in the same fixed order (the same bits
-// every time) and scales by the coefficient: nothing waits on the host.  Squares are formed and added in double: fp32
-// gradients of 1e-30 or 1e30 neither vanish nor overflow, and no order of summation shows in the fp32 result.
+// every time) and scales by the coefficient: nothing waits on the host.  Beyond one batch of tensors a launch of its own adds
+// them, once for all batches.  Squares are formed and added in double: fp32 gradients of 1e-30 or 1e30 neither vanish nor
+// overflow, and no order of summation shows in the fp32 result.
 // Tensors are described in the kernel's arguments (no table in device memory to keep or upload): a launch covers up to
 // CLIP_BATCH of them, cut into chunks of CHUNK elements, each loaded whole before its first value is used.
 // Bound by memory: 400 M bf16 / fp32 gradients into fp32 194 + 535 us (4.1 and 4.5 TB/s; element by element it took 1285); the
@@ -162,15 +163,23 @@ __device__ __forceinline__ void scale_to(int out_type, const void* in, void* out
   else scale_chunk<TI, DVAE_F16>(in, out, base, n, k);
 }
 
-// Chunks from the last to the first: the norm pass read the last ones last, so they are still in the 256 MB cache.  Every
-// workgroup adds the partial sums (a few thousand at most, 4 us less than a launch of their own).
+// Chunks from the last to the first: the norm pass read the last ones last, so they are still in the 256 MB cache.  JOIN: every
+// workgroup adds the partial sums, of one batch at most MAX_GRID (4 us less than a launch of their own), and the first writes
+// norm and coefficient; else out2 holds them (with every batch's workgroups adding every batch's sums, work that grows with the
+// square of the batches, 400 tensors of 400,000 fp32 took 470 us instead of 444).
+template <bool JOIN>
 __global__ __launch_bounds__(256) void scale_kernel(Batch b, const double* __restrict__ part, int n_part, double max_norm,
                                                     float* __restrict__ out2) {
-  const Sum sum = join(part, n_part, max_norm);
-  const float k = (float)sum.coef;
-  if (out2 && blockIdx.x == 0 && threadIdx.x == 0) {
-    out2[0] = (float)sum.norm;
-    out2[1] = k;
+  float k;
+  if (JOIN) {
+    const Sum sum = join(part, n_part, max_norm);
+    k = (float)sum.coef;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      out2[0] = (float)sum.norm;
+      out2[1] = k;
+    }
+  } else {
+    k = out2[1];
   }
   const int chunks = b.start[b.count];
   const Lookup tensor_of(b);
@@ -269,19 +278,20 @@ extern "C" size_t dvae_clip_ws_bytes(int n) {
 
 namespace {
 
-// partial sums of all tensors -> ws; `used` their number
-int partials(const dvae_tensor* tensors, int n, double max_norm, const float* norm_coef, void* ws, int* used, const char* who,
-             hipStream_t st) {
+// partial sums of all tensors -> ws; `used` their number, `batches` how many batches left them
+int partials(const dvae_tensor* tensors, int n, double max_norm, const float* norm_coef, void* ws, int* used, int* batches,
+             const char* who, hipStream_t st) {
   DVAE_REQUIRE(norm_coef && ws, "%s: null pointer", who);
   DVAE_REQUIRE(max_norm >= 0.0, "%s: max_norm must not be negative", who);
   double* part = (double*)ws;
   const size_t room = dvae_clip_ws_bytes(n) / sizeof(double);
-  *used = 0;
+  *used = *batches = 0;
   return for_batches(tensors, n, [&](const Batch& b, int grid) -> int {
     DVAE_REQUIRE((size_t)*used + grid <= room, "%s: too many batches", who);
     hipLaunchKernelGGL(norm_kernel, dim3(grid), dim3(256), 0, st, b, part + *used);
     DVAE_LAUNCH_CHECK();
     *used += grid;
+    ++*batches;
     return DVAE_OK;
   });
 }
@@ -290,8 +300,8 @@ int partials(const dvae_tensor* tensors, int n, double max_norm, const float* no
 
 extern "C" int dvae_grad_norm(const dvae_tensor* tensors, int n, double max_norm, float* norm_coef, void* ws, void* stream) {
   DVAE_TRY(check_tensors(tensors, n, false, "grad_norm"));
-  int used;
-  DVAE_TRY(partials(tensors, n, max_norm, norm_coef, ws, &used, "grad_norm", (hipStream_t)stream));
+  int used, batches;
+  DVAE_TRY(partials(tensors, n, max_norm, norm_coef, ws, &used, &batches, "grad_norm", (hipStream_t)stream));
   hipLaunchKernelGGL(norm_join_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, (const double*)ws, used, max_norm, norm_coef);
   DVAE_LAUNCH_CHECK();
   return DVAE_OK;
@@ -300,18 +310,18 @@ extern "C" int dvae_grad_norm(const dvae_tensor* tensors, int n, double max_norm
 extern "C" int dvae_clip_grads(const dvae_tensor* tensors, int n, double max_norm, float* norm_coef, void* ws, void* stream) {
   DVAE_TRY(check_tensors(tensors, n, true, "clip_grads"));
   hipStream_t st = (hipStream_t)stream;
-  int used;
-  DVAE_TRY(partials(tensors, n, max_norm, norm_coef, ws, &used, "clip_grads", st));
-  float* out2 = norm_coef;              // written by the first batch's launch
-  DVAE_TRY(for_batches(tensors, n, [&](const Batch& b, int grid) -> int {
-    hipLaunchKernelGGL(scale_kernel, dim3(grid), dim3(256), 0, st, b, (const double*)ws, used, max_norm, out2);
-    DVAE_LAUNCH_CHECK();
-    out2 = nullptr;
-    return DVAE_OK;
-  }));
-  if (out2) {                           // no elements at all
-    hipLaunchKernelGGL(norm_join_kernel, dim3(1), dim3(256), 0, st, (const double*)ws, 0, max_norm, norm_coef);
+  int used, batches;
+  DVAE_TRY(partials(tensors, n, max_norm, norm_coef, ws, &used, &batches, "clip_grads", st));
+  if (batches != 1) {                   // several, or no elements at all
+    hipLaunchKernelGGL(norm_join_kernel, dim3(1), dim3(256), 0, st, (const double*)ws, used, max_norm, norm_coef);
     DVAE_LAUNCH_CHECK();
   }
-  return DVAE_OK;
+  return for_batches(tensors, n, [&](const Batch& b, int grid) -> int {
+    if (batches == 1)
+      hipLaunchKernelGGL(scale_kernel<true>, dim3(grid), dim3(256), 0, st, b, (const double*)ws, used, max_norm, norm_coef);
+    else
+      hipLaunchKernelGGL(scale_kernel<false>, dim3(grid), dim3(256), 0, st, b, nullptr, 0, max_norm, norm_coef);
+    DVAE_LAUNCH_CHECK();
+    return DVAE_OK;
+  });
 }
