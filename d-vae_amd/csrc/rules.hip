@@ -617,6 +617,9 @@ __device__ __forceinline__ double token_value(const Rules& q, const RowP& p, lon
   return c ? counted64(p, x, c, b) : (double)x + (double)b;
 }
 
+// what the running sum has to exceed; from u = 1 on nothing does (and the last token with a weight is taken)
+__device__ __forceinline__ double edge_of(float u, double Z) { return u < 1.f ? fmax((double)u, 0.0) * Z : INFINITY; }
+
 // a row's results: its token, `at` the token's value, Z the row's sum against the reference `top` (its maximum); `rounded`: the
 // weights in Z are those of values rounded to fp32
 template <int MODE>
@@ -833,7 +836,7 @@ __global__ __launch_bounds__(256, sum_waves(T, HIST, MODE, ROWWAVE)) void rules_
   }
   // a row of one segment: its wave decides it
   const bool ok = finite && p.fine;
-  const double base = reference<MODE>(r.top, p.k);
+  const double Z = ok ? r.s * exp2_64(reference<MODE>(r.top, p.k) - r.top, p.k) : 0.0;
   long long tok = -1;
   const auto count = [&](int v) { return HIST ? count_at<HIST ? HIST : 1>(cnt, v) : 0u; };
   // values of EV tokens, -inf where there is none
@@ -872,7 +875,7 @@ __global__ __launch_bounds__(256, sum_waves(T, HIST, MODE, ROWWAVE)) void rules_
   } else if (ok && MODE == M_DRAW) {
     const float u = a.o.uniforms[row];
     if (u == u) {
-      const double edge = fmax((double)u, 0.0) * r.s;
+      const double edge = edge_of(u, Z);
       double before = 0.0;
       int last = -1;
       for (int first = 0; first < end && tok < 0; first += 64 * EV) {
@@ -881,7 +884,7 @@ __global__ __launch_bounds__(256, sum_waves(T, HIST, MODE, ROWWAVE)) void rules_
         if (v < end) values(v, w);
 #pragma unroll
         for (int e = 0; e < EV; ++e) {
-          w[e] = v < end ? exp2_64(w[e] - base, p.k) : 0.0;
+          w[e] = v < end ? exp2_64(w[e] - r.top, p.k) : 0.0;
           sum += w[e];
           if (w[e] > 0.0) last = v + e;
         }
@@ -913,7 +916,7 @@ __global__ __launch_bounds__(256, sum_waves(T, HIST, MODE, ROWWAVE)) void rules_
   if (lane) return;
   const bool have = tok >= 0 && tok < V;
   const double at = have ? token_value<T>(q, p, row, (int)tok, count((int)tok)) : 0.0;
-  end_row<MODE>(q, a.o, p, row, tok, at, r.top, ok, ok ? r.s * exp2_64(base - r.top, p.k) : 0.0, !DRAW && !far);
+  end_row<MODE>(q, a.o, p, row, tok, at, r.top, ok, Z, !DRAW && !far);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -1012,8 +1015,10 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
     for (int i = i0 + 1; i < i1; ++i) top = fmax(top, seg[i].top);
     top = block_reduce(top, shd, [](double x, double y) { return fmax(x, y); });
   }
+  // (a segment below 2^-990 of the largest weight counts as 0: what a draw picks has tokens whose own weights, cut at 2^-1000,
+  // are none)
   const auto scaled = [&](const Seg& s) {
-    return s.top > -INFINITY ? s.s * exp2_64(reference<MODE>(s.top, p.k) - top, p.k) : 0.0;
+    return (s.top - top) * p.k >= -990.0 ? s.s * exp2_64(reference<MODE>(s.top, p.k) - top, p.k) : 0.0;
   };
   double z0 = 0.0, z = 0.0;
   if (ok) {
@@ -1093,7 +1098,7 @@ __global__ __launch_bounds__(256) void rules_join_kernel(JoinArgs a) {
   }
 
   // the segment where the running sum passes u Z; beyond the end (u >= 1, or rounding): the last one with a weight
-  const double edge = fmax((double)uf, 0.0) * Z;
+  const double edge = edge_of(uf, Z);
   int first = INT32_MAX, last = -1;
   double first_before = 0.0, last_before = 0.0, run = before;
   for (int i = i0; i < i1; ++i) {
@@ -1318,7 +1323,7 @@ __global__ __launch_bounds__(256) void rules_group_kernel(GroupArgs a) {
       tok = idx < V ? idx : -1;
     } else if (ok && MODE == M_DRAW) {
       const float u = a.o.uniforms[row];
-      const double edge = fmax((double)u, 0.0) * Z;
+      const double edge = edge_of(u, Z);
       double at = run - sum;
       int hit = INT32_MAX, last = -1;
 #pragma unroll

@@ -367,9 +367,9 @@ def choose(logits, rules=None, history=None, lengths=None, state=None, temperatu
     """One token per row -> ``Choice(tokens int64, logprob fp32, state int32 or None)``.
 
     Without ``uniforms`` the largest x4, the lowest index of equal ones.  With ``uniforms`` (fp32, one per row, in [0, 1)) the
-    first token at which the running sum of p exceeds u; either decision is the one of 64-bit arithmetic.  ``logprob`` is
-    log p of the token (detached), ``state`` the grammar's next state where the grammar has ``next_state`` (a row without
-    a token keeps its state)."""
+    first token at which the running sum of p exceeds u (a p below 2^-990 of the largest is 0); either decision is the one of
+    64-bit arithmetic.  ``logprob`` is log p of the token (detached), ``state`` the grammar's next state where the grammar has
+    ``next_state`` (a row without a token keeps its state)."""
     c = _Call(logits, rules, history, lengths, state, temperature)
     u = None
     if uniforms is not None:

@@ -531,8 +531,8 @@ size_t dvae_rules_ws_bytes(const dvae_rules* rules);
 int dvae_rules_apply(const dvae_rules* rules, void* out, long long out_ld, void* stream);
 /* One token per row and its log-probability log p.  uniforms NULL: the largest x4, the lowest index of equal ones.
  * uniforms [rows] in [0, 1): the first v at which the running sum of p exceeds u (u below 0 counts as 0, from 1 on the
- * last token with a probability, NaN as token -1).  The decision is that of 64-bit arithmetic.  A row whose rules leave
- * nothing has token -1 and log-probability -inf.  next [states][vocab] / state_out [rows] (together, or NULL):
+ * last token with a probability, NaN as token -1; one below 2^-990 of the largest is none).  The decision is that of 64-bit
+ * arithmetic.  A row whose rules leave nothing has token -1 and log-probability -inf.  next [states][vocab] / state_out [rows] (together, or NULL):
  * state_out[r] = next[state[r]][token]; a row without a token or a state keeps its state.  state_out may be `state`. */
 int dvae_rules_choose(const dvae_rules* rules, const float* uniforms, const int* next, long long* tokens, float* logprob,
                       int* state_out, void* ws, void* stream);

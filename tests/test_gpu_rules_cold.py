@@ -244,3 +244,17 @@ def test_a_repetition_penalty_near_zero(cuda):
         x[:, 0], x[:, 1] = 2.0, -3.0
         got = apply_rules(x, TokenRules(1e-310), torch.tensor([0, 1, 2], device=cuda))
         assert torch.isinf(got[:, 0]).all() and (got[:, 0] > 0).all() and (got[:, 1:] == 0).all()
+
+
+@pytest.mark.parametrize("vocab", [6, 200, 700, 9000])
+def test_the_smallest_uniform_number_before_improbable_tokens(cuda, vocab):
+    """u = 0 draws the first token that counts as probable -- here 2^-1010 of the largest is none, 2^-980 is one --, u = 1 the
+    last one: never no token at all."""
+    from dvae_amd.rules import choose
+    for low, first in ((-200.0, vocab - 1), (-179.0, 0)):
+        x = torch.full((2, vocab), low, device=cuda)
+        x[0, vocab - 1] = 500.0
+        x[1, 0] = 500.0
+        got = choose(x, uniforms=torch.tensor([0.0, 1.0], device=cuda))
+        assert got.tokens.tolist() == [first, 0 if first else vocab - 1]
+        assert torch.isfinite(got.logprob).all()
