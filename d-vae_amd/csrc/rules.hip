@@ -635,7 +635,7 @@ __device__ __forceinline__ void end_row(const Rules& q, const RowOut& o, const R
     // w e^d - w = w (d + d^2 / 2), |d| <= 4e-5
     const double near = (float)at, d = (at - near) * (p.k * LN2);
     double z = Z;
-    if (rounded && at != near) z += exp2_64(near - top, p.k) * fma(0.5 * d, d, d);
+    if (rounded && at != near && near > -INFINITY) z += exp2_64(near - top, p.k) * fma(0.5 * d, d, d);
     lp = (float)((at - top) * (p.k * LN2) - log_64(z));
   }
   o.logprob[row] = lp;
@@ -1292,6 +1292,7 @@ __global__ __launch_bounds__(256) void rules_group_kernel(GroupArgs a) {
 #pragma unroll
     for (int j = 1; j < K; ++j) top = max_nan(top, y[j]);
     for (int o = W >> 1; o > 0; o >>= 1) top = max_nan(top, __shfl_xor(top, o));
+    if ((float)top == -INFINITY) top = -INFINITY;      // beyond fp32 is forbidden, as in longer rows
     const bool ok = top > -INFINITY && (float)top < INFINITY && p.fine;
     double w[K], sum = 0.0;
 #pragma unroll

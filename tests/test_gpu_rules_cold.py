@@ -258,3 +258,25 @@ def test_the_smallest_uniform_number_before_improbable_tokens(cuda, vocab):
         got = choose(x, uniforms=torch.tensor([0.0, 1.0], device=cuda))
         assert got.tokens.tolist() == [first, 0 if first else vocab - 1]
         assert torch.isfinite(got.logprob).all()
+
+
+@pytest.mark.parametrize("vocab", [6, 200, 700, 9000])
+def test_values_beyond_fp32(cuda, vocab):
+    """The lowest number times a penalty of 1.3 is -inf in fp32: log p -inf and no gradient from it, a row of nothing else is one
+    whose rules leave nothing -- in every kernel."""
+    from dvae_amd.rules import TokenRules, choose, token_logprob
+    low = torch.finfo(torch.float32).min
+    x = torch.zeros(3, vocab, device=cuda)
+    x[:, 1] = low
+    x[1, :] = low
+    h = torch.tensor([[1] * vocab, list(range(vocab)), [1] * vocab], device=cuda)
+    r = TokenRules(1.3)
+    for u in (None, torch.full((3,), 0.5, device=cuda)):
+        got = choose(x, r, h, uniforms=u)
+        assert got.tokens.tolist()[1] == -1 and float(got.logprob[1]) == -math.inf
+        assert got.tokens.tolist()[0] == got.tokens.tolist()[2] >= 0
+    x.requires_grad_(True)
+    lp = token_logprob(x, torch.tensor([1, 1, 0], device=cuda), r, h)
+    dx, = torch.autograd.grad(lp, x, torch.ones(3, device=cuda))
+    assert lp.tolist()[:2] == [-math.inf, -math.inf] and abs(float(lp[2]) + math.log(vocab - 1)) <= 1e-5
+    assert torch.isfinite(dx).all() and (dx[1] == 0).all() and float(dx[2, 1]) == 0.0 and float(dx[0, 0]) < 0.0
