@@ -460,7 +460,7 @@ struct Bwd {
   float m, coef, spread, kf, up, down;
   int tok;
   bool zero;                      // an ignored row, or one whose rules leave nothing
-  bool far;                       // no ordinary maximum: far_gradient instead
+  bool far;                       // no ordinary maximum: struct Far instead
   __device__ __forceinline__ Bwd() {}
   __device__ __forceinline__ Bwd(const SegArgs& a, const RowP& p, long long row) {
     const long long t = a.o.given[row];
@@ -527,19 +527,59 @@ __device__ __forceinline__ double any_value(const RowP& p, const Counted& t) {
   return t.c ? counted64(p, t.x, t.c, t.b) : (double)t.x + (double)t.b;
 }
 
-// one token's gradient in a far row, in doubles: writes the logit's, returns the value's
-template <int T, int HIST>
-__device__ __forceinline__ float far_gradient(const SegArgs& a, const RowP& p, long long row, const Bwd& b, const char* lrow,
-                                              typename Elem<T>::type* orow, const uint32_t* cnt, int v0, int d) {
-  const Counted t = load_counted<T, HIST>(a.q, p, lrow, cnt, v0, d);
-  float y = 0.f;
-  if (t.kept && !b.zero) {
-    const double w = exp2_rare(any_value<T>(p, t) - a.o.stat[2 * row], p.k) * a.o.stat[2 * row + 1];
-    y = (float)((double)a.d_logprob[row] * (p.k * LN2) * ((v0 + d == b.tok ? 1.0 : 0.0) - w));
-  }
-  if (a.out) orow[v0 + d] = Elem<T>::cast(t.c ? y * (t.x > 0.f ? b.down : b.up) : y);
-  return y;
+// ---- rows whose maximum is no ordinary one: token by token in doubles, a few in flight.  What lies `exponents` below the maximum
+// (and by more than any rounding) is passed over after an fp32 sum and a comparison: nearly everything, at low temperatures.
+__device__ __forceinline__ float far_reach(float m, float k, float exponents) {
+  return m - (exponents / k + fabsf(m) * 0x1p-21f);
 }
+
+// the exact maximum of n tokens from v0 on and the sum of their weights against it, over a wave; weights below 2^-200 of the
+// largest are left out
+template <int T, int HIST, int N>
+__device__ __forceinline__ void far_sum(const Rules& q, const RowP& p, const char* lrow, const uint32_t* cnt, int v0, int n,
+                                        int lane, float m, double& top, double& sum) {
+  const float reach = far_reach(m, (float)p.k, 200.f);
+  double best = -INFINITY, s = 0.0;
+#pragma unroll 1
+  for (int d = lane; d < n; d += 64 * N) {
+    Counted t[N];
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+      if (d + 64 * u < n) t[u] = load_counted<T, HIST>(q, p, lrow, cnt, v0, d + 64 * u);
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      if (d + 64 * u >= n || !t[u].kept || (!t[u].c && t[u].x + t[u].b < reach)) continue;
+      const double y = any_value<T>(p, t[u]);
+      const double w = exp2_rare(-fabs(y - best), p.k);
+      s = y > best ? fma(s, w, 1.0) : s + w;
+      best = fmax(best, y);
+    }
+  }
+  top = wave_max(best);
+  sum = wave_sum(best > -INFINITY ? s * exp2_rare(best - top, p.k) : 0.0);
+}
+
+// the gradients of a far row
+struct Far {
+  double top, iz, g;
+  float reach;
+  __device__ __forceinline__ Far(const SegArgs& a, const RowP& p, long long row, const Bwd& b) {
+    top = a.o.stat[2 * row];
+    iz = a.o.stat[2 * row + 1];
+    g = (double)a.d_logprob[row] * (p.k * LN2);
+    // 2^-400 of an ordinary g is no float; a NaN or infinite one shows everywhere
+    reach = fabs(g) < INFINITY ? far_reach(b.m, b.kf, 400.f) : -INFINITY;
+  }
+  // d value of token v
+  template <int T>
+  __device__ __forceinline__ float value(const RowP& p, const Bwd& b, const Counted& t, int v) const {
+    if (!t.kept || b.zero || (!t.c && t.x + t.b < reach && v != b.tok)) return 0.f;
+    return (float)(g * ((v == b.tok ? 1.0 : 0.0) - exp2_rare(any_value<T>(p, t) - top, p.k) * iz));
+  }
+  static __device__ __forceinline__ float slope(const Bwd& b, const Counted& t, float y) {
+    return t.c ? y * (t.x > 0.f ? b.down : b.up) : y;
+  }
+};
 
 // APPLY and BWD: a value written for every logit
 template <int T, int HIST, int MODE, bool ROWWAVE>
@@ -582,10 +622,21 @@ __global__ __launch_bounds__(256) void rules_map_kernel(SegArgs a) {
   if (MODE == M_BWD) {
     b = Bwd(a, p, row);
     if (__builtin_expect(b.far, 0)) {
+      const Far far(a, p, row, b);
 #pragma unroll 1
-      for (int d = lane; d < end - v0; d += 64) {
-        const float y = far_gradient<T, HIST>(a, p, row, b, lrow, orow, cnt, v0, d);
-        if (a.d_bias_rows) a.d_bias_rows[row * V + v0 + d] = y;
+      for (int d = lane; d < end - v0; d += 256) {
+        Counted t[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (d + 64 * u < end - v0) t[u] = load_counted<T, HIST>(q, p, lrow, cnt, v0, d + 64 * u);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int v = v0 + d + 64 * u;
+          if (v >= end) continue;
+          const float y = far.template value<T>(p, b, t[u], v);
+          if (a.d_bias_rows) a.d_bias_rows[row * V + v] = y;
+          if (a.out) orow[v] = E::cast(far.slope(b, t[u], y));
+        }
       }
       return;
     }
@@ -788,7 +839,8 @@ __global__ __launch_bounds__(256, sum_waves(T, HIST, MODE, ROWWAVE)) void rules_
     }
   });
   if (HIST) {
-    const RowP late = DRAW ? p : params_anew(q, row);        // (5 to 9 registers less in the steps)
+    // 5 to 9 registers less in the steps, a wave more or none spilled; a draw of halves has the room (512 x 131072 112 us, 114 so)
+    const RowP late = DRAW && T != DVAE_F32 ? p : params_anew(q, row);
     const auto one = [&](double y) {
       take((float)y);
       if (DRAW) weigh(y);
@@ -818,15 +870,7 @@ __global__ __launch_bounds__(256, sum_waves(T, HIST, MODE, ROWWAVE)) void rules_
   r.s = 0.0; r.top = m;
   if (__builtin_expect(far, 0)) {
     const RowP p = params_anew(q, row);
-    const auto value = [&](int d) { return any_value<T>(p, load_counted<T, HIST>(q, p, lrow, cnt, v0, d)); };
-    double top = -INFINITY;
-#pragma unroll 1
-    for (int d = lane; d < end - v0; d += 64) top = fmax(top, value(d));
-    r.top = top = wave_max(top);
-    zd = 0.0;
-#pragma unroll 1
-    for (int d = lane; d < end - v0; d += 64) zd += exp2_rare(value(d) - top, p.k);
-    r.s = wave_sum(zd);
+    far_sum<T, HIST, 4>(q, p, lrow, cnt, v0, end - v0, lane, m, r.top, r.s);
   } else if (finite) {
     r.s = DRAW ? wave_sum(zd) : (double)wave_sum(z * __builtin_amdgcn_exp2f((ref - m) * kf));
   }
@@ -1377,10 +1421,11 @@ struct ColArgs {
 constexpr int COL_STEPS = 4;
 
 template <int T, int HIST>
-__global__ __launch_bounds__(256, T == DVAE_F32 ? 4 : 2) void rules_bwd_col_kernel(ColArgs ca) {
+__global__ __launch_bounds__(256, T == DVAE_F32 && HIST < 2 ? 4 : 2) void rules_bwd_col_kernel(ColArgs ca) {
   typedef Elem<T> E;
   constexpr int EV = E::EV, STEP = 64 * EV, SPAN = COL_STEPS * STEP, PER = HIST ? Counts<HIST ? HIST : 1>::PER_WORD : 1;
   __shared__ uint32_t lds[4 * SPAN];              // counts of each wave's row, then each wave's sums
+  __shared__ float turn[4][STEP];
   const SegArgs& a = ca.s;
   const Rules& q = a.q;
   const int V = q.vocab, v0 = blockIdx.x * SPAN, lane = threadIdx.x & 63;
@@ -1393,6 +1438,18 @@ __global__ __launch_bounds__(256, T == DVAE_F32 ? 4 : 2) void rules_bwd_col_kern
   for (int j = 0; j < COL_STEPS; ++j)
 #pragma unroll
     for (int e = 0; e < EV; ++e) acc[j][e] = 0.f;
+  const auto sync = [] {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  };
+  const auto count = [&](const RowP& p) {
+    if (!HIST) return;
+    for (int i = lane * 4; i < SPAN / PER; i += 256) *reinterpret_cast<u32x4*>(&cnt[i]) = u32x4{0, 0, 0, 0};
+    sync();
+    count_history<HIST ? HIST : 1>(p, q.history_i64, v0, min(SPAN, V - v0), cnt, nullptr, lane, 64);
+    sync();
+  };
+  bool some_far = false;
   for (long long row = r0 + wave; row < r1; row += 4) {
     const RowP p = row_params(q, row);
     const Bwd b(a, p, row);
@@ -1405,26 +1462,11 @@ __global__ __launch_bounds__(256, T == DVAE_F32 ? 4 : 2) void rules_bwd_col_kern
       if (v0 + (j + 1) * STEP <= V) in[j] = load_step<T, true>(p, lrow, v, V);
       else in[j] = load_step<T, false>(p, lrow, v, V);
     }
-    if (HIST) {
-      for (int i = lane * 4; i < SPAN / PER; i += 256) *reinterpret_cast<u32x4*>(&cnt[i]) = u32x4{0, 0, 0, 0};
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      count_history<HIST>(p, q.history_i64, v0, min(SPAN, V - v0), cnt, nullptr, lane, 64);
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-    }
     if (__builtin_expect(b.far, 0)) {
-#pragma unroll 1
-      for (int i = 0; i < COL_STEPS * EV; ++i) {
-        const int d = i / EV * STEP + lane * EV + i % EV;
-        const float y = v0 + d < V ? far_gradient<T, HIST>(a, p, row, b, lrow, orow, cnt, v0, d) : 0.f;
-#pragma unroll
-        for (int j = 0; j < COL_STEPS; ++j)
-#pragma unroll
-          for (int e = 0; e < EV; ++e) acc[j][e] += i == j * EV + e ? y : 0.f;
-      }
+      some_far = true;
       continue;
     }
+    count(p);
 #pragma unroll
     for (int j = 0; j < COL_STEPS; ++j) {
       const int d = j * STEP + lane * EV, v = v0 + d;
@@ -1440,6 +1482,41 @@ __global__ __launch_bounds__(256, T == DVAE_F32 ? 4 : 2) void rules_bwd_col_kern
       };
       if (v0 + (j + 1) * STEP <= V) step(std::true_type{});
       else if (v < V) step(std::false_type{});
+    }
+  }
+  if (__builtin_expect(some_far, 0)) {
+#pragma unroll 1
+    for (long long row = r0 + wave; row < r1; row += 4) {
+      const RowP p = row_params(q, row);
+      const Bwd b(a, p, row);
+      if (!b.far) continue;
+      const char* lrow = static_cast<const char*>(q.logits) + row * q.ld * (long long)sizeof(typename E::type);
+      typename E::type* orow = static_cast<typename E::type*>(a.out) + row * a.out_ld;
+      const Far far(a, p, row, b);
+      count(p);
+#pragma unroll 1
+      for (int i = 0; i < COL_STEPS; ++i) {         // tokens side by side, then to the lanes that add them up
+#pragma unroll 1
+        for (int c = lane; c < STEP; c += 256) {
+          Counted t[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (v0 + i * STEP + c + 64 * u < V) t[u] = load_counted<T, HIST>(q, p, lrow, cnt, v0, i * STEP + c + 64 * u);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int v = v0 + i * STEP + c + 64 * u;
+            const float y = v < V ? far.template value<T>(p, b, t[u], v) : 0.f;
+            if (a.out && v < V) orow[v] = E::cast(far.slope(b, t[u], y));
+            turn[wave][c + 64 * u] = y;
+          }
+        }
+        sync();
+#pragma unroll
+        for (int j = 0; j < COL_STEPS; ++j)
+#pragma unroll
+          for (int e = 0; e < EV; ++e) acc[j][e] += i == j ? turn[wave][lane * EV + e] : 0.f;
+        sync();
+      }
     }
   }
   __syncthreads();
