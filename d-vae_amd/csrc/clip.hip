@@ -6,7 +6,7 @@
 // overflow, and no order of summation shows in the fp32 result.
 // Tensors are described in the kernel's arguments (no table in device memory to keep or upload): a launch covers up to
 // CLIP_BATCH of them, cut into chunks of CHUNK elements, each loaded whole before its first value is used.
-// Bound by memory: 400 M bf16 / fp32 gradients into fp32 194 + 535 us (4.1 and 4.5 TB/s; element by element it took 1285); the
+// Bound by memory: 400 M bf16 / fp32 gradients into fp32 191 + 524 us (4.2 and 4.6 TB/s; element by element it took 1285); the
 // 40 tensors of a model with 6.9 M parameters 10 + 15 us, most of it the way to the memory and back.
 #include <algorithm>
 #include <cmath>

@@ -16,22 +16,23 @@
 // matter).
 //
 // Bounds.  apply and log p move the logits once each way and are bound by memory: 256 x 131072 bf16 under all rules 31 us
-// (137 MB, 4.4 TB/s), log p of 4096 x 65536 bf16 105 + 10 us, its gradients 175 us (1.07 GB, 6.1 TB/s).  A drawn batch is
-// bound by its sums of doubles: 512 x 131072 bf16 under all rules 105 us for 41 M wave instructions -- 39 per element, 15 of
-// them the exp, 10 its value and masks, the rest counting and reductions -- where the bytes alone would take 29 us; + 17 us
-// join.
+// (137 MB, 4.4 TB/s), log p of 4096 x 65536 bf16 99 + 10 us, its gradients 179 us (1.07 GB, 6.0 TB/s).  A drawn batch is
+// bound by its sums of doubles: 512 x 131072 bf16 under all rules 102 us for 41 M wave instructions -- 39 per element, 15 of
+// them the exp, 10 its value and masks, the rest counting and reductions -- where the bytes alone would take 29 us; + 16 us
+// join.  The same batch taken greedily: 57 us for 25 M (24 per element; without rules 25 us for 10.6 M) + 13 us join.
 //
 // Numbers.  A token the history does not hold has the value x + b, one fp32 rounding; a counted one is computed in double
 // and rounded once.  Decisions do not rest on that rounding: rounding is monotone, so the largest exact value is among the
 // elements whose rounded value is the largest; those few are compared as doubles.  A drawn token is decided where a running
-// sum over the whole vocabulary crosses u Z.  With thousands of probable tokens fp32 weights (off by 5e-8) would decide 3 to 6
-// rows in a thousand otherwise (131072 tokens, normal logits of deviation 2.7, T 0.75 to 1.5), and a bound of their error flags
-// 8 to 37 % of the rows: so weights and sums are doubles, with an exp2 of 4e-14.
+// sum over the whole vocabulary crosses u Z: weights and sums are doubles, with an exp2 of 4e-14.  (131072 tokens, normal logits
+// of deviation 2.7, T 0.5 to 1.5: fp32 weights would decide up to 0.8 rows in a thousand otherwise, fp32 sums of them 10 to
+// 27, and a bound of the weights' error leaves 4 to 17 % of the rows open to a second pass; fp32 operations are hardly quicker,
+// 4.7 cycles a wave against 5.4.)
 // A low temperature magnifies what the rounding dropped: against the largest value as rounded, a weight 2^((x4 - ref) k) may
 // be 2^1000 or 0 where it is 1.  So doubles are summed against the exact largest value, and a segment whose largest |x4| k is
 // no ordinary one (`ordinary`: beyond 2^-400 .. 2^900, a T below 0.02 for a logit of 13) is summed in doubles throughout, token
-// by token, as is its gradient; within these bounds the rounding of the other tokens moves a log p of fp32 sums by at most
-// 900 ln2 2^-24 = 4e-5.
+// by token, as is its gradient (512 x 131072 bf16 with penalties: greedy 53 us, at T 0.01 125); within these bounds the rounding
+// of the other tokens moves a log p of fp32 sums by at most 900 ln2 2^-24 = 4e-5.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

@@ -74,7 +74,7 @@ def _limit(max_norm, what):
 def grad_norm(grads, max_norm=math.inf):
     """-> (norm, coef): the norm of all gradients taken as one vector, and min(1, max_norm / (norm + 1e-6)), both scalars
     on the device (nothing waits for them).  ``grads``: tensors (fp32 / bf16 / fp16, each one stretch of memory; None is
-    left out).  Sums are 64-bit in a fixed order: the same bits every time."""
+    left out).  Sums are 64-bit in a fixed order: the same bits every time.  Neither result carries a gradient."""
     m = _limit(max_norm, "grad_norm")
     ts = _as_list(grads)
     ins = _flat_list(ts, "grad_norm", "gradient")
